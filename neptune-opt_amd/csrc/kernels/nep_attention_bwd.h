@@ -1,0 +1,903 @@
+// nep_attention_bwd.h -- gradients of the online-softmax attention fold on gfx950 MFMA (bf16 or
+// fp16 in, fp32 accumulation).
+//
+// With t_ij = scale q_i.k_j, P_ij = exp(t_ij - lse_i) on the visible pairs (0 elsewhere) and the
+// forward pass's O and lse,
+//   delta_i = dO_i.O_i - dlse_i        dP_ij = dO_i.v_j       dS_ij = P_ij (dP_ij - delta_i)
+//   dV_j = sum_i P_ij dO_i             dK_j = scale sum_i dS_ij q_i
+//   dQ_i = scale sum_j dS_ij k_j
+// P is recomputed tile by tile from lse, so no score matrix is stored.
+//
+// Three kernels per call, none with an atomic: results do not depend on the order of workgroups.
+//  * attention_bwd_rows: delta of every query row, and the rows' start values -lse/scale.
+//  * attention_bwd_kv: a workgroup keeps K and V of its keys in registers and walks the query tiles
+//    (dK and dV stay in registers, four products per pair).
+//  * attention_bwd_q: a workgroup keeps Q and dO of its queries and walks the key tiles (three
+//    products per pair).
+// One kernel with five products instead of seven would add dQ across key blocks: fp32 atomics,
+// whose order changes results, or an fp32 copy of dQ per key block.
+//
+// Mapping (v_mfma_f32_32x32x16): attention_bwd_kv computes S[i][j] with A = Q rows from LDS and
+// B = K rows in registers, so lane l holds key l % 32 and registers hold queries
+// 8*(r/4) + 4*(l/32) + r%4.  That register order is the contraction order of dV^T += dO^T P and
+// dK^T += Q^T dS with P and dS straight from the registers as B; their A operand, rows of dO^T and
+// Q^T, comes from the same LDS tiles through ds_read_b64_tr_b16 (4 rows of 16 columns per 16
+// lanes, transposed), two reads of 4 queries per operand.  attention_bwd_q is the mirror image:
+// S^T with A = K rows, B = Q rows in registers, dQ^T += K^T dS^T.
+//
+// -lse_i/scale and -delta_i are the start values of the S and dP accumulators in attention_bwd_kv
+// (per register there), so P = exp2(c S) and dS = P dP without another operation.
+//
+// P and dS are rounded to the input type for their products (half a step, bf16 2^-8, fp16 2^-11
+// relative; the sums are fp32), the rounding that Q, K, V and dO themselves carry.  fp16 holds
+// 2^8 P (P alone would be subnormal below 2^-14) and dS times a power of two per head, from
+// bounds on |dO_i| and |v_j|, that keeps it below 2^15 and out of the subnormals; both are divided
+// out of the fp32 sums exactly.
+#pragma once
+
+namespace nep {
+
+constexpr int kBwdTile = 64;            // rows per staged tile
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct BwdIn;
+template <>
+struct BwdIn<__bf16> {
+  static constexpr bool kScaled = false;
+  static constexpr float kLift = 0.0f;              // log2 of the factor on P
+  static constexpr u32 kExponent = 0x7f807f80u;     // exponent bits of a packed pair
+};
+template <>
+struct BwdIn<_Float16> {
+  static constexpr bool kScaled = true;
+  static constexpr float kLift = 8.0f;
+  static constexpr u32 kExponent = 0x7c007c00u;
+};
+
+// Whether one of the two 16-bit values of a word is infinite or NaN (exponent all ones: the
+// xor leaves a zero half).  A finite pair never reports; with a non-finite low half the other
+// half does not matter.
+template <typename T>
+__device__ __forceinline__ u32 pair_nonfinite(u32 w) {
+  const u32 t = (w & BwdIn<T>::kExponent) ^ BwdIn<T>::kExponent;
+  return (t - 0x00010001u) & ~t & 0x80008000u;
+}
+
+// Row r of a tile (D 16-bit values, CH = D/8 chunks of 16 bytes) keeps chunk c at position
+// c ^ bwd_swizzle(r).  Two kinds of reads meet the 64 LDS banks (256 bytes a clock): 16 consecutive
+// rows of one chunk, which must spread over the 16 chunk positions of a bank sweep, and for the
+// transposed reads 4 consecutive rows of 4 chunks (one 64-byte window each), so rows differing in
+// their low two bits go to different windows.
+template <int D>
+__device__ __forceinline__ int bwd_swizzle(int row) {
+  if constexpr (D >= 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);   // two rows per sweep
+}
+
+// One tile operand's way into LDS: piece i of wave w fills the 1 KB block i*W + w.  LDS chunk L is
+// row L / CH, position L % CH.  Where the rows of one round of all waves are a multiple of 16 the
+// swizzle is the same in every piece and one offset serves them.
+template <int D, int W, int ROWS = kBwdTile>
+struct BwdTile {
+  static constexpr int CH = D / 8;
+  static constexpr int BYTES = ROWS * D * 2;
+  static constexpr int PIECES = BYTES / 1024 / W;
+  static constexpr int ROUND = 64 * W / CH;            // rows per round
+  static constexpr int OFFS = ROUND % 16 == 0 ? 1 : PIECES;
+  static_assert(PIECES >= 1, "a wave moves at least one block");
+  int offs[OFFS];
+  int step;
+
+  __device__ __forceinline__ BwdTile(int wave, int lane, i64 stride) {
+#pragma unroll
+    for (int i = 0; i < OFFS; ++i) {
+      const int chunk = (i * W + wave) * 64 + lane, row = chunk / CH, p = chunk % CH;
+      offs[i] = (int)((i64)row * stride * 2) + ((p ^ bwd_swizzle<D>(row)) << 4);
+    }
+    step = (int)((i64)ROUND * stride * 2);
+  }
+  // rows [row0, row0 + ROWS) of `base`; those at or past `count` read as zero
+  template <typename T>
+  __device__ __forceinline__ void load(const T* base, i64 stride, int row0, int count, int wave,
+                                       unsigned char* dst) const {
+    const int rows = min(ROWS, count - row0);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(base + (i64)row0 * stride), (short)0, (int)(((i64)(rows - 1) * stride + D) * 2),
+        (int)kRawBufferWord3);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      if constexpr (OFFS == 1) dma16(r, dst + (i * W + wave) * 1024, offs[0] + i * step, 0);
+      else dma16(r, dst + (i * W + wave) * 1024, offs[i], 0);
+    }
+  }
+};
+
+// Operand reads of the 32 rows from `sub` of a tile.
+template <typename T, int D>
+struct BwdRead {
+  typedef typename AttnIn<T>::vec8 vec8;
+  int row_off, sw, tr_off[2], tr_sw[2];
+
+  __device__ __forceinline__ explicit BwdRead(int lane) {
+    const int l32 = lane & 31, hi = lane >> 5;
+    row_off = l32 * (D * 2);
+    sw = bwd_swizzle<D>(l32) ^ hi;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = 8 * u + 4 * hi + ((lane & 15) >> 2);
+      tr_off[u] = row * (D * 2) + (lane & 1) * 8;
+      tr_sw[u] = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ bwd_swizzle<D>(row);
+    }
+  }
+  // row lane % 32, columns [16 s + 8 (lane / 32), + 8)
+  __device__ __forceinline__ vec8 row(const unsigned char* tile, int sub, int s) const {
+    return *(const vec8*)(tile + sub * (D * 2) + row_off + (((2 * (s & 7)) ^ sw) << 4) + (s >> 3) * 256);
+  }
+  // column 32 a + lane % 32 of the rows 16 cs + {4 hi + 0..3, 8 + 4 hi + 0..3}
+  __device__ __forceinline__ vec8 column(const unsigned char* tile, int sub, int cs, int a) const {
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    const unsigned char* p = tile + (sub + 16 * cs) * (D * 2);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4)(p + tr_off[0] + (((4 * (a & 3)) ^ tr_sw[0]) << 4) + (a >> 2) * 256));
+    const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4)(p + tr_off[1] + (((4 * (a & 3)) ^ tr_sw[1]) << 4) + (a >> 2) * 256));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 w = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(vec8, w);
+  }
+  // whether the 32 rows hold an infinity or NaN (the answer is the wave's)
+  __device__ __forceinline__ bool nonfinite(const unsigned char* tile, int sub) const {
+    u32 bad = 0;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const u32x4 w = *(const u32x4*)(tile + sub * (D * 2) + row_off +
+                                      (((2 * (s & 7)) ^ sw) << 4) + (s >> 3) * 256);
+      bad |= pair_nonfinite<T>(w.x) | pair_nonfinite<T>(w.y) | pair_nonfinite<T>(w.z) |
+             pair_nonfinite<T>(w.w);
+    }
+    return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  }
+};
+
+// B operand of contraction step cs from a 32x32 accumulator's packed pairs.
+template <typename T>
+__device__ __forceinline__ typename AttnIn<T>::vec8 packed_operand(const u32* pk, int cs) {
+  u32x4 w;
+  w.x = pk[4 * cs + 0];
+  w.y = pk[4 * cs + 1];
+  w.z = pk[4 * cs + 2];
+  w.w = pk[4 * cs + 3];
+  return __builtin_bit_cast(typename AttnIn<T>::vec8, w);
+}
+
+// The head's power of two on fp16 dS: |dP_ij - delta_i| <= 2 max|dO_i| max|v_j| + max|dlse_i|
+// (Cauchy-Schwarz; delta_i + dlse_i averages the dP_ij), below 2^e; 2^8 P dS 2^(7 - e) stays below
+// 2^15.  Returns 7 - e.  bounds: per 64 rows of queries (|dO|, |dlse|), then per 64 keys |v|.
+__device__ __forceinline__ int bwd_exponent(const float* __restrict__ rows, int nq,
+                                            const float* __restrict__ keys, int nk, int lane) {
+  float g = 0.0f, l = 0.0f, v = 0.0f;
+  for (int i = lane; i < nq; i += 64) {
+    g = __builtin_fmaxf(g, rows[2 * i]);
+    l = __builtin_fmaxf(l, rows[2 * i + 1]);
+  }
+  for (int i = lane; i < nk; i += 64) v = __builtin_fmaxf(v, keys[i]);
+  const float bound = 2.0f * group_max<64>(g) * group_max<64>(v) + group_max<64>(l);
+  const int e = (int)(as_u32(bound) >> 23) - 126;   // bound < 2^e
+  return 7 - min(max(e, -100), 100);
+}
+
+// delta_i and the start values of every query row, and fp16's bounds.  start[bh][sqp] holds
+// -lse/scale + lift (with rows from sq to sqp, a multiple of 64, at -inf: their P is 0), and
+// ndelta[bh][sqp] -delta_i (0 there).  A workgroup of 256 threads takes 64 query rows, D/8 lanes a
+// row; with fp16 the workgroups behind them take 64 keys each and bound |v|.  Rows with an infinity
+// or NaN are left out of the bounds: what they reach is not finite whatever the scale.
+// HBM-bound: O and dO are read once (and V in fp16).
+template <typename T, int D>
+__device__ __forceinline__ void attention_bwd_rows(
+    const T* __restrict__ o, const T* __restrict__ go, const T* __restrict__ v,
+    const float* __restrict__ lse, const float* __restrict__ glse, float* __restrict__ start,
+    float* __restrict__ ndelta, float* __restrict__ bounds, int heads, int sq, int sk, int units,
+    i64 osb, i64 osh, i64 oss, i64 gsb, i64 gsh, i64 gss, i64 vsb, i64 vsh, i64 vss, float scale) {
+  typedef AttnIn<T> In;
+  constexpr int LPR = D / 8, RPP = 256 / LPR;     // lanes per row, rows per pass
+  constexpr bool kScaled = BwdIn<T>::kScaled;
+  __shared__ float wmax[2][4];
+  const int nq = (sq + kBwdTile - 1) / kBwdTile, nk = (sk + kBwdTile - 1) / kBwdTile;
+  const int tid = threadIdx.x, c = tid % LPR;
+  const bool keys = kScaled && (int)blockIdx.x >= units * nq;
+  const int id = keys ? blockIdx.x - units * nq : blockIdx.x, n = keys ? nk : nq;
+  const int bh = id / n, t = id % n;
+  const int b = bh / heads, h = bh % heads;
+  float gm = 0.0f, lm = 0.0f;
+  if (!keys) {
+    const T* op = o + b * osb + h * osh;
+    const T* gp = go + b * gsb + h * gsh;
+    const i64 row0 = (i64)bh * nq * kBwdTile;
+    u32x4 ow[kBwdTile / RPP], gw[kBwdTile / RPP];
+#pragma unroll
+    for (int i = 0; i < kBwdTile / RPP; ++i) {
+      const int row = t * kBwdTile + i * RPP + tid / LPR;
+      ow[i] = gw[i] = u32x4{0u, 0u, 0u, 0u};
+      if (row < sq) {
+        ow[i] = load16_cached(op + (i64)row * oss + 8 * c);
+        gw[i] = load16_cached(gp + (i64)row * gss + 8 * c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBwdTile / RPP; ++i) {
+      const int row = t * kBwdTile + i * RPP + tid / LPR;
+      float dot = 0.0f, g2 = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        dot = __builtin_fmaf(In::lo(ow[i][w]), In::lo(gw[i][w]), dot);
+        dot = __builtin_fmaf(In::hi(ow[i][w]), In::hi(gw[i][w]), dot);
+        if constexpr (kScaled) {
+          g2 = __builtin_fmaf(In::lo(gw[i][w]), In::lo(gw[i][w]), g2);
+          g2 = __builtin_fmaf(In::hi(gw[i][w]), In::hi(gw[i][w]), g2);
+        }
+      }
+      dot = group_sum<LPR>(dot);
+      float dl = 0.0f;
+      if (row < sq && glse != nullptr) dl = glse[(i64)bh * sq + row];
+      if constexpr (kScaled) {
+        g2 = group_sum<LPR>(g2);
+        gm = is_finite(g2) ? __builtin_fmaxf(gm, g2) : gm;
+        lm = is_finite(dl) ? __builtin_fmaxf(lm, __builtin_fabsf(dl)) : lm;
+      }
+      if (c == 0) {
+        start[row0 + row] =
+            row < sq ? -lse[(i64)bh * sq + row] / scale + BwdIn<T>::kLift / (scale * kLog2e) : -kInf;
+        ndelta[row0 + row] = row < sq ? dl - dot : 0.0f;
+      }
+    }
+  } else {
+    const T* vp = v + b * vsb + h * vsh;
+#pragma unroll
+    for (int i = 0; i < kBwdTile / RPP; ++i) {
+      const int row = t * kBwdTile + i * RPP + tid / LPR;
+      float v2 = 0.0f;
+      if (row < sk) {
+        const u32x4 w = load16_cached(vp + (i64)row * vss + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v2 = __builtin_fmaf(In::lo(w[j]), In::lo(w[j]), v2);
+          v2 = __builtin_fmaf(In::hi(w[j]), In::hi(w[j]), v2);
+        }
+      }
+      v2 = group_sum<LPR>(v2);
+      gm = is_finite(v2) ? __builtin_fmaxf(gm, v2) : gm;
+    }
+  }
+  if constexpr (kScaled) {
+    gm = group_max<64>(gm);
+    lm = group_max<64>(lm);
+    if ((tid & 63) == 0) {
+      wmax[0][tid >> 6] = gm;
+      wmax[1][tid >> 6] = lm;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      float m[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        m[i] = __builtin_fmaxf(__builtin_fmaxf(wmax[i][0], wmax[i][1]),
+                               __builtin_fmaxf(wmax[i][2], wmax[i][3]));
+      // the fp32 sum of up to 256 squares is within 2^-15 of its value
+      const float norm = __builtin_sqrtf(m[0]) * 1.001f;
+      if (keys) {
+        bounds[(i64)units * nq * 2 + id] = norm;
+      } else {
+        bounds[2 * id] = norm;
+        bounds[2 * id + 1] = m[1];
+      }
+    }
+  }
+}
+
+// Gradients of [j0, j0 + count) keys in plain fp32, for a workgroup whose key range shares a tile
+// with queries hidden from some of its keys and holding inf or NaN in Q or dO (0 * inf in the
+// products above would reach those keys).  16 adjacent lanes hold a key's row (D/16 dims each);
+// hidden pairs are skipped.  Of the queries [i_begin, i_end).
+template <typename T, int D, bool CAUSAL, int W, class Store>
+__device__ void attention_bwd_exact_kv(const T* __restrict__ qp, const T* __restrict__ kp,
+                                       const T* __restrict__ vp, const T* __restrict__ gp,
+                                       const float* __restrict__ start,
+                                       const float* __restrict__ ndelta, int j0, int count, int sk,
+                                       int i_begin, int i_end, i64 qss, i64 kss, i64 vss, i64 gss,
+                                       float scale, float scale_log2, Store store) {
+  typedef AttnIn<T> In;
+  constexpr int DQ = D / 16;
+  const int tid = threadIdx.x, c = tid & 15;
+  for (int r0 = j0; r0 < j0 + count; r0 += W * 4) {
+    const int j = r0 + (tid >> 4);
+    const bool active = j < sk;
+    float kv[DQ], vv[DQ], dk[DQ], dv[DQ];
+#pragma unroll
+    for (int d = 0; d < DQ; d += 2) {
+      const u32 a = active ? *(const u32*)(kp + (i64)j * kss + c * DQ + d) : 0u;
+      const u32 b = active ? *(const u32*)(vp + (i64)j * vss + c * DQ + d) : 0u;
+      kv[d] = In::lo(a);
+      kv[d + 1] = In::hi(a);
+      vv[d] = In::lo(b);
+      vv[d + 1] = In::hi(b);
+      dk[d] = dk[d + 1] = dv[d] = dv[d + 1] = 0.0f;
+    }
+    for (int i = CAUSAL ? max(i_begin, r0) : i_begin; i < i_end; ++i) {
+      const T* qr = qp + (i64)i * qss + c * DQ;
+      const T* gr = gp + (i64)i * gss + c * DQ;
+      float s = 0.0f, dp = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DQ; d += 2) {
+        const u32 a = *(const u32*)(qr + d), b = *(const u32*)(gr + d);
+        s = __builtin_fmaf(In::lo(a), kv[d], s);
+        s = __builtin_fmaf(In::hi(a), kv[d + 1], s);
+        dp = __builtin_fmaf(In::lo(b), vv[d], dp);
+        dp = __builtin_fmaf(In::hi(b), vv[d + 1], dp);
+      }
+      s = group_sum<16>(s);
+      dp = group_sum<16>(dp);
+      if (active && (!CAUSAL || i >= j)) {
+        const float p =
+            __builtin_amdgcn_exp2f((s + start[i]) * scale_log2) * exp2_int(-(int)BwdIn<T>::kLift);
+        const float ds = p * (dp + ndelta[i]) * scale;
+#pragma unroll
+        for (int d = 0; d < DQ; d += 2) {
+          const u32 a = *(const u32*)(qr + d), b = *(const u32*)(gr + d);
+          dk[d] = __builtin_fmaf(ds, In::lo(a), dk[d]);
+          dk[d + 1] = __builtin_fmaf(ds, In::hi(a), dk[d + 1]);
+          dv[d] = __builtin_fmaf(p, In::lo(b), dv[d]);
+          dv[d + 1] = __builtin_fmaf(p, In::hi(b), dv[d + 1]);
+        }
+      }
+    }
+    if (active) {
+#pragma unroll
+      for (int d = 0; d < DQ; d += 4) {
+        store(0, j, c * DQ + d, dk[d], dk[d + 1], dk[d + 2], dk[d + 3]);
+        store(1, j, c * DQ + d, dv[d], dv[d + 1], dv[d + 2], dv[d + 3]);
+      }
+    }
+  }
+}
+
+// The same for dQ of the queries [i0, i0 + count), over the keys [j_begin, j_end).
+template <typename T, int D, bool CAUSAL, int W, class Store>
+__device__ void attention_bwd_exact_q(const T* __restrict__ qp, const T* __restrict__ kp,
+                                      const T* __restrict__ vp, const T* __restrict__ gp,
+                                      const float* __restrict__ start,
+                                      const float* __restrict__ ndelta, int i0, int count, int sq,
+                                      int j_begin, int j_end, i64 qss, i64 kss, i64 vss, i64 gss,
+                                      float scale, float scale_log2, Store store) {
+  typedef AttnIn<T> In;
+  constexpr int DQ = D / 16;
+  const int tid = threadIdx.x, c = tid & 15;
+  for (int r0 = i0; r0 < i0 + count; r0 += W * 4) {
+    const int i = r0 + (tid >> 4);
+    const bool active = i < sq;
+    float qv[DQ], gv[DQ], dq[DQ];
+#pragma unroll
+    for (int d = 0; d < DQ; d += 2) {
+      const u32 a = active ? *(const u32*)(qp + (i64)i * qss + c * DQ + d) : 0u;
+      const u32 b = active ? *(const u32*)(gp + (i64)i * gss + c * DQ + d) : 0u;
+      qv[d] = In::lo(a);
+      qv[d + 1] = In::hi(a);
+      gv[d] = In::lo(b);
+      gv[d + 1] = In::hi(b);
+      dq[d] = dq[d + 1] = 0.0f;
+    }
+    const float st = active ? start[i] : -kInf, nd = active ? ndelta[i] : 0.0f;
+    const int end = CAUSAL ? min(j_end, r0 + W * 4) : j_end;
+    for (int j = j_begin; j < end; ++j) {
+      const T* kr = kp + (i64)j * kss + c * DQ;
+      const T* vr = vp + (i64)j * vss + c * DQ;
+      float s = 0.0f, dp = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DQ; d += 2) {
+        const u32 a = *(const u32*)(kr + d), b = *(const u32*)(vr + d);
+        s = __builtin_fmaf(In::lo(a), qv[d], s);
+        s = __builtin_fmaf(In::hi(a), qv[d + 1], s);
+        dp = __builtin_fmaf(In::lo(b), gv[d], dp);
+        dp = __builtin_fmaf(In::hi(b), gv[d + 1], dp);
+      }
+      s = group_sum<16>(s);
+      dp = group_sum<16>(dp);
+      if (active && (!CAUSAL || j <= i)) {
+        const float p =
+            __builtin_amdgcn_exp2f((s + st) * scale_log2) * exp2_int(-(int)BwdIn<T>::kLift);
+        const float ds = p * (dp + nd) * scale;
+#pragma unroll
+        for (int d = 0; d < DQ; d += 2) {
+          const u32 a = *(const u32*)(kr + d);
+          dq[d] = __builtin_fmaf(ds, In::lo(a), dq[d]);
+          dq[d + 1] = __builtin_fmaf(ds, In::hi(a), dq[d + 1]);
+        }
+      }
+    }
+    if (active) {
+#pragma unroll
+      for (int d = 0; d < DQ; d += 4)
+        store(i, c * DQ + d, dq[d], dq[d + 1], dq[d + 2], dq[d + 3]);
+    }
+  }
+}
+
+// c += a b with c in vector registers.  The compiler keeps the accumulators of every MFMA of a
+// kernel that needs more than 256 registers in AGPRs, of which there are 256: dK and dV take them
+// all from head dim 128 up, and S and dP beside them would spill.  (`mfma_settle` stands between
+// the last of a chain and the first other use of c: the wait states are the program's here.)
+template <typename T>
+__device__ __forceinline__ void mfma_vgpr(typename AttnIn<T>::vec8 a, typename AttnIn<T>::vec8 b,
+                                          f32x16& c) {
+  if constexpr (__is_same(T, __bf16))
+    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  else
+    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_settle(f32x16& c, f32x16& d) {
+  asm volatile("s_nop 7\ns_nop 7\ns_nop 7" : "+v"(c), "+v"(d));
+}
+
+// dK and dV.  W waves of 32 KB keys each; a wave's K and V rows and its dK^T and dV^T stay in
+// registers, the workgroup's Q and dO tiles are staged for all of its waves.  One wave per SIMD:
+// at KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1
+// (at 32 keys a wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock).
+// PARTS: the queries of a head are split into `parts` of `per` tiles and each part's fp32 sums go
+// to `sums` [part][bh][key][dK, dV][D] for attention_bwd_join.
+template <typename T, int D, bool CAUSAL, int W, int KB, bool PARTS>
+__device__ __forceinline__ void attention_bwd_kv(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    const T* __restrict__ go, const float* __restrict__ start, const float* __restrict__ ndelta,
+    const float* __restrict__ bounds, T* __restrict__ dk, T* __restrict__ dv,
+    float* __restrict__ sums, int units, int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss,
+    i64 ksb, i64 ksh, i64 kss, i64 vsb, i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale,
+    float scale_log2, int parts, int per) {
+  typedef AttnIn<T> In;
+  typedef typename In::vec8 vec8;
+  constexpr int BN = 32 * KB * W;                    // keys per workgroup
+  constexpr int KSTEPS = D / 16, DBLK = D / 32;
+  constexpr int ROWS = D <= 128 ? kBwdTile : 32;     // queries per staged tile
+  constexpr int TILE = ROWS * D * 2;
+  constexpr bool kFull = D * KB >= 256;              // dK and dV take every AGPR
+  constexpr bool kKeysInLds = kFull;                 // and K no vector register
+  constexpr bool kScaled = BwdIn<T>::kScaled;
+  __shared__ __attribute__((aligned(1024))) unsigned char qbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char qbuf1[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char gbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char gbuf1[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char kall[kKeysInLds ? BN * D * 2 : 16];
+  __shared__ __attribute__((aligned(1024))) float sbuf0[2 * kBwdTile];
+  __shared__ __attribute__((aligned(1024))) float sbuf1[2 * kBwdTile];
+
+  const int nkb = (sk + BN - 1) / BN, nq = (sq + kBwdTile - 1) / kBwdTile;
+  const int bh = blockIdx.x % units, id = blockIdx.x / units;
+  const int kb_id = PARTS ? id / parts : id, part = PARTS ? id % parts : 0;
+  if (kb_id >= nkb) return;
+  const int b = bh / heads, h = bh % heads;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const int k0 = kb_id * BN, kw = k0 + wave * 32 * KB;
+  const T* qp = q + b * qsb + h * qsh;
+  const T* kp = k + b * ksb + h * ksh;
+  const T* vp = v + b * vsb + h * vsh;
+  const T* gp = go + b * gsb + h * gsh;
+  const float* st = start + (i64)bh * nq * kBwdTile;
+  const float* nd = ndelta + (i64)bh * nq * kBwdTile;
+  // causal: key j is seen by the queries from j on
+  constexpr int PER = kBwdTile / ROWS;
+  const int tiles = (sq + ROWS - 1) / ROWS, first = CAUSAL ? k0 / ROWS : 0;
+  const int t0 = PARTS ? max(first, part * per * PER) : first;
+  const int t1 = PARTS ? min(tiles, (part + 1) * per * PER) : tiles;
+
+  vec8 kreg[kKeysInLds ? 1 : KB][kKeysInLds ? 1 : KSTEPS], vreg[KB][KSTEPS];
+#pragma unroll
+  for (int x = 0; x < KB; ++x) {
+    const int j = kw + 32 * x + l32;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      vreg[x][s] = vec8{};
+      if constexpr (!kKeysInLds) kreg[x][s] = vec8{};
+      if (j < sk) {
+        if constexpr (!kKeysInLds) kreg[x][s] = *(const vec8*)(kp + (i64)j * kss + 16 * s + 8 * hi);
+        vreg[x][s] = *(const vec8*)(vp + (i64)j * vss + 16 * s + 8 * hi);
+      }
+    }
+  }
+  int lift = 0;
+  if constexpr (kScaled)
+    lift = bwd_exponent(bounds + 2 * (i64)bh * nq, nq,
+                        bounds + 2 * (i64)units * nq + (i64)bh * ((sk + kBwdTile - 1) / kBwdTile),
+                        (sk + kBwdTile - 1) / kBwdTile, lane);
+  const float ds_mul = exp2_int(lift);
+
+  const BwdTile<D, W, ROWS> qdma(wave, lane, qss), gdma(wave, lane, gss);
+  const BwdRead<T, D> rd(lane);
+  auto issue = [&](int tile, unsigned char* qd, unsigned char* gd, float* sd) {
+    qdma.load(qp, qss, tile * ROWS, sq, wave, qd);
+    gdma.load(gp, gss, tile * ROWS, sq, wave, gd);
+    if (wave < 2) {
+      const float* src = (wave == 0 ? st : nd) + (i64)tile * ROWS;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)src, (short)0, ROWS * 4, (int)kRawBufferWord3);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(sd + wave * kBwdTile), 4, lane * 4, 0, 0, 0);
+    }
+  };
+
+  f32x16 dka[KB][DBLK], dva[KB][DBLK];
+#pragma unroll
+  for (int x = 0; x < KB; ++x)
+#pragma unroll
+    for (int a = 0; a < DBLK; ++a) dka[x][a] = dva[x][a] = f32x16{};
+  bool bad = false;
+
+  auto body = [&](int tile, const unsigned char* qt, const unsigned char* gt, const float* sv) {
+#pragma unroll
+    for (int sub = 0; sub < ROWS; sub += 32) {
+      const int i0 = tile * ROWS + sub;
+      if (CAUSAL && i0 + 31 < kw) continue;          // every pair hidden
+      f32x16 s[KB], dp[KB];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 a = *(const f32x4*)(sv + sub + 8 * g + 4 * hi);
+        const f32x4 c = *(const f32x4*)(sv + kBwdTile + sub + 8 * g + 4 * hi);
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[x][4 * g + r] = a[r];
+            dp[x][4 * g + r] = c[r];
+          }
+      }
+      if constexpr (kFull) {
+#pragma unroll
+        for (int x = 0; x < KB; ++x) asm volatile("s_nop 1" : "+v"(s[x]), "+v"(dp[x]));
+      }
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        const vec8 a = rd.row(qt, sub, t);
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          if constexpr (kFull) mfma_vgpr<T>(a, rd.row(kall, wave * 32 * KB + 32 * x, t), s[x]);
+          else s[x] = In::mfma(a, kreg[x][t], s[x]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        const vec8 a = rd.row(gt, sub, t);
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          if constexpr (kFull) mfma_vgpr<T>(a, vreg[x][t], dp[x]);
+          else dp[x] = In::mfma(a, vreg[x][t], dp[x]);
+        }
+      }
+      if constexpr (kFull) {
+#pragma unroll
+        for (int x = 0; x < KB; ++x) mfma_settle(s[x], dp[x]);
+      }
+      u32 pk[KB][8], dk2[KB][8];
+#pragma unroll
+      for (int x = 0; x < KB; ++x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][r] = __builtin_amdgcn_exp2f(s[x][r] * scale_log2);
+      }
+      // rows past the end are zero and P = 2^-inf, but not where K or V of the lane's key is
+      // infinite or NaN: they are hidden too
+      if ((CAUSAL && i0 < kw + 32 * KB - 1) || i0 + 32 > sq) {
+        if (CAUSAL) bad |= rd.nonfinite(qt, sub) | rd.nonfinite(gt, sub);
+        const int end = sq - i0 - 4 * hi;
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          const int first_seen = CAUSAL ? kw + 32 * x + l32 - i0 - 4 * hi : 0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int row = 8 * (r >> 2) + (r & 3);
+            if (row < first_seen || row >= end) s[x][r] = dp[x][r] = 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < KB; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          pk[x][r >> 1] = In::pack2(s[x][r], s[x][r + 1]);
+          float a = s[x][r], c = s[x][r + 1];
+          if constexpr (kScaled) {
+            a *= ds_mul;
+            c *= ds_mul;
+          }
+          dk2[x][r >> 1] = In::pack2(a * dp[x][r], c * dp[x][r + 1]);
+        }
+#pragma unroll
+      for (int cs = 0; cs < 2; ++cs)
+#pragma unroll
+        for (int a = 0; a < DBLK; ++a) {
+          const vec8 t = rd.column(gt, sub, cs, a);
+#pragma unroll
+          for (int x = 0; x < KB; ++x)
+            dva[x][a] = In::mfma(t, packed_operand<T>(pk[x], cs), dva[x][a]);
+        }
+#pragma unroll
+      for (int cs = 0; cs < 2; ++cs)
+#pragma unroll
+        for (int a = 0; a < DBLK; ++a) {
+          const vec8 t = rd.column(qt, sub, cs, a);
+#pragma unroll
+          for (int x = 0; x < KB; ++x)
+            dka[x][a] = In::mfma(t, packed_operand<T>(dk2[x], cs), dka[x][a]);
+        }
+    }
+  };
+
+  // Tile t is used from buffers t % 2 while the loads of tile t+1 fill the others (last read in
+  // iteration t-1, before this iteration's barrier).
+  auto landed = []() { __builtin_amdgcn_s_waitcnt(0x0F70); };   // vmcnt(0)
+  if (t0 < t1) {
+    if constexpr (kKeysInLds) {
+      const BwdTile<D, W, ROWS> kdma(wave, lane, kss);
+#pragma unroll
+      for (int r = 0; r < BN; r += ROWS)
+        if (k0 + r < sk) kdma.load(kp, kss, k0 + r, sk, wave, kall + r * D * 2);
+    }
+    issue(t0, qbuf0, gbuf0, sbuf0);
+    for (int tile = t0; tile < t1; tile += 2) {
+      landed();
+      __syncthreads();
+      if (tile + 1 < t1) issue(tile + 1, qbuf1, gbuf1, sbuf1);
+      body(tile, qbuf0, gbuf0, sbuf0);
+      landed();
+      __syncthreads();
+      if (tile + 2 < t1) issue(tile + 2, qbuf0, gbuf0, sbuf0);
+      if (tile + 1 < t1) body(tile + 1, qbuf1, gbuf1, sbuf1);
+    }
+  }
+
+  const i64 row0 = (i64)bh * sk;
+  float* const part_rows = PARTS ? sums + ((i64)part * units + bh) * sk * 2 * D : nullptr;
+  auto store = [&](int which, int j, int d, float a0, float a1, float a2, float a3) {
+    if constexpr (PARTS) {
+      *(f32x4*)(part_rows + ((i64)j * 2 + which) * D + d) = f32x4{a0, a1, a2, a3};
+    } else {
+      u32x2 w;
+      w.x = In::pack2(a0, a1);
+      w.y = In::pack2(a2, a3);
+      *(u32x2*)((which ? dv : dk) + (row0 + j) * D + d) = w;
+    }
+  };
+  if constexpr (CAUSAL) {
+    if (__syncthreads_or(bad)) {
+      attention_bwd_exact_kv<T, D, CAUSAL, W>(qp, kp, vp, gp, st, nd, k0, BN, sk, t0 * ROWS,
+                                              min(sq, t1 * ROWS), qss, kss, vss, gss, scale,
+                                              scale_log2, store);
+      return;
+    }
+  }
+  const float pf = exp2_int(-(int)BwdIn<T>::kLift), sf = scale * pf * exp2_int(-lift);
+#pragma unroll
+  for (int x = 0; x < KB; ++x) {
+    const int j = kw + 32 * x + l32;
+    if (j >= sk) continue;
+#pragma unroll
+    for (int a = 0; a < DBLK; ++a)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * a + 8 * g + 4 * hi;
+        store(0, j, d, dka[x][a][4 * g] * sf, dka[x][a][4 * g + 1] * sf, dka[x][a][4 * g + 2] * sf,
+              dka[x][a][4 * g + 3] * sf);
+        store(1, j, d, dva[x][a][4 * g] * pf, dva[x][a][4 * g + 1] * pf, dva[x][a][4 * g + 2] * pf,
+              dva[x][a][4 * g + 3] * pf);
+      }
+  }
+}
+
+// dQ.  W waves of 32 QB queries each; a wave's Q and dO rows and its dQ^T stay in registers, the
+// workgroup's K and V tiles are staged for all of its waves.  PARTS: a head's keys are split into
+// `parts` of `per` tiles, the parts' fp32 sums go to `sums` [part][bh][query][D].
+template <typename T, int D, bool CAUSAL, int W, int QB, bool PARTS>
+__device__ __forceinline__ void attention_bwd_q(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    const T* __restrict__ go, const float* __restrict__ start, const float* __restrict__ ndelta,
+    const float* __restrict__ bounds, T* __restrict__ dq, float* __restrict__ sums, int units,
+    int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss, i64 ksb, i64 ksh, i64 kss, i64 vsb,
+    i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale, float scale_log2, int parts,
+    int per) {
+  typedef AttnIn<T> In;
+  typedef typename In::vec8 vec8;
+  constexpr int BM = 32 * QB * W;
+  constexpr int KSTEPS = D / 16, DBLK = D / 32;
+  constexpr int TILE = kBwdTile * D * 2;
+  constexpr bool kScaled = BwdIn<T>::kScaled;
+  __shared__ __attribute__((aligned(1024))) unsigned char kbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char kbuf1[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char vbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char vbuf1[TILE];
+
+  const int nqb = (sq + BM - 1) / BM, nq = (sq + kBwdTile - 1) / kBwdTile;
+  const int nk = (sk + kBwdTile - 1) / kBwdTile;
+  const int bh = blockIdx.x % units, id = blockIdx.x / units;
+  const int qb = nqb - 1 - (PARTS ? id / parts : id), part = PARTS ? id % parts : 0;   // heaviest first
+  if (qb < 0) return;
+  const int b = bh / heads, h = bh % heads;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const int q0 = qb * BM, qw = q0 + wave * 32 * QB;
+  const T* qp = q + b * qsb + h * qsh;
+  const T* kp = k + b * ksb + h * ksh;
+  const T* vp = v + b * vsb + h * vsh;
+  const T* gp = go + b * gsb + h * gsh;
+  const float* st = start + (i64)bh * nq * kBwdTile;
+  const float* nd = ndelta + (i64)bh * nq * kBwdTile;
+  const int last = CAUSAL ? min(nk, (q0 + BM + kBwdTile - 1) / kBwdTile) : nk;
+  const int t0 = PARTS ? part * per : 0;
+  const int t1 = PARTS ? min(last, t0 + per) : last;
+
+  vec8 qreg[QB][KSTEPS], greg[QB][KSTEPS];
+  float shift[QB], minus[QB];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int i = qw + 32 * x + l32;
+    shift[x] = i < sq ? st[i] * scale_log2 : -kInf;
+    minus[x] = i < sq ? nd[i] : 0.0f;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      qreg[x][s] = greg[x][s] = vec8{};
+      if (i < sq) {
+        qreg[x][s] = *(const vec8*)(qp + (i64)i * qss + 16 * s + 8 * hi);
+        greg[x][s] = *(const vec8*)(gp + (i64)i * gss + 16 * s + 8 * hi);
+      }
+    }
+  }
+  int lift = 0;
+  if constexpr (kScaled)
+    lift = bwd_exponent(bounds + 2 * (i64)bh * nq, nq, bounds + 2 * (i64)units * nq + (i64)bh * nk,
+                        nk, lane);
+  const float ds_mul = exp2_int(lift);
+
+  const BwdTile<D, W> kdma(wave, lane, kss), vdma(wave, lane, vss);
+  const BwdRead<T, D> rd(lane);
+  auto issue = [&](int tile, unsigned char* kd, unsigned char* vd) {
+    kdma.load(kp, kss, tile * kBwdTile, sk, wave, kd);
+    vdma.load(vp, vss, tile * kBwdTile, sk, wave, vd);
+  };
+
+  f32x16 dqa[QB][DBLK];
+#pragma unroll
+  for (int x = 0; x < QB; ++x)
+#pragma unroll
+    for (int a = 0; a < DBLK; ++a) dqa[x][a] = f32x16{};
+  bool bad = false;
+
+  auto body = [&](int tile, const unsigned char* kt, const unsigned char* vt) {
+#pragma unroll
+    for (int sub = 0; sub < kBwdTile; sub += 32) {
+      const int j0 = tile * kBwdTile + sub;
+      if (CAUSAL && j0 > qw + 32 * QB - 1) continue;   // every pair hidden
+      if (j0 >= sk) continue;
+      f32x16 s[QB], dp[QB];
+#pragma unroll
+      for (int x = 0; x < QB; ++x) s[x] = dp[x] = f32x16{};
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        const vec8 a = rd.row(kt, sub, t);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) s[x] = In::mfma(a, qreg[x][t], s[x]);
+      }
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        const vec8 a = rd.row(vt, sub, t);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) dp[x] = In::mfma(a, greg[x][t], dp[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], scale_log2, shift[x]));
+          if constexpr (kScaled) p *= ds_mul;
+          s[x][r] = p * (dp[x][r] + minus[x]);
+        }
+      const bool masked = (CAUSAL && j0 + 31 > qw) || j0 + 32 > sk;
+      if (masked) {
+        if (CAUSAL) bad |= rd.nonfinite(kt, sub);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+          const int i = qw + 32 * x + l32;
+          const int end = (CAUSAL ? min(sk, i + 1) : sk) - j0 - 4 * hi;   // register rows from it on
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) >= end) s[x][r] = 0.0f;
+        }
+      }
+      u32 pk[QB][8];
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) pk[x][r >> 1] = In::pack2(s[x][r], s[x][r + 1]);
+#pragma unroll
+      for (int cs = 0; cs < 2; ++cs)
+#pragma unroll
+        for (int a = 0; a < DBLK; ++a) {
+          const vec8 t = rd.column(kt, sub, cs, a);
+#pragma unroll
+          for (int x = 0; x < QB; ++x)
+            dqa[x][a] = In::mfma(t, packed_operand<T>(pk[x], cs), dqa[x][a]);
+        }
+    }
+  };
+
+  auto landed = []() { __builtin_amdgcn_s_waitcnt(0x0F70); };   // vmcnt(0)
+  if (t0 < t1) {
+    issue(t0, kbuf0, vbuf0);
+    for (int tile = t0; tile < t1;) {
+      landed();
+      __syncthreads();
+      if (tile + 1 < t1) issue(tile + 1, kbuf1, vbuf1);
+      body(tile, kbuf0, vbuf0);
+      if (++tile >= t1) break;
+      landed();
+      __syncthreads();
+      if (tile + 1 < t1) issue(tile + 1, kbuf0, vbuf0);
+      body(tile, kbuf1, vbuf1);
+      ++tile;
+    }
+  }
+
+  const i64 row0 = (i64)bh * sq;
+  float* const part_rows = PARTS ? sums + ((i64)part * units + bh) * sq * D : nullptr;
+  auto store = [&](int i, int d, float a0, float a1, float a2, float a3) {
+    if constexpr (PARTS) {
+      *(f32x4*)(part_rows + (i64)i * D + d) = f32x4{a0, a1, a2, a3};
+    } else {
+      u32x2 w;
+      w.x = In::pack2(a0, a1);
+      w.y = In::pack2(a2, a3);
+      *(u32x2*)(dq + (row0 + i) * D + d) = w;
+    }
+  };
+  if constexpr (CAUSAL) {
+    if (__syncthreads_or(bad)) {
+      attention_bwd_exact_q<T, D, CAUSAL, W>(qp, kp, vp, gp, st, nd, q0, BM, sq, t0 * kBwdTile,
+                                             min(sk, t1 * kBwdTile), qss, kss, vss, gss, scale,
+                                             scale_log2, store);
+      return;
+    }
+  }
+  const float sf = scale * exp2_int(-(int)BwdIn<T>::kLift) * exp2_int(-lift);
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int i = qw + 32 * x + l32;
+    if (i >= sq) continue;
+#pragma unroll
+    for (int a = 0; a < DBLK; ++a)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store(i, 32 * a + 8 * g + 4 * hi, dqa[x][a][4 * g] * sf, dqa[x][a][4 * g + 1] * sf,
+              dqa[x][a][4 * g + 2] * sf, dqa[x][a][4 * g + 3] * sf);
+  }
+}
+
+// The parts' fp32 sums [part][n] added in the order of the parts and rounded once; pairs (dK, dV)
+// of a row lie side by side and part into two outputs.
+template <typename T, int D, bool PAIR>
+__device__ __forceinline__ void attention_bwd_join(const float* __restrict__ sums, T* __restrict__ a,
+                                                   T* __restrict__ b, i64 rows, int parts) {
+  typedef AttnIn<T> In;
+  constexpr int N = PAIR ? 2 * D : D;
+  const i64 at = ((i64)blockIdx.x * 256 + threadIdx.x) * 4;
+  const i64 all = rows * N;
+  if (at >= all) return;
+  f32x4 t = *(const f32x4*)(sums + at);
+  for (int p = 1; p < parts; ++p) t += *(const f32x4*)(sums + p * all + at);
+  const i64 row = at / N;
+  const int c = (int)(at % N);
+  u32x2 w;
+  w.x = In::pack2(t[0], t[1]);
+  w.y = In::pack2(t[2], t[3]);
+  T* out = PAIR && c >= D ? b + row * D + (c - D) : a + row * D + c;
+  *(u32x2*)out = w;
+}
+
+}  // namespace nep

@@ -18,6 +18,7 @@ from neptune_codegen.algebra import (_BRANCH_CUT, MergeCertificate, StateCertifi
                                      repair_pair, term_expr, vanishes)
 from neptune_codegen.attention import (as_attention_op, attention_fold, exact_path_taken,
                                        launch_attention, run_attention)
+from neptune_codegen.attention_backward import as_attention_grad_op, run_attention_backward
 from neptune_codegen.autotune import best_config, machine_key, op_key, parameter_tag
 from neptune_codegen.emitters import (check_supported, derived_producer_expr, emit_fold_policy,
                                       emit_kernel_source, emit_rms_state_source,
@@ -65,6 +66,7 @@ __all__ = [
     "state_op_handle", "as_segment_op", "segment_op_handle", "run_segment_pool",
     "compile_segment_reduction", "validate_segment_inputs",
     "run_attention", "attention_fold", "as_attention_op", "launch_attention", "exact_path_taken",
+    "run_attention_backward", "as_attention_grad_op",
     "compile_readout", "run_readout", "run_log_softmax", "as_readout_op", "readout_op_handle",
     "best_config", "machine_key", "op_key", "parameter_tag", "prebuilt_programs",
     # internals the reference package also exports: the algebra's quotient-power marker and

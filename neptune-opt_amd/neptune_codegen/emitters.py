@@ -701,3 +701,74 @@ def emit_attention_short_source(head_dim: int, causal: bool, dtype="bfloat16") -
         f'extern "C" __global__ void __launch_bounds__(256) {merge}(const float* po, const float* pml, '
         "void* o, float* lse, long long rows, int chunks) {\n"
         f"  nep::attention_short_merge<{ctype}, {head_dim}>(po, pml, ({ctype}*)o, lse, rows, chunks);\n}}\n"])
+
+
+# Attention's gradients: workgroups of 4 wave64s, each of one or two blocks of 32 keys (of 32 queries,
+# for dQ) -- one at head dim 256, whose gradients take twice the registers.
+ATTN_BWD_TILE, ATTN_BWD_WAVES = 64, 4
+
+
+def attention_backward_blocks(head_dim: int) -> int:
+    """The most 32-row blocks per wave."""
+    return 2 if head_dim <= 128 else 1
+
+
+def attention_backward_kernel_names(head_dim: int, causal: bool, dtype="bfloat16", kv_blocks: int = 1,
+                                    q_blocks: int = 1, kv_parts: bool = False,
+                                    q_parts: bool = False) -> dict:
+    """Symbols of one unit of attention's gradients, by stage."""
+    tag, _ = _attn_dtype(dtype)
+    mask = "causal" if causal else "full"
+    return {"rows": f"attention_bwd_rows_{tag}_d{head_dim}",
+            "kv": f"attention_bwd_kv_{tag}_d{head_dim}_{mask}_b{kv_blocks}{'_parts' if kv_parts else ''}",
+            "q": f"attention_bwd_q_{tag}_d{head_dim}_{mask}_b{q_blocks}{'_parts' if q_parts else ''}",
+            "kv_join": f"attention_bwd_kv_join_{tag}_d{head_dim}",
+            "q_join": f"attention_bwd_q_join_{tag}_d{head_dim}"}
+
+
+def emit_attention_backward_source(head_dim: int, causal: bool, dtype="bfloat16", kv_blocks: int = 1,
+                                   q_blocks: int = 1, kv_parts: bool = False,
+                                   q_parts: bool = False) -> str:
+    """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics, dK and dV,
+    dQ, and the joins of split key or query ranges."""
+    if head_dim not in ATTN_HEAD_DIMS:
+        raise NotImplementedError("attention fold supports head_dim 64, 128 and 256")
+    tag, ctype = _attn_dtype(dtype)
+    names = attention_backward_kernel_names(head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts, q_parts)
+    if not (1 <= kv_blocks <= attention_backward_blocks(head_dim) >= q_blocks >= 1):
+        raise ValueError("attention backward has no kernel of so many blocks per wave")
+    cz, waves, threads = "true" if causal else "false", ATTN_BWD_WAVES, 64 * ATTN_BWD_WAVES
+    c = f"(const {ctype}*)"
+    strides = ("long long qsb, long long qsh, long long qss, long long ksb, long long ksh, long long kss, "
+               "long long vsb, long long vsh, long long vss, long long gsb, long long gsh, long long gss, "
+               "float scale, float scale_log2, int parts, int per")
+    given = "qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, parts, per"
+    operands = ("const void* q, const void* k, const void* v, const void* go, const float* start, "
+                "const float* ndelta, const float* bounds, ")
+    parts = [
+        "// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
+        f"// gradients of the online-softmax attention fold: head_dim={head_dim}, causal={causal}, {tag}\n",
+        kernel_header("nep_device.h", "nep_attention.h", "nep_attention_bwd.h"),
+        f'extern "C" __global__ void __launch_bounds__(256) {names["rows"]}(const void* o, const void* go, '
+        "const void* v, const float* lse, const float* glse, float* start, float* ndelta, float* bounds, "
+        "int heads, int sq, int sk, int units, long long osb, long long osh, long long oss, long long gsb, "
+        "long long gsh, long long gss, long long vsb, long long vsh, long long vss, float scale) {\n"
+        f"  nep::attention_bwd_rows<{ctype}, {head_dim}>({c}o, {c}go, {c}v, lse, glse, start, ndelta, "
+        "bounds, heads, sq, sk, units, osb, osh, oss, gsb, gsh, gss, vsb, vsh, vss, scale);\n}\n",
+        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {names["kv"]}({operands}'
+        f"void* dk, void* dv, float* sums, int units, int heads, int sq, int sk, {strides}) {{\n"
+        f"  nep::attention_bwd_kv<{ctype}, {head_dim}, {cz}, {waves}, {kv_blocks}, {str(kv_parts).lower()}>("
+        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, ({ctype}*)dk, ({ctype}*)dv, sums, units, heads, "
+        f"sq, sk, {given});\n}}\n",
+        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {names["q"]}({operands}'
+        f"void* dq, float* sums, int units, int heads, int sq, int sk, {strides}) {{\n"
+        f"  nep::attention_bwd_q<{ctype}, {head_dim}, {cz}, {waves}, {q_blocks}, {str(q_parts).lower()}>("
+        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, ({ctype}*)dq, sums, units, heads, sq, sk, {given});\n}}\n"]
+    for stage, split, pair in (("kv_join", kv_parts, "true"), ("q_join", q_parts, "false")):
+        if split:
+            parts.append(
+                f'extern "C" __global__ void __launch_bounds__(256) {names[stage]}(const float* sums, void* a, '
+                "void* b, long long rows, int parts) {\n"
+                f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, rows, "
+                "parts);\n}\n")
+    return "\n".join(parts)
