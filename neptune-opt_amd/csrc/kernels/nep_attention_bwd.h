@@ -439,12 +439,43 @@ __device__ __forceinline__ void mfma_settle(f32x16& c, f32x16& d) {
   asm volatile("s_nop 7\ns_nop 7\ns_nop 7" : "+v"(c), "+v"(d));
 }
 
+// A wave's 32 output rows (acc holds their transpose) go through its own 32 * D * 2 bytes of LDS,
+// 16-byte chunks XORed by row, and out as whole rows of 16 bytes per lane.  Written from the
+// accumulators they would be 8-byte pieces of 32 rows each (a workgroup's end at head dim 128 took
+// 8 us longer so).
+template <typename T, int D>
+__device__ __forceinline__ void bwd_store_rows(unsigned char* stage, const f32x16 (&acc)[D / 32],
+                                               float factor, T* __restrict__ out, int row0, int rows,
+                                               int lane) {
+  typedef AttnIn<T> In;
+  constexpr int CPR = D / 8, SW = CPR < 16 ? CPR - 1 : 15, RPI = 64 / CPR;
+  const int l32 = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int a = 0; a < D / 32; ++a)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u32x2 w;
+      w.x = In::pack2(acc[a][4 * g] * factor, acc[a][4 * g + 1] * factor);
+      w.y = In::pack2(acc[a][4 * g + 2] * factor, acc[a][4 * g + 3] * factor);
+      *(u32x2*)(stage + l32 * (D * 2) + (((4 * a + g) ^ (l32 & SW)) << 4) + 8 * hi) = w;
+    }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int row = RPI * i + lane / CPR, c = lane % CPR;
+    const u32x4 w = *(const u32x4*)(stage + row * (D * 2) + ((c ^ (row & SW)) << 4));
+    if (row0 + row < rows) store16(out + (i64)(row0 + row) * D + 8 * c, w);
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
 // dK and dV.  W waves of 32 KB keys each; a wave's K and V rows and its dK^T and dV^T stay in
 // registers, the workgroup's Q and dO tiles are staged for all of its waves.  One wave per SIMD:
 // at KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1
 // (at 32 keys a wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock).
-// PARTS: the queries of a head are split into `parts` of `per` tiles and each part's fp32 sums go
-// to `sums` [part][bh][key][dK, dV][D] for attention_bwd_join.
+// PARTS: each block's query tiles are taken in parts of `per` (64-row tiles, from the block's first);
+// of a block with more than one, each part's fp32 sums go to `sums` [part][bh][key][dK, dV][D] for
+// attention_bwd_join.
 template <typename T, int D, bool CAUSAL, int W, int KB, bool PARTS>
 __device__ __forceinline__ void attention_bwd_kv(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -452,7 +483,7 @@ __device__ __forceinline__ void attention_bwd_kv(
     const float* __restrict__ bounds, T* __restrict__ dk, T* __restrict__ dv,
     float* __restrict__ sums, int units, int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss,
     i64 ksb, i64 ksh, i64 kss, i64 vsb, i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale,
-    float scale_log2, int parts, int per) {
+    float scale_log2, int per) {
   typedef AttnIn<T> In;
   typedef typename In::vec8 vec8;
   constexpr int BN = 32 * KB * W;                    // keys per workgroup
@@ -472,8 +503,7 @@ __device__ __forceinline__ void attention_bwd_kv(
 
   const int nkb = (sk + BN - 1) / BN, nq = (sq + kBwdTile - 1) / kBwdTile;
   const int bh = blockIdx.x % units, id = blockIdx.x / units;
-  const int kb_id = PARTS ? id / parts : id, part = PARTS ? id % parts : 0;
-  if (kb_id >= nkb) return;
+  const int kb_id = PARTS ? id % nkb : id, part = PARTS ? id / nkb : 0;   // whole parts first
   const int b = bh / heads, h = bh % heads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -488,8 +518,10 @@ __device__ __forceinline__ void attention_bwd_kv(
   // causal: key j is seen by the queries from j on
   constexpr int PER = kBwdTile / ROWS;
   const int tiles = (sq + ROWS - 1) / ROWS, first = CAUSAL ? k0 / ROWS : 0;
-  const int t0 = PARTS ? max(first, part * per * PER) : first;
-  const int t1 = PARTS ? min(tiles, (part + 1) * per * PER) : tiles;
+  const int t0 = first + part * per * PER;
+  const int t1 = PARTS ? min(tiles, t0 + per * PER) : tiles;
+  if (PARTS && part > 0 && t0 >= tiles) return;      // the block has fewer parts
+  const bool whole = !PARTS || tiles - first <= per * PER;
 
   vec8 kreg[kKeysInLds ? 1 : KB][kKeysInLds ? 1 : KSTEPS], vreg[KB][KSTEPS];
 #pragma unroll
@@ -657,7 +689,7 @@ __device__ __forceinline__ void attention_bwd_kv(
   const i64 row0 = (i64)bh * sk;
   float* const part_rows = PARTS ? sums + ((i64)part * units + bh) * sk * 2 * D : nullptr;
   auto store = [&](int which, int j, int d, float a0, float a1, float a2, float a3) {
-    if constexpr (PARTS) {
+    if (!whole) {
       *(f32x4*)(part_rows + ((i64)j * 2 + which) * D + d) = f32x4{a0, a1, a2, a3};
     } else {
       u32x2 w;
@@ -675,34 +707,44 @@ __device__ __forceinline__ void attention_bwd_kv(
     }
   }
   const float pf = exp2_int(-(int)BwdIn<T>::kLift), sf = scale * pf * exp2_int(-lift);
+  if (whole) {
+    if constexpr (!CAUSAL) __syncthreads();          // every wave is done with the tiles
+    static_assert(W <= 4, "one tile buffer for each wave");
+    unsigned char* stage = wave == 0 ? qbuf0 : wave == 1 ? qbuf1 : wave == 2 ? gbuf0 : gbuf1;
 #pragma unroll
-  for (int x = 0; x < KB; ++x) {
-    const int j = kw + 32 * x + l32;
-    if (j >= sk) continue;
+    for (int x = 0; x < KB; ++x) {
+      bwd_store_rows<T, D>(stage, dka[x], sf, dk + row0 * D, kw + 32 * x, sk, lane);
+      bwd_store_rows<T, D>(stage, dva[x], pf, dv + row0 * D, kw + 32 * x, sk, lane);
+    }
+  } else {
 #pragma unroll
-    for (int a = 0; a < DBLK; ++a)
+    for (int x = 0; x < KB; ++x) {
+      const int j = kw + 32 * x + l32;
+      if (j >= sk) continue;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * a + 8 * g + 4 * hi;
-        store(0, j, d, dka[x][a][4 * g] * sf, dka[x][a][4 * g + 1] * sf, dka[x][a][4 * g + 2] * sf,
-              dka[x][a][4 * g + 3] * sf);
-        store(1, j, d, dva[x][a][4 * g] * pf, dva[x][a][4 * g + 1] * pf, dva[x][a][4 * g + 2] * pf,
-              dva[x][a][4 * g + 3] * pf);
-      }
+      for (int a = 0; a < DBLK; ++a)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * a + 8 * g + 4 * hi;
+          store(0, j, d, dka[x][a][4 * g] * sf, dka[x][a][4 * g + 1] * sf,
+                dka[x][a][4 * g + 2] * sf, dka[x][a][4 * g + 3] * sf);
+          store(1, j, d, dva[x][a][4 * g] * pf, dva[x][a][4 * g + 1] * pf,
+                dva[x][a][4 * g + 2] * pf, dva[x][a][4 * g + 3] * pf);
+        }
+    }
   }
 }
 
 // dQ.  W waves of 32 QB queries each; a wave's Q and dO rows and its dQ^T stay in registers, the
-// workgroup's K and V tiles are staged for all of its waves.  PARTS: a head's keys are split into
-// `parts` of `per` tiles, the parts' fp32 sums go to `sums` [part][bh][query][D].
+// workgroup's K and V tiles are staged for all of its waves.  PARTS: as above, over the key tiles, with
+// `sums` [part][bh][query][D].
 template <typename T, int D, bool CAUSAL, int W, int QB, bool PARTS>
 __device__ __forceinline__ void attention_bwd_q(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     const T* __restrict__ go, const float* __restrict__ start, const float* __restrict__ ndelta,
     const float* __restrict__ bounds, T* __restrict__ dq, float* __restrict__ sums, int units,
     int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss, i64 ksb, i64 ksh, i64 kss, i64 vsb,
-    i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale, float scale_log2, int parts,
-    int per) {
+    i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale, float scale_log2, int per) {
   typedef AttnIn<T> In;
   typedef typename In::vec8 vec8;
   constexpr int BM = 32 * QB * W;
@@ -717,8 +759,7 @@ __device__ __forceinline__ void attention_bwd_q(
   const int nqb = (sq + BM - 1) / BM, nq = (sq + kBwdTile - 1) / kBwdTile;
   const int nk = (sk + kBwdTile - 1) / kBwdTile;
   const int bh = blockIdx.x % units, id = blockIdx.x / units;
-  const int qb = nqb - 1 - (PARTS ? id / parts : id), part = PARTS ? id % parts : 0;   // heaviest first
-  if (qb < 0) return;
+  const int qb = nqb - 1 - (PARTS ? id % nqb : id), part = PARTS ? id / nqb : 0;   // heaviest first
   const int b = bh / heads, h = bh % heads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -733,6 +774,8 @@ __device__ __forceinline__ void attention_bwd_q(
   const int last = CAUSAL ? min(nk, (q0 + BM + kBwdTile - 1) / kBwdTile) : nk;
   const int t0 = PARTS ? part * per : 0;
   const int t1 = PARTS ? min(last, t0 + per) : last;
+  if (PARTS && part > 0 && t0 >= last) return;       // the block has fewer parts
+  const bool whole = !PARTS || last <= per;
 
   vec8 qreg[QB][KSTEPS], greg[QB][KSTEPS];
   float shift[QB], minus[QB];
@@ -831,24 +874,22 @@ __device__ __forceinline__ void attention_bwd_q(
   auto landed = []() { __builtin_amdgcn_s_waitcnt(0x0F70); };   // vmcnt(0)
   if (t0 < t1) {
     issue(t0, kbuf0, vbuf0);
-    for (int tile = t0; tile < t1;) {
+    for (int tile = t0; tile < t1; tile += 2) {
       landed();
       __syncthreads();
       if (tile + 1 < t1) issue(tile + 1, kbuf1, vbuf1);
       body(tile, kbuf0, vbuf0);
-      if (++tile >= t1) break;
       landed();
       __syncthreads();
-      if (tile + 1 < t1) issue(tile + 1, kbuf0, vbuf0);
-      body(tile, kbuf1, vbuf1);
-      ++tile;
+      if (tile + 2 < t1) issue(tile + 2, kbuf0, vbuf0);
+      if (tile + 1 < t1) body(tile + 1, kbuf1, vbuf1);
     }
   }
 
   const i64 row0 = (i64)bh * sq;
   float* const part_rows = PARTS ? sums + ((i64)part * units + bh) * sq * D : nullptr;
   auto store = [&](int i, int d, float a0, float a1, float a2, float a3) {
-    if constexpr (PARTS) {
+    if (!whole) {
       *(f32x4*)(part_rows + (i64)i * D + d) = f32x4{a0, a1, a2, a3};
     } else {
       u32x2 w;
@@ -866,37 +907,53 @@ __device__ __forceinline__ void attention_bwd_q(
     }
   }
   const float sf = scale * exp2_int(-(int)BwdIn<T>::kLift) * exp2_int(-lift);
+  if (whole) {
+    if constexpr (!CAUSAL) __syncthreads();          // every wave is done with the tiles
+    static_assert(W <= 4, "one tile buffer for each wave");
+    unsigned char* stage = wave == 0 ? kbuf0 : wave == 1 ? kbuf1 : wave == 2 ? vbuf0 : vbuf1;
 #pragma unroll
-  for (int x = 0; x < QB; ++x) {
-    const int i = qw + 32 * x + l32;
-    if (i >= sq) continue;
+    for (int x = 0; x < QB; ++x)
+      bwd_store_rows<T, D>(stage, dqa[x], sf, dq + row0 * D, qw + 32 * x, sq, lane);
+  } else {
 #pragma unroll
-    for (int a = 0; a < DBLK; ++a)
+    for (int x = 0; x < QB; ++x) {
+      const int i = qw + 32 * x + l32;
+      if (i >= sq) continue;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store(i, 32 * a + 8 * g + 4 * hi, dqa[x][a][4 * g] * sf, dqa[x][a][4 * g + 1] * sf,
-              dqa[x][a][4 * g + 2] * sf, dqa[x][a][4 * g + 3] * sf);
+      for (int a = 0; a < DBLK; ++a)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store(i, 32 * a + 8 * g + 4 * hi, dqa[x][a][4 * g] * sf, dqa[x][a][4 * g + 1] * sf,
+                dqa[x][a][4 * g + 2] * sf, dqa[x][a][4 * g + 3] * sf);
+    }
   }
 }
 
-// The parts' fp32 sums [part][n] added in the order of the parts and rounded once; pairs (dK, dV)
-// of a row lie side by side and part into two outputs.
-template <typename T, int D, bool PAIR>
+// The parts' fp32 sums of the rows whose block of `block` rows had more than one part of `per` tiles,
+// added in the order of the parts and rounded once.  KV: `len` keys a head and (dK, dV) of a key side by
+// side; a block's tiles are those of the `other` queries, from its own keys' on under the causal mask.
+// Otherwise `len` queries; the tiles are the keys', up to its own queries'.
+template <typename T, int D, bool KV>
 __device__ __forceinline__ void attention_bwd_join(const float* __restrict__ sums, T* __restrict__ a,
-                                                   T* __restrict__ b, i64 rows, int parts) {
+                                                   T* __restrict__ b, i64 rows, int len, int other,
+                                                   int block, int per, int causal) {
   typedef AttnIn<T> In;
-  constexpr int N = PAIR ? 2 * D : D;
+  constexpr int N = KV ? 2 * D : D;
   const i64 at = ((i64)blockIdx.x * 256 + threadIdx.x) * 4;
   const i64 all = rows * N;
   if (at >= all) return;
+  const i64 row = at / N;
+  const int c = (int)(at % N), r0 = (int)(row % len) / block * block;
+  int tiles = (other + kBwdTile - 1) / kBwdTile;
+  if (causal) tiles = KV ? tiles - r0 / kBwdTile : min(tiles, (r0 + block + kBwdTile - 1) / kBwdTile);
+  const int parts = (tiles + per - 1) / per;
+  if (parts <= 1) return;                            // written by its workgroup
   f32x4 t = *(const f32x4*)(sums + at);
   for (int p = 1; p < parts; ++p) t += *(const f32x4*)(sums + p * all + at);
-  const i64 row = at / N;
-  const int c = (int)(at % N);
   u32x2 w;
   w.x = In::pack2(t[0], t[1]);
   w.y = In::pack2(t[2], t[3]);
-  T* out = PAIR && c >= D ? b + row * D + (c - D) : a + row * D + c;
+  T* out = KV && c >= D ? b + row * D + (c - D) : a + row * D + c;
   *(u32x2*)out = w;
 }
 

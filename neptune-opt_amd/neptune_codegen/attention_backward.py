@@ -15,13 +15,14 @@ V or dO reaches only the gradients whose formula has it.
 """
 from __future__ import annotations
 
+import functools
 import math
 import threading
 
 from neptune_codegen import calls, hip
 from neptune_codegen.attention import K_ROW_STRIDE_MAX, LOG2E, validate_attention_inputs
 from neptune_codegen.emitters import (ATTN_BWD_TILE, ATTN_BWD_WAVES, BASE_OPTIONS,
-                                      attention_backward_blocks, attention_backward_kernel_names,
+                                      attention_backward_blocks, attention_backward_kernel_name,
                                       emit_attention_backward_source)
 
 _PROGRAMS: dict = {}
@@ -31,41 +32,44 @@ _SEEN = calls.Seen()
 _lock = threading.Lock()
 
 _ROWS_ARGS = (hip.PTR,) * 8 + (hip.I32,) * 4 + (hip.I64,) * 9 + (hip.F32,)
-_OPERAND_ARGS = (hip.I32,) * 4 + (hip.I64,) * 12 + (hip.F32,) * 2 + (hip.I32,) * 2
+_OPERAND_ARGS = (hip.I32,) * 4 + (hip.I64,) * 12 + (hip.F32,) * 2 + (hip.I32,)
 _KV_ARGS = (hip.PTR,) * 10 + _OPERAND_ARGS
 _Q_ARGS = (hip.PTR,) * 9 + _OPERAND_ARGS
 _THREADS = 64 * ATTN_BWD_WAVES
-_JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32)
+_JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64,) + (hip.I32,) * 5
 
 
-def _program(head_dim, causal, dtype, kv_blocks=1, q_blocks=1, kv_parts=False, q_parts=False) -> hip.Program:
-    key = (head_dim, causal, str(dtype).replace("torch.", ""), kv_blocks, q_blocks, kv_parts, q_parts)
+def _program(stage, head_dim, causal, dtype, blocks=1, parts=False) -> hip.Program:
+    causal = bool(causal) and stage != "rows"        # one unit for both masks
+    key = (stage, head_dim, causal, str(dtype).replace("torch.", ""), blocks, parts)
     with _lock:
         prog = _PROGRAMS.get(key)
         if prog is None:
-            source = emit_attention_backward_source(head_dim, causal, dtype, kv_blocks, q_blocks,
-                                                    kv_parts, q_parts)
-            name = attention_backward_kernel_names(head_dim, causal, dtype, kv_blocks, q_blocks,
-                                                   kv_parts, q_parts)["kv"]
-            prog = _PROGRAMS[key] = hip.Program(source, f"{name}_{q_blocks}{'p' if q_parts else ''}.hip",
-                                                BASE_OPTIONS)
+            name = attention_backward_kernel_name(stage, head_dim, causal, dtype, blocks, parts)
+            prog = _PROGRAMS[key] = hip.Program(
+                emit_attention_backward_source(stage, head_dim, causal, dtype, blocks, parts),
+                f"{name}.hip", BASE_OPTIONS)
         return prog
 
 
-def _kernels(device, head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts, q_parts) -> tuple:
-    """(rows, kv, q, kv join or None, q join or None), fetched once per device."""
-    key = (device, head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts, q_parts)
+def unit_kinds(head_dim):
+    """(stage, blocks per wave, parts) of the units a call at this head dim may launch."""
+    yield "rows", 1, False
+    for stage, dim, blocks in TILE_US:
+        if dim == head_dim:
+            yield stage, blocks, False
+            yield stage, blocks, True
+
+
+def _kernel(stage, device, head_dim, causal, dtype, blocks=1, parts=False) -> hip.Kernel:
+    key = (stage, device, head_dim, causal, dtype, blocks, parts)
     found = _KERNELS.get(key)
     if found is None:
-        prog = _program(head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts, q_parts)
-        names = attention_backward_kernel_names(head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts,
-                                                q_parts)
-        found = (prog.kernel(names["rows"], _ROWS_ARGS, 256, device),
-                 prog.kernel(names["kv"], _KV_ARGS, _THREADS, device),
-                 prog.kernel(names["q"], _Q_ARGS, _THREADS, device),
-                 prog.kernel(names["kv_join"], _JOIN_ARGS, 256, device) if kv_parts else None,
-                 prog.kernel(names["q_join"], _JOIN_ARGS, 256, device) if q_parts else None)
-        _KERNELS[key] = found
+        args, threads = {"rows": (_ROWS_ARGS, 256), "kv": (_KV_ARGS, _THREADS), "q": (_Q_ARGS, _THREADS),
+                         "kv_join": (_JOIN_ARGS, 256), "q_join": (_JOIN_ARGS, 256)}[stage]
+        prog = _program("rows" if stage.endswith("join") else stage, head_dim, causal, dtype, blocks, parts)
+        found = _KERNELS[key] = prog.kernel(
+            attention_backward_kernel_name(stage, head_dim, causal, dtype, blocks, parts), args, threads, device)
     return found
 
 
@@ -133,10 +137,69 @@ class _Call:
                 kernel.launch(grid, (sums, dq.data_ptr(), 0) + rest, stream)
 
 
+# What `_plan` prices a stage with, in us on MI355X (fits of replays over sixteen shapes): a workgroup's
+# pass over a 64-row tile with few workgroups on the chip, and with the chip full (the clock and the
+# caches are shared), and its start and end.  Head dim 64 has two workgroups of one block on a CU.
+# Two blocks a wave read each tile half as often and pass twice the rows in 1.7 to 2.1 times the time;
+# one block makes twice the workgroups.  Measured at head dim 128, one / two blocks: bf16 causal 4x32x4096x128 dK and dV
+# 1154 / 1074 us, dQ 1000 / 905; full 8x32x1024x128 319 / 293, 272 / 238; causal 4x16x512x128 23 / 42,
+# 21 / 35.  (At head dim 64 two were slower everywhere: full 8x12x777 49 / 58, 45 / 51.)
+TILE_US = {("kv", 64, 1): (1.03, 1.08, 4.0), ("kv", 128, 1): (1.72, 2.15, 8.0), ("kv", 128, 2): (3.7, 3.95, 14.0),
+           ("kv", 256, 1): (3.7, 4.1, 12.0), ("q", 64, 1): (1.12, 1.15, 3.0), ("q", 128, 1): (1.62, 1.88, 5.0),
+           ("q", 128, 2): (2.95, 3.3, 9.0), ("q", 256, 1): (3.6, 4.0, 8.0)}
+# A split's second launch and its fp32 sums, written and read (through the caches).
+JOIN_US, SUM_BYTES_PER_US, MAX_SUM_BYTES = 4.0, 4e6, 256 << 20
+CUS = 256
+
+
+def _stage_cost(stage, units, own, other, head_dim, causal, blocks, per):
+    """us of a stage with blocks of `own` rows walking the tiles of the `other` rows in parts of `per`."""
+    few, full, ends = TILE_US[stage, head_dim, blocks]
+    step = 32 * ATTN_BWD_WAVES * blocks // ATTN_BWD_TILE
+    count, tiles = -(-own // (step * ATTN_BWD_TILE)), -(-other // ATTN_BWD_TILE)
+    if not causal:
+        lengths = {tiles: count}
+    else:
+        lengths = {}
+        for i in range(count):
+            n = max(0, tiles - step * i) if stage == "kv" else min(tiles, step * (i + 1))
+            lengths[n] = lengths.get(n, 0) + 1
+    longest = min(per, max(lengths))
+    items = units * sum(m * max(1, -(-n // per)) for n, m in lengths.items())
+    total = units * sum(n * m for n, m in lengths.items())
+    tile = full if items > CUS // 2 else few
+    if causal or head_dim == 64:
+        # longest first, or two to a CU: the last to end are about half a part apart
+        cost = max(longest * few + ends, (total * full + items * ends) / CUS + longest * few / 2)
+    else:
+        cost = -(-items // CUS) * (longest * tile + ends)
+    if max(lengths) > per:
+        width = head_dim * (2 if stage == "kv" else 1)
+        cost += JOIN_US + 8.0 * width * units * own * max(lengths) / per / SUM_BYTES_PER_US
+    return cost
+
+
+@functools.lru_cache(maxsize=4096)
+def _stage_plan(stage, units, own_tiles, other_tiles, head_dim, causal):
+    """(blocks per wave, parts) of the cheapest launch of a stage."""
+    own, other = own_tiles * ATTN_BWD_TILE, other_tiles * ATTN_BWD_TILE
+    width, best = head_dim * (2 if stage == "kv" else 1), None
+    for blocks in range(1, attention_backward_blocks(head_dim) + 1):
+        for parts in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32):
+            if parts > 1 and (parts > other_tiles // 2
+                              or 4 * parts * units * own * width > MAX_SUM_BYTES):
+                break
+            cost = _stage_cost(stage, units, own, other, head_dim, causal, blocks, -(-other_tiles // parts))
+            if best is None or cost < best[0]:
+                best = (cost, blocks, parts)
+    return best[1:]
+
+
 def _plan(units, sq, sk, head_dim, causal):
-    """(kv blocks, kv parts, q blocks, q parts) of a call."""
-    b = attention_backward_blocks(head_dim)
-    return b, 1, b, 1
+    """(kv blocks, kv parts, q blocks, q parts) of a call; searched once for the same tile counts."""
+    nq, nk = -(-sq // ATTN_BWD_TILE), -(-sk // ATTN_BWD_TILE)
+    return (_stage_plan("kv", units, nk, nq, head_dim, causal)
+            + _stage_plan("q", units, nq, nk, head_dim, causal))
 
 
 def _prepare(q, k, strides, scale, causal, plan=None) -> _Call:
@@ -148,8 +211,7 @@ def _prepare(q, k, strides, scale, causal, plan=None) -> _Call:
     nq, nk = -(-Sq // ATTN_BWD_TILE), -(-Sk // ATTN_BWD_TILE)
     kv_per, q_per = -(-nq // kv_parts), -(-nk // q_parts)
     kv_parts, q_parts = -(-nq // kv_per), -(-nk // q_per)
-    rows, kv, q_kernel, kv_join, q_join = _kernels(device, D, causal, q.dtype, kv_blocks, q_blocks,
-                                                   kv_parts > 1, q_parts > 1)
+    kind = (device, D, causal, q.dtype)
     call = _Call()
     call.device = device
     # start values and deltas of every padded query row; fp16's bounds; the parts' fp32 sums
@@ -167,12 +229,17 @@ def _prepare(q, k, strides, scale, causal, plan=None) -> _Call:
     for n, threads in ((groups, 256), (kv_groups, _THREADS), (q_groups, _THREADS),
                        (max(join), 256)):
         calls.check_grid(n, threads, "attention backward")
-    call.rows = (rows, (groups,), (H, Sq, Sk, units) + os + gs + vs + (scale,))
+    call.rows = (_kernel("rows", *kind), (groups,), (H, Sq, Sk, units) + os + gs + vs + (scale,))
     tail = (units, H, Sq, Sk) + qs + ks + vs + gs + (scale, scale * LOG2E)
-    call.kv = (kv, (kv_groups,), tail + (kv_parts, kv_per))
-    call.q = (q_kernel, (q_groups,), tail + (q_parts, q_per))
-    call.kv_join = (kv_join, (join[0],), (units * Sk, kv_parts)) if kv_parts > 1 else None
-    call.q_join = (q_join, (join[1],), (units * Sq, q_parts)) if q_parts > 1 else None
+    call.kv = (_kernel("kv", *kind, kv_blocks, kv_parts > 1), (kv_groups,), tail + (kv_per,))
+    call.q = (_kernel("q", *kind, q_blocks, q_parts > 1), (q_groups,), tail + (q_per,))
+    call.kv_join = call.q_join = None
+    if kv_parts > 1:
+        call.kv_join = (_kernel("kv_join", *kind), (join[0],),
+                        (units * Sk, Sk, Sq, 32 * ATTN_BWD_WAVES * kv_blocks, kv_per, int(causal)))
+    if q_parts > 1:
+        call.q_join = (_kernel("q_join", *kind), (join[1],),
+                       (units * Sq, Sq, Sk, 32 * ATTN_BWD_WAVES * q_blocks, q_per, int(causal)))
     return call
 
 

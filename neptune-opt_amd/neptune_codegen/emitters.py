@@ -703,72 +703,66 @@ def emit_attention_short_source(head_dim: int, causal: bool, dtype="bfloat16") -
         f"  nep::attention_short_merge<{ctype}, {head_dim}>(po, pml, ({ctype}*)o, lse, rows, chunks);\n}}\n"])
 
 
-# Attention's gradients: workgroups of 4 wave64s, each of one or two blocks of 32 keys (of 32 queries,
-# for dQ) -- one at head dim 256, whose gradients take twice the registers.
+# Attention's gradients: workgroups of 4 wave64s, each of one block of 32 keys (of 32 queries, for dQ);
+# at head dim 128 of one or two (two at 64 were slower at every shape, at 256 they would not fit).
 ATTN_BWD_TILE, ATTN_BWD_WAVES = 64, 4
 
 
 def attention_backward_blocks(head_dim: int) -> int:
     """The most 32-row blocks per wave."""
-    return 2 if head_dim <= 128 else 1
+    return 2 if head_dim == 128 else 1
 
 
-def attention_backward_kernel_names(head_dim: int, causal: bool, dtype="bfloat16", kv_blocks: int = 1,
-                                    q_blocks: int = 1, kv_parts: bool = False,
-                                    q_parts: bool = False) -> dict:
-    """Symbols of one unit of attention's gradients, by stage."""
+def attention_backward_kernel_name(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
+                                   blocks: int = 1, parts: bool = False) -> str:
+    """Symbol of one stage of attention's gradients: "rows", "kv", "q", "kv_join" or "q_join"."""
     tag, _ = _attn_dtype(dtype)
-    mask = "causal" if causal else "full"
-    return {"rows": f"attention_bwd_rows_{tag}_d{head_dim}",
-            "kv": f"attention_bwd_kv_{tag}_d{head_dim}_{mask}_b{kv_blocks}{'_parts' if kv_parts else ''}",
-            "q": f"attention_bwd_q_{tag}_d{head_dim}_{mask}_b{q_blocks}{'_parts' if q_parts else ''}",
-            "kv_join": f"attention_bwd_kv_join_{tag}_d{head_dim}",
-            "q_join": f"attention_bwd_q_join_{tag}_d{head_dim}"}
+    if stage not in ("kv", "q"):
+        return f"attention_bwd_{stage}_{tag}_d{head_dim}"
+    return (f"attention_bwd_{stage}_{tag}_d{head_dim}_{'causal' if causal else 'full'}_b{blocks}"
+            f"{'_parts' if parts else ''}")
 
 
-def emit_attention_backward_source(head_dim: int, causal: bool, dtype="bfloat16", kv_blocks: int = 1,
-                                   q_blocks: int = 1, kv_parts: bool = False,
-                                   q_parts: bool = False) -> str:
-    """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics, dK and dV,
-    dQ, and the joins of split key or query ranges."""
+def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
+                                   blocks: int = 1, parts: bool = False) -> str:
+    """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics with the joins
+    of split ranges ("rows"; the mask does not matter), dK and dV ("kv"), or dQ ("q")."""
     if head_dim not in ATTN_HEAD_DIMS:
         raise NotImplementedError("attention fold supports head_dim 64, 128 and 256")
-    tag, ctype = _attn_dtype(dtype)
-    names = attention_backward_kernel_names(head_dim, causal, dtype, kv_blocks, q_blocks, kv_parts, q_parts)
-    if not (1 <= kv_blocks <= attention_backward_blocks(head_dim) >= q_blocks >= 1):
+    if not 1 <= blocks <= attention_backward_blocks(head_dim):
         raise ValueError("attention backward has no kernel of so many blocks per wave")
+    tag, ctype = _attn_dtype(dtype)
     cz, waves, threads = "true" if causal else "false", ATTN_BWD_WAVES, 64 * ATTN_BWD_WAVES
-    c = f"(const {ctype}*)"
-    strides = ("long long qsb, long long qsh, long long qss, long long ksb, long long ksh, long long kss, "
-               "long long vsb, long long vsh, long long vss, long long gsb, long long gsh, long long gss, "
-               "float scale, float scale_log2, int parts, int per")
-    given = "qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, parts, per"
-    operands = ("const void* q, const void* k, const void* v, const void* go, const float* start, "
-                "const float* ndelta, const float* bounds, ")
-    parts = [
-        "// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
-        f"// gradients of the online-softmax attention fold: head_dim={head_dim}, causal={causal}, {tag}\n",
-        kernel_header("nep_device.h", "nep_attention.h", "nep_attention_bwd.h"),
-        f'extern "C" __global__ void __launch_bounds__(256) {names["rows"]}(const void* o, const void* go, '
-        "const void* v, const float* lse, const float* glse, float* start, float* ndelta, float* bounds, "
-        "int heads, int sq, int sk, int units, long long osb, long long osh, long long oss, long long gsb, "
-        "long long gsh, long long gss, long long vsb, long long vsh, long long vss, float scale) {\n"
-        f"  nep::attention_bwd_rows<{ctype}, {head_dim}>({c}o, {c}go, {c}v, lse, glse, start, ndelta, "
-        "bounds, heads, sq, sk, units, osb, osh, oss, gsb, gsh, gss, vsb, vsh, vss, scale);\n}\n",
-        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {names["kv"]}({operands}'
-        f"void* dk, void* dv, float* sums, int units, int heads, int sq, int sk, {strides}) {{\n"
-        f"  nep::attention_bwd_kv<{ctype}, {head_dim}, {cz}, {waves}, {kv_blocks}, {str(kv_parts).lower()}>("
-        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, ({ctype}*)dk, ({ctype}*)dv, sums, units, heads, "
-        f"sq, sk, {given});\n}}\n",
-        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {names["q"]}({operands}'
-        f"void* dq, float* sums, int units, int heads, int sq, int sk, {strides}) {{\n"
-        f"  nep::attention_bwd_q<{ctype}, {head_dim}, {cz}, {waves}, {q_blocks}, {str(q_parts).lower()}>("
-        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, ({ctype}*)dq, sums, units, heads, sq, sk, {given});\n}}\n"]
-    for stage, split, pair in (("kv_join", kv_parts, "true"), ("q_join", q_parts, "false")):
-        if split:
-            parts.append(
-                f'extern "C" __global__ void __launch_bounds__(256) {names[stage]}(const float* sums, void* a, '
-                "void* b, long long rows, int parts) {\n"
-                f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, rows, "
-                "parts);\n}\n")
-    return "\n".join(parts)
+    c, name = f"(const {ctype}*)", attention_backward_kernel_name(stage, head_dim, causal, dtype, blocks, parts)
+    head = ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
+            f"// gradients of the online-softmax attention fold: {stage}, head_dim={head_dim}, {tag}\n"
+            + kernel_header("nep_device.h", "nep_attention.h", "nep_attention_bwd.h"))
+    if stage == "rows":
+        units = [
+            head,
+            f'extern "C" __global__ void __launch_bounds__(256) {name}(const void* o, const void* go, '
+            "const void* v, const float* lse, const float* glse, float* start, float* ndelta, float* bounds, "
+            "int heads, int sq, int sk, int units, long long osb, long long osh, long long oss, long long gsb, "
+            "long long gsh, long long gss, long long vsb, long long vsh, long long vss, float scale) {\n"
+            f"  nep::attention_bwd_rows<{ctype}, {head_dim}>({c}o, {c}go, {c}v, lse, glse, start, ndelta, "
+            "bounds, heads, sq, sk, units, osb, osh, oss, gsb, gsh, gss, vsb, vsh, vss, scale);\n}\n"]
+        for join, pair in (("kv_join", "true"), ("q_join", "false")):
+            symbol = attention_backward_kernel_name(join, head_dim, causal, dtype)
+            units.append(
+                f'extern "C" __global__ void __launch_bounds__(256) {symbol}(const float* sums, void* a, '
+                "void* b, long long rows, int len, int other, int block, int per, int causal) {\n"
+                f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, "
+                "rows, len, other, block, per, causal);\n}\n")
+        return "\n".join(units)
+    outs, args = (("void* dk, void* dv", f"({ctype}*)dk, ({ctype}*)dv") if stage == "kv"
+                  else ("void* dq", f"({ctype}*)dq"))
+    return "\n".join([
+        head,
+        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {name}(const void* q, const void* k, '
+        f"const void* v, const void* go, const float* start, const float* ndelta, const float* bounds, {outs}, "
+        "float* sums, int units, int heads, int sq, int sk, long long qsb, long long qsh, long long qss, "
+        "long long ksb, long long ksh, long long kss, long long vsb, long long vsh, long long vss, "
+        "long long gsb, long long gsh, long long gss, float scale, float scale_log2, int per) {\n"
+        f"  nep::attention_bwd_{stage}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
+        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {args}, sums, units, heads, sq, sk, qsb, qsh, qss, "
+        "ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, per);\n}\n"])

@@ -91,5 +91,15 @@ def _attention_programs():
     return out
 
 
+def _attention_backward_programs():
+    from neptune_codegen.attention_backward import _program, unit_kinds
+
+    return [_program(stage, dim, causal, dt, blocks, parts)
+            for dt in ("bfloat16", "float16") for dim in (64, 128, 256)
+            for stage, blocks, parts in unit_kinds(dim)
+            for causal in ((True, False) if stage != "rows" else (False,))]
+
+
 def programs():
-    return _fold_programs() + _row_programs() + _segment_programs() + _attention_programs()
+    return (_fold_programs() + _row_programs() + _segment_programs() + _attention_programs()
+            + _attention_backward_programs())
