@@ -1,0 +1,312 @@
+// nep_distill.h -- distillation from a teacher's top logits, and its gradient (gfx950).
+//
+// Per row, student logits z[0..n), temperature T, and a teacher's list of entries (t_k, i_k):
+//   p = softmax(t / T) over the list's present entries (i_k >= 0)      q = softmax(z / T)
+//   loss = T^2 sum_k p_k (log p_k - log q_{i_k})
+//   dloss/dz_i = T (q_i - sum of p_k with i_k = i), times the row's upstream gradient
+// The row's state (max m, sum s of exp((z - m) / T)) is kept for the gradient instead of its
+// logsumexp: (z - m) is exact to an ulp of itself where z - lse would lose lse's ulp.
+//
+// A list without a present entry, or with all of them -inf, has loss 0 and gradient 0 whatever the
+// row holds.  An entry with p = 0 adds nothing; one with p > 0 at a student logit of -inf makes the
+// loss +inf (its gradient is finite).  An index of n or more makes the row's loss and gradient NaN,
+// and is never read through.
+//
+// HBM-bound: the loss reads the row once (running max and sum per lane, rescaled when the max
+// moves), the gradient reads it once and writes it once.
+#pragma once
+
+namespace nep {
+
+// TPR lanes hold a row: a wavefront (WG holds several rows, no barrier) or the whole workgroup.
+template <int TPR>
+struct RowLanes {
+  static constexpr int kWaves = TPR > 64 ? TPR / 64 : 1;
+  static_assert(TPR >= 64, "a row has a wavefront at least");
+  __device__ static __forceinline__ void sync() {
+    if constexpr (TPR > 64) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+  }
+  // `lds` has kWaves floats; the caller's next reduction may use the same
+  template <class Pair, class Group>
+  __device__ static __forceinline__ float reduce(float v, float* lds, Group group, Pair pair) {
+    v = group(v);
+    if constexpr (TPR > 64) {
+      __syncthreads();
+      if (lane_id() == 0) lds[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = lds[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v = pair(v, lds[w]);
+    }
+    return v;
+  }
+  __device__ static __forceinline__ float max(float v, float* lds) {
+    return reduce(v, lds, [](float x) { return group_max<64>(x); },
+                  [](float a, float b) { return __builtin_fmaxf(a, b); });
+  }
+  __device__ static __forceinline__ float sum(float v, float* lds) {
+    return reduce(v, lds, [](float x) { return group_sum<64>(x); },
+                  [](float a, float b) { return a + b; });
+  }
+};
+
+// A row's entries, EPL per lane: entry k of lane t is t + k TPR.
+template <class Lt, typename Ix, int TPR, int EPL>
+struct TeacherList {
+  float e[EPL];      // t_k, then exp((t_k - max) / T) / sum = p_k
+  float d[EPL];      // (t_k - max)
+  int at[EPL];       // column, -1 where absent
+  float top, total;  // max and sum of the exponentials
+  bool empty, bad;
+
+  __device__ __forceinline__ void load(const typename Lt::T* t, const Ix* ix, int count, i64 n,
+                                       int lane, bool live) {
+    bad = false;
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) {
+      const int i = lane + k * TPR;
+      at[k] = -1;
+      e[k] = -kInf;
+      if (live && i < count) {
+        const Ix x = ix[i];
+        const float v = Lt::load(t + i);
+        bad |= (i64)x >= n;
+        if (x >= 0 && (i64)x < n) {
+          at[k] = (int)x;
+          e[k] = v;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void weigh(float c, float* lds) {
+    typedef RowLanes<TPR> R;
+    float m = -kInf;
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) {
+      m = __builtin_fmaxf(m, e[k]);
+      // a NaN is no maximum; it counts as present all the same
+      if (is_nan(e[k])) m = __builtin_fmaxf(m, -3.0e38f);
+    }
+    top = R::max(m, lds);
+    bad = R::max(bad ? 1.0f : 0.0f, lds) != 0.0f;
+    empty = top == -kInf && !bad;
+    const float ref = top == -kInf ? 0.0f : top;
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) {
+      d[k] = e[k] - ref;
+      e[k] = at[k] < 0 ? 0.0f : __builtin_amdgcn_exp2f(d[k] * c);
+      s += e[k];
+    }
+    total = R::sum(s, lds);
+    const float inv = 1.0f / total;
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) e[k] = e[k] * inv;
+  }
+};
+
+// Loss and state of each row.  c = log2(e) / T, inv_t = 1 / T, t2 = T^2.
+template <class St, class Lt, typename Ix, int TPR, int UNROLL, int ACCESS, int EPL, int WG>
+__device__ __forceinline__ void distill_forward(const typename St::T* __restrict__ z,
+                                                const typename Lt::T* __restrict__ top_logits,
+                                                const Ix* __restrict__ index,
+                                                float* __restrict__ loss,
+                                                float* __restrict__ stats, i64 rows, i64 n,
+                                                i64 stride_z, i64 stride_t, i64 stride_i,
+                                                int count, float c, float inv_t, float t2) {
+  typedef RowLanes<TPR> R;
+  typedef Span<St, TPR, ACCESS> Sp;
+  constexpr int VEC = St::kVec, STEP = TPR * VEC;
+  __shared__ float lds[R::kWaves];
+  const int t = threadIdx.x % TPR;
+  const i64 row = (i64)blockIdx.x * (WG / TPR) + threadIdx.x / TPR;
+  const bool live = row < rows;
+  const typename St::T* rp = z + (live ? row : 0) * stride_z;
+  TeacherList<Lt, Ix, TPR, EPL> list;
+  list.load(top_logits + (live ? row : 0) * stride_t, index + (live ? row : 0) * stride_i, count, n, t, live);
+  float zk[EPL];                                   // in flight under the row's walk
+#pragma unroll
+  for (int k = 0; k < EPL; ++k) zk[k] = list.at[k] >= 0 ? St::load(rp + list.at[k]) : 0.0f;
+
+  const Sp sp(rp, 0, live ? n : 0);
+  float m = -kInf, s = 0.0f;
+  u32x4 cur[UNROLL];
+  auto fetch = [&](i64 e0, u32x4* w) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const i64 e = e0 + (i64)(u * TPR + t) * VEC;
+      w[u] = e < sp.v1 ? load16(rp + e) : u32x4{St::kNegInfWord, St::kNegInfWord, St::kNegInfWord, St::kNegInfWord};
+    }
+  };
+  auto move = [&](float tile_max) {
+    if (tile_max > m) {
+      s *= m == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m - tile_max) * c);
+      m = tile_max;
+    }
+    return m == -kInf ? 0.0f : m;
+  };
+  fetch(sp.v0, cur);
+  typename Sp::Rest rest;
+  if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
+  for (i64 e0 = sp.v0; e0 < sp.v1; e0 += (i64)UNROLL * STEP) {
+    u32x4 next[UNROLL];
+    fetch(e0 + (i64)UNROLL * STEP, next);
+    float tm = -kInf;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float v[VEC];
+      St::unpack(cur[u], v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) tm = __builtin_fmaxf(tm, v[j]);
+    }
+    const float ref = move(tm);
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float v[VEC];
+      St::unpack(cur[u], v);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        a += __builtin_amdgcn_exp2f((v[j] - ref) * c);
+        b += __builtin_amdgcn_exp2f((v[j + 1] - ref) * c);
+      }
+    }
+    s += a + b;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) cur[u] = next[u];
+  }
+  if constexpr (ACCESS == kRagged) {
+    float tm = -kInf;
+#pragma unroll
+    for (int u = 0; u < Sp::RU; ++u) tm = __builtin_fmaxf(tm, rest.s[u]);
+    const float ref = move(tm);
+#pragma unroll
+    for (int u = 0; u < Sp::RU; ++u) s += __builtin_amdgcn_exp2f((rest.s[u] - ref) * c);
+  }
+  const float top = R::max(m, lds);
+  const float total = R::sum(m == -kInf ? s : s * __builtin_amdgcn_exp2f((m - top) * c), lds);
+  list.weigh(c, lds);
+  // log p_k - log q_k = ((t_k - max t) - (z_k - max z)) / T - log(total t) + log(total z)
+  const float gap = logf(total) - logf(list.total);
+  float term = 0.0f;
+#pragma unroll
+  for (int k = 0; k < EPL; ++k)
+    if (list.at[k] >= 0 && !(list.e[k] == 0.0f))
+      term += list.e[k] * ((list.d[k] - (zk[k] - top)) * inv_t + gap);
+  term = R::sum(term, lds);
+  if (live && t == 0) {
+    loss[row] = list.bad ? __builtin_nanf("") : list.empty ? 0.0f : t2 * term;
+    if (stats != nullptr) {
+      stats[2 * row] = top;
+      stats[2 * row + 1] = total;
+    }
+  }
+}
+
+// Gradient of each row.  The row is written as T g q first; the list's columns are then written
+// again, whole, by the lanes that hold their entries, after a barrier behind which the first writes
+// are complete.  An index that comes twice is found by a hash of LDS bits (never missed; a false
+// alarm costs the search): each of its entries then sums p over the list in the list's order, so
+// all of them write the same value.
+template <class St, class Lt, typename Ix, int TPR, int UNROLL, int ACCESS, int EPL, int WG>
+__device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
+                                                 const typename St::T* __restrict__ z,
+                                                 const typename Lt::T* __restrict__ top_logits,
+                                                 const Ix* __restrict__ index,
+                                                 const float* __restrict__ stats,
+                                                 typename St::T* __restrict__ dz, i64 rows, i64 n,
+                                                 i64 stride_g, i64 stride_z, i64 stride_t,
+                                                 i64 stride_i, int count, float c, float temperature) {
+  typedef RowLanes<TPR> R;
+  typedef Span<St, TPR, ACCESS> Sp;
+  constexpr int VEC = St::kVec, STEP = TPR * VEC, RPW = WG / TPR;
+  constexpr int HASH = 1 << 15;                    // bits of a row's table
+  __shared__ float lds[R::kWaves];
+  __shared__ u32 seen[RPW][HASH / 32];
+  __shared__ float list_p[RPW][TPR * EPL];
+  __shared__ int list_at[RPW][TPR * EPL];
+  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const i64 row = (i64)blockIdx.x * RPW + slot;
+  const bool live = row < rows;
+  const typename St::T* rp = z + (live ? row : 0) * stride_z;
+  typename St::T* op = dz + (live ? row : 0) * n;
+  const Sp sp(rp, 0, live ? n : 0);
+  u32x4 cur[UNROLL];
+  auto fetch = [&](i64 e0, u32x4* w) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const i64 e = e0 + (i64)(u * TPR + t) * VEC;
+      w[u] = e < sp.v1 ? load16(rp + e) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  fetch(sp.v0, cur);
+  TeacherList<Lt, Ix, TPR, EPL> list;
+  list.load(top_logits + (live ? row : 0) * stride_t, index + (live ? row : 0) * stride_i, count, n, t, live);
+  float zk[EPL];
+#pragma unroll
+  for (int k = 0; k < EPL; ++k) zk[k] = list.at[k] >= 0 ? St::load(rp + list.at[k]) : 0.0f;
+  const float g = live ? grad[row * stride_g] * temperature : 0.0f;
+  const float top = live ? stats[2 * row] : 0.0f, total = live ? stats[2 * row + 1] : 1.0f;
+#pragma unroll
+  for (int i = t; i < HASH / 32; i += TPR) seen[slot][i] = 0u;
+  list.weigh(c, lds);                              // (its barriers stand between the table's two uses)
+  R::sync();
+  bool twice = false;
+#pragma unroll
+  for (int k = 0; k < EPL; ++k) {
+    list_p[slot][t + k * TPR] = list.e[k];
+    list_at[slot][t + k * TPR] = list.at[k];
+    if (list.at[k] >= 0) {
+      const u32 h = (u32)list.at[k] & (HASH - 1);
+      twice |= (atomicOr(&seen[slot][h >> 5], 1u << (h & 31)) >> (h & 31)) & 1u;
+    }
+  }
+  // NaN where the list's probabilities are (their sum is 1 otherwise), and for an index past the row
+  const float scale = list.bad || is_nan(list.total) ? __builtin_nanf("") : g / total;
+  const float ref = top == -kInf ? 0.0f : top;
+  auto value = [&](float v) { return scale * __builtin_amdgcn_exp2f((v - ref) * c); };
+  if (list.empty) {
+    for (i64 e = sp.v0 + (i64)t * VEC; e < sp.v1; e += STEP) store_vec<ACCESS>(op + e, u32x4{0u, 0u, 0u, 0u});
+    if constexpr (ACCESS == kRagged)
+      for (int i = t; i < sp.rest; i += TPR) St::store(op + sp.column(i), 0.0f);
+  } else {
+    typename Sp::Rest rest;
+    if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
+    for (i64 e0 = sp.v0; e0 < sp.v1; e0 += (i64)UNROLL * STEP) {
+      u32x4 next[UNROLL];
+      fetch(e0 + (i64)UNROLL * STEP, next);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const i64 e = e0 + (i64)(u * TPR + t) * VEC;
+        if (e >= sp.v1) continue;
+        float v[VEC];
+        St::unpack(cur[u], v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
+        store_vec<ACCESS>(op + e, St::pack(v));
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) cur[u] = next[u];
+    }
+    if constexpr (ACCESS == kRagged) sp.store_rest(rest, op, t, value);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): this wave's writes are done
+  R::sync();
+  if (list.empty || list.bad) twice = false;
+  if constexpr (TPR > 64) twice = __syncthreads_or(twice) != 0;
+  else twice = __builtin_amdgcn_ballot_w64(twice) != 0;
+  if (list.empty || list.bad) return;
+#pragma unroll
+  for (int k = 0; k < EPL; ++k) {
+    if (list.at[k] < 0) continue;
+    float p = list.e[k];
+    if (twice) {
+      p = 0.0f;
+      for (int i = 0; i < count; ++i) p += list_at[slot][i] == list.at[k] ? list_p[slot][i] : 0.0f;
+    }
+    St::store(op + list.at[k], g * (__builtin_amdgcn_exp2f((zk[k] - ref) * c) / total - p));
+  }
+}
+
+}  // namespace nep

@@ -20,6 +20,7 @@ from neptune_codegen.attention import (as_attention_op, attention_fold, exact_pa
                                        launch_attention, run_attention)
 from neptune_codegen.attention_backward import as_attention_grad_op, run_attention_backward
 from neptune_codegen.autotune import best_config, machine_key, op_key, parameter_tag
+from neptune_codegen.distill import as_distill_op, run_distill, run_distill_backward
 from neptune_codegen.emitters import (check_supported, derived_producer_expr, emit_fold_policy,
                                       emit_kernel_source, emit_rms_state_source,
                                       emit_segment_source, param_bindings)
@@ -67,6 +68,7 @@ __all__ = [
     "compile_segment_reduction", "validate_segment_inputs",
     "run_attention", "attention_fold", "as_attention_op", "launch_attention", "exact_path_taken",
     "run_attention_backward", "as_attention_grad_op",
+    "run_distill", "run_distill_backward", "as_distill_op",
     "compile_readout", "run_readout", "run_log_softmax", "as_readout_op", "readout_op_handle",
     "best_config", "machine_key", "op_key", "parameter_tag", "prebuilt_programs",
     # internals the reference package also exports: the algebra's quotient-power marker and

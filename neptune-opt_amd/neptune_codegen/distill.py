@@ -1,0 +1,267 @@
+"""Distillation from a teacher's top logits: loss and gradient.
+
+There is no reference function for this path; the row state is the logsumexp fold's (max, sum of
+exponentials).  Per row of student logits z, with temperature T and the teacher's list (t_k, i_k):
+
+    p = softmax(t / T) over the list's entries with i_k >= 0,   q = softmax(z / T)
+    loss = T^2 sum_k p_k (log p_k - log q_{i_k}),   dloss/dz_i = T (q_i - sum of p_k with i_k = i)
+
+Layout contract: logits [..., n] in float32, bfloat16 or float16; top_logits [..., k] in float32 or the
+logits' dtype and top_index [..., k] in int32 or int64, with the same leading sizes, 1 <= k <= 1024.  A
+negative index marks an absent entry (lists may differ in length); a list without an entry has loss 0
+and gradient 0; an index of n or more makes its row's loss and gradient NaN.  Loss and state are fp32,
+the gradient has the logits' dtype.  Edge values (infinities, repeated indices) are described in
+csrc/kernels/nep_distill.h.
+"""
+from __future__ import annotations
+
+import math
+import threading
+
+from neptune_codegen import calls, hip
+from neptune_codegen.emitters import (BASE_OPTIONS, DistillVariant, distill_kernel_name,
+                                      emit_distill_source)
+from neptune_codegen.template import _row_last_layout, _validate_row_last
+
+MAX_ENTRIES = 1024
+_PROGRAMS: dict = {}
+_OPS: dict = {}
+_SEEN = calls.Seen()
+_lock = threading.Lock()
+
+_FORWARD_ARGS = (hip.PTR,) * 5 + (hip.I64,) * 5 + (hip.I32,) + (hip.F32,) * 3
+_BACKWARD_ARGS = (hip.PTR,) * 6 + (hip.I64,) * 6 + (hip.I32,) + (hip.F32,) * 2
+
+
+def _program(stage: str, var: DistillVariant) -> hip.Program:
+    with _lock:
+        prog = _PROGRAMS.get((stage, var))
+        if prog is None:
+            prog = _PROGRAMS[stage, var] = hip.Program(
+                emit_distill_source(stage, var), f"{distill_kernel_name(stage, var)}.hip", BASE_OPTIONS)
+        return prog
+
+
+def _temperature(temperature) -> float:
+    if type(temperature) not in (int, float) or not math.isfinite(temperature) or temperature <= 0:
+        raise ValueError("distillation needs a finite positive temperature")
+    return float(temperature)
+
+
+def validate_distill_inputs(logits, top_logits, top_index, *, metadata: bool = False):
+    """Leading sizes of a call."""
+    import torch
+
+    for t, name in ((logits, "logits"), (top_logits, "top_logits"), (top_index, "top_index")):
+        calls.check_tensor(t, f"distillation {name}", metadata=metadata)
+    _validate_row_last(logits, metadata=metadata)
+    lead = logits.shape[:-1]
+    if top_logits.ndim != logits.ndim or top_logits.shape[:-1] != lead:
+        raise ValueError(f"distillation top_logits {tuple(top_logits.shape)} must have the leading sizes of "
+                         f"the logits {tuple(logits.shape)}")
+    if top_index.shape != top_logits.shape:
+        raise ValueError(f"distillation top_index {tuple(top_index.shape)} must have the shape of top_logits "
+                         f"{tuple(top_logits.shape)}")
+    if top_logits.dtype not in (torch.float32, logits.dtype):
+        raise TypeError(f"distillation top_logits must be float32 or the logits' dtype, got {top_logits.dtype}")
+    if top_index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"distillation top_index must be int32 or int64, got {top_index.dtype}")
+    if top_logits.device != logits.device or top_index.device != logits.device:
+        raise ValueError("distillation tensors must be on the same device")
+    if not 1 <= top_logits.shape[-1] <= MAX_ENTRIES:
+        raise NotImplementedError(f"distillation takes lists of 1 to {MAX_ENTRIES} entries")
+    if logits.shape[-1] >= 1 << 31:
+        raise NotImplementedError("distillation takes rows of less than 2^31 logits")
+    return lead
+
+
+def _check_rows(t, name, shape, logits, *, metadata):
+    import torch
+
+    calls.check_tensor(t, f"distillation {name}", metadata=metadata)
+    if t.shape != shape or t.dtype != torch.float32 or t.device != logits.device:
+        raise ValueError(f"distillation {name} must be float32 {tuple(shape)} on the logits' device, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _variant(z, top, index, rows: int, n: int, count: int) -> DistillVariant:
+    """Lanes per row: a wavefront up to 512 slots of 16 bytes, a workgroup of 256 lanes beyond; 1024
+    where the rows leave most CUs idle otherwise."""
+    vec = 16 // z.element_size()
+    slots = -(-n // vec)
+    aligned = n % vec == 0 and z.data_ptr() % 16 == 0 and (z.stride(0) * z.element_size()) % 16 == 0
+    tpr = 64 if slots <= 512 and count <= 256 else 256
+    if rows <= 512 and slots > 1024:
+        tpr = 1024
+    unroll = 1
+    while unroll < 4 and tpr * unroll * 2 < slots * 1.5:
+        unroll *= 2
+    entries = 1
+    while entries * tpr < count:
+        entries *= 2
+    name = lambda t: str(t.dtype).replace("torch.", "")  # noqa: E731
+    return DistillVariant(name(z), name(top), name(index), not aligned, tpr, unroll, entries)
+
+
+def _rows_of(t):
+    """[rows, columns] of unit column stride."""
+    flat, rows, cols = _row_last_layout(t)
+    if flat.stride(1) != 1 and cols > 1:
+        flat = flat.contiguous()
+    return flat, rows, cols
+
+
+class _Call:
+    __slots__ = ("kernel", "grid", "rest", "device", "lead", "copied")
+
+    def __init__(self, stage, logits, top, index, temperature, grad_stride=None):
+        self.lead = logits.shape[:-1]
+        z, rows, n = _rows_of(logits)
+        t, _, count = _rows_of(top)
+        i, _, _ = _rows_of(index)
+        self.copied = [a if a.data_ptr() != b.data_ptr() else None
+                       for a, b in ((z, logits), (t, top), (i, index))]
+        var = _variant(z, t, i, rows, n, count)
+        self.device = calls.device_index(logits)
+        self.kernel = _program(stage, var).kernel(
+            distill_kernel_name(stage, var), _FORWARD_ARGS if stage == "forward" else _BACKWARD_ARGS,
+            var.wg, self.device)
+        groups = -(-rows // var.rows)
+        calls.check_grid(groups, var.wg, "distillation")
+        self.grid = (groups,)
+        c = math.log2(math.e) / temperature
+        strides = (z.stride(0), t.stride(0), i.stride(0))
+        if stage == "forward":
+            self.rest = (rows, n) + strides + (count, c, 1.0 / temperature, temperature * temperature)
+        else:
+            self.rest = (rows, n, grad_stride) + strides + (count, c, temperature)
+
+    def operands(self, *given):
+        return [(c if c is not None else g).data_ptr() for c, g in zip(self.copied, given)]
+
+    @property
+    def reusable(self) -> bool:
+        return all(c is None for c in self.copied)
+
+
+def run_distill(logits, top_logits, top_index, *, temperature: float = 1.0, return_stats: bool = False):
+    """Loss [...] of each row in fp32, and with `return_stats` the state [..., 2] (max, sum of
+    exponentials) that run_distill_backward takes, on the current stream.  A call whose tensor layouts
+    and temperature were seen before reuses that call's kernel and launch shape."""
+    import torch
+
+    key = calls.tensors_key(logits, top_logits, top_index)
+    call = None
+    if key is not None and type(temperature) in (int, float):
+        key += ("forward", temperature)
+        call = _SEEN.get(key)
+    else:
+        key = None
+    if call is None:
+        metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
+        lead = validate_distill_inputs(logits, top_logits, top_index, metadata=metadata)
+        temperature = _temperature(temperature)
+        if not metadata and logits.numel() != 0:
+            call = _Call("forward", logits, top_logits, top_index, temperature)
+            if key is not None and call.reusable:
+                _SEEN.keep(key, call)
+    else:
+        lead = call.lead
+    loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    stats = torch.empty((*lead, 2), dtype=torch.float32, device=logits.device) if return_stats else None
+    if call is not None:
+        with calls.on_device(call.device):
+            call.kernel.launch(call.grid, (*call.operands(logits, top_logits, top_index), loss.data_ptr(),
+                                           0 if stats is None else stats.data_ptr()) + call.rest,
+                               hip.current_stream(call.device))
+    return (loss, stats) if return_stats else loss
+
+
+def run_distill_backward(grad, logits, top_logits, top_index, stats, *, temperature: float = 1.0):
+    """Gradient [..., n] of the logits, in their dtype, for the losses' gradient `grad` [...] in fp32 and
+    the state that run_distill returned; fresh and contiguous."""
+    import torch
+
+    key = calls.tensors_key(grad, logits, top_logits, top_index, stats)
+    call = None
+    if key is not None and type(temperature) in (int, float):
+        key += ("backward", temperature)
+        call = _SEEN.get(key)
+    else:
+        key = None
+    if call is None:
+        metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
+        lead = validate_distill_inputs(logits, top_logits, top_index, metadata=metadata)
+        _check_rows(grad, "grad", lead, logits, metadata=metadata)
+        _check_rows(stats, "stats", (*lead, 2), logits, metadata=metadata)
+        temperature = _temperature(temperature)
+        if metadata or logits.numel() == 0:
+            return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        plain = stats.is_contiguous()
+        stats = stats.contiguous()
+        flat = grad.reshape(-1)           # a view where the rows have one stride (a mean's is 0)
+        call = _Call("backward", logits, top_logits, top_index, temperature, flat.stride(0))
+        if key is not None and call.reusable and plain and flat.data_ptr() == grad.data_ptr():
+            _SEEN.keep(key, call)
+        grad = flat
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    with calls.on_device(call.device):
+        call.kernel.launch(call.grid, (grad.data_ptr(), *call.operands(logits, top_logits, top_index),
+                                       stats.data_ptr(), out.data_ptr()) + call.rest,
+                           hip.current_stream(call.device))
+    return out
+
+
+def as_distill_op(temperature: float = 1.0, lib: str = "neptune"):
+    """Differentiable custom op `(Tensor logits, Tensor top_logits, Tensor top_index) -> (Tensor loss,
+    Tensor stats)` with the temperature in its name; the gradient is the logits'."""
+    import torch
+
+    from neptune_codegen.autotune import parameter_tag
+
+    temperature = _temperature(temperature)
+    key = (lib, temperature)
+    with _lock:
+        if key in _OPS:
+            return _OPS[key]
+    name = f"distill{parameter_tag({'t': temperature})}"
+
+    def _forward(logits, top_logits, top_index):
+        return run_distill(logits, top_logits, top_index, temperature=temperature, return_stats=True)
+
+    def _forward_fake(logits, top_logits, top_index):
+        lead = validate_distill_inputs(logits, top_logits, top_index, metadata=True)
+        return (torch.empty(lead, dtype=torch.float32, device=logits.device),
+                torch.empty((*lead, 2), dtype=torch.float32, device=logits.device))
+
+    def _backward(grad, logits, top_logits, top_index, stats):
+        return run_distill_backward(grad, logits, top_logits, top_index, stats, temperature=temperature)
+
+    def _backward_fake(grad, logits, top_logits, top_index, stats):
+        validate_distill_inputs(logits, top_logits, top_index, metadata=True)
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+    define = torch.library.custom_op
+    op = define(f"{lib}::{name}", mutates_args=(),
+                schema="(Tensor logits, Tensor top_logits, Tensor top_index) -> (Tensor, Tensor)")(_forward)
+    op.register_fake(_forward_fake)
+    back = define(f"{lib}::{name}_backward", mutates_args=(),
+                  schema="(Tensor grad, Tensor logits, Tensor top_logits, Tensor top_index, Tensor stats) "
+                         "-> Tensor")(_backward)
+    back.register_fake(_backward_fake)
+
+    def _setup(ctx, inputs, output):
+        loss, stats = output
+        ctx.save_for_backward(*inputs, stats)
+        ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
+
+    def _grad(ctx, grad, _):
+        if grad is None:
+            return None, None, None
+        return back(grad, *ctx.saved_tensors), None, None
+
+    op.register_autograd(_grad, setup_context=_setup)
+    with _lock:
+        _OPS[key] = op
+    return op

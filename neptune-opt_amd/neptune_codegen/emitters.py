@@ -766,3 +766,57 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
         f"  nep::attention_bwd_{stage}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
         f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {args}, sums, units, heads, sq, sk, qsb, qsh, qss, "
         "ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, per);\n}\n"])
+
+
+# ---------------------------------------------------------------- distillation from top logits
+@dataclasses.dataclass(frozen=True)
+class DistillVariant:
+    """One launch shape of the distillation kernels."""
+
+    dtype: str          # of the logits
+    top_dtype: str      # of the teacher's logits
+    index: str          # "int32" or "int64"
+    ragged: bool        # rows of any alignment and width (nep_device.h kRagged)
+    tpr: int            # lanes per row: a wavefront, or the workgroup
+    unroll: int         # 16-byte slots per lane and step
+    entries: int        # list entries per lane
+
+    @property
+    def wg(self) -> int:
+        return max(256, self.tpr)
+
+    @property
+    def rows(self) -> int:
+        return self.wg // self.tpr
+
+    def tag(self) -> str:
+        return (f"{dtype_tag(self.dtype)[0]}_{dtype_tag(self.top_dtype)[0]}_{self.index[0]}{self.index[3:]}"
+                f"_{access_tag(True, self.ragged)}{self.tpr}u{self.unroll}e{self.entries}")
+
+
+def distill_kernel_name(stage: str, var: DistillVariant) -> str:
+    return f"distill_{stage}_{var.tag()}"
+
+
+def emit_distill_source(stage: str, var: DistillVariant) -> str:
+    """hiprtc unit of the distillation loss ("forward") or its gradient ("backward"), nep_distill.h."""
+    st, lt = dtype_tag(var.dtype)[1], dtype_tag(var.top_dtype)[1]
+    ix = {"int32": "int", "int64": "long long"}[var.index]
+    targs = (f"<{st}, {lt}, {ix}, {var.tpr}, {var.unroll}, {access_name(True, var.ragged)}, "
+             f"{var.entries}, {var.wg}>")
+    head = ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
+            f"// distillation from a teacher's top logits: {stage}, {var.tag()}\n"
+            + kernel_header("nep_device.h", "nep_distill.h"))
+    bound = f'extern "C" __global__ void __launch_bounds__({var.wg}) {distill_kernel_name(stage, var)}'
+    if stage == "forward":
+        return (f"{head}\n{bound}(const void* z, const void* t, const void* ix, float* loss, float* stats, "
+                "long long rows, long long n, long long stride_z, long long stride_t, long long stride_i, "
+                "int count, float c, float inv_t, float t2) {\n"
+                f"  nep::distill_forward{targs}((const {st}::T*)z, (const {lt}::T*)t, (const {ix}*)ix, loss, "
+                "stats, rows, n, stride_z, stride_t, stride_i, count, c, inv_t, t2);\n}\n")
+    return (f"{head}\n{bound}(const float* grad, const void* z, const void* t, const void* ix, "
+            "const float* stats, void* dz, long long rows, long long n, long long stride_g, "
+            "long long stride_z, long long stride_t, long long stride_i, int count, float c, "
+            "float temperature) {\n"
+            f"  nep::distill_backward{targs}(grad, (const {st}::T*)z, (const {lt}::T*)t, (const {ix}*)ix, "
+            f"stats, ({st}::T*)dz, rows, n, stride_g, stride_z, stride_t, stride_i, count, c, temperature);\n}}\n")
