@@ -24,6 +24,8 @@ from neptune_codegen.distill import as_distill_op, run_distill, run_distill_back
 from neptune_codegen.emitters import (check_supported, derived_producer_expr, emit_fold_policy,
                                       emit_kernel_source, emit_rms_state_source,
                                       emit_segment_source, param_bindings)
+from neptune_codegen.residual_norm import (as_residual_norm_op, run_residual_norm,
+                                           run_residual_norm_backward)
 from neptune_codegen.skeleton import (NEGATIVE_CONTROLS, SKELETONS, STATE_REDUCTIONS,
                                       NumericalContract, Skeleton, StateField, StateReduction,
                                       all_registered, param_defaults, register,
@@ -69,6 +71,7 @@ __all__ = [
     "run_attention", "attention_fold", "as_attention_op", "launch_attention", "exact_path_taken",
     "run_attention_backward", "as_attention_grad_op",
     "run_distill", "run_distill_backward", "as_distill_op",
+    "run_residual_norm", "run_residual_norm_backward", "as_residual_norm_op",
     "compile_readout", "run_readout", "run_log_softmax", "as_readout_op", "readout_op_handle",
     "best_config", "machine_key", "op_key", "parameter_tag", "prebuilt_programs",
     # internals the reference package also exports: the algebra's quotient-power marker and

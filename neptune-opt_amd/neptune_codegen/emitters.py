@@ -820,3 +820,59 @@ def emit_distill_source(stage: str, var: DistillVariant) -> str:
             "float temperature) {\n"
             f"  nep::distill_backward{targs}(grad, (const {st}::T*)z, (const {lt}::T*)t, (const {ix}*)ix, "
             f"stats, ({st}::T*)dz, rows, n, stride_g, stride_z, stride_t, stride_i, count, c, temperature);\n}}\n")
+
+
+# ---------------------------------------------------------------- residual norm
+@dataclasses.dataclass(frozen=True)
+class ResidualNormVariant:
+    """One launch shape of the residual norm's kernels."""
+
+    dtype: str
+    any: bool           # rows of any alignment and width
+    tpr: int            # lanes per row
+    nv: int             # 16-byte slots per lane
+    wg: int             # lanes per workgroup
+    after: bool         # a norm behind the block
+    gate: str           # "none", "rows" (one per row) or "group" (one per group of rows)
+
+    def tag(self) -> str:
+        return (f"{dtype_tag(self.dtype)[0]}_{'a' if self.any else 'v'}{self.tpr}n{self.nv}w{self.wg}"
+                f"{'_after' if self.after else ''}{'' if self.gate == 'none' else '_' + self.gate}")
+
+
+def residual_norm_kernel_name(stage: str, var: ResidualNormVariant) -> str:
+    if stage == "join":
+        return f"residual_norm_join_{dtype_tag(var.dtype)[0]}"
+    return f"residual_norm_{stage}_{var.tag()}"
+
+
+def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
+    """hiprtc unit of the residual norm ("forward") or its gradients with their join ("backward"),
+    nep_residual_norm.h."""
+    st = dtype_tag(var.dtype)[1]
+    gate = {"none": "nep::kGateNone", "rows": "nep::kGateRows", "group": "nep::kGateGroup"}[var.gate]
+    flags = f"{str(var.any).lower()}, {str(var.after).lower()}, {gate}, {var.wg}"
+    c, m = f"(const {st}::T*)", f"({st}::T*)"
+    head = ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
+            f"// residual norm: {stage}, {var.tag()}\n"
+            + kernel_header("nep_device.h", "nep_residual_norm.h"))
+    bound = f'extern "C" __global__ void __launch_bounds__({var.wg}) {residual_norm_kernel_name(stage, var)}'
+    if stage == "forward":
+        return (f"{head}\n{bound}(const void* x, const void* y, const void* gate, const void* after, "
+                "const void* before, void* residual, void* normed, float* stats, long long rows, int n, "
+                "long long stride_x, long long stride_y, long long group, float scale, float eps) {\n"
+                f"  nep::residual_norm_forward<{st}, {var.tpr}, {var.nv}, {flags}>({c}x, {c}y, {c}gate, "
+                f"{c}after, {c}before, {m}residual, {m}normed, stats, rows, n, stride_x, stride_y, group, "
+                "scale, eps);\n}\n")
+    return (f"{head}\n{bound}(const void* dres, const void* dnormed, const void* x, const void* y, "
+            "const void* gate, const void* after, const void* before, const float* stats, void* dx, void* dy, "
+            "void* dgate, void* dafter, void* dbefore, float* sums, long long rows, int n, "
+            "long long stride_dr, long long stride_dn, long long stride_x, long long stride_y, "
+            "long long group, long long chunk, long long per_group, float scale) {\n"
+            f"  nep::residual_norm_backward<{st}, {var.tpr}, {var.nv}, {flags}>({c}dres, {c}dnormed, {c}x, "
+            f"{c}y, {c}gate, {c}after, {c}before, stats, {m}dx, {m}dy, {m}dgate, {m}dafter, {m}dbefore, sums, "
+            "rows, n, stride_dr, stride_dn, stride_x, stride_y, group, chunk, per_group, scale);\n}\n"
+            f'extern "C" __global__ void __launch_bounds__(256) {residual_norm_kernel_name("join", var)}('
+            "const float* sums, void* dafter, void* dbefore, void* dgate, int n, long long chunks, "
+            "long long per_group) {\n"
+            f"  nep::residual_norm_join<{st}>(sums, {m}dafter, {m}dbefore, {m}dgate, n, chunks, per_group);\n}}\n")
