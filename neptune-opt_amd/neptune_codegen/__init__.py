@@ -26,6 +26,7 @@ from neptune_codegen.emitters import (check_supported, derived_producer_expr, em
                                       emit_segment_source, param_bindings)
 from neptune_codegen.residual_norm import (as_residual_norm_op, run_residual_norm,
                                            run_residual_norm_backward)
+from neptune_codegen.rotary import as_rotary_op, rotary_frequencies, run_rotary, run_rotary_backward
 from neptune_codegen.skeleton import (NEGATIVE_CONTROLS, SKELETONS, STATE_REDUCTIONS,
                                       NumericalContract, Skeleton, StateField, StateReduction,
                                       all_registered, param_defaults, register,
@@ -70,6 +71,7 @@ __all__ = [
     "compile_segment_reduction", "validate_segment_inputs",
     "run_attention", "attention_fold", "as_attention_op", "launch_attention", "exact_path_taken",
     "run_attention_backward", "as_attention_grad_op",
+    "run_rotary", "run_rotary_backward", "rotary_frequencies", "as_rotary_op",
     "run_distill", "run_distill_backward", "as_distill_op",
     "run_residual_norm", "run_residual_norm_backward", "as_residual_norm_op",
     "compile_readout", "run_readout", "run_log_softmax", "as_readout_op", "readout_op_handle",
