@@ -18,8 +18,15 @@
 //
 // Calls whose Python body makes a copy of an input, or whose inputs alias one another, leave
 // no plan and keep going through Python.
+//
+// The training operators' direct entry points (neptune_codegen/calls.py) keep their calls here too:
+// CallPlan is one call layout's buffers and launches, CallTable finds it again by the layout of the
+// tensors and the numbers of a call.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
@@ -261,6 +268,184 @@ py::object key_of(const std::vector<at::Tensor>& tensors) {
   return py::cast(key);
 }
 
+// ---------------------------------------------------------------- direct entry points
+// One call layout of an entry point: the buffers it allocates (results first, then scratch) and its
+// launches, whose pointer arguments are each an input, or a buffer at a byte offset.
+class CallPlan {
+ public:
+  struct Patch {
+    uint32_t offset;        // in the image
+    int32_t source;         // input `source`, or buffer -1 - source
+    int64_t add;            // bytes
+  };
+  struct CallLaunch {
+    Launch launch;
+    std::vector<Patch> patches;
+  };
+
+  // buffers: (dtype code, sizes); returns: buffer per result, -1 for None, and whether a single result
+  // comes bare; launches: (kernel, grid, block, lds, image, ((offset, source, add), ...))
+  CallPlan(int n_inputs, const py::tuple& buffers, std::vector<int> returns, bool bare,
+           const py::tuple& launches)
+      : n_inputs_(n_inputs), returns_(std::move(returns)), bare_(bare) {
+    for (py::handle b : buffers) {
+      py::tuple t = b.cast<py::tuple>();
+      dtypes_.push_back(static_cast<c10::ScalarType>(t[0].cast<int>()));
+      sizes_.push_back(t[1].cast<std::vector<int64_t>>());
+    }
+    const int n = static_cast<int>(sizes_.size());
+    for (int r : returns_) TORCH_CHECK(r >= -1 && r < n, "CallPlan: no such result");
+    TORCH_CHECK(!bare_ || (returns_.size() == 1 && returns_[0] >= 0), "CallPlan: one bare result");
+    for (py::handle l : launches) {
+      py::tuple t = l.cast<py::tuple>();
+      CallLaunch c;
+      c.launch.kernel = t[0].cast<uint64_t>();
+      py::tuple grid = t[1].cast<py::tuple>();
+      for (int d = 0; d < 3; ++d) c.launch.grid[d] = grid[d].cast<uint32_t>();
+      c.launch.block = t[2].cast<uint32_t>();
+      c.launch.lds = t[3].cast<uint32_t>();
+      const std::string image = t[4].cast<std::string>();
+      c.launch.image.assign(image.begin(), image.end());
+      TORCH_CHECK(c.launch.kernel != 0 && image.size() <= nep_plan::kMaxImage, "CallPlan: bad launch");
+      for (py::handle p : t[5].cast<py::tuple>()) {
+        py::tuple pt = p.cast<py::tuple>();
+        Patch patch{pt[0].cast<uint32_t>(), pt[1].cast<int32_t>(), pt[2].cast<int64_t>()};
+        TORCH_CHECK(patch.offset + sizeof(void*) <= image.size() && patch.source < n_inputs_ &&
+                        -1 - patch.source < n, "CallPlan: bad pointer");
+        c.patches.push_back(patch);
+      }
+      launches_.push_back(std::move(c));
+    }
+  }
+
+  py::object run(const py::tuple& tensors) const {
+    TORCH_CHECK(static_cast<int>(tensors.size()) == n_inputs_, "CallPlan: expected ", n_inputs_, " tensors");
+    constexpr int kMostInputs = 16;
+    TORCH_CHECK(n_inputs_ <= kMostInputs, "CallPlan: too many tensors");
+    char* inputs[kMostInputs];
+    const at::Tensor* first = nullptr;
+    for (int i = 0; i < n_inputs_; ++i) {
+      PyObject* o = PyTuple_GET_ITEM(tensors.ptr(), i);
+      inputs[i] = nullptr;
+      if (o == Py_None) continue;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      inputs[i] = static_cast<char*>(t.data_ptr());
+      if (first == nullptr) first = &t;
+    }
+    TORCH_CHECK(first != nullptr, "CallPlan: no tensor");
+    const c10::Device device = first->device();
+    const c10::DeviceGuard guard(device);
+    const at::TensorOptions options = at::TensorOptions().device(device);
+    std::vector<at::Tensor> buffers;
+    buffers.reserve(sizes_.size());
+    for (size_t i = 0; i < sizes_.size(); ++i)
+      buffers.push_back(at::empty(sizes_[i], options.dtype(dtypes_[i])));
+    if (!launches_.empty()) {
+      hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
+      uint8_t image[nep_plan::kMaxImage];
+      for (const CallLaunch& c : launches_) {
+        const Launch& l = c.launch;
+        std::memcpy(image, l.image.data(), l.image.size());
+        for (const Patch& p : c.patches) {
+          char* ptr = p.source >= 0 ? inputs[p.source]
+                                    : static_cast<char*>(buffers[-1 - p.source].data_ptr()) + p.add;
+          std::memcpy(image + p.offset, &ptr, sizeof(ptr));
+        }
+        const int rc = nep_launch_packed(l.kernel, l.grid[0], l.grid[1], l.grid[2], l.block, l.lds,
+                                         stream, image, l.image.size());
+        TORCH_CHECK(rc == NEP_OK, "neptune launch failed: ", nep_last_error());
+      }
+    }
+    if (bare_) return py::cast(buffers[returns_[0]]);
+    py::tuple out(returns_.size());
+    for (size_t i = 0; i < returns_.size(); ++i)
+      out[i] = returns_[i] < 0 ? py::object(py::none()) : py::cast(buffers[returns_[i]]);
+    return out;
+  }
+
+ private:
+  const int n_inputs_;
+  std::vector<c10::ScalarType> dtypes_;
+  std::vector<std::vector<int64_t>> sizes_;
+  const std::vector<int> returns_;
+  const bool bare_;
+  std::vector<CallLaunch> launches_;
+};
+
+// Plans by (layout of the tensors, numbers): dtype, device, sizes, strides and address mod 16 of plain
+// strided device tensors, None for an absent one, and the type and value of each number.  A call with
+// anything else among them has no key.
+class CallTable {
+ public:
+  py::object run(const py::tuple& tensors, const py::tuple& numbers) {
+    Key key;
+    if (!make_key(tensors, numbers, key)) return py::none();
+    auto it = plans_.find(key);                      // under the GIL
+    if (it == plans_.end()) return py::none();
+    const std::shared_ptr<CallPlan> plan = it->second;
+    return plan->run(tensors);
+  }
+  bool keep(const py::tuple& tensors, const py::tuple& numbers, std::shared_ptr<CallPlan> plan) {
+    Key key;
+    if (!make_key(tensors, numbers, key)) return false;
+    if (plans_.size() >= kMostPlans) plans_.clear();
+    plans_[std::move(key)] = std::move(plan);
+    return true;
+  }
+  size_t size() const { return plans_.size(); }
+  void clear() { plans_.clear(); }
+
+ private:
+  static constexpr size_t kMostPlans = 4096;
+
+  static bool make_key(const py::tuple& tensors, const py::tuple& numbers, Key& key) {
+    key.reserve(tensors.size() * 14 + numbers.size() * 2);
+    for (py::handle h : tensors) {
+      PyObject* o = h.ptr();
+      if (o == Py_None) {
+        key.push_back(-1);
+        continue;
+      }
+      if (!THPVariable_CheckExact(o)) return false;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!t.defined() || !t.device().is_cuda() || t.layout() != c10::kStrided || t.is_neg() || t.is_conj() ||
+          t.key_set().has(c10::DispatchKey::Python))
+        return false;
+      key.push_back(static_cast<int64_t>(t.scalar_type()));
+      key.push_back(t.get_device());
+      key.push_back(t.dim());
+      for (int64_t s : t.sizes()) key.push_back(s);
+      for (int64_t s : t.strides()) key.push_back(s);
+      key.push_back(static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16));
+    }
+    for (py::handle h : numbers) {
+      PyObject* o = h.ptr();
+      if (o == Py_None) {
+        key.push_back(0);
+      } else if (PyBool_Check(o)) {
+        key.push_back(o == Py_True ? 2 : 1);
+      } else if (PyFloat_CheckExact(o)) {
+        const double d = PyFloat_AS_DOUBLE(o);
+        int64_t bits;
+        std::memcpy(&bits, &d, sizeof(bits));
+        key.push_back(3);
+        key.push_back(bits);
+      } else if (PyLong_CheckExact(o)) {
+        int overflow = 0;
+        const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+        if (overflow != 0) return false;
+        key.push_back(4);
+        key.push_back(v);
+      } else {
+        return false;
+      }
+    }
+    return true;
+  }
+
+  std::unordered_map<Key, std::shared_ptr<CallPlan>, KeyHash> plans_;
+};
+
 int64_t dtype_code(const at::Tensor& t) { return static_cast<int64_t>(t.scalar_type()); }
 
 bool installed(const std::string& qualname) {
@@ -279,4 +464,14 @@ PYBIND11_MODULE(_neptune_dispatch, m) {
   m.def("installed", &installed, py::arg("qualname"));
   m.def("key_of", &key_of, py::arg("tensors"));
   m.def("dtype_code", &dtype_code, py::arg("tensor"));
+  py::class_<CallPlan, std::shared_ptr<CallPlan>>(m, "CallPlan")
+      .def(py::init<int, const py::tuple&, std::vector<int>, bool, const py::tuple&>(), py::arg("n_inputs"),
+           py::arg("buffers"), py::arg("returns"), py::arg("bare"), py::arg("launches"))
+      .def("run", &CallPlan::run, py::arg("tensors"));
+  py::class_<CallTable>(m, "CallTable")
+      .def(py::init<>())
+      .def("run", &CallTable::run, py::arg("tensors"), py::arg("numbers"))
+      .def("keep", &CallTable::keep, py::arg("tensors"), py::arg("numbers"), py::arg("plan"))
+      .def("size", &CallTable::size)
+      .def("clear", &CallTable::clear);
 }

@@ -28,7 +28,7 @@ from neptune_codegen.emitters import (ATTN_BWD_TILE, ATTN_BWD_WAVES, BASE_OPTION
 _PROGRAMS: dict = {}
 _KERNELS: dict = {}
 _OPS: dict = {}
-_SEEN = calls.Seen()
+_TABLE = calls.Table()
 _lock = threading.Lock()
 
 _ROWS_ARGS = (hip.PTR,) * 8 + (hip.I32,) * 4 + (hip.I64,) * 9 + (hip.F32,)
@@ -105,38 +105,6 @@ def _operand(t):
     return t, (sb, sh, ss)
 
 
-class _Call:
-    """The launches of one call layout: kernels, grids and the arguments that are not pointers."""
-
-    __slots__ = ("device", "q_shape", "k_shape", "nbytes", "offsets", "sums", "rows", "kv", "q",
-                 "kv_join", "q_join")
-
-    def run(self, grad, q, k, v, out, lse, grad_lse, dq, dk, dv):
-        import torch
-
-        work = torch.empty(self.nbytes, dtype=torch.uint8, device=q.device)
-        base = work.data_ptr()
-        start, ndelta, bounds, sums = (base + o for o in self.offsets)
-        pq, pk, pv, pg = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad.data_ptr()
-        with calls.on_device(self.device):
-            stream = hip.current_stream(self.device)
-            kernel, grid, rest = self.rows
-            kernel.launch(grid, (out.data_ptr(), pg, pv, lse.data_ptr(),
-                                 0 if grad_lse is None else grad_lse.data_ptr(), start, ndelta, bounds)
-                          + rest, stream)
-            kernel, grid, rest = self.kv
-            kernel.launch(grid, (pq, pk, pv, pg, start, ndelta, bounds, dk.data_ptr(), dv.data_ptr(), sums)
-                          + rest, stream)
-            if self.kv_join is not None:
-                kernel, grid, rest = self.kv_join
-                kernel.launch(grid, (sums, dk.data_ptr(), dv.data_ptr()) + rest, stream)
-            kernel, grid, rest = self.q
-            kernel.launch(grid, (pq, pk, pv, pg, start, ndelta, bounds, dq.data_ptr(), sums) + rest, stream)
-            if self.q_join is not None:
-                kernel, grid, rest = self.q_join
-                kernel.launch(grid, (sums, dq.data_ptr(), 0) + rest, stream)
-
-
 # What `_plan` prices a stage with, in us on MI355X (fits of replays over sixteen shapes): a workgroup's
 # pass over a 64-row tile with few workgroups on the chip, and with the chip full (the clock and the
 # caches are shared), and its start and end.  Head dim 64 has two workgroups of one block on a CU.
@@ -202,7 +170,8 @@ def _plan(units, sq, sk, head_dim, causal):
             + _stage_plan("q", units, nq, nk, head_dim, causal))
 
 
-def _prepare(q, k, strides, scale, causal, plan=None) -> _Call:
+def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
+    """Launches of a call; its tensors are (grad, q, k, v, out, lse, grad_lse)."""
     import torch
 
     B, H, Sq, D = q.shape
@@ -211,36 +180,35 @@ def _prepare(q, k, strides, scale, causal, plan=None) -> _Call:
     nq, nk = -(-Sq // ATTN_BWD_TILE), -(-Sk // ATTN_BWD_TILE)
     kv_per, q_per = -(-nq // kv_parts), -(-nk // q_parts)
     kv_parts, q_parts = -(-nq // kv_per), -(-nk // q_per)
+    kv_rows, q_rows = 32 * ATTN_BWD_WAVES * kv_blocks, 32 * ATTN_BWD_WAVES * q_blocks
     kind = (device, D, causal, q.dtype)
-    call = _Call()
-    call.device = device
-    # start values and deltas of every padded query row; fp16's bounds; the parts' fp32 sums
+    # scratch: start values and deltas of every padded query row; fp16's bounds; the parts' fp32 sums
     stats = 4 * units * nq * ATTN_BWD_TILE
     bounds = -(-4 * units * (2 * nq + nk) // 256) * 256
     sums = max(8 * kv_parts * units * Sk * D if kv_parts > 1 else 0,
                4 * q_parts * units * Sq * D if q_parts > 1 else 0)
-    call.offsets = (0, stats, 2 * stats, 2 * stats + bounds)
-    call.nbytes = 2 * stats + bounds + sums
+    buffers = [(q.shape, q.dtype), (k.shape, q.dtype), (k.shape, q.dtype),
+               ((2 * stats + bounds + sums,), torch.uint8)]
+    grad, tq, tk, tv, out, lse, glse = map(calls.tensor, range(7))
+    dq, dk, dv = map(calls.buffer, range(3))
+    start, ndelta, limit, part = (calls.buffer(3, o) for o in (0, stats, 2 * stats, 2 * stats + bounds))
     qs, ks, vs, gs, os = strides
+    sizes, steps = (units, H, Sq, Sk), qs + ks + vs + gs + (scale, scale * LOG2E)
     groups = units * (nq + (nk if q.dtype == torch.float16 else 0))
-    kv_groups = units * kv_parts * -(-Sk // (32 * ATTN_BWD_WAVES * kv_blocks))
-    q_groups = units * q_parts * -(-Sq // (32 * ATTN_BWD_WAVES * q_blocks))
-    join = tuple(-(-units * n * D // 1024) for n in (2 * Sk, Sq))
-    for n, threads in ((groups, 256), (kv_groups, _THREADS), (q_groups, _THREADS),
-                       (max(join), 256)):
-        calls.check_grid(n, threads, "attention backward")
-    call.rows = (_kernel("rows", *kind), (groups,), (H, Sq, Sk, units) + os + gs + vs + (scale,))
-    tail = (units, H, Sq, Sk) + qs + ks + vs + gs + (scale, scale * LOG2E)
-    call.kv = (_kernel("kv", *kind, kv_blocks, kv_parts > 1), (kv_groups,), tail + (kv_per,))
-    call.q = (_kernel("q", *kind, q_blocks, q_parts > 1), (q_groups,), tail + (q_per,))
-    call.kv_join = call.q_join = None
+    launches = [
+        (_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start, ndelta,
+                                             limit, H, Sq, Sk, units) + os + gs + vs + (scale,)),
+        (_kernel("kv", *kind, kv_blocks, kv_parts > 1), (units * kv_parts * -(-Sk // kv_rows),),
+         (tq, tk, tv, grad, start, ndelta, limit, dk, dv, part) + sizes + steps + (kv_per,))]
     if kv_parts > 1:
-        call.kv_join = (_kernel("kv_join", *kind), (join[0],),
-                        (units * Sk, Sk, Sq, 32 * ATTN_BWD_WAVES * kv_blocks, kv_per, int(causal)))
+        launches.append((_kernel("kv_join", *kind), (-(-units * 2 * Sk * D // 1024),),
+                         (part, dk, dv, units * Sk, Sk, Sq, kv_rows, kv_per, int(causal))))
+    launches.append((_kernel("q", *kind, q_blocks, q_parts > 1), (units * q_parts * -(-Sq // q_rows),),
+                     (tq, tk, tv, grad, start, ndelta, limit, dq, part) + sizes + steps + (q_per,)))
     if q_parts > 1:
-        call.q_join = (_kernel("q_join", *kind), (join[1],),
-                       (units * Sq, Sq, Sk, 32 * ATTN_BWD_WAVES * q_blocks, q_per, int(causal)))
-    return call
+        launches.append((_kernel("q_join", *kind), (-(-units * Sq * D // 1024),),
+                         (part, dq, 0, units * Sq, Sq, Sk, q_rows, q_per, int(causal))))
+    return calls.Plan(device, 7, buffers, (0, 1, 2), launches)
 
 
 def run_attention_backward(grad, q, k, v, out, lse, *, grad_lse=None, scale: float | None = None,
@@ -249,42 +217,35 @@ def run_attention_backward(grad, q, k, v, out, lse, *, grad_lse=None, scale: flo
     gradient `grad` of its output (and `grad_lse` of its logsumexp), on the current stream.  `out`
     and `lse` are what that call returned.  See the module docstring for the contract.  A call whose
     tensor layouts and options were seen before reuses that call's kernels and launch shapes."""
-    key = call = None
-    if scale is None or type(scale) in (int, float):
-        key = calls.tensors_key(grad, q, k, v, out, lse, grad_lse)
-    if key is not None:
-        key += (type(scale), scale, bool(causal))
-        call = _SEEN.get(key)
-    return _run(grad, q, k, v, out, lse, grad_lse, scale, causal, key, call)
+    causal = bool(causal)
+    found = _TABLE.run((grad, q, k, v, out, lse, grad_lse), (scale, causal))
+    if found is not None:
+        return found
+    return _run(grad, q, k, v, out, lse, grad_lse, scale, causal)
 
 
-def _run(grad, q, k, v, out, lse, grad_lse, scale, causal, key=None, call=None, plan=None):
+def _run(grad, q, k, v, out, lse, grad_lse, scale, causal, plan=None):
     import torch
 
-    if call is None:
-        metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
-        validate_attention_backward_inputs(grad, q, k, v, out, lse, grad_lse, metadata=metadata)
-        scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-        if not math.isfinite(scale) or scale <= 0:
-            raise ValueError("attention scale must be finite and positive")
-        if metadata or q.numel() == 0:
-            # without a query nothing reaches the keys
-            return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                    torch.zeros(k.shape, dtype=k.dtype, device=k.device),
-                    torch.zeros(v.shape, dtype=v.dtype, device=v.device))
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    if call is None:
-        given = (q, k, v, grad, out, lse, grad_lse)
-        (q, qs), (k, ks), (v, vs), (grad, gs), (out, os) = map(_operand, given[:5])
-        lse = lse.contiguous()
-        grad_lse = grad_lse.contiguous() if grad_lse is not None else None
-        call = _prepare(q, k, (qs, ks, vs, gs, os), scale, bool(causal), plan)
-        if key is not None and all(a is b for a, b in zip(given, (q, k, v, grad, out, lse, grad_lse))):
-            _SEEN.keep(key, call)
-    call.run(grad, q, k, v, out, lse, grad_lse, dq, dk, dv)
-    return dq, dk, dv
+    metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
+    validate_attention_backward_inputs(grad, q, k, v, out, lse, grad_lse, metadata=metadata)
+    given, number = (grad, q, k, v, out, lse, grad_lse), scale
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("attention scale must be finite and positive")
+    if metadata or q.numel() == 0:
+        # without a query nothing reaches the keys
+        return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                torch.zeros(k.shape, dtype=k.dtype, device=k.device),
+                torch.zeros(v.shape, dtype=v.dtype, device=v.device))
+    (grad, gs), (q, qs), (k, ks), (v, vs), (out, os) = map(_operand, given[:5])
+    lse = lse.contiguous()
+    grad_lse = grad_lse.contiguous() if grad_lse is not None else None
+    used = (grad, q, k, v, out, lse, grad_lse)
+    call = _call_plan(q, k, (qs, ks, vs, gs, os), grad_lse, scale, causal, plan)
+    if plan is None and calls.same(given, used):
+        _TABLE.keep(given, (number, causal), call)
+    return call.run(used)
 
 
 def as_attention_grad_op(scale: float | None = None, causal: bool = True, lib: str = "neptune"):

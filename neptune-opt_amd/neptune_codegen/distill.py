@@ -21,12 +21,12 @@ import threading
 from neptune_codegen import calls, hip
 from neptune_codegen.emitters import (BASE_OPTIONS, DistillVariant, distill_kernel_name,
                                       emit_distill_source)
-from neptune_codegen.template import _row_last_layout, _validate_row_last
+from neptune_codegen.template import _validate_row_last
 
 MAX_ENTRIES = 1024
 _PROGRAMS: dict = {}
 _OPS: dict = {}
-_SEEN = calls.Seen()
+_FORWARD, _BACKWARD = calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _FORWARD_ARGS = (hip.PTR,) * 5 + (hip.I64,) * 5 + (hip.I32,) + (hip.F32,) * 3
@@ -84,12 +84,12 @@ def _check_rows(t, name, shape, logits, *, metadata):
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _variant(z, top, index, rows: int, n: int, count: int) -> DistillVariant:
+def _variant(z, stride: int, top, index, rows: int, n: int, count: int) -> DistillVariant:
     """Lanes per row: a wavefront up to 512 slots of 16 bytes, a workgroup of 256 lanes beyond; 1024
     where the rows leave most CUs idle otherwise."""
     vec = 16 // z.element_size()
     slots = -(-n // vec)
-    aligned = n % vec == 0 and z.data_ptr() % 16 == 0 and (z.stride(0) * z.element_size()) % 16 == 0
+    aligned = n % vec == 0 and z.data_ptr() % 16 == 0 and stride % vec == 0
     tpr = 64 if slots <= 512 and count <= 256 else 256
     if rows <= 512 and slots > 1024:
         tpr = 1024
@@ -103,45 +103,14 @@ def _variant(z, top, index, rows: int, n: int, count: int) -> DistillVariant:
     return DistillVariant(name(z), name(top), name(index), not aligned, tpr, unroll, entries)
 
 
-def _rows_of(t):
-    """[rows, columns] of unit column stride."""
-    flat, rows, cols = _row_last_layout(t)
-    if flat.stride(1) != 1 and cols > 1:
-        flat = flat.contiguous()
-    return flat, rows, cols
-
-
-class _Call:
-    __slots__ = ("kernel", "grid", "rest", "device", "lead", "copied")
-
-    def __init__(self, stage, logits, top, index, temperature, grad_stride=None):
-        self.lead = logits.shape[:-1]
-        z, rows, n = _rows_of(logits)
-        t, _, count = _rows_of(top)
-        i, _, _ = _rows_of(index)
-        self.copied = [a if a.data_ptr() != b.data_ptr() else None
-                       for a, b in ((z, logits), (t, top), (i, index))]
-        var = _variant(z, t, i, rows, n, count)
-        self.device = calls.device_index(logits)
-        self.kernel = _program(stage, var).kernel(
-            distill_kernel_name(stage, var), _FORWARD_ARGS if stage == "forward" else _BACKWARD_ARGS,
-            var.wg, self.device)
-        groups = -(-rows // var.rows)
-        calls.check_grid(groups, var.wg, "distillation")
-        self.grid = (groups,)
-        c = math.log2(math.e) / temperature
-        strides = (z.stride(0), t.stride(0), i.stride(0))
-        if stage == "forward":
-            self.rest = (rows, n) + strides + (count, c, 1.0 / temperature, temperature * temperature)
-        else:
-            self.rest = (rows, n, grad_stride) + strides + (count, c, temperature)
-
-    def operands(self, *given):
-        return [(c if c is not None else g).data_ptr() for c, g in zip(self.copied, given)]
-
-    @property
-    def reusable(self) -> bool:
-        return all(c is None for c in self.copied)
+def _launch(stage, z, top, index, strides, args, ends):
+    """(kernel, grid, arguments) of a stage; `args` are its pointers, `ends` what follows the strides."""
+    rows, n, count = z.numel() // z.shape[-1], z.shape[-1], top.shape[-1]
+    var = _variant(z, strides[-3], top, index, rows, n, count)
+    kernel = _program(stage, var).kernel(distill_kernel_name(stage, var),
+                                         _FORWARD_ARGS if stage == "forward" else _BACKWARD_ARGS,
+                                         var.wg, calls.device_index(z))
+    return kernel, (-(-rows // var.rows),), args + (rows, n) + strides + (count,) + ends
 
 
 def run_distill(logits, top_logits, top_index, *, temperature: float = 1.0, return_stats: bool = False):
@@ -150,31 +119,26 @@ def run_distill(logits, top_logits, top_index, *, temperature: float = 1.0, retu
     and temperature were seen before reuses that call's kernel and launch shape."""
     import torch
 
-    key = calls.tensors_key(logits, top_logits, top_index)
-    call = None
-    if key is not None and type(temperature) in (int, float):
-        key += ("forward", temperature)
-        call = _SEEN.get(key)
-    else:
-        key = None
-    if call is None:
-        metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
-        lead = validate_distill_inputs(logits, top_logits, top_index, metadata=metadata)
-        temperature = _temperature(temperature)
-        if not metadata and logits.numel() != 0:
-            call = _Call("forward", logits, top_logits, top_index, temperature)
-            if key is not None and call.reusable:
-                _SEEN.keep(key, call)
-    else:
-        lead = call.lead
-    loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
-    stats = torch.empty((*lead, 2), dtype=torch.float32, device=logits.device) if return_stats else None
-    if call is not None:
-        with calls.on_device(call.device):
-            call.kernel.launch(call.grid, (*call.operands(logits, top_logits, top_index), loss.data_ptr(),
-                                           0 if stats is None else stats.data_ptr()) + call.rest,
-                               hip.current_stream(call.device))
-    return (loss, stats) if return_stats else loss
+    given, return_stats = (logits, top_logits, top_index), bool(return_stats)
+    found = _FORWARD.run(given, (temperature, return_stats))
+    if found is not None:
+        return found
+    metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
+    lead = validate_distill_inputs(*given, metadata=metadata)
+    number, temperature = temperature, _temperature(temperature)
+    outputs = [(lead, torch.float32)] + ([((*lead, 2), torch.float32)] if return_stats else [])
+    if metadata or logits.numel() == 0:
+        made = tuple(torch.empty(shape, dtype=dtype, device=logits.device) for shape, dtype in outputs)
+        return made if return_stats else made[0]
+    (z, sz), (t, st), (i, si) = map(calls.rows_of, given)
+    stats = calls.buffer(1) if return_stats else 0
+    launch = _launch("forward", z, t, i, (sz, st, si),
+                     (calls.tensor(0), calls.tensor(1), calls.tensor(2), calls.buffer(0), stats),
+                     (math.log2(math.e) / temperature, 1.0 / temperature, temperature * temperature))
+    plan = calls.Plan(calls.device_index(z), 3, outputs, range(len(outputs)), [launch], bare=not return_stats)
+    if calls.same(given, (z, t, i)):
+        _FORWARD.keep(given, (number, return_stats), plan)
+    return plan.run((z, t, i))
 
 
 def run_distill_backward(grad, logits, top_logits, top_index, stats, *, temperature: float = 1.0):
@@ -182,34 +146,28 @@ def run_distill_backward(grad, logits, top_logits, top_index, stats, *, temperat
     the state that run_distill returned; fresh and contiguous."""
     import torch
 
-    key = calls.tensors_key(grad, logits, top_logits, top_index, stats)
-    call = None
-    if key is not None and type(temperature) in (int, float):
-        key += ("backward", temperature)
-        call = _SEEN.get(key)
-    else:
-        key = None
-    if call is None:
-        metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
-        lead = validate_distill_inputs(logits, top_logits, top_index, metadata=metadata)
-        _check_rows(grad, "grad", lead, logits, metadata=metadata)
-        _check_rows(stats, "stats", (*lead, 2), logits, metadata=metadata)
-        temperature = _temperature(temperature)
-        if metadata or logits.numel() == 0:
-            return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        plain = stats.is_contiguous()
-        stats = stats.contiguous()
-        flat = grad.reshape(-1)           # a view where the rows have one stride (a mean's is 0)
-        call = _Call("backward", logits, top_logits, top_index, temperature, flat.stride(0))
-        if key is not None and call.reusable and plain and flat.data_ptr() == grad.data_ptr():
-            _SEEN.keep(key, call)
-        grad = flat
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    with calls.on_device(call.device):
-        call.kernel.launch(call.grid, (grad.data_ptr(), *call.operands(logits, top_logits, top_index),
-                                       stats.data_ptr(), out.data_ptr()) + call.rest,
-                           hip.current_stream(call.device))
-    return out
+    given = (grad, logits, top_logits, top_index, stats)
+    found = _BACKWARD.run(given, (temperature,))
+    if found is not None:
+        return found
+    metadata = isinstance(logits, torch.Tensor) and calls.is_metadata(logits)
+    lead = validate_distill_inputs(logits, top_logits, top_index, metadata=metadata)
+    _check_rows(grad, "grad", lead, logits, metadata=metadata)
+    _check_rows(stats, "stats", (*lead, 2), logits, metadata=metadata)
+    number, temperature = temperature, _temperature(temperature)
+    if metadata or logits.numel() == 0:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    (z, sz), (t, st), (i, si) = map(calls.rows_of, given[1:4])
+    # the rows' gradients have one stride where that can be (a mean's is 0)
+    g, sg = calls.rows_of(grad.unsqueeze(-1))
+    used = (grad if g.data_ptr() == grad.data_ptr() else g, z, t, i, stats.contiguous())
+    launch = _launch("backward", z, t, i, (sg, sz, st, si),
+                     (calls.tensor(0), calls.tensor(1), calls.tensor(2), calls.tensor(3), calls.tensor(4),
+                      calls.buffer(0)), (math.log2(math.e) / temperature, temperature))
+    plan = calls.Plan(calls.device_index(z), 5, [(logits.shape, logits.dtype)], (0,), [launch], bare=True)
+    if calls.same(given, used):
+        _BACKWARD.keep(given, (number,), plan)
+    return plan.run(used)
 
 
 def as_distill_op(temperature: float = 1.0, lib: str = "neptune"):

@@ -24,13 +24,13 @@ import threading
 from neptune_codegen import calls, hip
 from neptune_codegen.emitters import (BASE_OPTIONS, ResidualNormVariant, emit_residual_norm_source,
                                       residual_norm_kernel_name)
-from neptune_codegen.template import _row_last_layout, _validate_row_last
+from neptune_codegen.template import _validate_row_last
 
 MAX_WIDTH = 16384
 CUS = 256
 _PROGRAMS: dict = {}
 _OPS: dict = {}
-_SEEN = calls.Seen()
+_FORWARD, _BACKWARD = calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _FORWARD_ARGS = (hip.PTR,) * 8 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,) * 2
@@ -107,20 +107,9 @@ def _eps(eps) -> float:
     return float(eps)
 
 
-def _rows_of(t):
-    """[rows, columns] of unit column stride."""
-    flat, _, cols = _row_last_layout(t)
-    if cols > 1 and flat.stride(1) != 1:
-        flat = flat.contiguous()
-    return flat
-
-
-def _variant(tensors, rows, n, after, gate_kind, backward) -> ResidualNormVariant:
+def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, backward: bool) -> ResidualNormVariant:
     """Lanes and slots of a row."""
-    size = tensors[0].element_size()
-    vec = 16 // size
-    aligned = n % vec == 0 and all(t.data_ptr() % 16 == 0 and (t.ndim == 1 or t.stride(0) * size % 16 == 0)
-                                   for t in tensors)
+    vec = 16 // x.element_size()
     slots = -(-n // vec)
     nv = 1
     if not backward and slots >= 256 and rows >= 4 * CUS:
@@ -129,41 +118,22 @@ def _variant(tensors, rows, n, after, gate_kind, backward) -> ResidualNormVarian
     while tpr > 1024:
         tpr, nv = tpr // 2, nv * 2
     wg = max(512 if backward else 256, tpr)
-    return ResidualNormVariant(str(tensors[0].dtype).replace("torch.", ""), not aligned, tpr, nv, wg, after,
-                               gate_kind)
+    return ResidualNormVariant(str(x.dtype).replace("torch.", ""), not aligned, tpr, nv, wg, after, gate_kind)
+
+
+def _operands(rows, vectors, n):
+    """(tensors, row strides, whether every row is whole 16-byte words): `rows` [..., n] as they are or as
+    contiguous copies, `vectors` contiguous."""
+    made = [(None, 0) if t is None else calls.rows_of(t) for t in rows]
+    used = [t for t, _ in made] + [None if t is None else t.contiguous() for t in vectors]
+    vec = 16 // used[-2].element_size()
+    aligned = (n % vec == 0 and all(s % vec == 0 for _, s in made)
+               and all(t is None or t.data_ptr() % 16 == 0 for t in used))
+    return tuple(used), tuple(s for _, s in made), aligned
 
 
 def _gate_kind(groups, group) -> str:
     return "none" if not groups else "rows" if group == 1 else "group"
-
-
-class _Forward:
-    __slots__ = ("kernel", "grid", "rest", "device", "shape", "copied")
-
-    def __init__(self, x, y, after, before, gate, groups, group, scale, eps):
-        self.shape = x.shape
-        given = (x, y, after, before, gate)
-        flat = [_rows_of(x), _rows_of(y)] + [t.contiguous() if t is not None else None for t in given[2:]]
-        self.copied = [f if f is not None and f.data_ptr() != t.data_ptr() else None for f, t in zip(flat, given)]
-        fx, fy = flat[:2]
-        rows, n = fx.shape
-        var = _variant([t for t in flat if t is not None], rows, n, after is not None,
-                       _gate_kind(groups, group), False)
-        self.device = calls.device_index(x)
-        self.kernel = _program("forward", var).kernel(residual_norm_kernel_name("forward", var), _FORWARD_ARGS,
-                                                      var.wg, self.device)
-        self.grid = (-(-rows // (var.wg // var.tpr)),)
-        calls.check_grid(self.grid[0], var.wg, "residual norm")
-        self.rest = (rows, n, fx.stride(0), fy.stride(0), max(group, 1), scale, eps)
-
-    def run(self, x, y, after, before, gate, residual, normed, stats):
-        x, y, after, before, gate = (
-            0 if t is None else (c if c is not None else t).data_ptr()
-            for c, t in zip(self.copied, (x, y, after, before, gate)))
-        with calls.on_device(self.device):
-            self.kernel.launch(self.grid, (x, y, gate, after, before, residual.data_ptr(), normed.data_ptr(),
-                                           0 if stats is None else stats.data_ptr()) + self.rest,
-                               hip.current_stream(self.device))
 
 
 def run_residual_norm(x, y, gamma_after, gamma_before, *, gate=None, residual_scale: float = 1.0,
@@ -174,27 +144,30 @@ def run_residual_norm(x, y, gamma_after, gamma_before, *, gate=None, residual_sc
     that call's kernel and launch shape."""
     import torch
 
-    key = calls.tensors_key(x, y, gamma_after, gamma_before, gate)
-    call = None
-    if key is not None and type(residual_scale) in (int, float) and type(eps) in (int, float):
-        key += ("forward", residual_scale, eps)
-        call = _SEEN.get(key)
-    else:
-        key = None
-    if call is None:
-        metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
-        groups, group = validate_residual_norm_inputs(x, y, gamma_after, gamma_before, gate, metadata=metadata)
-        scale, eps = _scale(residual_scale), _eps(eps)
-        if not metadata and x.numel() != 0:
-            call = _Forward(x, y, gamma_after, gamma_before, gate, groups, group, scale, eps)
-            if key is not None and all(c is None for c in call.copied):
-                _SEEN.keep(key, call)
-    residual = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=x.device) if return_stats else None
-    if call is not None:
-        call.run(x, y, gamma_after, gamma_before, gate, residual, normed, stats)
-    return (residual, normed, stats) if return_stats else (residual, normed)
+    given, return_stats = (x, y, gamma_after, gamma_before, gate), bool(return_stats)
+    found = _FORWARD.run(given, (residual_scale, eps, return_stats))
+    if found is not None:
+        return found
+    metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
+    groups, group = validate_residual_norm_inputs(*given, metadata=metadata)
+    numbers, scale, eps = (residual_scale, eps, return_stats), _scale(residual_scale), _eps(eps)
+    outputs = [(x.shape, x.dtype)] * 2 + ([((*x.shape[:-1], 2), torch.float32)] if return_stats else [])
+    if metadata or x.numel() == 0:
+        return tuple(torch.empty(shape, dtype=dtype, device=x.device) for shape, dtype in outputs)
+    n = x.shape[-1]
+    rows = x.numel() // n
+    used, strides, aligned = _operands((x, y), (gamma_after, gamma_before, gate), n)
+    var = _variant(x, aligned, rows, n, gamma_after is not None, _gate_kind(groups, group), False)
+    device = calls.device_index(x)
+    kernel = _program("forward", var).kernel(residual_norm_kernel_name("forward", var), _FORWARD_ARGS, var.wg, device)
+    tx, ty, after, before, tgate = map(calls.tensor, range(5))
+    launch = (kernel, (-(-rows // (var.wg // var.tpr)),),
+              (tx, ty, tgate, after, before, calls.buffer(0), calls.buffer(1),
+               calls.buffer(2) if return_stats else 0, rows, n) + strides + (max(group, 1), scale, eps))
+    plan = calls.Plan(device, 5, outputs, range(len(outputs)), [launch])
+    if calls.same(given, used):
+        _FORWARD.keep(given, numbers, plan)
+    return plan.run(used)
 
 
 def _chunks(rows, groups, group, gate_kind, rpw):
@@ -211,47 +184,6 @@ def _chunks(rows, groups, group, gate_kind, rpw):
     return groups * per_group, chunk, per_group
 
 
-class _Backward:
-    __slots__ = ("kernel", "join", "grid", "join_grid", "rest", "tail", "device", "floats", "copied", "shapes")
-
-    def __init__(self, dres, dnormed, x, y, after, before, gate, groups, group, scale):
-        given = (dres, dnormed, x, y, after, before, gate)
-        flat = [None if t is None else _rows_of(t) for t in given[:4]]
-        flat += [None if t is None else t.contiguous() for t in given[4:]]
-        self.copied = [f if f is not None and f.data_ptr() != t.data_ptr() else None for f, t in zip(flat, given)]
-        rows, n = flat[2].shape
-        kind = _gate_kind(groups, group)
-        var = _variant([t for t in flat if t is not None], rows, n, after is not None, kind, True)
-        self.device = calls.device_index(x)
-        prog = _program("backward", var)
-        self.kernel = prog.kernel(residual_norm_kernel_name("backward", var), _BACKWARD_ARGS, var.wg, self.device)
-        self.join = prog.kernel(residual_norm_kernel_name("join", var), _JOIN_ARGS, 256, self.device)
-        chunks, chunk, per_group = _chunks(rows, groups, group, kind, var.wg // var.tpr)
-        split_gate = kind == "group" and per_group > 1
-        self.grid = (chunks,)
-        self.join_grid = (-(-n // 32), 2 + (groups if split_gate else 0)) if chunks > 1 else None
-        self.floats = (2 + split_gate) * chunks * n if chunks > 1 else 0
-        strides = tuple(0 if t is None else t.stride(0) for t in flat[:4])
-        self.rest = (rows, n) + strides + (group if kind == "group" else rows, chunk, per_group, scale)
-        self.tail = (n, chunks, per_group)
-
-    def run(self, given, stats, dx, dy, dgate, dafter, dbefore):
-        import torch
-
-        dres, dnormed, x, y, after, before, gate = (
-            0 if t is None else (c if c is not None else t).data_ptr() for c, t in zip(self.copied, given))
-        pointer = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-        work = torch.empty(self.floats, dtype=torch.float32, device=dx.device) if self.floats else None
-        with calls.on_device(self.device):
-            stream = hip.current_stream(self.device)
-            self.kernel.launch(self.grid, (dres, dnormed, x, y, gate, after, before, stats.data_ptr(),
-                                           dx.data_ptr(), dy.data_ptr(), pointer(dgate), pointer(dafter),
-                                           dbefore.data_ptr(), pointer(work)) + self.rest, stream)
-            if self.join_grid is not None:
-                self.join.launch(self.join_grid, (work.data_ptr(), pointer(dafter), dbefore.data_ptr(),
-                                                  pointer(dgate)) + self.tail, stream)
-
-
 def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, gamma_before, stats, *,
                                gate=None, residual_scale: float = 1.0):
     """(dx, dy, dgamma_after, dgamma_before, dgate) of run_residual_norm's call with these x, y, gammas and
@@ -259,40 +191,56 @@ def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, ga
     be None (a residual that nothing else reads).  Gradients have their operand's shape and dtype."""
     import torch
 
-    given = (grad_residual, grad_normed, x, y, gamma_after, gamma_before, gate)
-    key = calls.tensors_key(*given, stats)
-    call = None
-    if key is not None and type(residual_scale) in (int, float):
-        key += ("backward", residual_scale)
-        call = _SEEN.get(key)
-    else:
-        key = None
-    metadata = False
-    if call is None:
-        metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
-        groups, group = validate_residual_norm_inputs(x, y, gamma_after, gamma_before, gate, metadata=metadata)
-        for t, name in ((grad_normed, "grad_normed"), (grad_residual, "grad_residual")):
-            if t is None and name == "grad_residual":
-                continue
-            calls.check_tensor(t, f"residual norm {name}", metadata=metadata)
-            if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
-                raise ValueError(f"residual norm {name} must have x's shape, dtype and device")
-        calls.check_tensor(stats, "residual norm stats", metadata=metadata)
-        if stats.shape != (*x.shape[:-1], 2) or stats.dtype != torch.float32 or stats.device != x.device:
-            raise ValueError(f"residual norm stats must be float32 {(*x.shape[:-1], 2)} on x's device")
-        scale = _scale(residual_scale)
-    make = torch.zeros if x.numel() == 0 else torch.empty
-    dx, dy, dafter, dbefore, dgate = (
-        None if t is None else make(t.shape, dtype=t.dtype, device=t.device)
-        for t in (x, y, gamma_after, gamma_before, gate))
-    if call is None and not metadata and x.numel() != 0:
-        call = _Backward(*given, groups, group, scale)
-        if key is not None and all(c is None for c in call.copied) and stats.is_contiguous():
-            _SEEN.keep(key, call)
-        stats = stats.contiguous()
-    if call is not None:
-        call.run(given, stats, dx, dy, dgate, dafter, dbefore)
-    return dx, dy, dafter, dbefore, dgate
+    given = (grad_residual, grad_normed, x, y, gamma_after, gamma_before, gate, stats)
+    found = _BACKWARD.run(given, (residual_scale,))
+    if found is not None:
+        return found
+    metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
+    groups, group = validate_residual_norm_inputs(x, y, gamma_after, gamma_before, gate, metadata=metadata)
+    for t, name in ((grad_normed, "grad_normed"), (grad_residual, "grad_residual")):
+        if t is None and name == "grad_residual":
+            continue
+        calls.check_tensor(t, f"residual norm {name}", metadata=metadata)
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"residual norm {name} must have x's shape, dtype and device")
+    calls.check_tensor(stats, "residual norm stats", metadata=metadata)
+    if stats.shape != (*x.shape[:-1], 2) or stats.dtype != torch.float32 or stats.device != x.device:
+        raise ValueError(f"residual norm stats must be float32 {(*x.shape[:-1], 2)} on x's device")
+    scale = _scale(residual_scale)
+    wanted = (x, y, gamma_after, gamma_before, gate)
+    if metadata or x.numel() == 0:
+        return tuple(None if t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in wanted)
+    n = x.shape[-1]
+    rows = x.numel() // n
+    used, strides, aligned = _operands((grad_residual, grad_normed, x, y), (gamma_after, gamma_before, gate), n)
+    used += (stats.contiguous(),)
+    kind = _gate_kind(groups, group)
+    var = _variant(x, aligned, rows, n, gamma_after is not None, kind, True)
+    device, prog = calls.device_index(x), _program("backward", var)
+    chunks, chunk, per_group = _chunks(rows, groups, group, kind, var.wg // var.tpr)
+    split_gate = kind == "group" and per_group > 1
+    buffers, returns = [], []
+    for t in wanted:
+        returns.append(None if t is None else len(buffers))
+        if t is not None:
+            buffers.append((t.shape, t.dtype))
+    dx, dy, dafter, dbefore, dgate = (0 if r is None else calls.buffer(r) for r in returns)
+    work = 0
+    if chunks > 1:
+        work = calls.buffer(len(buffers))
+        buffers.append((((2 + split_gate) * chunks * n,), torch.float32))
+    dres, dnormed, tx, ty, after, before, tgate, tstats = map(calls.tensor, range(8))
+    launches = [(prog.kernel(residual_norm_kernel_name("backward", var), _BACKWARD_ARGS, var.wg, device), (chunks,),
+                 (dres, dnormed, tx, ty, tgate, after, before, tstats, dx, dy, dgate, dafter, dbefore, work, rows, n)
+                 + strides + (group if kind == "group" else rows, chunk, per_group, scale))]
+    if chunks > 1:
+        launches.append((prog.kernel(residual_norm_kernel_name("join", var), _JOIN_ARGS, 256, device),
+                         (-(-n // 32), 2 + (groups if split_gate else 0)),
+                         (work, dafter, dbefore, dgate, n, chunks, per_group)))
+    plan = calls.Plan(device, 8, buffers, returns, launches)
+    if calls.same(given, used):
+        _BACKWARD.keep(given, (residual_scale,), plan)
+    return plan.run(used)
 
 
 def as_residual_norm_op(residual_scale: float = 1.0, eps: float = 1e-6, lib: str = "neptune"):

@@ -21,7 +21,7 @@ from neptune_codegen.emitters import BASE_OPTIONS, emit_rotary_source, rotary_ke
 
 _PROGRAMS: dict = {}
 _OPS: dict = {}
-_SEEN = calls.Seen()
+_TABLE = calls.Table()
 _lock = threading.Lock()
 _ARGS = (hip.PTR,) * 6 + (hip.I32,) * 9 + (hip.I64,) * 8 + (hip.F32,) * 2
 
@@ -105,7 +105,7 @@ def validate_rotary_inputs(q, k, positions, turns, *, metadata: bool = False) ->
         raise ValueError(f"rotary turns of {turns.shape[0]} pairs do not fit heads of {q.shape[3]} elements")
 
 
-def _plan(tokens, slots, heads):
+def _heads_per_lane(tokens, slots, heads):
     """Heads per lane: as many as leave 2^18 lanes (four wavefronts for each SIMD of 256 CUs), up to 8.
     More heads share a lane's angles; few tokens need the lanes."""
     per = 8
@@ -114,74 +114,46 @@ def _plan(tokens, slots, heads):
     return per
 
 
-class _Call:
-    __slots__ = ("kernel", "grid", "rest", "device", "copied")
-
-    def __init__(self, q, k, positions, turns, interleaved, sign, magnitude):
-        import torch
-
-        given = (q, k, positions, turns)
-        flat = [t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k)]
-        flat += [positions, turns.contiguous()]
-        self.copied = [a if a is not None and a.data_ptr() != b.data_ptr() else None for a, b in zip(flat, given)]
-        q, k, positions, turns = flat
-        batch, heads_q, seq, dim = q.shape
-        heads_k = k.shape[1] if k is not None else 0
-        part, vec = 2 * turns.shape[0], 16 // q.element_size()
-        run = part if interleaved else part // 2
-        any_rows = bool(dim % vec or run % vec or (dim - part) % vec
-                        or any(t is not None and (t.data_ptr() % 16 or any(s % vec for s in t.stride()[:3]))
-                               for t in (q, k)))
-        turned, rest = -(-run // vec), -(-(dim - part) // vec)
-        slots, heads = turned + rest, heads_q + heads_k
-        tokens = batch * seq
-        per = _plan(tokens, slots, heads)
-        self.device = calls.device_index(q)
-        index = "int32" if positions.dtype == torch.int32 else "int64"
-        name = rotary_kernel_name(q.dtype, index, interleaved, any_rows)
-        self.kernel = _program(q.dtype, index, interleaved, any_rows).kernel(name, _ARGS, 256, self.device)
-        self.grid = (-(-tokens * slots // 256), -(-heads // per))
-        calls.check_grid(self.grid[0], 256, "rotary")
-        if self.grid[1] > 65535 or tokens >= 1 << 31:
-            raise NotImplementedError("rotary: too many heads or tokens for one launch")
-        psb = positions.stride(0) if positions.ndim == 2 else 0
-        self.rest = (tokens, seq, dim, part, slots, turned, heads_q, heads_k, per, *q.stride()[:3],
-                     *(k.stride()[:3] if k is not None else (0, 0, 0)), psb, positions.stride(-1), sign, magnitude)
-
-    def run(self, q, k, positions, turns, qo, ko):
-        q, k, positions, turns = (0 if t is None else (c if c is not None else t).data_ptr()
-                                  for c, t in zip(self.copied, (q, k, positions, turns)))
-        with calls.on_device(self.device):
-            self.kernel.launch(self.grid, (q, k, positions, turns, qo.data_ptr(),
-                                           0 if ko is None else ko.data_ptr()) + self.rest,
-                               hip.current_stream(self.device))
-
-
 def _run(q, k, positions, turns, magnitude, interleaved, sign):
     import torch
 
-    key = calls.tensors_key(q, k, positions, turns)
-    call = None
-    if key is not None and type(magnitude) in (int, float):
-        key += (magnitude, bool(interleaved), sign)
-        call = _SEEN.get(key)
-    else:
-        key = None
-    metadata = False
-    if call is None:
-        metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
-        validate_rotary_inputs(q, k, positions, turns, metadata=metadata)
-        if type(magnitude) not in (int, float) or not math.isfinite(magnitude):
-            raise ValueError("rotary magnitude must be a finite number")
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
-    if call is None and not metadata and (q.numel() or (k is not None and k.numel())):
-        call = _Call(q, k, positions, turns, bool(interleaved), sign, float(magnitude))
-        if key is not None and all(c is None for c in call.copied):
-            _SEEN.keep(key, call)
-    if call is not None:
-        call.run(q, k, positions, turns, qo, ko)
-    return qo, ko
+    given, interleaved = (q, k, positions, turns), bool(interleaved)
+    found = _TABLE.run(given, (magnitude, interleaved, sign))
+    if found is not None:
+        return found
+    metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
+    validate_rotary_inputs(*given, metadata=metadata)
+    if type(magnitude) not in (int, float) or not math.isfinite(magnitude):
+        raise ValueError("rotary magnitude must be a finite number")
+    if metadata or not (q.numel() or (k is not None and k.numel())):
+        return tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    used = tuple(t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k))
+    used += (positions, turns.contiguous())
+    (batch, heads_q, seq, dim), heads_k = q.shape, k.shape[1] if k is not None else 0
+    part, vec = 2 * turns.shape[0], 16 // q.element_size()
+    run = part if interleaved else part // 2
+    any_rows = bool(dim % vec or run % vec or (dim - part) % vec
+                    or any(t is not None and (t.data_ptr() % 16 or any(s % vec for s in t.stride()[:3]))
+                           for t in used[:2]))
+    turned, rest = -(-run // vec), -(-(dim - part) // vec)
+    slots, heads, tokens = turned + rest, heads_q + heads_k, batch * seq
+    if tokens >= 1 << 31:
+        raise NotImplementedError("rotary takes less than 2^31 tokens")
+    per = _heads_per_lane(tokens, slots, heads)
+    device, index = calls.device_index(q), "int32" if positions.dtype == torch.int32 else "int64"
+    kernel = _program(q.dtype, index, interleaved, any_rows).kernel(
+        rotary_kernel_name(q.dtype, index, interleaved, any_rows), _ARGS, 256, device)
+    strides = used[0].stride()[:3] + (used[1].stride()[:3] if k is not None else (0, 0, 0))
+    strides += (positions.stride(0) if positions.ndim == 2 else 0, positions.stride(-1))
+    out = [calls.buffer(0), 0 if k is None else calls.buffer(1)]
+    launch = (kernel, (-(-tokens * slots // 256), -(-heads // per)),
+              (*map(calls.tensor, range(4)), *out, tokens, seq, dim, part, slots, turned, heads_q, heads_k, per)
+              + strides + (sign, float(magnitude)))
+    plan = calls.Plan(device, 4, [(t.shape, t.dtype) for t in (q, k) if t is not None],
+                      (0, None if k is None else 1), [launch])
+    if calls.same(given, used):
+        _TABLE.keep(given, (magnitude, interleaved, sign), plan)
+    return plan.run(used)
 
 
 def run_rotary(q, k, positions, turns, *, magnitude: float = 1.0, interleaved: bool = False):

@@ -86,7 +86,7 @@ def test_rows_fit_the_lanes():
         for dtype in (torch.float32, torch.bfloat16):
             for backward in (False, True):
                 for rows in (1, 100000):
-                    var = RN._variant([meta(rows, n, dtype=dtype)], rows, n, True, "group", backward)
+                    var = RN._variant(meta(rows, n, dtype=dtype), n % 8 == 0, rows, n, True, "group", backward)
                     vec = 16 // meta(1, dtype=dtype).element_size()
                     assert var.tpr * var.nv * vec >= n and var.tpr <= var.wg <= 1024
                     # the column sums' LDS
