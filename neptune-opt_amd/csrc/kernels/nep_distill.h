@@ -120,7 +120,7 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
   constexpr int VEC = St::kVec, STEP = TPR * VEC;
   __shared__ float lds[R::kWaves];
   const int t = threadIdx.x % TPR;
-  const i64 row = (i64)blockIdx.x * (WG / TPR) + threadIdx.x / TPR;
+  const i64 row = (i64)blockIdx.x * (WG / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const bool live = row < rows;
   const typename St::T* rp = z + (live ? row : 0) * stride_z;
   TeacherList<Lt, Ix, TPR, EPL> list;
@@ -226,7 +226,7 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   __shared__ u32 seen[RPW][HASH / 32];
   __shared__ float list_p[RPW][TPR * EPL];
   __shared__ int list_at[RPW][TPR * EPL];
-  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR, slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const i64 row = (i64)blockIdx.x * RPW + slot;
   const bool live = row < rows;
   const typename St::T* rp = z + (live ? row : 0) * stride_z;

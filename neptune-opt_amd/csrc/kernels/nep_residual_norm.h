@@ -17,48 +17,123 @@
 // 32 bits.
 //
 // HBM-bound: the forward pass reads x and y and writes r and h, the gradient reads x, y, dr and dh and
-// writes dx and dy, once each; rows stay in registers as packed words.
+// writes dx and dy, once each; rows stay in registers as packed words.  Forward bf16 16384 x 4096 91-95 us
+// (5.7-5.9 TB/s; one slot a lane, two and four within 4%), 65536 x 256 24 us; gradient 143-146 us, fp32
+// 8192 x 4096 138, bf16 16384 x 8192 280; 16384 columns 180-250 us per 0.8 GB, where registers run out.
 #pragma once
 
 namespace nep {
 
+typedef float f32x4n __attribute__((ext_vector_type(4)));
+
 constexpr int kGateNone = 0, kGateRows = 1, kGateGroup = 2;   // a gate row per row, or per group of rows
 
+// How rows are read: whole 16-byte words; any alignment and width from one word up; fewer columns than a
+// word holds, one by one.
+constexpr int kWords = 0, kAnyRows = 1, kFewColumns = 2;
+constexpr u32 kBufferWord3 = 0x00020000u;          // gfx9 raw buffer descriptor, dword 3
+constexpr u32 kNowhere = 0x80000000u;              // past every buffer: reads as zero, is not written
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, 0x7fffffff, (int)kBufferWord3);
+}
+
 // A row of up to TPR * NV * VEC columns: slot u of lane t holds the columns from (u TPR + t) VEC.
-// ANY: rows of any alignment and width (a slot over the end is taken element by element).
-template <class St, int TPR, int NV, bool ANY>
+//  * kWords: buffer accesses, lanes and rows past the end at an offset past the buffer, so that no
+//    access is in a branch: the waits for loads in flight then count the accesses behind them exactly.
+//    (In branches each wait is for everything in flight, the next row's loads among it.)
+//  * kAnyRows: a slot over the end is loaded from the row's last VEC columns and shifted when it is used
+//    (its columns one by one would be waited for in front of the row's arithmetic).
+template <class St, int TPR, int NV, int ACCESS>
 struct NormRow {
   typedef typename St::T T;
   static constexpr int VEC = St::kVec;
   static constexpr int COLS = TPR * NV * VEC;
   __device__ static __forceinline__ int at(int u, int t) { return (u * TPR + t) * VEC; }
-  __device__ static __forceinline__ u32x4 edge(const T* p, int e, int n) {
-    float v[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = e + j < n ? St::load(p + e + j) : 0.0f;
-    return St::pack(v);
-  }
-  // columns past n read as zero
+  // Words of the row `local` rows behind row0 (the wavefront's first); to be settled.
   template <bool STREAM>
-  __device__ static __forceinline__ void load(u32x4* w, const T* p, int n, int t, bool live) {
+  __device__ static __forceinline__ void load(u32x4* w, const T* p, i64 row0, i64 stride, int local, bool live,
+                                              int n, int t) {
+    if constexpr (ACCESS == kWords) {
+      const __amdgpu_buffer_rsrc_t r = buffer_at(p + row0 * stride);
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int e = at(u, t);
+        const u32 off = live && e < n ? (u32)(local * (int)stride + e) * (u32)sizeof(T) : kNowhere;
+        w[u] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, STREAM ? 2 : 0);
+      }
+    } else if constexpr (ACCESS == kAnyRows) {
+      const T* q = p + row0 * stride + (live ? (i64)local * stride : 0);
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int e = at(u, t);
+        w[u] = load16_any(q + (e + VEC <= n ? e : n - VEC));
+      }
+    } else {
+      const T* q = p + row0 * stride + (live ? (i64)local * stride : 0);
+      float v[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = j < n && t == 0 ? St::load(q + j) : 0.0f;
+      w[0] = St::pack(v);
+    }
+  }
+  // columns past n, and rows that are none, become zero
+  __device__ static __forceinline__ void settle(u32x4* w, int n, int t, bool live) {
+    if constexpr (ACCESS == kWords) return;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int e = at(u, t);
-      w[u] = u32x4{0u, 0u, 0u, 0u};
-      if (!live) continue;
-      if (e + VEC <= n) w[u] = ANY ? load16_any(p + e) : STREAM ? load16(p + e) : load16_cached(p + e);
-      else if (ANY && e < n) w[u] = edge(p, e, n);
+      const int over = ACCESS == kAnyRows ? at(u, t) + VEC - n : 0;
+      if (!live || over >= VEC) {
+        w[u] = u32x4{0u, 0u, 0u, 0u};
+      } else if (over > 0) {
+        u32x4 x = w[u];
+        if constexpr (VEC == 8) {
+          if (over & 4) x = u32x4{x.z, x.w, 0u, 0u};
+          if (over & 2) x = u32x4{x.y, x.z, x.w, 0u};
+          if (over & 1)
+            x = u32x4{__builtin_amdgcn_alignbit(x.y, x.x, 16), __builtin_amdgcn_alignbit(x.z, x.y, 16),
+                      __builtin_amdgcn_alignbit(x.w, x.z, 16), x.w >> 16};
+        } else {
+          if (over & 2) x = u32x4{x.z, x.w, 0u, 0u};
+          if (over & 1) x = u32x4{x.y, x.z, x.w, 0u};
+        }
+        w[u] = x;
+      }
     }
   }
-  __device__ static __forceinline__ void store(T* p, int e, int n, const float* v) {
-    if (e + VEC <= n) {
-      if constexpr (ANY) store16_any(p + e, St::pack(v));
-      else store16(p + e, St::pack(v));
-    } else if (ANY && e < n) {
+  // a vector of n columns, settled
+  __device__ static __forceinline__ void vector(u32x4* w, const T* p, int n, int t) {
+    load<false>(w, p, 0, 0, 0, true, n, t);
+    settle(w, n, t, true);
+  }
+  // words v[u] of the row `local` behind row0 of a contiguous output
+  __device__ static __forceinline__ void store(T* p, i64 row0, int local, bool live, int u, int n, int t,
+                                               const float* v) {
+    const int e = at(u, t);
+    if constexpr (ACCESS == kWords) {
+      const u32 off = live && e < n ? (u32)(local * n + e) * (u32)sizeof(T) : kNowhere;
+      __builtin_amdgcn_raw_buffer_store_b128(St::pack(v), buffer_at(p + row0 * n), off, 0, 2);
+    } else if (live) {
+      T* q = p + (row0 + local) * n + e;
+      if (e + VEC <= n) {
+        store16_any(q, St::pack(v));
+      } else if (e < n) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (e + j < n) St::store(p + e + j, v[j]);
+        for (int j = 0; j < VEC; ++j)
+          if (e + j < n) St::store(q + j, v[j]);
+      }
     }
+  }
+};
+
+// A lane's row: `local` rows behind the wavefront's first, which is `first` rows into the workgroup's
+// (the same in every lane, so that addresses are scalar).
+template <int TPR>
+struct LaneRow {
+  int first, local;
+  __device__ __forceinline__ LaneRow() {
+    constexpr int PER = TPR < 64 ? 64 / TPR : 1;     // rows of a wavefront
+    first = __builtin_amdgcn_readfirstlane(TPR < 64 ? (int)(threadIdx.x / 64) * PER : (int)(threadIdx.x / TPR));
+    local = TPR < 64 ? (int)(threadIdx.x % 64) / TPR : 0;
   }
 };
 
@@ -77,43 +152,43 @@ __device__ __forceinline__ void row_sums(float* v, float* lds) {
       for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
     }
     __syncthreads();
-    float r[WPR][N];
+    // every group of WPR lanes reads the waves' sums and adds them (held whole, they would take N WPR
+    // registers)
 #pragma unroll
-    for (int w = 0; w < WPR; ++w)
-#pragma unroll
-      for (int i = 0; i < N; ++i) r[w][i] = lds[(first + w) * N + i];
-#pragma unroll
-    for (int s = 1; s < WPR; s *= 2)
-#pragma unroll
-      for (int w = 0; w < WPR; w += 2 * s)
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[w][i] += r[w + s][i];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = r[0][i];
+    for (int i = 0; i < N; ++i) v[i] = group_sum<WPR>(lds[(first + lane_id() % WPR) * N + i]);
   }
 }
 
-template <class St, int TPR, int NV, bool ANY, bool AFTER, int GATE, int WG>
+template <class St, int TPR, int NV, int ACCESS, bool AFTER, int GATE, int WG>
 __device__ __forceinline__ void residual_norm_forward(
     const typename St::T* __restrict__ x, const typename St::T* __restrict__ y,
     const typename St::T* __restrict__ gate, const typename St::T* __restrict__ after,
     const typename St::T* __restrict__ before, typename St::T* __restrict__ residual,
     typename St::T* __restrict__ normed, float* __restrict__ stats, i64 rows, int n, i64 stride_x,
     i64 stride_y, i64 group, float scale, float eps) {
-  typedef NormRow<St, TPR, NV, ANY> Row;
+  typedef NormRow<St, TPR, NV, ACCESS> Row;
   constexpr int VEC = St::kVec;
   __shared__ float lds[2][WG / 64];
   const int t = threadIdx.x % TPR;
-  const i64 row = (i64)blockIdx.x * (WG / TPR) + threadIdx.x / TPR;
+  const LaneRow<TPR> lane;
+  const i64 row0 = (i64)blockIdx.x * (WG / TPR) + lane.first, row = row0 + lane.local;
   const bool live = row < rows;
-  const i64 at = live ? row : 0;
+  const i64 safe = row0 < rows ? row0 : 0;           // a wavefront without a row reads the first
   u32x4 xw[NV], yw[NV], gw[NV], aw[NV], bw[NV];
-  Row::template load<true>(yw, y + at * stride_y, n, t, live);
-  Row::template load<true>(xw, x + at * stride_x, n, t, live);
-  if constexpr (GATE == kGateRows) Row::template load<true>(gw, gate + at * n, n, t, live);
-  if constexpr (GATE == kGateGroup) Row::template load<false>(gw, gate + at / group * n, n, t, live);
-  if constexpr (AFTER) Row::template load<false>(aw, after, n, t, live);
-  Row::template load<false>(bw, before, n, t, live);
+  Row::template load<true>(yw, y, safe, stride_y, lane.local, live, n, t);
+  Row::template load<true>(xw, x, safe, stride_x, lane.local, live, n, t);
+  if constexpr (GATE == kGateRows) Row::template load<true>(gw, gate, safe, n, lane.local, live, n, t);
+  // (rows of one wavefront may be in different groups)
+  const i64 gate0 = safe / group;
+  if constexpr (GATE == kGateGroup)
+    Row::template load<false>(gw, gate, gate0, n, live ? (int)(row / group - gate0) : 0, live, n, t);
+  if constexpr (AFTER) Row::template load<false>(aw, after, 0, 0, 0, true, n, t);
+  Row::template load<false>(bw, before, 0, 0, 0, true, n, t);
+  Row::settle(yw, n, t, live);
+  Row::settle(xw, n, t, live);
+  if constexpr (GATE != kGateNone) Row::settle(gw, n, t, live);
+  if constexpr (AFTER) Row::settle(aw, n, t, true);
+  Row::settle(bw, n, t, true);
   const float mean = 1.0f / (float)n;
   float rate_y = 1.0f;
   if constexpr (AFTER) {
@@ -147,54 +222,99 @@ __device__ __forceinline__ void residual_norm_forward(
   }
   row_sums<TPR, 1>(&total, lds[1]);
   const float rate_r = frsq(__builtin_fmaf(total, mean, eps));
-  if (!live) return;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    const int e = Row::at(u, t);
     float b[VEC], h[VEC];
     St::unpack(bw[u], b);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) h[j] = r[u][j] * rate_r * b[j];
-    Row::store(residual + row * n, e, n, r[u]);
-    Row::store(normed + row * n, e, n, h);
+    Row::store(residual, row0, lane.local, live, u, n, t, r[u]);
+    Row::store(normed, row0, lane.local, live, u, n, t, h);
   }
-  if (stats != nullptr && t == 0) {
+  if (stats != nullptr && t == 0 && live) {
     stats[2 * row] = rate_y;
     stats[2 * row + 1] = rate_r;
   }
 }
 
-// The workgroup's sums of `acc` over its rows (WG / TPR at a time) into fp32 `out`, or rounded into
-// `rounded` where the workgroup has seen all rows.
-template <class St, int TPR, int NV, int WG>
-__device__ __forceinline__ void norm_columns(float (&acc)[NV][St::kVec], float* lds, float* out,
-                                             typename St::T* rounded, int n) {
-  constexpr int VEC = St::kVec, COLS = TPR * NV * VEC, RPW = WG / TPR;
-  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  __syncthreads();                                   // the last sums have been read
-#pragma unroll
-  for (int u = 0; u < NV; ++u)
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4)
-      *(u32x4*)(lds + slot * COLS + (u * TPR + t) * VEC + j) =
-          u32x4{as_u32(acc[u][j]), as_u32(acc[u][j + 1]), as_u32(acc[u][j + 2]), as_u32(acc[u][j + 3])};
-  __syncthreads();
-  for (int e = threadIdx.x; e < n; e += WG) {
-    float v = lds[e];
-    for (int s = 1; s < RPW; ++s) v += lds[s * COLS + e];
-    if (rounded != nullptr) St::store(rounded + e, v);
-    else out[e] = v;
-  }
-}
+// A workgroup's column sums, for each of the three quantities: in registers, or in LDS where a lane has
+// 16 columns (its own, so without a barrier).
+template <class St, int TPR, int NV, int WG, bool IN_LDS>
+struct ColumnSums {
+  typedef typename St::T T;
+  static constexpr int VEC = St::kVec, COLS = TPR * NV * VEC, RPW = WG / TPR;
+  static_assert(!IN_LDS || RPW == 1, "a lane owns its columns");
+  float acc[IN_LDS ? 1 : NV][VEC];
+  float* lds;      // COLS floats of its own (IN_LDS), or RPW * COLS shared by the workgroup's sums
 
-// A workgroup of WG lanes walks a chunk of rows, WG / TPR at a time, the next rows' words in flight
-// under the arithmetic of these, and keeps the column sums in registers: one partial row per workgroup
-// and quantity (256 workgroups: 3% of the bytes at 16384 x 4096).
-//   chunks: `per_group` chunks of `chunk` rows in each gate group, or (per_group 0) one chunk of
-//   `chunk` whole groups of `group` rows.
+  __device__ __forceinline__ ColumnSums(float* l, int t) : lds(l) { clear(t); }
+  __device__ __forceinline__ f32x4n* at(int u, int t, int j) const {
+    return (f32x4n*)(lds + (u * TPR + t) * VEC + j);
+  }
+  __device__ __forceinline__ void clear(int t) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        if constexpr (IN_LDS) *at(u, t, j) = f32x4n{0.0f, 0.0f, 0.0f, 0.0f};
+        else acc[u][j] = acc[u][j + 1] = acc[u][j + 2] = acc[u][j + 3] = 0.0f;
+      }
+  }
+  __device__ __forceinline__ void add(int u, int t, const float* v) {
+    if constexpr (IN_LDS) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) *at(u, t, j) += f32x4n{v[j], v[j + 1], v[j + 2], v[j + 3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[u][j] += v[j];
+    }
+  }
+  // over the workgroup's rows, into fp32 `out`, or rounded into `rounded` where it has seen them all
+  __device__ __forceinline__ void write(int slot, int t, float* out, T* rounded, int n) {
+    if constexpr (RPW > 1) {
+      __syncthreads();                               // the last sums have been read
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4)
+          *(f32x4n*)(lds + slot * COLS + (u * TPR + t) * VEC + j) =
+              f32x4n{acc[u][j], acc[u][j + 1], acc[u][j + 2], acc[u][j + 3]};
+      __syncthreads();
+      for (int e = threadIdx.x; e < n; e += WG) {
+        float v = lds[e];
+        for (int s = 1; s < RPW; ++s) v += lds[s * COLS + e];
+        if (rounded != nullptr) St::store(rounded + e, v);
+        else out[e] = v;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int e = (u * TPR + t) * VEC + j;
+          if (e >= n) continue;
+          float v;
+          if constexpr (IN_LDS) v = lds[e];
+          else v = acc[u][j];
+          if (rounded != nullptr) St::store(rounded + e, v);
+          else out[e] = v;
+        }
+    }
+  }
+};
+
+// A workgroup of WG lanes walks a chunk of rows, WG / TPR at a time, and keeps the column sums, one
+// partial row per workgroup and quantity (256 workgroups: 3% of the bytes at 16384 x 4096).  With up to 8
+// columns a lane the next rows' words are in flight under the arithmetic of these, the gammas and the
+// gate stay in registers in fp32, and an element's terms are kept from the sums to the results; with 16
+// there are no registers for that, and sums but dgamma_before's are in LDS.
+//   `per_group` workgroups share each group of `group` rows, or (per_group 0) each takes whole groups.
+//   Rows and groups are dealt in turn, so that the workgroups walk through memory together: in
+//   contiguous chunks, 512 KB apart at bf16 16384 x 4096, they meet in the same memory channels (160-166
+//   us; in turn 148-150; with exact waits, above, 143-146, 5.6 TB/s).
 //   sums: fp32 [2][chunks][n] for dgamma_after and dgamma_before, then [chunks][n] for the gate's
 //   (only with per_group > 1; a group that one workgroup sees whole is written rounded).
-template <class St, int TPR, int NV, bool ANY, bool AFTER, int GATE, int WG>
+template <class St, int TPR, int NV, int ACCESS, bool AFTER, int GATE, int WG>
 __device__ __forceinline__ void residual_norm_backward(
     const typename St::T* __restrict__ dres, const typename St::T* __restrict__ dnormed,
     const typename St::T* __restrict__ x, const typename St::T* __restrict__ y,
@@ -203,54 +323,65 @@ __device__ __forceinline__ void residual_norm_backward(
     typename St::T* __restrict__ dx, typename St::T* __restrict__ dy,
     typename St::T* __restrict__ dgate, typename St::T* __restrict__ dafter,
     typename St::T* __restrict__ dbefore, float* __restrict__ sums, i64 rows, int n, i64 stride_dr,
-    i64 stride_dn, i64 stride_x, i64 stride_y, i64 group, i64 chunk, i64 per_group, float scale) {
-  typedef NormRow<St, TPR, NV, ANY> Row;
+    i64 stride_dn, i64 stride_x, i64 stride_y, i64 group, i64 per_group, float scale) {
+  typedef NormRow<St, TPR, NV, ACCESS> Row;
   constexpr int VEC = St::kVec, RPW = WG / TPR, COLS = Row::COLS;
-  __shared__ __attribute__((aligned(16))) float lds[RPW * COLS];
+  constexpr bool kLean = NV * VEC >= 16;
+  constexpr int SHARED = kLean ? (AFTER + (GATE == kGateGroup)) * COLS : RPW > 1 ? RPW * COLS : 0;
+  __shared__ __attribute__((aligned(16))) float lds[SHARED ? SHARED : 4];
   __shared__ float sums3[2][3 * (WG / 64)];
-  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const LaneRow<TPR> lane;
+  const int slot = lane.first + lane.local;
   const float mean = 1.0f / (float)n;
   const i64 chunks = gridDim.x;
-  // 16 columns a lane and more: their sums and words leave no registers for the next row's words or
-  // for the gammas and the gate, which come from the caches at each row instead
-  constexpr bool kLean = NV * VEC >= 16;
-  u32x4 aw[NV], bw[NV], gw[NV];
-  auto weights = [&](i64 gi) {
-    if constexpr (AFTER) Row::template load<false>(aw, after, n, t, true);
-    Row::template load<false>(bw, before, n, t, true);
-    if constexpr (GATE == kGateGroup) Row::template load<false>(gw, gate + gi * n, n, t, true);
-  };
-  float da[NV][VEC], db[NV][VEC], dg[NV][VEC];
-#pragma unroll
-  for (int u = 0; u < NV; ++u)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) da[u][j] = db[u][j] = dg[u][j] = 0.0f;
+  ColumnSums<St, TPR, NV, WG, kLean> da(lds, AFTER ? t : 0);
+  ColumnSums<St, TPR, NV, WG, kLean && GATE == kGateGroup> dg(lds + (kLean && AFTER ? COLS : 0), t);
+  ColumnSums<St, TPR, NV, WG, false> db(lds, t);
 
-  const i64 g0 = per_group ? blockIdx.x / per_group : blockIdx.x * chunk;
-  const i64 g1 = per_group ? g0 + 1 : (g0 + chunk < rows / group ? g0 + chunk : rows / group);
+  // words of gamma_after, gamma_before and the group's gate
+  u32x4 aw[NV], bw[NV], gw[NV];
+  auto weights = [&](i64 gate_row) {
+    if constexpr (AFTER) Row::vector(aw, after, n, t);
+    Row::vector(bw, before, n, t);
+    if constexpr (GATE == kGateGroup) Row::vector(gw, gate + gate_row * n, n, t);
+  };
+
+  const i64 g0 = per_group ? blockIdx.x / per_group : blockIdx.x;
+  const i64 g1 = per_group ? g0 + 1 : rows / group, step = RPW * (per_group ? per_group : 1);
   int turn = 0;
-  for (i64 gi = g0; gi < g1; ++gi) {
-    const i64 first = gi * group + (per_group ? blockIdx.x % per_group * chunk : 0);
-    const i64 end = per_group && first + chunk < (gi + 1) * group ? first + chunk : (gi + 1) * group;
+  for (i64 gi = g0; gi < g1; gi += chunks) {
+    const i64 first = gi * group + (per_group ? blockIdx.x % per_group * RPW : 0), end = (gi + 1) * group;
     if constexpr (!kLean) weights(gi);
     u32x4 nx[NV], ny[NV], nr[NV], nh[NV], ng[GATE == kGateRows ? NV : 1];
-    float nrate_y = 0.0f, nrate_r = 0.0f;
+    u32x2 nrate;
+    // no row: zeros, for a lane group that has none adds them (the addresses are the first row's)
     auto fetch = [&](i64 base) {
-      const i64 row = base + slot;
-      const bool live = row < end;
-      const i64 at = live ? row : 0;
-      Row::template load<true>(nx, x + at * stride_x, n, t, live);
-      Row::template load<true>(ny, y + at * stride_y, n, t, live);
-      Row::template load<true>(nr, dres + at * stride_dr, n, t, live && dres != nullptr);
-      Row::template load<true>(nh, dnormed + at * stride_dn, n, t, live);
-      if constexpr (GATE == kGateRows) Row::template load<true>(ng, gate + at * n, n, t, live);
-      nrate_y = live ? stats[2 * at] : 0.0f;         // (a lane group without a row adds zeros)
-      nrate_r = live ? stats[2 * at + 1] : 0.0f;
+      const i64 row0 = base + lane.first, safe = row0 < end ? row0 : first;
+      const bool live = row0 + lane.local < end;
+      Row::template load<true>(nx, x, safe, stride_x, lane.local, live, n, t);
+      Row::template load<true>(ny, y, safe, stride_y, lane.local, live, n, t);
+      Row::template load<true>(nr, dres != nullptr ? dres : dnormed, safe, dres != nullptr ? stride_dr : stride_dn,
+                               lane.local, live && dres != nullptr, n, t);
+      Row::template load<true>(nh, dnormed, safe, stride_dn, lane.local, live, n, t);
+      if constexpr (GATE == kGateRows) Row::template load<true>(ng, gate, safe, n, lane.local, live, n, t);
+      nrate = __builtin_amdgcn_raw_buffer_load_b64(buffer_at(stats + 2 * safe), live ? 8u * lane.local : kNowhere,
+                                                   0, 0);
     };
-    if (!kLean && first < end) fetch(first);
-    for (i64 base = first; base < end; base += RPW) {
-      const i64 row = base + slot;
-      const bool live = row < end;
+    if (first >= end) continue;
+    if constexpr (!kLean) {
+      fetch(first);
+      // as many writes as a row makes, to nowhere: the first wait counts what every other does
+      if constexpr (ACCESS == kWords) {
+        const __amdgpu_buffer_rsrc_t none = buffer_at(dx);
+#pragma unroll
+        for (int i = 0; i < (GATE == kGateRows ? 3 : 2) * NV; ++i)
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{0u, 0u, 0u, 0u}, none, kNowhere, 0, 2);
+      }
+    }
+    for (i64 base = first; base < end; base += step) {
+      const i64 row0 = base + lane.first;
+      const bool live = row0 + lane.local < end;
       if constexpr (kLean) {
         fetch(base);
         weights(gi);
@@ -264,37 +395,61 @@ __device__ __forceinline__ void residual_norm_backward(
         hw[u] = nh[u];
         if constexpr (GATE == kGateRows) gw[u] = ng[u];
       }
-      const float rate_y = AFTER ? nrate_y : 1.0f, rate_r = nrate_r;
-      if (!kLean && base + RPW < end) fetch(base + RPW);
-      // per element: the block's unit output, s g, its share of r, r / its norm, gamma_before dh
-      auto element = [&](int u, int j, const float* xv, const float* yv, const float* hv, const float* gv,
-                         const float* av, const float* bv, float& unit, float& w, float& c, float& k, float& a) {
-        unit = yv[j] * rate_y;
-        c = AFTER ? unit * av[j] : unit;
-        w = GATE != kGateNone ? scale * gv[j] : scale;
-        k = __builtin_fmaf(w, c, xv[j]) * rate_r;
-        a = hv[j] * bv[j];
+      const u32x2 rate = nrate;
+      if constexpr (!kLean) {
+        fetch(base + step);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      Row::settle(xw, n, t, live);
+      Row::settle(yw, n, t, live);
+      Row::settle(rw, n, t, live && dres != nullptr);
+      Row::settle(hw, n, t, live);
+      if constexpr (GATE == kGateRows) Row::settle(gw, n, t, live);
+      const float rate_y = AFTER ? as_f32(rate.x) : 1.0f, rate_r = as_f32(rate.y);
+      // an element's unit output, the residual over its norm k, gamma_before dh; its share c and s g are
+      // made again from the words (kept too, they would not fit the 128 registers of 1024 lanes)
+      struct Terms {
+        float unit[VEC], k[VEC], a[VEC];
       };
+      auto share = [&](int u, const Terms& e, float* g2, float* c, float* w) {
+        if constexpr (AFTER) St::reunpack(aw[u], g2);
+        if constexpr (GATE != kGateNone) St::reunpack(gw[u], w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          w[j] = GATE != kGateNone ? scale * w[j] : scale;
+          c[j] = AFTER ? e.unit[j] * g2[j] : e.unit[j];
+        }
+      };
+      auto terms = [&](int u, Terms& e, float* g2, float* c, float* w) {
+        float xv[VEC], yv[VEC], hv[VEC], bv[VEC];
+        St::reunpack(xw[u], xv);
+        St::reunpack(yw[u], yv);
+        St::reunpack(hw[u], hv);
+        St::reunpack(bw[u], bv);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e.unit[j] = yv[j] * rate_y;
+        share(u, e, g2, c, w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          e.k[j] = __builtin_fmaf(w[j], c[j], xv[j]) * rate_r;
+          e.a[j] = hv[j] * bv[j];
+        }
+      };
+      Terms kept[kLean ? 1 : NV];
       float s3[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        float xv[VEC], yv[VEC], rv[VEC], hv[VEC], gv[VEC], av[VEC], bv[VEC];
-        St::unpack(xw[u], xv);
-        St::unpack(yw[u], yv);
-        St::unpack(rw[u], rv);
-        St::unpack(hw[u], hv);
-        if constexpr (GATE != kGateNone) St::unpack(gw[u], gv);
-        if constexpr (AFTER) St::unpack(aw[u], av);
-        St::unpack(bw[u], bv);
+        Terms& e = kept[kLean ? 0 : u];
+        float rv[VEC], g2[VEC], c[VEC], w[VEC];
+        terms(u, e, g2, c, w);
+        St::reunpack(rw[u], rv);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          float unit, w, c, k, a;
-          element(u, j, xv, yv, hv, gv, av, bv, unit, w, c, k, a);
-          s3[0] = __builtin_fmaf(a, k, s3[0]);
+          s3[0] = __builtin_fmaf(e.a[j], e.k[j], s3[0]);
           if constexpr (AFTER) {
-            const float wc = w * c;
-            s3[1] = __builtin_fmaf(wc, __builtin_fmaf(rate_r, a, rv[j]), s3[1]);
-            s3[2] = __builtin_fmaf(wc, k, s3[2]);
+            const float wc = w[j] * c[j];
+            s3[1] = __builtin_fmaf(wc, __builtin_fmaf(rate_r, e.a[j], rv[j]), s3[1]);
+            s3[2] = __builtin_fmaf(wc, e.k[j], s3[2]);
           }
         }
       }
@@ -304,52 +459,36 @@ __device__ __forceinline__ void residual_norm_backward(
       const float m2 = AFTER ? (s3[1] - rate_r * m1 * s3[2]) * mean : 0.0f;
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        const int e = Row::at(u, t);
-        float xv[VEC], yv[VEC], rv[VEC], hv[VEC], gv[VEC], av[VEC], bv[VEC], ox[VEC], oy[VEC], og[VEC];
-        St::reunpack(xw[u], xv);
-        St::reunpack(yw[u], yv);
+        Terms& e = kept[kLean ? 0 : u];
+        float rv[VEC], hv[VEC], ox[VEC], oy[VEC], og[VEC], ca[VEC], cb[VEC], g2[VEC], c[VEC], w[VEC];
+        if constexpr (kLean) terms(u, e, g2, c, w);
+        else share(u, e, g2, c, w);
         St::reunpack(rw[u], rv);
         St::reunpack(hw[u], hv);
-        if constexpr (GATE != kGateNone) St::reunpack(gw[u], gv);
-        if constexpr (AFTER) St::reunpack(aw[u], av);
-        St::reunpack(bw[u], bv);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          float unit, w, c, k, a;
-          element(u, j, xv, yv, hv, gv, av, bv, unit, w, c, k, a);
-          ox[j] = __builtin_fmaf(rate_r, __builtin_fmaf(-k, m1, a), rv[j]);
-          const float dc = w * ox[j];
-          if constexpr (AFTER) {
-            oy[j] = rate_y * __builtin_fmaf(-unit, m2, dc * av[j]);
-            da[u][j] = __builtin_fmaf(dc, unit, da[u][j]);
-          } else {
-            oy[j] = dc;
-          }
-          db[u][j] = __builtin_fmaf(hv[j], k, db[u][j]);
-          if constexpr (GATE != kGateNone) {
-            og[j] = scale * ox[j] * c;
-            if constexpr (GATE == kGateGroup) dg[u][j] += og[j];
-          }
+          ox[j] = __builtin_fmaf(rate_r, __builtin_fmaf(-e.k[j], m1, e.a[j]), rv[j]);
+          const float dc = w[j] * ox[j];
+          oy[j] = AFTER ? rate_y * __builtin_fmaf(-e.unit[j], m2, dc * g2[j]) : dc;
+          ca[j] = dc * e.unit[j];
+          cb[j] = hv[j] * e.k[j];
+          og[j] = scale * ox[j] * c[j];
         }
-        if (!live) continue;
-        Row::store(dx + row * n, e, n, ox);
-        Row::store(dy + row * n, e, n, oy);
-        if constexpr (GATE == kGateRows) Row::store(dgate + row * n, e, n, og);
+        if constexpr (AFTER) da.add(u, t, ca);
+        db.add(u, t, cb);
+        if constexpr (GATE == kGateGroup) dg.add(u, t, og);
+        Row::store(dx, row0, lane.local, live, u, n, t, ox);
+        Row::store(dy, row0, lane.local, live, u, n, t, oy);
+        if constexpr (GATE == kGateRows) Row::store(dgate, row0, lane.local, live, u, n, t, og);
       }
     }
     if constexpr (GATE == kGateGroup) {
-      const bool whole = per_group <= 1;
-      norm_columns<St, TPR, NV, WG>(dg, lds, sums + (2 * chunks + blockIdx.x) * n,
-                                    whole ? dgate + gi * n : nullptr, n);
-#pragma unroll
-      for (int u = 0; u < NV; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) dg[u][j] = 0.0f;
+      dg.write(slot, t, sums + (2 * chunks + blockIdx.x) * n, per_group <= 1 ? dgate + gi * n : nullptr, n);
+      dg.clear(t);
     }
   }
-  if constexpr (AFTER)
-    norm_columns<St, TPR, NV, WG>(da, lds, sums + (i64)blockIdx.x * n, chunks == 1 ? dafter : nullptr, n);
-  norm_columns<St, TPR, NV, WG>(db, lds, sums + (chunks + blockIdx.x) * n, chunks == 1 ? dbefore : nullptr, n);
+  if constexpr (AFTER) da.write(slot, t, sums + (i64)blockIdx.x * n, chunks == 1 ? dafter : nullptr, n);
+  db.write(slot, t, sums + (chunks + blockIdx.x) * n, chunks == 1 ? dbefore : nullptr, n);
 }
 
 // Column sums of `count` fp32 partial rows, in their order within each of 8 interleaved runs and

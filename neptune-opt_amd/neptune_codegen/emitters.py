@@ -828,7 +828,7 @@ class ResidualNormVariant:
     """One launch shape of the residual norm's kernels."""
 
     dtype: str
-    any: bool           # rows of any alignment and width
+    access: str         # rows of whole 16-byte "words", of "any" alignment and width, of "few" columns
     tpr: int            # lanes per row
     nv: int             # 16-byte slots per lane
     wg: int             # lanes per workgroup
@@ -836,7 +836,7 @@ class ResidualNormVariant:
     gate: str           # "none", "rows" (one per row) or "group" (one per group of rows)
 
     def tag(self) -> str:
-        return (f"{dtype_tag(self.dtype)[0]}_{'a' if self.any else 'v'}{self.tpr}n{self.nv}w{self.wg}"
+        return (f"{dtype_tag(self.dtype)[0]}_{self.access}{self.tpr}n{self.nv}w{self.wg}"
                 f"{'_after' if self.after else ''}{'' if self.gate == 'none' else '_' + self.gate}")
 
 
@@ -851,7 +851,8 @@ def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
     nep_residual_norm.h."""
     st = dtype_tag(var.dtype)[1]
     gate = {"none": "nep::kGateNone", "rows": "nep::kGateRows", "group": "nep::kGateGroup"}[var.gate]
-    flags = f"{str(var.any).lower()}, {str(var.after).lower()}, {gate}, {var.wg}"
+    access = {"words": "nep::kWords", "any": "nep::kAnyRows", "few": "nep::kFewColumns"}[var.access]
+    flags = f"{access}, {str(var.after).lower()}, {gate}, {var.wg}"
     c, m = f"(const {st}::T*)", f"({st}::T*)"
     head = ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n"
             f"// residual norm: {stage}, {var.tag()}\n"
@@ -868,10 +869,10 @@ def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
             "const void* gate, const void* after, const void* before, const float* stats, void* dx, void* dy, "
             "void* dgate, void* dafter, void* dbefore, float* sums, long long rows, int n, "
             "long long stride_dr, long long stride_dn, long long stride_x, long long stride_y, "
-            "long long group, long long chunk, long long per_group, float scale) {\n"
+            "long long group, long long per_group, float scale) {\n"
             f"  nep::residual_norm_backward<{st}, {var.tpr}, {var.nv}, {flags}>({c}dres, {c}dnormed, {c}x, "
             f"{c}y, {c}gate, {c}after, {c}before, stats, {m}dx, {m}dy, {m}dgate, {m}dafter, {m}dbefore, sums, "
-            "rows, n, stride_dr, stride_dn, stride_x, stride_y, group, chunk, per_group, scale);\n}\n"
+            "rows, n, stride_dr, stride_dn, stride_x, stride_y, group, per_group, scale);\n}\n"
             f'extern "C" __global__ void __launch_bounds__(256) {residual_norm_kernel_name("join", var)}('
             "const float* sums, void* dafter, void* dbefore, void* dgate, int n, long long chunks, "
             "long long per_group) {\n"

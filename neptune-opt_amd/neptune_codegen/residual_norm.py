@@ -27,6 +27,7 @@ from neptune_codegen.emitters import (BASE_OPTIONS, ResidualNormVariant, emit_re
 from neptune_codegen.template import _validate_row_last
 
 MAX_WIDTH = 16384
+MAX_STRIDE = 1 << 22
 CUS = 256
 _PROGRAMS: dict = {}
 _OPS: dict = {}
@@ -34,7 +35,7 @@ _FORWARD, _BACKWARD = calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _FORWARD_ARGS = (hip.PTR,) * 8 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,) * 2
-_BACKWARD_ARGS = (hip.PTR,) * 14 + (hip.I64, hip.I32) + (hip.I64,) * 7 + (hip.F32,)
+_BACKWARD_ARGS = (hip.PTR,) * 14 + (hip.I64, hip.I32) + (hip.I64,) * 6 + (hip.F32,)
 _JOIN_ARGS = (hip.PTR,) * 4 + (hip.I32,) + (hip.I64,) * 2
 
 
@@ -108,7 +109,10 @@ def _eps(eps) -> float:
 
 
 def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, backward: bool) -> ResidualNormVariant:
-    """Lanes and slots of a row."""
+    """Lanes and slots of a row.  The forward pass takes two slots a lane once the rows fill the chip (bf16
+    16384 x 4096 93-95 us with one, two or four; 3000 x 3001 17 us, one 20).  The gradient takes one, on
+    workgroups of 512 lanes (1024 would hold its state in 128 registers: bf16 16384 x 4096 gated by sequence
+    174 us, 512 lanes 145; two slots on 256 lanes 209), or of 1024 where a row needs them."""
     vec = 16 // x.element_size()
     slots = -(-n // vec)
     nv = 1
@@ -118,13 +122,16 @@ def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, b
     while tpr > 1024:
         tpr, nv = tpr // 2, nv * 2
     wg = max(512 if backward else 256, tpr)
-    return ResidualNormVariant(str(x.dtype).replace("torch.", ""), not aligned, tpr, nv, wg, after, gate_kind)
+    access = "few" if n < vec else "words" if aligned else "any"
+    return ResidualNormVariant(str(x.dtype).replace("torch.", ""), access, tpr, nv, wg, after, gate_kind)
 
 
 def _operands(rows, vectors, n):
     """(tensors, row strides, whether every row is whole 16-byte words): `rows` [..., n] as they are or as
     contiguous copies, `vectors` contiguous."""
     made = [(None, 0) if t is None else calls.rows_of(t) for t in rows]
+    # (a wavefront's rows are addressed with 32-bit byte offsets from its first)
+    made = [(t, s) if t is None or s < MAX_STRIDE else (t.contiguous(), n) for t, s in made]
     used = [t for t, _ in made] + [None if t is None else t.contiguous() for t in vectors]
     vec = 16 // used[-2].element_size()
     aligned = (n % vec == 0 and all(s % vec == 0 for _, s in made)
@@ -171,17 +178,17 @@ def run_residual_norm(x, y, gamma_after, gamma_before, *, gate=None, residual_sc
 
 
 def _chunks(rows, groups, group, gate_kind, rpw):
-    """(chunks, rows or groups per chunk, chunks per group) of the gradient's launch: about one workgroup
-    per CU; chunks of whole groups (0 per group) where there are more groups than that."""
+    """(workgroups, workgroups per group) of the gradient's launch: one per CU, or fewer where their partial
+    sums would cost more than the rows (a row takes a workgroup about 1.7 us, a partial row 0.03 us to write and
+    join: bf16 256 x 4096 18 us with 256 workgroups, 15 with 128; 16384 x 4096 148 with 256, 157-176 with 512); 0 per group
+    where there are more groups than workgroups and each takes whole ones."""
     if gate_kind != "group":
         groups, group = 1, rows
-    if groups > CUS:
-        chunk = -(-groups // CUS)
-        return -(-groups // chunk), chunk, 0
-    per_group = max(1, min(CUS // groups, -(-group // rpw)))
-    chunk = -(-(-(-group // per_group)) // rpw) * rpw
-    per_group = -(-group // chunk)
-    return groups * per_group, chunk, per_group
+    most = min(CUS, math.isqrt(64 * -(-rows // rpw)) + 1)
+    if groups > most:
+        return most, 0
+    per_group = max(1, min(most // groups, -(-group // rpw)))
+    return groups * per_group, per_group
 
 
 def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, gamma_before, stats, *,
@@ -217,7 +224,7 @@ def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, ga
     kind = _gate_kind(groups, group)
     var = _variant(x, aligned, rows, n, gamma_after is not None, kind, True)
     device, prog = calls.device_index(x), _program("backward", var)
-    chunks, chunk, per_group = _chunks(rows, groups, group, kind, var.wg // var.tpr)
+    chunks, per_group = _chunks(rows, groups, group, kind, var.wg // var.tpr)
     split_gate = kind == "group" and per_group > 1
     buffers, returns = [], []
     for t in wanted:
@@ -232,7 +239,7 @@ def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, ga
     dres, dnormed, tx, ty, after, before, tgate, tstats = map(calls.tensor, range(8))
     launches = [(prog.kernel(residual_norm_kernel_name("backward", var), _BACKWARD_ARGS, var.wg, device), (chunks,),
                  (dres, dnormed, tx, ty, tgate, after, before, tstats, dx, dy, dgate, dafter, dbefore, work, rows, n)
-                 + strides + (group if kind == "group" else rows, chunk, per_group, scale))]
+                 + strides + (group if kind == "group" else rows, per_group, scale))]
     if chunks > 1:
         launches.append((prog.kernel(residual_norm_kernel_name("join", var), _JOIN_ARGS, 256, device),
                          (-(-n // 32), 2 + (groups if split_gate else 0)),

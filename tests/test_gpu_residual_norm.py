@@ -220,4 +220,4 @@ def test_no_rows():
     assert r.shape == h.shape == (0, 64) and s.shape == (0, 2)
     grads = CG.run_residual_norm_backward(x, x, x, x, g, g, s, gate=g)
     assert grads[0].shape == (0, 64) and not grads[2].any() and not grads[3].any() and not grads[4].any()
-    assert RN._chunks(5, 1, 5, "none", 8) == (1, 8, 1)
+    assert RN._chunks(5, 1, 5, "none", 8) == (1, 1)

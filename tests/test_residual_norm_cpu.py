@@ -61,24 +61,24 @@ def test_gate_groups(shape, gate, want):
     assert RN._gate_groups(meta(*gate), meta(*shape)) == want
 
 
-def test_chunks_cover_the_rows_once():
+def test_workgroups_cover_the_rows_once():
     for rows, groups in ((1, 1), (7, 7), (1000, 1), (1000, 8), (1000, 500), (60000, 30000), (16384, 8), (300, 300),
                          (512, 256), (514, 257)):
         group = rows // groups
         for kind in ("none", "rows", "group"):
             for rpw in (1, 2, 8, 64):
-                chunks, chunk, per_group = RN._chunks(rows, groups, group, kind, rpw)
+                chunks, per_group = RN._chunks(rows, groups, group, kind, rpw)
                 seen = [0] * rows
                 gr, gn = (group, groups) if kind == "group" else (rows, 1)
                 for c in range(chunks):          # as the kernel walks them
-                    g0 = c // per_group if per_group else c * chunk
-                    for gi in range(g0, g0 + 1 if per_group else min(g0 + chunk, gn)):
-                        first = gi * gr + (c % per_group * chunk if per_group else 0)
-                        end = min(first + chunk, (gi + 1) * gr) if per_group else (gi + 1) * gr
+                    g0 = c // per_group if per_group else c
+                    for gi in range(g0, g0 + 1 if per_group else gn, chunks):
+                        first, end = gi * gr + (c % per_group * rpw if per_group else 0), (gi + 1) * gr
                         assert first < end
-                        for r in range(first, end):
-                            seen[r] += 1
-                assert seen == [1] * rows and chunks <= 512
+                        for base in range(first, end, rpw * max(per_group, 1)):
+                            for r in range(base, min(base + rpw, end)):
+                                seen[r] += 1
+                assert seen == [1] * rows and chunks <= 256
 
 
 def test_rows_fit_the_lanes():
