@@ -22,34 +22,51 @@ namespace nep {
 template <int TPR>
 struct RowLanes {
   static constexpr int kWaves = TPR > 64 ? TPR / 64 : 1;
-  static_assert(TPR >= 64, "a row has a wavefront at least");
+  static_assert(TPR >= 64 && TPR <= 1024, "a row has a wavefront at least");
   __device__ static __forceinline__ void sync() {
     if constexpr (TPR > 64) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
   }
-  // `lds` has kWaves floats; the caller's next reduction may use the same
-  template <class Pair, class Group>
-  __device__ static __forceinline__ float reduce(float v, float* lds, Group group, Pair pair) {
-    v = group(v);
+  // N reductions in one exchange; `lds` has N floats a wave, and the next call may use the same
+  template <bool MAX, int N>
+  __device__ static __forceinline__ void reduce(float (&v)[N], float* lds) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = MAX ? group_max<64>(v[i]) : group_sum<64>(v[i]);
     if constexpr (TPR > 64) {
       __syncthreads();
-      if (lane_id() == 0) lds[threadIdx.x >> 6] = v;
-      __syncthreads();
-      v = lds[0];
+      if (lane_id() == 0) {
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) v = pair(v, lds[w]);
+        for (int i = 0; i < N; ++i) lds[(threadIdx.x >> 6) * N + i] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = lds[(lane_id() % kWaves) * N + i];
+        v[i] = MAX ? group_max<kWaves>(w) : group_sum<kWaves>(w);
+      }
     }
-    return v;
   }
-  __device__ static __forceinline__ float max(float v, float* lds) {
-    return reduce(v, lds, [](float x) { return group_max<64>(x); },
-                  [](float a, float b) { return __builtin_fmaxf(a, b); });
-  }
-  __device__ static __forceinline__ float sum(float v, float* lds) {
-    return reduce(v, lds, [](float x) { return group_sum<64>(x); },
-                  [](float a, float b) { return a + b; });
+  __device__ static __forceinline__ bool any(bool b) {
+    if constexpr (TPR > 64) return __syncthreads_or(b ? 1 : 0) != 0;
+    else return __builtin_amdgcn_ballot_w64(b) != 0;
   }
 };
+
+// The whole words of a row (those of its Span), read through a buffer: word i of the row, zero past
+// the end.  No access is in a branch, so a wait for one tile leaves the next one in flight (in branches
+// the waits are for everything, and a tile is not started until the one before it is done).
+constexpr u32 kPastRow = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, 0x7fffffff, 0x00020000);
+}
+template <int TPR, int UNROLL>
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t row, int first, int words, int t, u32x4* w) {
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const int i = first + u * TPR + t;
+    w[u] = __builtin_amdgcn_raw_buffer_load_b128(row, i < words ? (u32)i * 16u : kPastRow, 0, 2);
+  }
+}
 
 // A row's entries, EPL per lane: entry k of lane t is t + k TPR.
 template <class Lt, typename Ix, int TPR, int EPL>
@@ -79,18 +96,16 @@ struct TeacherList {
       }
     }
   }
-  __device__ __forceinline__ void weigh(float c, float* lds) {
-    typedef RowLanes<TPR> R;
+  // this lane's largest t (a NaN is no maximum, but it counts as present)
+  __device__ __forceinline__ float largest() const {
     float m = -kInf;
 #pragma unroll
-    for (int k = 0; k < EPL; ++k) {
-      m = __builtin_fmaxf(m, e[k]);
-      // a NaN is no maximum; it counts as present all the same
-      if (is_nan(e[k])) m = __builtin_fmaxf(m, -3.0e38f);
-    }
-    top = R::max(m, lds);
-    bad = R::max(bad ? 1.0f : 0.0f, lds) != 0.0f;
-    empty = top == -kInf && !bad;
+    for (int k = 0; k < EPL; ++k) m = __builtin_fmaxf(m, is_nan(e[k]) ? -3.0e38f : e[k]);
+    return m;
+  }
+  // with the list's largest: the exponentials, this lane's sum of them
+  __device__ __forceinline__ float exponentials(float list_top, float c) {
+    top = list_top;
     const float ref = top == -kInf ? 0.0f : top;
     float s = 0.0f;
 #pragma unroll
@@ -99,10 +114,15 @@ struct TeacherList {
       e[k] = at[k] < 0 ? 0.0f : __builtin_amdgcn_exp2f(d[k] * c);
       s += e[k];
     }
-    total = R::sum(s, lds);
-    const float inv = 1.0f / total;
+    return s;
+  }
+  __device__ __forceinline__ void normalise(float list_total, bool any_bad) {
+    total = list_total;
+    bad = any_bad;
+    empty = top == -kInf && !bad;
+    const float inv = __builtin_amdgcn_rcpf(total);   // total is at least 1
 #pragma unroll
-    for (int k = 0; k < EPL; ++k) e[k] = e[k] * inv;
+    for (int k = 0; k < EPL; ++k) e[k] *= inv;
   }
 };
 
@@ -117,8 +137,8 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
                                                 int count, float c, float inv_t, float t2) {
   typedef RowLanes<TPR> R;
   typedef Span<St, TPR, ACCESS> Sp;
-  constexpr int VEC = St::kVec, STEP = TPR * VEC;
-  __shared__ float lds[R::kWaves];
+  constexpr int VEC = St::kVec;
+  __shared__ float lds[2 * R::kWaves];
   const int t = threadIdx.x % TPR;
   const i64 row = (i64)blockIdx.x * (WG / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const bool live = row < rows;
@@ -130,15 +150,10 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
   for (int k = 0; k < EPL; ++k) zk[k] = list.at[k] >= 0 ? St::load(rp + list.at[k]) : 0.0f;
 
   const Sp sp(rp, 0, live ? n : 0);
+  const __amdgpu_buffer_rsrc_t row_words = row_buffer(rp + sp.v0);
+  const int words = (int)((sp.v1 - sp.v0) / VEC);
   float m = -kInf, s = 0.0f;
   u32x4 cur[UNROLL];
-  auto fetch = [&](i64 e0, u32x4* w) {
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const i64 e = e0 + (i64)(u * TPR + t) * VEC;
-      w[u] = e < sp.v1 ? load16(rp + e) : u32x4{St::kNegInfWord, St::kNegInfWord, St::kNegInfWord, St::kNegInfWord};
-    }
-  };
   auto move = [&](float tile_max) {
     if (tile_max > m) {
       s *= m == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m - tile_max) * c);
@@ -146,12 +161,7 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
     }
     return m == -kInf ? 0.0f : m;
   };
-  fetch(sp.v0, cur);
-  typename Sp::Rest rest;
-  if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
-  for (i64 e0 = sp.v0; e0 < sp.v1; e0 += (i64)UNROLL * STEP) {
-    u32x4 next[UNROLL];
-    fetch(e0 + (i64)UNROLL * STEP, next);
+  auto tile = [&]() {
     float tm = -kInf;
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -173,8 +183,24 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
       }
     }
     s += a + b;
+  };
+  load_words<TPR, UNROLL>(row_words, 0, words, t, cur);
+  typename Sp::Rest rest;
+  if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
+  int at = 0;
+  for (; at + UNROLL * TPR <= words; at += UNROLL * TPR) {
+    u32x4 next[UNROLL];
+    load_words<TPR, UNROLL>(row_words, at + UNROLL * TPR, words, t, next);
+    tile();
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) cur[u] = next[u];
+  }
+  if (at < words) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (at + u * TPR + t >= words)
+        cur[u] = u32x4{St::kNegInfWord, St::kNegInfWord, St::kNegInfWord, St::kNegInfWord};
+    tile();
   }
   if constexpr (ACCESS == kRagged) {
     float tm = -kInf;
@@ -184,19 +210,25 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
 #pragma unroll
     for (int u = 0; u < Sp::RU; ++u) s += __builtin_amdgcn_exp2f((rest.s[u] - ref) * c);
   }
-  const float top = R::max(m, lds);
-  const float total = R::sum(m == -kInf ? s : s * __builtin_amdgcn_exp2f((m - top) * c), lds);
-  list.weigh(c, lds);
-  // log p_k - log q_k = ((t_k - max t) - (z_k - max z)) / T - log(total t) + log(total z)
-  const float gap = logf(total) - logf(list.total);
+  float tops[2] = {m, list.largest()};
+  R::template reduce<true, 2>(tops, lds);
+  const float top = tops[0];
+  float totals[2] = {m == -kInf ? s : s * __builtin_amdgcn_exp2f((m - top) * c), list.exponentials(tops[1], c)};
+  R::template reduce<false, 2>(totals, lds);
+  const float total = totals[0];
+  list.normalise(totals[1], R::any(list.bad));
+  // log p_k - log q_k = ((t_k - max t) - (z_k - max z)) / T - log(total t) + log(total z), with the
+  // hardware's logarithm (an ulp; both arguments are at least 1)
+  const float gap = (__builtin_amdgcn_logf(total) - __builtin_amdgcn_logf(list.total)) * 0.6931471805599453f;
   float term = 0.0f;
 #pragma unroll
   for (int k = 0; k < EPL; ++k)
     if (list.at[k] >= 0 && !(list.e[k] == 0.0f))
       term += list.e[k] * ((list.d[k] - (zk[k] - top)) * inv_t + gap);
-  term = R::sum(term, lds);
+  float terms[1] = {term};
+  R::template reduce<false, 1>(terms, lds);
   if (live && t == 0) {
-    loss[row] = list.bad ? __builtin_nanf("") : list.empty ? 0.0f : t2 * term;
+    loss[row] = list.bad ? __builtin_nanf("") : list.empty ? 0.0f : t2 * terms[0];
     if (stats != nullptr) {
       stats[2 * row] = top;
       stats[2 * row + 1] = total;
@@ -232,15 +264,10 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   const typename St::T* rp = z + (live ? row : 0) * stride_z;
   typename St::T* op = dz + (live ? row : 0) * n;
   const Sp sp(rp, 0, live ? n : 0);
+  const __amdgpu_buffer_rsrc_t row_words = row_buffer(rp + sp.v0);
+  const int words = (int)((sp.v1 - sp.v0) / VEC);
   u32x4 cur[UNROLL];
-  auto fetch = [&](i64 e0, u32x4* w) {
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const i64 e = e0 + (i64)(u * TPR + t) * VEC;
-      w[u] = e < sp.v1 ? load16(rp + e) : u32x4{0u, 0u, 0u, 0u};
-    }
-  };
-  fetch(sp.v0, cur);
+  load_words<TPR, UNROLL>(row_words, 0, words, t, cur);
   TeacherList<Lt, Ix, TPR, EPL> list;
   list.load(top_logits + (live ? row : 0) * stride_t, index + (live ? row : 0) * stride_i, count, n, t, live);
   float zk[EPL];
@@ -250,8 +277,12 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   const float top = live ? stats[2 * row] : 0.0f, total = live ? stats[2 * row + 1] : 1.0f;
 #pragma unroll
   for (int i = t; i < HASH / 32; i += TPR) seen[slot][i] = 0u;
-  list.weigh(c, lds);                              // (its barriers stand between the table's two uses)
-  R::sync();
+  float reduced[1] = {list.largest()};
+  R::template reduce<true, 1>(reduced, lds);
+  reduced[0] = list.exponentials(reduced[0], c);
+  R::template reduce<false, 1>(reduced, lds);
+  list.normalise(reduced[0], R::any(list.bad));
+  R::sync();                                       // the table is clear
   bool twice = false;
 #pragma unroll
   for (int k = 0; k < EPL; ++k) {
@@ -273,29 +304,36 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   } else {
     typename Sp::Rest rest;
     if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
-    for (i64 e0 = sp.v0; e0 < sp.v1; e0 += (i64)UNROLL * STEP) {
+    typename St::T* ow = op + sp.v0 + (i64)t * VEC;
+    auto put = [&](int u, int at) {
+      float v[VEC];
+      St::unpack(cur[u], v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
+      store_vec<ACCESS>(ow + (i64)(at + u * TPR) * VEC, St::pack(v));
+    };
+    // as many writes as a tile makes, to nowhere: the first wait counts what every other does
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      __builtin_amdgcn_raw_buffer_store_b32(0u, row_words, kPastRow + 4u * u, 0, 0);
+    int at = 0;
+    for (; at + UNROLL * TPR <= words; at += UNROLL * TPR) {
       u32x4 next[UNROLL];
-      fetch(e0 + (i64)UNROLL * STEP, next);
+      load_words<TPR, UNROLL>(row_words, at + UNROLL * TPR, words, t, next);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const i64 e = e0 + (i64)(u * TPR + t) * VEC;
-        if (e >= sp.v1) continue;
-        float v[VEC];
-        St::unpack(cur[u], v);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
-        store_vec<ACCESS>(op + e, St::pack(v));
-      }
+      for (int u = 0; u < UNROLL; ++u) put(u, at);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) cur[u] = next[u];
     }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (at + u * TPR + t < words) put(u, at);
     if constexpr (ACCESS == kRagged) sp.store_rest(rest, op, t, value);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): this wave's writes are done
   R::sync();
   if (list.empty || list.bad) twice = false;
-  if constexpr (TPR > 64) twice = __syncthreads_or(twice) != 0;
-  else twice = __builtin_amdgcn_ballot_w64(twice) != 0;
+  twice = R::any(twice);
   if (list.empty || list.bad) return;
 #pragma unroll
   for (int k = 0; k < EPL; ++k) {

@@ -10,9 +10,11 @@
 // cosine see at most pi/4: their Taylor series to x^9 and x^10 are within 2^-28 of the value there, and
 // the quarter turns are exact.
 //
-// HBM-bound: every element is read once and written once.  A lane owns one 16-byte slot of a token (a
-// pair of slots half a part apart in the half layout), computes its angles once and walks `per` heads
-// with them, queries and keys alike; consecutive lanes are consecutive slots, then tokens.
+// HBM-bound: every element is read once and written once.  A lane owns one 16-byte slot of a token,
+// computes its angles once and walks `per` heads with them, queries and keys alike; consecutive lanes are
+// consecutive slots, then tokens.  In the half layout a lane has the two slots of its pairs, half a part
+// apart; where a head's slots are a power of two and all turned, each lane has one slot instead and the
+// two of a pair exchange their words, so that a wavefront reads whole rows of a head.
 #pragma once
 
 namespace nep {
@@ -37,6 +39,21 @@ __device__ __forceinline__ void sincos_turns(double turn, float& s, float& c) {
   c = (q & 1) ? sx : cx;
   if (q & 2) s = -s;
   if (q == 1 || q == 2) c = -c;
+}
+
+constexpr int kHalves = 0, kPairs = 1, kExchanged = 2;
+// the word of lane ^ distance (a power of two below 64)
+__device__ __forceinline__ u32x4 exchanged(const u32x4& w, int distance) {
+  u32x4 r;
+  if (distance == 8) {                               // row_ror:8 inside 16 lanes
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (u32)__builtin_amdgcn_mov_dpp((int)w[i], 0x128, 0xF, 0xF, false);
+  } else {
+    const int from = (lane_id() ^ distance) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (u32)__builtin_amdgcn_ds_bpermute(from, (int)w[i]);
+  }
+  return r;
 }
 
 // One 16-byte slot of a row from element e; ANY: of any alignment, up to `count` elements.
@@ -66,7 +83,7 @@ __device__ __forceinline__ void slot_store(typename St::T* p, const u32x4& w, in
 
 // tokens = batch * seq; a token has `turned` slots of pairs and then the slots of its copied rest,
 // `slots` in all.  Outputs are contiguous [batch, heads, seq, dim].
-template <class St, typename Px, bool INTERLEAVED, bool ANY>
+template <class St, typename Px, int LAYOUT, bool ANY>
 __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
                                        const typename St::T* __restrict__ k,
                                        const Px* __restrict__ positions,
@@ -77,7 +94,8 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
                                        int per, i64 qsb, i64 qsh, i64 qss, i64 ksb, i64 ksh, i64 kss,
                                        i64 psb, i64 pss, float sign, float magnitude) {
   typedef typename St::T T;
-  constexpr int VEC = St::kVec, PAIRS = INTERLEAVED ? VEC / 2 : VEC;
+  constexpr int VEC = St::kVec, PAIRS = LAYOUT == kPairs ? VEC / 2 : VEC;
+  static_assert(LAYOUT != kExchanged || !ANY, "whole words");
   constexpr int AHEAD = 4;                          // heads in flight per lane
   const u32 id = blockIdx.x * 256u + threadIdx.x;
   const u32 token = id / slots, slot = id - token * slots;
@@ -87,16 +105,17 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
   const bool turn = slot < turned;
   // first element, elements of the slot, and for the half layout the distance to their partners
   const int e = turn ? (int)slot * VEC : part + (int)(slot - turned) * VEC;
-  const int count = (turn ? (INTERLEAVED ? part : half) : dim) - e;
+  const int count = (turn ? (LAYOUT == kHalves ? half : part) : dim) - e;
   float cs[PAIRS], sn[PAIRS];
   if (turn) {
     const double at = (double)positions[b * psb + s * pss];
-    const int first = INTERLEAVED ? e / 2 : e;
+    const int first = LAYOUT == kPairs ? e / 2 : LAYOUT == kExchanged && e >= half ? e - half : e;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       const double t = first + i < half ? at * turns[first + i] : 0.0;
       sincos_turns(t, sn[i], cs[i]);
-      sn[i] *= sign * magnitude;
+      // (exchanged: the second half's slot is b, and b' = b cos + a sin)
+      sn[i] *= LAYOUT == kExchanged && e < half ? -(sign * magnitude) : sign * magnitude;
       cs[i] *= magnitude;
     }
   }
@@ -113,14 +132,21 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
       if (h + i >= end) continue;
       const T* p = h + i < heads_q ? qrow + (h + i) * qsh : krow + (h + i - heads_q) * ksh;
       w0[i] = slot_load<St, ANY>(p, count);
-      if (!INTERLEAVED && turn) w1[i] = slot_load<St, ANY>(p + half, count);
+      if (LAYOUT == kHalves && turn) w1[i] = slot_load<St, ANY>(p + half, count);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (h + i >= end) continue;
       T* o = h + i < heads_q ? qout + (h + i) * ostep : kout + (h + i - heads_q) * ostep;
       if (turn) {
-        if constexpr (INTERLEAVED) {
+        if constexpr (LAYOUT == kExchanged) {
+          float own[VEC], other[VEC];
+          St::unpack(w0[i], own);
+          St::unpack(exchanged(w0[i], half / VEC), other);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) own[j] = __builtin_fmaf(other[j], sn[j], own[j] * cs[j]);
+          w0[i] = St::pack(own);
+        } else if constexpr (LAYOUT == kPairs) {
           float v[VEC];
           St::unpack(w0[i], v);
 #pragma unroll

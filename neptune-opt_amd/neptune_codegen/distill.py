@@ -70,8 +70,8 @@ def validate_distill_inputs(logits, top_logits, top_index, *, metadata: bool = F
         raise ValueError("distillation tensors must be on the same device")
     if not 1 <= top_logits.shape[-1] <= MAX_ENTRIES:
         raise NotImplementedError(f"distillation takes lists of 1 to {MAX_ENTRIES} entries")
-    if logits.shape[-1] >= 1 << 31:
-        raise NotImplementedError("distillation takes rows of less than 2^31 logits")
+    if logits.shape[-1] >= 1 << 29:
+        raise NotImplementedError("distillation takes rows of less than 2^29 logits")
     return lead
 
 
@@ -84,17 +84,31 @@ def _check_rows(t, name, shape, logits, *, metadata):
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _variant(z, stride: int, top, index, rows: int, n: int, count: int) -> DistillVariant:
-    """Lanes per row: a wavefront up to 512 slots of 16 bytes, a workgroup of 256 lanes beyond; 1024
-    where the rows leave most CUs idle otherwise."""
+def _variant(z, stride: int, top, index, rows: int, n: int, count: int, stage: str) -> DistillVariant:
+    """Lanes per row and 16-byte slots a lane has in flight.
+
+    Forward: a wavefront up to 512 slots (16384 rows of 4096 bf16: 31 us, 42 with 256 lanes), 256 lanes
+    beyond (16384 rows of 32000: 157 us, 164 with 512, 201 with 1024), 1024 where 512 rows or fewer would
+    leave CUs idle (64 rows of 128256: 11.1 us, 13.4 with 256).  Eight slots in flight where a CU has four
+    workgroups (7168 rows of 32003: 73.5 us, 77.1 with four), four below (600 rows of 50000: 15.7 us, 17.4).
+    Backward, which reads and writes and so wants few rows open at once: a wavefront up to 256 slots (16384
+    rows of 1000: 21.4 us, 24.6 with 128), 256 lanes up to 2048 (16384 rows of 4096: 63 us, 69 with a
+    wavefront), 1024 beyond (7168 rows of 32003: 169 us, 193 with 256; fp32 4096 rows of 32000: 176, 190).
+    A tile of lanes x slots is never wider than the row: 16384 rows of 32000 by 1024 lanes take 368 us with
+    two slots, 442 with four."""
     vec = 16 // z.element_size()
     slots = -(-n // vec)
     aligned = n % vec == 0 and z.data_ptr() % 16 == 0 and stride % vec == 0
-    tpr = 64 if slots <= 512 and count <= 256 else 256
-    if rows <= 512 and slots > 1024:
-        tpr = 1024
+    if stage == "forward":
+        tpr = 64 if slots <= 512 and count <= 256 else 1024 if rows <= 512 and slots > 1024 else 256
+        most = 8 if rows >= 1024 else 4
+    else:
+        tpr = 64 if slots <= 256 and count <= 256 else 256 if slots < 2048 else 1024
+        if rows <= 512 and slots > 1024:
+            tpr = 1024
+        most = 4
     unroll = 1
-    while unroll < 4 and tpr * unroll * 2 < slots * 1.5:
+    while unroll < most and tpr * unroll * 2 <= slots:
         unroll *= 2
     entries = 1
     while entries * tpr < count:
@@ -106,7 +120,7 @@ def _variant(z, stride: int, top, index, rows: int, n: int, count: int) -> Disti
 def _launch(stage, z, top, index, strides, args, ends):
     """(kernel, grid, arguments) of a stage; `args` are its pointers, `ends` what follows the strides."""
     rows, n, count = z.numel() // z.shape[-1], z.shape[-1], top.shape[-1]
-    var = _variant(z, strides[-3], top, index, rows, n, count)
+    var = _variant(z, strides[-3], top, index, rows, n, count, stage)
     kernel = _program(stage, var).kernel(distill_kernel_name(stage, var),
                                          _FORWARD_ARGS if stage == "forward" else _BACKWARD_ARGS,
                                          var.wg, calls.device_index(z))

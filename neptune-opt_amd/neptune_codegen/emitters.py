@@ -880,26 +880,28 @@ def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
 
 
 # ---------------------------------------------------------------- rotary positions
-def rotary_kernel_name(dtype, index: str, interleaved: bool, any_rows: bool) -> str:
-    return (f"rotary_{dtype_tag(dtype)[0]}_{index[0]}{index[3:]}_{'pairs' if interleaved else 'halves'}"
-            f"{'_any' if any_rows else ''}")
+ROTARY_LAYOUTS = {"halves": "nep::kHalves", "pairs": "nep::kPairs", "exchanged": "nep::kExchanged"}
 
 
-def emit_rotary_source(dtype, index: str, interleaved: bool, any_rows: bool) -> str:
-    """hiprtc unit of the rotary positions (nep_rotary.h); `index` is the positions' dtype, `any_rows`
-    takes rows of any alignment and sizes that are no multiple of 16 bytes."""
+def rotary_kernel_name(dtype, index: str, layout: str, any_rows: bool) -> str:
+    return f"rotary_{dtype_tag(dtype)[0]}_{index[0]}{index[3:]}_{layout}{'_any' if any_rows else ''}"
+
+
+def emit_rotary_source(dtype, index: str, layout: str, any_rows: bool) -> str:
+    """hiprtc unit of the rotary positions (nep_rotary.h); `index` is the positions' dtype, `layout` one of
+    ROTARY_LAYOUTS, `any_rows` takes rows of any alignment and sizes that are no multiple of 16 bytes."""
     st = dtype_tag(dtype)[1]
     px = {"int32": "int", "int64": "long long"}[index]
     c, m = f"(const {st}::T*)", f"({st}::T*)"
     return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// rotary positions\n"
             + kernel_header("nep_device.h", "nep_rotary.h")
             + '\nextern "C" __global__ void __launch_bounds__(256) '
-            f"{rotary_kernel_name(dtype, index, interleaved, any_rows)}(const void* q, const void* k, "
+            f"{rotary_kernel_name(dtype, index, layout, any_rows)}(const void* q, const void* k, "
             "const void* positions, const double* turns, void* qo, void* ko, int tokens, int seq, int dim, "
             "int part, int slots, int turned, int heads_q, int heads_k, int per, long long qsb, long long qsh, "
             "long long qss, long long ksb, long long ksh, long long kss, long long psb, long long pss, "
             "float sign, float magnitude) {\n"
-            f"  nep::rotary<{st}, {px}, {str(interleaved).lower()}, {str(any_rows).lower()}>({c}q, {c}k, "
+            f"  nep::rotary<{st}, {px}, {ROTARY_LAYOUTS[layout]}, {str(any_rows).lower()}>({c}q, {c}k, "
             f"(const {px}*)positions, turns, {m}qo, {m}ko, (nep::u32)tokens, (nep::u32)seq, dim, part, "
             "(nep::u32)slots, (nep::u32)turned, heads_q, heads_k, per, qsb, qsh, qss, ksb, ksh, kss, psb, pss, "
             "sign, magnitude);\n}\n")

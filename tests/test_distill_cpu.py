@@ -61,6 +61,7 @@ def test_lists_fit_the_lanes():
                 for dtype in (torch.float32, torch.bfloat16):
                     z = meta((rows, n), dtype)
                     t, i = meta((rows, k), torch.float32), meta((rows, k), torch.int64)
-                    var = DI._variant(z, n, t, i, rows, n, k)
-                    assert var.tpr * var.entries >= k and var.tpr in (64, 256, 1024) and var.unroll <= 4
-                    assert DI._program("forward", var).source
+                    for stage in ("forward", "backward"):
+                        var = DI._variant(z, n, t, i, rows, n, k, stage)
+                        assert var.tpr * var.entries >= k and var.tpr in (64, 256, 1024) and var.unroll <= 8
+                        assert DI._program(stage, var).source
