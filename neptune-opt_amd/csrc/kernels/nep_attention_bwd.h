@@ -469,6 +469,13 @@ __device__ __forceinline__ void bwd_store_rows(unsigned char* stage, const f32x1
   __builtin_amdgcn_wave_barrier();
 }
 
+// A tile buffer, an object of its own, the same for both stages where one kernel holds them.
+template <int BYTES, int ID>
+__device__ __forceinline__ unsigned char* bwd_tile() {
+  __shared__ __attribute__((aligned(1024))) unsigned char tile[BYTES];
+  return tile;
+}
+
 // dK and dV.  W waves of 32 KB keys each; a wave's K and V rows and its dK^T and dV^T stay in
 // registers, the workgroup's Q and dO tiles are staged for all of its waves.  One wave per SIMD:
 // at KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1
@@ -483,7 +490,7 @@ __device__ __forceinline__ void attention_bwd_kv(
     const float* __restrict__ bounds, T* __restrict__ dk, T* __restrict__ dv,
     float* __restrict__ sums, int units, int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss,
     i64 ksb, i64 ksh, i64 kss, i64 vsb, i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale,
-    float scale_log2, int per) {
+    float scale_log2, int per, int group) {
   typedef AttnIn<T> In;
   typedef typename In::vec8 vec8;
   constexpr int BN = 32 * KB * W;                    // keys per workgroup
@@ -493,22 +500,21 @@ __device__ __forceinline__ void attention_bwd_kv(
   constexpr bool kFull = D * KB >= 256;              // dK and dV take every AGPR
   constexpr bool kKeysInLds = kFull;                 // and K no vector register
   constexpr bool kScaled = BwdIn<T>::kScaled;
-  __shared__ __attribute__((aligned(1024))) unsigned char qbuf0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char qbuf1[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char gbuf0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char gbuf1[TILE];
+  unsigned char *const qbuf0 = bwd_tile<TILE, 0>(), *const qbuf1 = bwd_tile<TILE, 1>(),
+                *const gbuf0 = bwd_tile<TILE, 2>(), *const gbuf1 = bwd_tile<TILE, 3>();
   __shared__ __attribute__((aligned(1024))) unsigned char kall[kKeysInLds ? BN * D * 2 : 16];
   __shared__ __attribute__((aligned(1024))) float sbuf0[2 * kBwdTile];
   __shared__ __attribute__((aligned(1024))) float sbuf1[2 * kBwdTile];
 
   const int nkb = (sk + BN - 1) / BN, nq = (sq + kBwdTile - 1) / kBwdTile;
-  const int bh = blockIdx.x % units, id = blockIdx.x / units;
+  const int bh = group % units, id = group / units;
   const int kb_id = PARTS ? id % nkb : id, part = PARTS ? id / nkb : 0;   // whole parts first
   const int b = bh / heads, h = bh % heads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
   const int k0 = kb_id * BN, kw = k0 + wave * 32 * KB;
+  const bool idle = kw >= sk;                        // a wave without a key
   const T* qp = q + b * qsb + h * qsh;
   const T* kp = k + b * ksb + h * ksh;
   const T* vp = v + b * vsb + h * vsh;
@@ -570,6 +576,7 @@ __device__ __forceinline__ void attention_bwd_kv(
     for (int sub = 0; sub < ROWS; sub += 32) {
       const int i0 = tile * ROWS + sub;
       if (CAUSAL && i0 + 31 < kw) continue;          // every pair hidden
+      if (i0 >= sq) continue;
       f32x16 s[KB], dp[KB];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -678,11 +685,11 @@ __device__ __forceinline__ void attention_bwd_kv(
       landed();
       __syncthreads();
       if (tile + 1 < t1) issue(tile + 1, qbuf1, gbuf1, sbuf1);
-      body(tile, qbuf0, gbuf0, sbuf0);
+      if (!idle) body(tile, qbuf0, gbuf0, sbuf0);
       landed();
       __syncthreads();
       if (tile + 2 < t1) issue(tile + 2, qbuf0, gbuf0, sbuf0);
-      if (tile + 1 < t1) body(tile + 1, qbuf1, gbuf1, sbuf1);
+      if (!idle && tile + 1 < t1) body(tile + 1, qbuf1, gbuf1, sbuf1);
     }
   }
 
@@ -744,27 +751,27 @@ __device__ __forceinline__ void attention_bwd_q(
     const T* __restrict__ go, const float* __restrict__ start, const float* __restrict__ ndelta,
     const float* __restrict__ bounds, T* __restrict__ dq, float* __restrict__ sums, int units,
     int heads, int sq, int sk, i64 qsb, i64 qsh, i64 qss, i64 ksb, i64 ksh, i64 kss, i64 vsb,
-    i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale, float scale_log2, int per) {
+    i64 vsh, i64 vss, i64 gsb, i64 gsh, i64 gss, float scale, float scale_log2, int per, int group) {
   typedef AttnIn<T> In;
   typedef typename In::vec8 vec8;
   constexpr int BM = 32 * QB * W;
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
   constexpr int TILE = kBwdTile * D * 2;
   constexpr bool kScaled = BwdIn<T>::kScaled;
-  __shared__ __attribute__((aligned(1024))) unsigned char kbuf0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char kbuf1[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char vbuf0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char vbuf1[TILE];
+  unsigned char *const kbuf0 = bwd_tile<TILE, 0>(), *const kbuf1 = bwd_tile<TILE, 1>(),
+                *const vbuf0 = bwd_tile<TILE, 2>(), *const vbuf1 = bwd_tile<TILE, 3>();
 
   const int nqb = (sq + BM - 1) / BM, nq = (sq + kBwdTile - 1) / kBwdTile;
   const int nk = (sk + kBwdTile - 1) / kBwdTile;
-  const int bh = blockIdx.x % units, id = blockIdx.x / units;
-  const int qb = nqb - 1 - (PARTS ? id % nqb : id), part = PARTS ? id / nqb : 0;   // heaviest first
+  const int bh = group % units, id = group / units;
+  // heaviest first: under the causal mask those of the most keys, otherwise the whole ones
+  const int at = PARTS ? id % nqb : id, qb = CAUSAL ? nqb - 1 - at : at, part = PARTS ? id / nqb : 0;
   const int b = bh / heads, h = bh % heads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
   const int q0 = qb * BM, qw = q0 + wave * 32 * QB;
+  const bool idle = qw >= sq;                        // a wave without a query
   const T* qp = q + b * qsb + h * qsh;
   const T* kp = k + b * ksb + h * ksh;
   const T* vp = v + b * vsb + h * vsh;
@@ -878,11 +885,11 @@ __device__ __forceinline__ void attention_bwd_q(
       landed();
       __syncthreads();
       if (tile + 1 < t1) issue(tile + 1, kbuf1, vbuf1);
-      body(tile, kbuf0, vbuf0);
+      if (!idle) body(tile, kbuf0, vbuf0);
       landed();
       __syncthreads();
       if (tile + 2 < t1) issue(tile + 2, kbuf0, vbuf0);
-      if (tile + 1 < t1) body(tile + 1, kbuf1, vbuf1);
+      if (!idle && tile + 1 < t1) body(tile + 1, kbuf1, vbuf1);
     }
   }
 

@@ -35,6 +35,7 @@ _ROWS_ARGS = (hip.PTR,) * 8 + (hip.I32,) * 4 + (hip.I64,) * 9 + (hip.F32,)
 _OPERAND_ARGS = (hip.I32,) * 4 + (hip.I64,) * 12 + (hip.F32,) * 2 + (hip.I32,)
 _KV_ARGS = (hip.PTR,) * 10 + _OPERAND_ARGS
 _Q_ARGS = (hip.PTR,) * 9 + _OPERAND_ARGS
+_KVQ_ARGS = (hip.PTR,) * 12 + _OPERAND_ARGS + (hip.I32,) * 2
 _THREADS = 64 * ATTN_BWD_WAVES
 _JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64,) + (hip.I32,) * 5
 
@@ -55,8 +56,8 @@ def _program(stage, head_dim, causal, dtype, blocks=1, parts=False) -> hip.Progr
 def unit_kinds(head_dim):
     """(stage, blocks per wave, parts) of the units a call at this head dim may launch."""
     yield "rows", 1, False
-    for stage, dim, blocks in TILE_US:
-        if dim == head_dim:
+    for blocks in range(1, attention_backward_blocks(head_dim) + 1):
+        for stage in ("kvq",) if _joint(head_dim, blocks) else ("kv", "q"):
             yield stage, blocks, False
             yield stage, blocks, True
 
@@ -66,6 +67,7 @@ def _kernel(stage, device, head_dim, causal, dtype, blocks=1, parts=False) -> hi
     found = _KERNELS.get(key)
     if found is None:
         args, threads = {"rows": (_ROWS_ARGS, 256), "kv": (_KV_ARGS, _THREADS), "q": (_Q_ARGS, _THREADS),
+                         "kvq": (_KVQ_ARGS, _THREADS),
                          "kv_join": (_JOIN_ARGS, 256), "q_join": (_JOIN_ARGS, 256)}[stage]
         prog = _program("rows" if stage.endswith("join") else stage, head_dim, causal, dtype, blocks, parts)
         found = _KERNELS[key] = prog.kernel(
@@ -105,69 +107,94 @@ def _operand(t):
     return t, (sb, sh, ss)
 
 
-# What `_plan` prices a stage with, in us on MI355X (fits of replays over sixteen shapes): a workgroup's
-# pass over a 64-row tile with few workgroups on the chip, and with the chip full (the clock and the
-# caches are shared), and its start and end.  Head dim 64 has two workgroups of one block on a CU.
-# Two blocks a wave read each tile half as often and pass twice the rows in 1.7 to 2.1 times the time;
-# one block makes twice the workgroups.  Measured at head dim 128, one / two blocks: bf16 causal 4x32x4096x128 dK and dV
-# 1154 / 1074 us, dQ 1000 / 905; full 8x32x1024x128 319 / 293, 272 / 238; causal 4x16x512x128 23 / 42,
-# 21 / 35.  (At head dim 64 two were slower everywhere: full 8x12x777 49 / 58, 45 / 51.)
-TILE_US = {("kv", 64, 1): (1.03, 1.08, 4.0), ("kv", 128, 1): (1.72, 2.15, 8.0), ("kv", 128, 2): (3.7, 3.95, 14.0),
-           ("kv", 256, 1): (3.7, 4.1, 12.0), ("q", 64, 1): (1.12, 1.15, 3.0), ("q", 128, 1): (1.62, 1.88, 5.0),
+# What `_plan` prices a launch with, in us on MI355X (fits of timings over sixteen shapes): a workgroup's
+# pass over a 64-row tile with few workgroups on the chip, and a CU's with the chip full (the clock and
+# the caches are shared; head dim 64 has two workgroups on a CU), and a workgroup's start and end.
+TILE_US = {("kv", 64, 1): (1.0, 0.9, 4.0), ("kv", 128, 1): (1.72, 2.15, 8.0), ("kv", 128, 2): (3.7, 3.95, 14.0),
+           ("kv", 256, 1): (3.7, 4.1, 12.0), ("q", 64, 1): (1.05, 0.86, 3.0), ("q", 128, 1): (1.62, 1.88, 5.0),
            ("q", 128, 2): (2.95, 3.3, 9.0), ("q", 256, 1): (3.6, 4.0, 8.0)}
-# A split's second launch and its fp32 sums, written and read (through the caches).
-JOIN_US, SUM_BYTES_PER_US, MAX_SUM_BYTES = 4.0, 4e6, 256 << 20
+# A split's further launch and its fp32 sums, written and read (through the caches).
+JOIN_US, SUM_BYTES_PER_US, MAX_SUM_BYTES = 4.0, 7e6, 256 << 20
 CUS = 256
+PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32)
 
 
-def _stage_cost(stage, units, own, other, head_dim, causal, blocks, per):
-    """us of a stage with blocks of `own` rows walking the tiles of the `other` rows in parts of `per`."""
-    few, full, ends = TILE_US[stage, head_dim, blocks]
-    step = 32 * ATTN_BWD_WAVES * blocks // ATTN_BWD_TILE
-    count, tiles = -(-own // (step * ATTN_BWD_TILE)), -(-other // ATTN_BWD_TILE)
-    if not causal:
-        lengths = {tiles: count}
-    else:
-        lengths = {}
-        for i in range(count):
-            n = max(0, tiles - step * i) if stage == "kv" else min(tiles, step * (i + 1))
-            lengths[n] = lengths.get(n, 0) + 1
-    longest = min(per, max(lengths))
-    items = units * sum(m * max(1, -(-n // per)) for n, m in lengths.items())
-    total = units * sum(n * m for n, m in lengths.items())
-    tile = full if items > CUS // 2 else few
-    if causal or head_dim == 64:
-        # longest first, or two to a CU: the last to end are about half a part apart
-        cost = max(longest * few + ends, (total * full + items * ends) / CUS + longest * few / 2)
-    else:
-        cost = -(-items // CUS) * (longest * tile + ends)
-    if max(lengths) > per:
-        width = head_dim * (2 if stage == "kv" else 1)
-        cost += JOIN_US + 8.0 * width * units * own * max(lengths) / per / SUM_BYTES_PER_US
-    return cost
+def _joint(head_dim, blocks):
+    """Whether one launch holds both stages: where a wave's accumulators leave registers for either.  The
+    second stage's workgroups then run beside the last of the first: causal 2x8x1500x128 97 us apart, 57
+    together; 1x4x8192x128 438 and 284; 2x4x77x64 16.4 and 10.9; full 8x12x777x64 95 and 90.  (Long calls
+    of head dim 64 lose a little, their dQ workgroups being three to a CU alone: causal 4x32x4096 964, 977.)"""
+    return head_dim * blocks < 256
+
+
+def _work(stage, units, own, other, head_dim, causal, blocks, per):
+    """(items, tiles, longest item's tiles, bytes of split sums) of a stage with blocks of `own` rows
+    walking the tiles of the `other` rows in parts of `per`."""
+    step = ATTN_BWD_WAVES * blocks // 2              # tiles of a block's own rows
+    rows = step * ATTN_BWD_TILE
+    count, tiles = -(-own // rows), -(-other // ATTN_BWD_TILE)
+    width = head_dim * (2 if stage == "kv" else 1)
+    items = total = longest = sums = 0
+    for i in range(count):
+        n = tiles if not causal else max(0, tiles - step * i) if stage == "kv" else min(tiles, step * (i + 1))
+        m = count if not causal else 1
+        parts = max(1, -(-n // per))
+        items, total, longest = items + m * parts, total + m * n, max(longest, min(n, per))
+        sums += m * parts * rows * width * 8 if parts > 1 else 0
+        if not causal:
+            break
+    return units * items, units * total, longest, units * sums
+
+
+def _launch_cost(works, head_dim, causal, blocks):
+    """us of a launch of `works`, {stage: _work(...)}, and of the joins of what it splits."""
+    items = sum(w[0] for w in works.values())
+    busy = longest = joins = 0.0
+    for stage, (n, tiles, most, sums) in works.items():
+        few, full, ends = TILE_US[stage, head_dim, blocks]
+        # two workgroups on a CU take turns
+        tile = 1.7 * full if head_dim == 64 and items > CUS else few
+        longest = max(longest, most * tile + ends)
+        busy += (tiles * full + n * ends) / CUS
+        joins += JOIN_US + sums / SUM_BYTES_PER_US if sums else 0.0
+    if items <= CUS:
+        return longest + joins
+    if not causal and len(works) == 1:               # equal items: whole rounds
+        return -(-items // CUS) * (most * full + ends) + joins
+    # the heaviest start first, and the last to end are short, unless those of the second stage are longer
+    late = list(works.values())[-1][2] > 2 * list(works.values())[0][2]
+    return max(longest, busy + longest / (2 if late else 8)) + joins
 
 
 @functools.lru_cache(maxsize=4096)
-def _stage_plan(stage, units, own_tiles, other_tiles, head_dim, causal):
-    """(blocks per wave, parts) of the cheapest launch of a stage."""
-    own, other = own_tiles * ATTN_BWD_TILE, other_tiles * ATTN_BWD_TILE
-    width, best = head_dim * (2 if stage == "kv" else 1), None
+def _plan_tiles(units, q_tiles, k_tiles, head_dim, causal):
+    sq, sk, best = q_tiles * ATTN_BWD_TILE, k_tiles * ATTN_BWD_TILE, None
     for blocks in range(1, attention_backward_blocks(head_dim) + 1):
-        for parts in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32):
-            if parts > 1 and (parts > other_tiles // 2
-                              or 4 * parts * units * own * width > MAX_SUM_BYTES):
-                break
-            cost = _stage_cost(stage, units, own, other, head_dim, causal, blocks, -(-other_tiles // parts))
-            if best is None or cost < best[0]:
-                best = (cost, blocks, parts)
-    return best[1:]
+        found = {}
+        for stage, own, other in (("kv", sk, sq), ("q", sq, sk)):
+            width, tiles = head_dim * (2 if stage == "kv" else 1), other // ATTN_BWD_TILE
+            found[stage] = [(p, _work(stage, units, own, other, head_dim, causal, blocks, -(-tiles // p)))
+                            for p in PARTS
+                            if p == 1 or p <= tiles // 2 and 4 * p * units * own * width <= MAX_SUM_BYTES]
+        if _joint(head_dim, blocks):
+            cost, kv, q = min((_launch_cost({"kv": kv, "q": q}, head_dim, causal, blocks), i, j)
+                              for i, kv in found["kv"] for j, q in found["q"])
+        else:
+            (kv_cost, kv), (q_cost, q) = (
+                min((_launch_cost({stage: w}, head_dim, causal, blocks), p) for p, w in found[stage])
+                for stage in ("kv", "q"))
+            cost = kv_cost + q_cost
+        if best is None or cost < best[0]:
+            best = (cost, (blocks, kv, blocks, q))
+    return best[1]
 
 
 def _plan(units, sq, sk, head_dim, causal):
-    """(kv blocks, kv parts, q blocks, q parts) of a call; searched once for the same tile counts."""
-    nq, nk = -(-sq // ATTN_BWD_TILE), -(-sk // ATTN_BWD_TILE)
-    return (_stage_plan("kv", units, nk, nq, head_dim, causal)
-            + _stage_plan("q", units, nq, nk, head_dim, causal))
+    """(kv blocks, kv parts, q blocks, q parts) of a call, the cheapest by TILE_US; searched once for the
+    same tile counts.  Two blocks a wave (head dim 128) read each tile half as often and pass twice the rows
+    in 1.7 to 2.1 times the time, one makes twice the workgroups: bf16 causal 4x32x4096x128 dK and dV 1154 us
+    by one block and 1074 by two, dQ 1000 and 905; causal 4x16x512x128 23 and 42, 21 and 35."""
+    return _plan_tiles(units, -(-sq // ATTN_BWD_TILE), -(-sk // ATTN_BWD_TILE), head_dim, causal)
 
 
 def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
@@ -185,8 +212,8 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
     # scratch: start values and deltas of every padded query row; fp16's bounds; the parts' fp32 sums
     stats = 4 * units * nq * ATTN_BWD_TILE
     bounds = -(-4 * units * (2 * nq + nk) // 256) * 256
-    sums = max(8 * kv_parts * units * Sk * D if kv_parts > 1 else 0,
-               4 * q_parts * units * Sq * D if q_parts > 1 else 0)
+    kv_sums = 8 * kv_parts * units * Sk * D if kv_parts > 1 else 0
+    sums = kv_sums + (4 * q_parts * units * Sq * D if q_parts > 1 else 0)
     buffers = [(q.shape, q.dtype), (k.shape, q.dtype), (k.shape, q.dtype),
                ((2 * stats + bounds + sums,), torch.uint8)]
     grad, tq, tk, tv, out, lse, glse = map(calls.tensor, range(7))
@@ -195,19 +222,28 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
     qs, ks, vs, gs, os = strides
     sizes, steps = (units, H, Sq, Sk), qs + ks + vs + gs + (scale, scale * LOG2E)
     groups = units * (nq + (nk if q.dtype == torch.float16 else 0))
-    launches = [
-        (_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start, ndelta,
-                                             limit, H, Sq, Sk, units) + os + gs + vs + (scale,)),
-        (_kernel("kv", *kind, kv_blocks, kv_parts > 1), (units * kv_parts * -(-Sk // kv_rows),),
-         (tq, tk, tv, grad, start, ndelta, limit, dk, dv, part) + sizes + steps + (kv_per,))]
+    joint = kv_blocks == q_blocks == 1 and _joint(D, 1)
+    kv_groups, q_groups = units * kv_parts * -(-Sk // kv_rows), units * q_parts * -(-Sq // q_rows)
+    read = (tq, tk, tv, grad, start, ndelta, limit)
+    launches = [(_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start,
+                                                     ndelta, limit, H, Sq, Sk, units) + os + gs + vs + (scale,))]
+    if joint:
+        qpart = calls.buffer(3, 2 * stats + bounds + kv_sums)
+        launches.append((_kernel("kvq", *kind, 1, kv_parts > 1 or q_parts > 1), (kv_groups + q_groups,),
+                         read + (dk, dv, dq, part, qpart) + sizes + steps + (kv_per, q_per, kv_groups)))
+    else:
+        qpart = part
+        launches.append((_kernel("kv", *kind, kv_blocks, kv_parts > 1), (kv_groups,),
+                         read + (dk, dv, part) + sizes + steps + (kv_per,)))
     if kv_parts > 1:
         launches.append((_kernel("kv_join", *kind), (-(-units * 2 * Sk * D // 1024),),
                          (part, dk, dv, units * Sk, Sk, Sq, kv_rows, kv_per, int(causal))))
-    launches.append((_kernel("q", *kind, q_blocks, q_parts > 1), (units * q_parts * -(-Sq // q_rows),),
-                     (tq, tk, tv, grad, start, ndelta, limit, dq, part) + sizes + steps + (q_per,)))
+    if not joint:
+        launches.append((_kernel("q", *kind, q_blocks, q_parts > 1), (q_groups,),
+                         read + (dq, part) + sizes + steps + (q_per,)))
     if q_parts > 1:
         launches.append((_kernel("q_join", *kind), (-(-units * Sq * D // 1024),),
-                         (part, dq, 0, units * Sq, Sq, Sk, q_rows, q_per, int(causal))))
+                         (qpart, dq, 0, units * Sq, Sq, Sk, q_rows, q_per, int(causal))))
     return calls.Plan(device, 7, buffers, (0, 1, 2), launches)
 
 

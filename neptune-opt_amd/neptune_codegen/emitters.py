@@ -754,18 +754,29 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
                 f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, "
                 "rows, len, other, block, per, causal);\n}\n")
         return "\n".join(units)
-    outs, args = (("void* dk, void* dv", f"({ctype}*)dk, ({ctype}*)dv") if stage == "kv"
-                  else ("void* dq", f"({ctype}*)dq"))
+    outs = {"kv": "void* dk, void* dv", "q": "void* dq", "kvq": "void* dk, void* dv, void* dq"}[stage]
+    sums = "float* sums" + (", float* qsums" if stage == "kvq" else "")
+    pers = "int per" + (", int qper, int groups" if stage == "kvq" else "")
+
+    def call(which, total, per, group):
+        args = f"({ctype}*)dk, ({ctype}*)dv" if which == "kv" else f"({ctype}*)dq"
+        return (f"nep::attention_bwd_{which}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
+                f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {args}, {total}, units, heads, sq, sk, qsb, "
+                "qsh, qss, ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, "
+                f"{per}, {group});\n")
+
+    body = f"  {call(stage, 'sums', 'per', 'blockIdx.x')}"
+    if stage == "kvq":
+        body = ("  if ((int)blockIdx.x < groups) " + call("kv", "sums", "per", "blockIdx.x")
+                + "  else " + call("q", "qsums", "qper", "(int)blockIdx.x - groups"))
     return "\n".join([
         head,
-        f'extern "C" __global__ void __launch_bounds__({threads}, 1) {name}(const void* q, const void* k, '
-        f"const void* v, const void* go, const float* start, const float* ndelta, const float* bounds, {outs}, "
-        "float* sums, int units, int heads, int sq, int sk, long long qsb, long long qsh, long long qss, "
+        f'extern "C" __global__ void __launch_bounds__({threads}, {2 if head_dim == 64 else 1}) {name}('
+        f"const void* q, const void* k, const void* v, const void* go, const float* start, const float* ndelta, const float* bounds, {outs}, "
+        f"{sums}, int units, int heads, int sq, int sk, long long qsb, long long qsh, long long qss, "
         "long long ksb, long long ksh, long long kss, long long vsb, long long vsh, long long vss, "
-        "long long gsb, long long gsh, long long gss, float scale, float scale_log2, int per) {\n"
-        f"  nep::attention_bwd_{stage}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
-        f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {args}, sums, units, heads, sq, sk, qsb, qsh, qss, "
-        "ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, per);\n}\n"])
+        f"long long gsb, long long gsh, long long gss, float scale, float scale_log2, {pers}) {{\n"
+        + body + "}\n"])
 
 
 # ---------------------------------------------------------------- distillation from top logits
