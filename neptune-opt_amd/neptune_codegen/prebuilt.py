@@ -100,6 +100,49 @@ def _attention_backward_programs():
             for causal in ((True, False) if stage != "rows" else (False,))]
 
 
+def _distill_programs():
+    import torch
+
+    from neptune_codegen.distill import _program, _variant
+
+    out = []
+    for rows, n, dtype in ((16384, 32000, torch.bfloat16), (7168, 32003, torch.bfloat16),
+                           (16384, 4096, torch.bfloat16), (64, 128256, torch.bfloat16),
+                           (4096, 32000, torch.float32), (16, 1000, torch.float32)):
+        z = torch.empty((rows, n), device="meta", dtype=dtype)
+        top = torch.empty((rows, 64), device="meta", dtype=torch.float32)
+        index = torch.empty((rows, 64), device="meta", dtype=torch.int64)
+        out += [_program(stage, _variant(z, n, top, index, rows, n, 64, stage))
+                for stage in ("forward", "backward")]
+    return out
+
+
+def _residual_norm_programs():
+    import torch
+
+    from neptune_codegen.residual_norm import _program, _variant
+
+    out = []
+    for dtype in (torch.bfloat16, torch.float32):
+        for rows, n in ((16384, 4096), (64, 4096), (8, 1024), (16384, 8192)):
+            x = torch.empty((rows, n), device="meta", dtype=dtype)
+            for after, gate in ((True, "group"), (True, "none"), (False, "none")):
+                out += [_program(stage, _variant(x, True, rows, n, after, gate, stage == "backward"))
+                        for stage in ("forward", "backward")]
+    return out
+
+
+def _rotary_programs():
+    from neptune_codegen.rotary import _program
+
+    return [_program(dtype, index, layout, any_rows)
+            for dtype in ("bfloat16", "float16", "float32") for index in ("int32", "int64")
+            for layout, any_rows in (("halves", False), ("halves", True), ("pairs", False), ("pairs", True),
+                                     ("exchanged", False))]
+
+
 def programs():
-    return (_fold_programs() + _row_programs() + _segment_programs() + _attention_programs()
-            + _attention_backward_programs())
+    # (a launch shape that two sizes share is listed once)
+    return list(dict.fromkeys(_fold_programs() + _row_programs() + _segment_programs() + _attention_programs()
+                              + _attention_backward_programs() + _distill_programs()
+                              + _residual_norm_programs() + _rotary_programs()))
