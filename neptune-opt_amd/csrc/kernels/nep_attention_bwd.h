@@ -8,14 +8,26 @@
 //   dQ_i = scale sum_j dS_ij k_j
 // P is recomputed tile by tile from lse, so no score matrix is stored.
 //
-// Three kernels per call, none with an atomic: results do not depend on the order of workgroups.
+// Three stages per call, none with an atomic: results do not depend on the order of workgroups.
 //  * attention_bwd_rows: delta of every query row, and the rows' start values -lse/scale.
-//  * attention_bwd_kv: a workgroup keeps K and V of its keys in registers and walks the query tiles
-//    (dK and dV stay in registers, four products per pair).
+//  * attention_bwd_kv: a workgroup keeps K and V of its keys (in registers, K in LDS where dK and dV take
+//    every AGPR) and walks the query tiles (dK and dV stay in registers, four products per pair).
 //  * attention_bwd_q: a workgroup keeps Q and dO of its queries and walks the key tiles (three
 //    products per pair).
-// One kernel with five products instead of seven would add dQ across key blocks: fp32 atomics,
+// The last two share a launch where a wave has registers for either (head dim 64, and 128 with one block a
+// wave).  Five products instead of seven, with one stage, would add dQ across key blocks: fp32 atomics,
 // whose order changes results, or an fp32 copy of dQ per key block.
+//
+// Bound by the matrix cores at the rate that this card's power allows a product: full bf16 2x16x4096x128
+// runs 550 GFLOP of kv in 422 us (1300 TFLOP/s) and 412 of q in 340 (1210), a library product of 8192^3
+// 1165 to 1220.  Causal 4x32x4096x128: 1003 and 802 us, with the tiles on the diagonal passed whole by
+// the waves that need them and a workgroup's start and end (14 and 9 us: its K and V rows, its gradients)
+// not overlapped, there being one to a CU.  Head dim 64 (fp16 full 8x12x777: 69 us for both stages) passes
+// as many LDS reads and exponentials for half the products, and 7% of rows past the end.
+//
+// Inside a tile the S products stand alone, P is computed beside those of dP, dS beside those of dV (in
+// attention_bwd_q beside the first half of dQ's), each LDS read two steps before its MFMAs: causal
+// 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1867 so; full 2x16x4096x128 874 and 774.
 //
 // Mapping (v_mfma_f32_32x32x16): attention_bwd_kv computes S[i][j] with A = Q rows from LDS and
 // B = K rows in registers, so lane l holds key l % 32 and registers hold queries
@@ -423,21 +435,58 @@ __device__ void attention_bwd_exact_q(const T* __restrict__ qp, const T* __restr
   }
 }
 
-// c += a b with c in vector registers.  The compiler keeps the accumulators of every MFMA of a
-// kernel that needs more than 256 registers in AGPRs, of which there are 256: dK and dV take them
-// all from head dim 128 up, and S and dP beside them would spill.  (`mfma_settle` stands between
-// the last of a chain and the first other use of c: the wait states are the program's here.)
-template <typename T>
+// S and dP of kernels with more than 256 registers: d = c + a b with d in vector registers, from a zero,
+// a given or its own c.  The compiler keeps the accumulators of every MFMA of such a kernel in AGPRs, of
+// which there are 256: the gradients take them (all, for dK and dV from head dim 128 up), S and dP beside
+// them would spill, and each of their values would cost a move before its exponential.  (`mfma_settle`
+// stands between the last of a chain and the first other use of d: the wait states are the program's here,
+// 12 after an MFMA of 8 passes, as the compiler leaves after its own.)
+// B_AGPR: b is kept in AGPRs.
+template <typename T, bool B_AGPR>
 __device__ __forceinline__ void mfma_vgpr(typename AttnIn<T>::vec8 a, typename AttnIn<T>::vec8 b,
                                           f32x16& c) {
+  if constexpr (__is_same(T, __bf16)) {
+    if constexpr (B_AGPR) asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+    else asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  } else {
+    if constexpr (B_AGPR) asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+    else asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  }
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_vgpr_from(typename AttnIn<T>::vec8 a, typename AttnIn<T>::vec8 b,
+                                                 const f32x16& c) {
+  f32x16 d;
   if constexpr (__is_same(T, __bf16))
-    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %3" : "=&v"(d) : "v"(a), "v"(b), "v"(c));
   else
-    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %3" : "=&v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
 }
-__device__ __forceinline__ void mfma_settle(f32x16& c, f32x16& d) {
-  asm volatile("s_nop 7\ns_nop 7\ns_nop 7" : "+v"(c), "+v"(d));
+template <typename T, bool B_AGPR>
+__device__ __forceinline__ f32x16 mfma_vgpr_zero(typename AttnIn<T>::vec8 a, typename AttnIn<T>::vec8 b) {
+  f32x16 d;
+  if constexpr (__is_same(T, __bf16)) {
+    if constexpr (B_AGPR) asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+    else asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  } else {
+    if constexpr (B_AGPR) asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+    else asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  }
+  return d;
 }
+template <int N>
+__device__ __forceinline__ void mfma_settle(f32x16 (&c)[N]) {
+  static_assert(N == 1 || N == 2, "one or two");
+  if constexpr (N == 1) asm volatile("s_nop 15" : "+v"(c[0]));
+  else asm volatile("s_nop 15" : "+v"(c[0]), "+v"(c[1]));
+}
+// Nothing moves across: the steps of the loops below stand in the order they were written, each with the
+// next step's LDS reads in flight and vector operations beside its MFMAs.
+// The registers of an MFMA's c are free for other values once the next MFMA has been issued.
+__device__ __forceinline__ void mfma_read(const f32x16& c) { asm volatile("" : : "v"(c)); }
+__device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
+constexpr int kAhead = 2;               // steps that an LDS read is issued before its MFMAs
 
 // A wave's 32 output rows (acc holds their transpose) go through its own 32 * D * 2 bytes of LDS,
 // 16-byte chunks XORed by row, and out as whole rows of 16 bytes per lane.  Written from the
@@ -479,7 +528,8 @@ __device__ __forceinline__ unsigned char* bwd_tile() {
 // dK and dV.  W waves of 32 KB keys each; a wave's K and V rows and its dK^T and dV^T stay in
 // registers, the workgroup's Q and dO tiles are staged for all of its waves.  One wave per SIMD:
 // at KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1
-// (at 32 keys a wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock).
+// (at 32 keys a wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock: full
+// 2x16x4096x128 955 us, 907 with two blocks).
 // PARTS: each block's query tiles are taken in parts of `per` (64-row tiles, from the block's first);
 // of a block with more than one, each part's fp32 sums go to `sums` [part][bh][key][dK, dV][D] for
 // attention_bwd_join.
@@ -577,51 +627,76 @@ __device__ __forceinline__ void attention_bwd_kv(
       const int i0 = tile * ROWS + sub;
       if (CAUSAL && i0 + 31 < kw) continue;          // every pair hidden
       if (i0 >= sq) continue;
-      f32x16 s[KB], dp[KB];
+      auto starts = [&](const float* p) {            // per register: its query's value
+        f32x16 c;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 a = *(const f32x4*)(sv + sub + 8 * g + 4 * hi);
-        const f32x4 c = *(const f32x4*)(sv + kBwdTile + sub + 8 * g + 4 * hi);
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 w = *(const f32x4*)(p + sub + 8 * g + 4 * hi);
 #pragma unroll
-        for (int x = 0; x < KB; ++x)
+          for (int r = 0; r < 4; ++r) c[4 * g + r] = w[r];
+        }
+        return c;
+      };
+      auto kop = [&](int x, int t) {
+        if constexpr (kKeysInLds) return rd.row(kall, wave * 32 * KB + 32 * x, t);
+        else return kreg[x][t];
+      };
+      // every step's operands, read kAhead steps before
+      vec8 rows[2 * KSTEPS + kAhead], keys[KB][KSTEPS + kAhead], columns[4 * DBLK + kAhead];
+      auto read_step = [&](int n) {
+        if (n < 2 * KSTEPS) rows[n] = n < KSTEPS ? rd.row(qt, sub, n) : rd.row(gt, sub, n - KSTEPS);
+        if (n < KSTEPS) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[x][4 * g + r] = a[r];
-            dp[x][4 * g + r] = c[r];
+          for (int x = 0; x < KB; ++x) keys[x][n] = kop(x, n);
+        }
+        if (n >= 2 * KSTEPS) {
+          const int m = n - 2 * KSTEPS, cs = m / DBLK % 2;
+          if (m < 4 * DBLK) columns[m] = rd.column(m < 2 * DBLK ? gt : qt, sub, cs, m % DBLK);
+        }
+      };
+      f32x16 s[KB], dp[KB], c = starts(sv);
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) read_step(n);
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        read_step(t + kAhead);
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          if constexpr (kFull) {
+            if (t == 0) s[x] = mfma_vgpr_from<T>(rows[t], keys[x][t], c);
+            else mfma_vgpr<T, false>(rows[t], keys[x][t], s[x]);
+          } else {
+            s[x] = In::mfma(rows[t], keys[x][t], t == 0 ? c : s[x]);
           }
+        }
+        if (kFull && t == 1) mfma_read(c);
+        if (t == KSTEPS - 2) c = starts(sv + kBwdTile);
+        if constexpr (kFull) step_end();
       }
-      if constexpr (kFull) {
-#pragma unroll
-        for (int x = 0; x < KB; ++x) asm volatile("s_nop 1" : "+v"(s[x]), "+v"(dp[x]));
-      }
+      // P of the first elements while the products of dP go on
+      constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 * KB + KSTEPS - LATE - 1) / (KSTEPS - LATE);
 #pragma unroll
       for (int t = 0; t < KSTEPS; ++t) {
-        const vec8 a = rd.row(qt, sub, t);
+        read_step(KSTEPS + t + kAhead);
 #pragma unroll
         for (int x = 0; x < KB; ++x) {
-          if constexpr (kFull) mfma_vgpr<T>(a, rd.row(kall, wave * 32 * KB + 32 * x, t), s[x]);
-          else s[x] = In::mfma(a, kreg[x][t], s[x]);
+          if constexpr (kFull) {
+            if (t == 0) dp[x] = mfma_vgpr_from<T>(rows[KSTEPS + t], vreg[x][t], c);
+            else mfma_vgpr<T, false>(rows[KSTEPS + t], vreg[x][t], dp[x]);
+          } else {
+            dp[x] = In::mfma(rows[KSTEPS + t], vreg[x][t], t == 0 ? c : dp[x]);
+          }
         }
-      }
+        if (kFull && t == 1) mfma_read(c);
+        if (kFull && t == LATE) mfma_settle(s);
+        if (t >= LATE) {
 #pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        const vec8 a = rd.row(gt, sub, t);
-#pragma unroll
-        for (int x = 0; x < KB; ++x) {
-          if constexpr (kFull) mfma_vgpr<T>(a, vreg[x][t], dp[x]);
-          else dp[x] = In::mfma(a, vreg[x][t], dp[x]);
+          for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * KB; ++e)
+            s[e / 16][e % 16] = __builtin_amdgcn_exp2f(s[e / 16][e % 16] * scale_log2);
         }
+        if constexpr (kFull) step_end();
       }
-      if constexpr (kFull) {
-#pragma unroll
-        for (int x = 0; x < KB; ++x) mfma_settle(s[x], dp[x]);
-      }
-      u32 pk[KB][8], dk2[KB][8];
-#pragma unroll
-      for (int x = 0; x < KB; ++x) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[x][r] = __builtin_amdgcn_exp2f(s[x][r] * scale_log2);
-      }
+      if constexpr (kFull) mfma_settle(dp);
       // rows past the end are zero and P = 2^-inf, but not where K or V of the lane's key is
       // infinite or NaN: they are hidden too
       if ((CAUSAL && i0 < kw + 32 * KB - 1) || i0 + 32 > sq) {
@@ -637,36 +712,47 @@ __device__ __forceinline__ void attention_bwd_kv(
           }
         }
       }
+      u32 pk[KB][8], dk2[KB][8];
+      auto pack_p = [&](int x, int w) { pk[x][w] = In::pack2(s[x][2 * w], s[x][2 * w + 1]); };
+      auto pack_ds = [&](int x, int w) {
+        float u = s[x][2 * w], v = s[x][2 * w + 1];
+        if constexpr (kScaled) {
+          u *= ds_mul;
+          v *= ds_mul;
+        }
+        dk2[x][w] = In::pack2(u * dp[x][2 * w], v * dp[x][2 * w + 1]);
+      };
 #pragma unroll
       for (int x = 0; x < KB; ++x)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          pk[x][r >> 1] = In::pack2(s[x][r], s[x][r + 1]);
-          float a = s[x][r], c = s[x][r + 1];
-          if constexpr (kScaled) {
-            a *= ds_mul;
-            c *= ds_mul;
-          }
-          dk2[x][r >> 1] = In::pack2(a * dp[x][r], c * dp[x][r + 1]);
+        for (int w = 0; w < 4; ++w) pack_p(x, w);
+      if constexpr (kFull) step_end();
+      // dV; beside it the rest of P, then dS
+      constexpr int WORDS_STEP = (4 * KB + DBLK - 1) / DBLK, LATER = (8 * KB + DBLK - 1) / DBLK;
+#pragma unroll
+      for (int n = 0; n < 2 * DBLK; ++n) {
+        read_step(2 * KSTEPS + n + kAhead);
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+          dva[x][n % DBLK] = In::mfma(columns[n], packed_operand<T>(pk[x], n / DBLK), dva[x][n % DBLK]);
+        // words in the order they are needed: P's 4..7 before the second half, then dS's 0..7
+        if (n < DBLK) {
+#pragma unroll
+          for (int w = n * WORDS_STEP; w < (n + 1) * WORDS_STEP && w < 4 * KB; ++w) pack_p(w / 4, 4 + w % 4);
+        } else {
+#pragma unroll
+          for (int w = (n - DBLK) * LATER; w < (n - DBLK + 1) * LATER && w < 8 * KB; ++w) pack_ds(w / 8, w % 8);
         }
+        if constexpr (kFull) step_end();
+      }
 #pragma unroll
-      for (int cs = 0; cs < 2; ++cs)
+      for (int n = 0; n < 2 * DBLK; ++n) {
+        read_step(2 * KSTEPS + 2 * DBLK + n + kAhead);
 #pragma unroll
-        for (int a = 0; a < DBLK; ++a) {
-          const vec8 t = rd.column(gt, sub, cs, a);
-#pragma unroll
-          for (int x = 0; x < KB; ++x)
-            dva[x][a] = In::mfma(t, packed_operand<T>(pk[x], cs), dva[x][a]);
-        }
-#pragma unroll
-      for (int cs = 0; cs < 2; ++cs)
-#pragma unroll
-        for (int a = 0; a < DBLK; ++a) {
-          const vec8 t = rd.column(qt, sub, cs, a);
-#pragma unroll
-          for (int x = 0; x < KB; ++x)
-            dka[x][a] = In::mfma(t, packed_operand<T>(dk2[x], cs), dka[x][a]);
-        }
+        for (int x = 0; x < KB; ++x)
+          dka[x][n % DBLK] = In::mfma(columns[2 * DBLK + n], packed_operand<T>(dk2[x], n / DBLK), dka[x][n % DBLK]);
+        if constexpr (kFull) step_end();
+      }
     }
   };
 
@@ -758,6 +844,7 @@ __device__ __forceinline__ void attention_bwd_q(
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
   constexpr int TILE = kBwdTile * D * 2;
   constexpr bool kScaled = BwdIn<T>::kScaled;
+  constexpr bool kFull = D * QB >= 256;              // more than 256 registers
   unsigned char *const kbuf0 = bwd_tile<TILE, 0>(), *const kbuf1 = bwd_tile<TILE, 1>(),
                 *const vbuf0 = bwd_tile<TILE, 2>(), *const vbuf1 = bwd_tile<TILE, 3>();
 
@@ -800,11 +887,18 @@ __device__ __forceinline__ void attention_bwd_q(
       }
     }
   }
+  if constexpr (kFull) {
+#pragma unroll
+    for (int x = 0; x < QB; ++x)
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) asm("" : "+a"(greg[x][s]));
+  }
   int lift = 0;
   if constexpr (kScaled)
     lift = bwd_exponent(bounds + 2 * (i64)bh * nq, nq, bounds + 2 * (i64)units * nq + (i64)bh * nk,
                         nk, lane);
-  const float ds_mul = exp2_int(lift);
+#pragma unroll
+  for (int x = 0; x < QB; ++x) shift[x] += (float)lift;   // P times the power of two of dS
 
   const BwdTile<D, W> kdma(wave, lane, kss), vdma(wave, lane, vss);
   const BwdRead<T, D> rd(lane);
@@ -826,29 +920,57 @@ __device__ __forceinline__ void attention_bwd_q(
       const int j0 = tile * kBwdTile + sub;
       if (CAUSAL && j0 > qw + 32 * QB - 1) continue;   // every pair hidden
       if (j0 >= sk) continue;
+      // every step's operands, read kAhead steps before
+      vec8 rows[2 * KSTEPS + kAhead], columns[2 * DBLK + kAhead];
+      auto read_step = [&](int n) {
+        if (n < 2 * KSTEPS) {
+          rows[n] = n < KSTEPS ? rd.row(kt, sub, n) : rd.row(vt, sub, n - KSTEPS);
+        } else {
+          const int m = n - 2 * KSTEPS;
+          if (m < 2 * DBLK) columns[m] = rd.column(kt, sub, m / DBLK, m % DBLK);
+        }
+      };
       f32x16 s[QB], dp[QB];
 #pragma unroll
-      for (int x = 0; x < QB; ++x) s[x] = dp[x] = f32x16{};
+      for (int n = 0; n < kAhead; ++n) read_step(n);
 #pragma unroll
       for (int t = 0; t < KSTEPS; ++t) {
-        const vec8 a = rd.row(kt, sub, t);
+        read_step(t + kAhead);
 #pragma unroll
-        for (int x = 0; x < QB; ++x) s[x] = In::mfma(a, qreg[x][t], s[x]);
-      }
-#pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        const vec8 a = rd.row(vt, sub, t);
-#pragma unroll
-        for (int x = 0; x < QB; ++x) dp[x] = In::mfma(a, greg[x][t], dp[x]);
-      }
-#pragma unroll
-      for (int x = 0; x < QB; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], scale_log2, shift[x]));
-          if constexpr (kScaled) p *= ds_mul;
-          s[x][r] = p * (dp[x][r] + minus[x]);
+        for (int x = 0; x < QB; ++x) {
+          if constexpr (kFull) {
+            if (t == 0) s[x] = mfma_vgpr_zero<T, false>(rows[t], qreg[x][t]);
+            else mfma_vgpr<T, false>(rows[t], qreg[x][t], s[x]);
+          } else {
+            s[x] = In::mfma(rows[t], qreg[x][t], t == 0 ? f32x16{} : s[x]);
+          }
         }
+        if constexpr (kFull) step_end();
+      }
+      // P of the first elements while the products of dP go on
+      constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 * QB + KSTEPS - LATE - 1) / (KSTEPS - LATE);
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        read_step(KSTEPS + t + kAhead);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+          if constexpr (kFull) {
+            if (t == 0) dp[x] = mfma_vgpr_zero<T, true>(rows[KSTEPS + t], greg[x][t]);
+            else mfma_vgpr<T, true>(rows[KSTEPS + t], greg[x][t], dp[x]);
+          } else {
+            dp[x] = In::mfma(rows[KSTEPS + t], greg[x][t], t == 0 ? f32x16{} : dp[x]);
+          }
+        }
+        if (kFull && t == LATE) mfma_settle(s);
+        if (t >= LATE) {
+#pragma unroll
+          for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * QB; ++e)
+            s[e / 16][e % 16] =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], scale_log2, shift[e / 16]));
+        }
+        if constexpr (kFull) step_end();
+      }
+      if constexpr (kFull) mfma_settle(dp);
       const bool masked = (CAUSAL && j0 + 31 > qw) || j0 + 32 > sk;
       if (masked) {
         if (CAUSAL) bad |= rd.nonfinite(kt, sub);
@@ -858,23 +980,35 @@ __device__ __forceinline__ void attention_bwd_q(
           const int end = (CAUSAL ? min(sk, i + 1) : sk) - j0 - 4 * hi;   // register rows from it on
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (8 * (r >> 2) + (r & 3) >= end) s[x][r] = 0.0f;
+            if (8 * (r >> 2) + (r & 3) >= end) {
+              s[x][r] = 0.0f;
+              dp[x][r] = -minus[x];
+            }
         }
       }
       u32 pk[QB][8];
+      auto pack_ds = [&](int x, int w) {
+        pk[x][w] = In::pack2(s[x][2 * w] * (dp[x][2 * w] + minus[x]),
+                             s[x][2 * w + 1] * (dp[x][2 * w + 1] + minus[x]));
+      };
 #pragma unroll
       for (int x = 0; x < QB; ++x)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) pk[x][r >> 1] = In::pack2(s[x][r], s[x][r + 1]);
+        for (int w = 0; w < 4; ++w) pack_ds(x, w);
+      if constexpr (kFull) step_end();
+      constexpr int WORDS_STEP = (4 * QB + DBLK - 1) / DBLK;
 #pragma unroll
-      for (int cs = 0; cs < 2; ++cs)
+      for (int n = 0; n < 2 * DBLK; ++n) {
+        read_step(2 * KSTEPS + n + kAhead);
 #pragma unroll
-        for (int a = 0; a < DBLK; ++a) {
-          const vec8 t = rd.column(kt, sub, cs, a);
+        for (int x = 0; x < QB; ++x)
+          dqa[x][n % DBLK] = In::mfma(columns[n], packed_operand<T>(pk[x], n / DBLK), dqa[x][n % DBLK]);
+        if (n < DBLK) {
 #pragma unroll
-          for (int x = 0; x < QB; ++x)
-            dqa[x][a] = In::mfma(t, packed_operand<T>(pk[x], cs), dqa[x][a]);
+          for (int w = n * WORDS_STEP; w < (n + 1) * WORDS_STEP && w < 4 * QB; ++w) pack_ds(w / 4, 4 + w % 4);
         }
+        if constexpr (kFull) step_end();
+      }
     }
   };
 
