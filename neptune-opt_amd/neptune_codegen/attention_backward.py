@@ -268,8 +268,9 @@ def _run(grad, q, k, v, out, lse, grad_lse, scale, causal, plan=None):
     validate_attention_backward_inputs(grad, q, k, v, out, lse, grad_lse, metadata=metadata)
     given, number = (grad, q, k, v, out, lse, grad_lse), scale
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-    if not math.isfinite(scale) or scale <= 0:
-        raise ValueError("attention scale must be finite and positive")
+    # (the kernels hold lse / scale in fp32)
+    if not 2.0 ** -100 <= scale <= calls.MOST_FLOAT:
+        raise ValueError("attention scale must be finite and positive, from 2^-100 to 2^125")
     if metadata or q.numel() == 0:
         # without a query nothing reaches the keys
         return (torch.empty(q.shape, dtype=q.dtype, device=q.device),

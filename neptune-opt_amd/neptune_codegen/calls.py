@@ -13,6 +13,8 @@ from neptune_codegen import dispatch, hip
 
 # a launch has fewer than 2^32 work-items in each dimension of its grid
 MOST_THREADS = (1 << 32) - 1
+# what kernels take as an fp32 number, and as its product with a number below 4
+LEAST_FLOAT, MOST_FLOAT = 2.0 ** -126, 2.0 ** 125
 
 
 class tensor:

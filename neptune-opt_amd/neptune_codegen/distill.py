@@ -43,8 +43,9 @@ def _program(stage: str, var: DistillVariant) -> hip.Program:
 
 
 def _temperature(temperature) -> float:
-    if type(temperature) not in (int, float) or not math.isfinite(temperature) or temperature <= 0:
-        raise ValueError("distillation needs a finite positive temperature")
+    # (its square and its reciprocal are fp32 numbers)
+    if type(temperature) not in (int, float) or not 1e-18 <= temperature <= 1e18:
+        raise ValueError("distillation needs a temperature from 1e-18 to 1e18")
     return float(temperature)
 
 

@@ -97,14 +97,15 @@ def validate_residual_norm_inputs(x, y, gamma_after, gamma_before, gate=None, *,
 
 
 def _scale(residual_scale) -> float:
-    if type(residual_scale) not in (int, float) or not math.isfinite(residual_scale):
-        raise ValueError("residual norm needs a finite residual_scale")
+    if type(residual_scale) not in (int, float) or not abs(residual_scale) <= calls.MOST_FLOAT:
+        raise ValueError("residual norm needs a residual_scale that is finite in fp32")
     return float(residual_scale)
 
 
 def _eps(eps) -> float:
-    if type(eps) not in (int, float) or not math.isfinite(eps) or eps <= 0:
-        raise ValueError("residual norm needs a finite positive eps")
+    # (a smaller one would be 0 or a denormal in fp32, and a row of zeros NaN)
+    if type(eps) not in (int, float) or not calls.LEAST_FLOAT <= eps <= calls.MOST_FLOAT:
+        raise ValueError("residual norm needs a positive eps that is a normal number in fp32")
     return float(eps)
 
 

@@ -124,8 +124,8 @@ def _run(q, k, positions, turns, magnitude, interleaved, sign):
         return found
     metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
     validate_rotary_inputs(*given, metadata=metadata)
-    if type(magnitude) not in (int, float) or not math.isfinite(magnitude):
-        raise ValueError("rotary magnitude must be a finite number")
+    if type(magnitude) not in (int, float) or not abs(magnitude) <= calls.MOST_FLOAT:
+        raise ValueError("rotary magnitude must be a number that is finite in fp32")
     if metadata or not (q.numel() or (k is not None and k.numel())):
         return tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     used = tuple(t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k))
@@ -179,8 +179,8 @@ def as_rotary_op(magnitude: float = 1.0, interleaved: bool = False, lib: str = "
 
     from neptune_codegen.autotune import parameter_tag
 
-    if type(magnitude) not in (int, float) or not math.isfinite(magnitude):
-        raise ValueError("rotary magnitude must be a finite number")
+    if type(magnitude) not in (int, float) or not abs(magnitude) <= calls.MOST_FLOAT:
+        raise ValueError("rotary magnitude must be a number that is finite in fp32")
     magnitude, interleaved = float(magnitude), bool(interleaved)
     key = (lib, magnitude, interleaved)
     with _lock:
