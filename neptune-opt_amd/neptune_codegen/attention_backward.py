@@ -127,7 +127,7 @@ def _joint(head_dim, blocks):
     return head_dim * blocks < 256
 
 
-def _work(stage, units, own, other, head_dim, causal, blocks, per):
+def _stage_work(stage, units, own, other, head_dim, causal, blocks, per):
     """(items, tiles, longest item's tiles, bytes of split sums) of a stage with blocks of `own` rows
     walking the tiles of the `other` rows in parts of `per`."""
     step = ATTN_BWD_WAVES * blocks // 2              # tiles of a block's own rows
@@ -147,7 +147,7 @@ def _work(stage, units, own, other, head_dim, causal, blocks, per):
 
 
 def _launch_cost(works, head_dim, causal, blocks):
-    """us of a launch of `works`, {stage: _work(...)}, and of the joins of what it splits."""
+    """us of a launch of `works`, {stage: _stage_work(...)}, and of the joins of what it splits."""
     items = sum(w[0] for w in works.values())
     busy = longest = joins = 0.0
     for stage, (n, tiles, most, sums) in works.items():
@@ -173,7 +173,7 @@ def _plan_tiles(units, q_tiles, k_tiles, head_dim, causal):
         found = {}
         for stage, own, other in (("kv", sk, sq), ("q", sq, sk)):
             width, tiles = head_dim * (2 if stage == "kv" else 1), other // ATTN_BWD_TILE
-            found[stage] = [(p, _work(stage, units, own, other, head_dim, causal, blocks, -(-tiles // p)))
+            found[stage] = [(p, _stage_work(stage, units, own, other, head_dim, causal, blocks, -(-tiles // p)))
                             for p in PARTS
                             if p == 1 or p <= tiles // 2 and 4 * p * units * own * width <= MAX_SUM_BYTES]
         if _joint(head_dim, blocks):

@@ -715,9 +715,10 @@ def attention_backward_blocks(head_dim: int) -> int:
 
 def attention_backward_kernel_name(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
                                    blocks: int = 1, parts: bool = False) -> str:
-    """Symbol of one stage of attention's gradients: "rows", "kv", "q", "kv_join" or "q_join"."""
+    """Symbol of one stage of attention's gradients: "rows", "kv", "q", "kvq", "kv_join" or
+    "q_join"."""
     tag, _ = _attn_dtype(dtype)
-    if stage not in ("kv", "q"):
+    if stage not in ("kv", "q", "kvq"):
         return f"attention_bwd_{stage}_{tag}_d{head_dim}"
     return (f"attention_bwd_{stage}_{tag}_d{head_dim}_{'causal' if causal else 'full'}_b{blocks}"
             f"{'_parts' if parts else ''}")
@@ -726,7 +727,9 @@ def attention_backward_kernel_name(stage: str, head_dim: int, causal: bool, dtyp
 def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
                                    blocks: int = 1, parts: bool = False) -> str:
     """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics with the joins
-    of split ranges ("rows"; the mask does not matter), dK and dV ("kv"), or dQ ("q")."""
+    of split ranges ("rows"; the mask does not matter), dK and dV ("kv"), dQ ("q"), or the last two in one
+    launch ("kvq": its first `groups` workgroups take dK and dV).  At head dim 64 two workgroups share a
+    CU, and so a SIMD's 512 registers."""
     if head_dim not in ATTN_HEAD_DIMS:
         raise NotImplementedError("attention fold supports head_dim 64, 128 and 256")
     if not 1 <= blocks <= attention_backward_blocks(head_dim):
