@@ -52,21 +52,37 @@ struct RowLanes {
   }
 };
 
-// The whole words of a row (those of its Span), read through a buffer: word i of the row, zero past
-// the end.  No access is in a branch, so a wait for one tile leaves the next one in flight (in branches
-// the waits are for everything, and a tile is not started until the one before it is done).
+// The whole words of a row (those of its Span), read through a buffer, zero past the end.  No access is in a
+// branch, so a wait for one tile leaves the next one in flight (in branches the waits are for everything,
+// and a tile is not started until the one before it is done).
+// LINES: word 0 is the start of the cache line that the row's first word is in, and the lanes before `skip`
+// take the first word too (and write the same value): a wavefront's words are whole lines.  For the gradient
+// of wide rows, which writes them: 7168 rows of 32003 159 us, 167 from the first word on; the loss, and
+// rows that a wavefront holds, lose by the longer row (16384 rows of 1000 13.6 us, 14.7).
 constexpr u32 kPastRow = 0x80000000u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* p) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, 0x7fffffff, 0x00020000);
-}
-template <int TPR, int UNROLL>
-__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t row, int first, int words, int t, u32x4* w) {
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const int i = first + u * TPR + t;
-    w[u] = __builtin_amdgcn_raw_buffer_load_b128(row, i < words ? (u32)i * 16u : kPastRow, 0, 2);
+template <class St, class Sp, bool LINES>
+struct RowWords {
+  __amdgpu_buffer_rsrc_t row;
+  int skip, words;
+  i64 line;                                          // column of word 0
+
+  __device__ __forceinline__ RowWords(const typename St::T* rp, const Sp& sp) {
+    skip = LINES ? (int)(((u64)(rp + sp.v0) >> 4) & 7) : 0;
+    line = sp.v0 - skip * St::kVec;
+    words = sp.v1 > sp.v0 ? skip + (int)((sp.v1 - sp.v0) / St::kVec) : 0;
+    row = __builtin_amdgcn_make_buffer_rsrc((void*)(rp + line), (short)0, 0x7fffffff, 0x00020000);
   }
-}
+  // words first + u TPR + t of a tile
+  template <int TPR, int UNROLL>
+  __device__ __forceinline__ void load(int first, int t, u32x4* w) const {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = first + u * TPR + t;
+      w[u] = __builtin_amdgcn_raw_buffer_load_b128(row, i < words ? (u32)at(i) * 16u : kPastRow, 0, 2);
+    }
+  }
+  __device__ __forceinline__ int at(int i) const { return LINES && i < skip ? skip : i; }
+};
 
 // A row's entries, EPL per lane: entry k of lane t is t + k TPR.
 template <class Lt, typename Ix, int TPR, int EPL>
@@ -150,8 +166,8 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
   for (int k = 0; k < EPL; ++k) zk[k] = list.at[k] >= 0 ? St::load(rp + list.at[k]) : 0.0f;
 
   const Sp sp(rp, 0, live ? n : 0);
-  const __amdgpu_buffer_rsrc_t row_words = row_buffer(rp + sp.v0);
-  const int words = (int)((sp.v1 - sp.v0) / VEC);
+  const RowWords<St, Sp, false> row_words(rp, sp);
+  const int words = row_words.words;
   float m = -kInf, s = 0.0f;
   u32x4 cur[UNROLL];
   auto move = [&](float tile_max) {
@@ -184,13 +200,13 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
     }
     s += a + b;
   };
-  load_words<TPR, UNROLL>(row_words, 0, words, t, cur);
+  row_words.template load<TPR, UNROLL>(0, t, cur);
   typename Sp::Rest rest;
   if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
   int at = 0;
   for (; at + UNROLL * TPR <= words; at += UNROLL * TPR) {
     u32x4 next[UNROLL];
-    load_words<TPR, UNROLL>(row_words, at + UNROLL * TPR, words, t, next);
+    row_words.template load<TPR, UNROLL>(at + UNROLL * TPR, t, next);
     tile();
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) cur[u] = next[u];
@@ -264,10 +280,10 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   const typename St::T* rp = z + (live ? row : 0) * stride_z;
   typename St::T* op = dz + (live ? row : 0) * n;
   const Sp sp(rp, 0, live ? n : 0);
-  const __amdgpu_buffer_rsrc_t row_words = row_buffer(rp + sp.v0);
-  const int words = (int)((sp.v1 - sp.v0) / VEC);
+  const RowWords<St, Sp, (TPR > 64)> row_words(rp, sp);
+  const int words = row_words.words;
   u32x4 cur[UNROLL];
-  load_words<TPR, UNROLL>(row_words, 0, words, t, cur);
+  row_words.template load<TPR, UNROLL>(0, t, cur);
   TeacherList<Lt, Ix, TPR, EPL> list;
   list.load(top_logits + (live ? row : 0) * stride_t, index + (live ? row : 0) * stride_i, count, n, t, live);
   float zk[EPL];
@@ -304,22 +320,22 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   } else {
     typename Sp::Rest rest;
     if constexpr (ACCESS == kRagged) sp.load_rest(rest, rp, t);
-    typename St::T* ow = op + sp.v0 + (i64)t * VEC;
+    typename St::T* ow = op + row_words.line;
     auto put = [&](int u, int at) {
       float v[VEC];
       St::unpack(cur[u], v);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
-      store_vec<ACCESS>(ow + (i64)(at + u * TPR) * VEC, St::pack(v));
+      store_vec<ACCESS>(ow + (i64)row_words.at(at + u * TPR + t) * VEC, St::pack(v));
     };
     // as many writes as a tile makes, to nowhere: the first wait counts what every other does
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      __builtin_amdgcn_raw_buffer_store_b32(0u, row_words, kPastRow + 4u * u, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(0u, row_words.row, kPastRow + 4u * u, 0, 0);
     int at = 0;
     for (; at + UNROLL * TPR <= words; at += UNROLL * TPR) {
       u32x4 next[UNROLL];
-      load_words<TPR, UNROLL>(row_words, at + UNROLL * TPR, words, t, next);
+      row_words.template load<TPR, UNROLL>(at + UNROLL * TPR, t, next);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) put(u, at);
 #pragma unroll

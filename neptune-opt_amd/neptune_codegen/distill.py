@@ -71,8 +71,8 @@ def validate_distill_inputs(logits, top_logits, top_index, *, metadata: bool = F
         raise ValueError("distillation tensors must be on the same device")
     if not 1 <= top_logits.shape[-1] <= MAX_ENTRIES:
         raise NotImplementedError(f"distillation takes lists of 1 to {MAX_ENTRIES} entries")
-    if logits.shape[-1] >= 1 << 29:
-        raise NotImplementedError("distillation takes rows of less than 2^29 logits")
+    if logits.shape[-1] >= 1 << 28:
+        raise NotImplementedError("distillation takes rows of less than 2^28 logits")
     return lead
 
 
