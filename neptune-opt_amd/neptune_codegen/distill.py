@@ -88,29 +88,36 @@ def _check_rows(t, name, shape, logits, *, metadata):
 def _variant(z, stride: int, top, index, rows: int, n: int, count: int, stage: str) -> DistillVariant:
     """Lanes per row and 16-byte slots a lane has in flight.
 
-    Forward: a wavefront up to 512 slots (16384 rows of 4096 bf16: 31 us, 42 with 256 lanes), 256 lanes
-    beyond (16384 rows of 32000: 157 us, 164 with 512, 201 with 1024), 1024 where 512 rows or fewer would
-    leave CUs idle (64 rows of 128256: 11.1 us, 13.4 with 256).  Eight slots in flight where a CU has four
-    workgroups (7168 rows of 32003: 73.5 us, 77.1 with four), four below (600 rows of 50000: 15.7 us, 17.4).
+    Forward: a wavefront up to 512 slots (16384 rows of 4096 bf16: 27 us, 37 with 256 lanes) and, where the
+    rows fill the chip with wavefronts, up to 1536 (8192 rows of 10007: 32 us, 36); 256 lanes beyond (16384
+    rows of 32000: 151 us, 164 with 512, 201 with 1024), 1024 where 512 rows or fewer would leave CUs idle
+    (64 rows of 128256: 11 us, 13.4 with 256).  Eight slots in flight where a CU has four workgroups (7168
+    rows of 32003: 73.5 us, 77.1 with four), four below (600 rows of 50000: 15.7 us, 17.4).
     Backward, which reads and writes and so wants few rows open at once: a wavefront up to 256 slots (16384
-    rows of 1000: 21.4 us, 24.6 with 128), 256 lanes up to 2048 (16384 rows of 4096: 63 us, 69 with a
-    wavefront), 1024 beyond (7168 rows of 32003: 169 us, 193 with 256; fp32 4096 rows of 32000: 176, 190).
-    A tile of lanes x slots is never wider than the row: 16384 rows of 32000 by 1024 lanes take 368 us with
-    two slots, 442 with four."""
+    rows of 1000: 20.4 us, 24.6 with 128), 256 lanes up to 2048 (16384 rows of 4096: 58 us, 67 with a
+    wavefront), 1024 beyond (16384 rows of 32000: 368 us, 392 with 256; fp32 4096 rows of 32000: 176, 190).
+    A tile of lanes x slots is never wider than the row (16384 rows of 32000 by 1024 lanes take 355 us with
+    two slots, 442 with four), and half as wide where a wavefront or 256 lanes that write hold a row, for the
+    next tile's loads (4096 columns, forward 27.4 us with four slots, 28.7 with eight; backward 61.7 with one,
+    64.1 with two); a row of up to two slots a lane is one tile (16384 rows of 1000: 12.0 us, 13.1)."""
     vec = 16 // z.element_size()
     slots = -(-n // vec)
     aligned = n % vec == 0 and z.data_ptr() % 16 == 0 and stride % vec == 0
     if stage == "forward":
-        tpr = 64 if slots <= 512 and count <= 256 else 1024 if rows <= 512 and slots > 1024 else 256
+        alone = 1536 if rows >= 4096 else 512
+        tpr = 64 if slots <= alone and count <= 256 else 1024 if rows <= 512 and slots > 1024 else 256
         most = 8 if rows >= 1024 else 4
     else:
         tpr = 64 if slots <= 256 and count <= 256 else 256 if slots < 2048 else 1024
         if rows <= 512 and slots > 1024:
             tpr = 1024
         most = 4
-    unroll = 1
-    while unroll < most and tpr * unroll * 2 <= slots:
+    half = tpr == (64 if stage == "forward" else 256)
+    unroll, widest = 1, slots // 2 if half else slots
+    while unroll < most and tpr * unroll * 2 <= widest:
         unroll *= 2
+    if stage == "forward" and tpr < slots <= 2 * tpr:
+        unroll = 2
     entries = 1
     while entries * tpr < count:
         entries *= 2
