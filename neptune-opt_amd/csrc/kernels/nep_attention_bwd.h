@@ -547,8 +547,8 @@ __device__ __forceinline__ void attention_bwd_kv(
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
   constexpr int ROWS = D <= 128 ? kBwdTile : 32;     // queries per staged tile
   constexpr int TILE = ROWS * D * 2;
-  constexpr bool kFull = D * KB >= 256;              // dK and dV take every AGPR
-  constexpr bool kKeysInLds = kFull;                 // and K no vector register
+  constexpr bool kOwn = D * KB >= 128;               // more than 256 registers
+  constexpr bool kKeysInLds = D * KB >= 256;         // dK and dV take every AGPR, and K no vector register
   constexpr bool kScaled = BwdIn<T>::kScaled;
   unsigned char *const qbuf0 = bwd_tile<TILE, 0>(), *const qbuf1 = bwd_tile<TILE, 1>(),
                 *const gbuf0 = bwd_tile<TILE, 2>(), *const gbuf1 = bwd_tile<TILE, 3>();
@@ -662,16 +662,16 @@ __device__ __forceinline__ void attention_bwd_kv(
         read_step(t + kAhead);
 #pragma unroll
         for (int x = 0; x < KB; ++x) {
-          if constexpr (kFull) {
+          if constexpr (kOwn) {
             if (t == 0) s[x] = mfma_vgpr_from<T>(rows[t], keys[x][t], c);
             else mfma_vgpr<T, false>(rows[t], keys[x][t], s[x]);
           } else {
             s[x] = In::mfma(rows[t], keys[x][t], t == 0 ? c : s[x]);
           }
         }
-        if (kFull && t == 1) mfma_read(c);
+        if (kOwn && t == 1) mfma_read(c);
         if (t == KSTEPS - 2) c = starts(sv + kBwdTile);
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
       // P of the first elements while the products of dP go on
       constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 * KB + KSTEPS - LATE - 1) / (KSTEPS - LATE);
@@ -680,23 +680,23 @@ __device__ __forceinline__ void attention_bwd_kv(
         read_step(KSTEPS + t + kAhead);
 #pragma unroll
         for (int x = 0; x < KB; ++x) {
-          if constexpr (kFull) {
+          if constexpr (kOwn) {
             if (t == 0) dp[x] = mfma_vgpr_from<T>(rows[KSTEPS + t], vreg[x][t], c);
             else mfma_vgpr<T, false>(rows[KSTEPS + t], vreg[x][t], dp[x]);
           } else {
             dp[x] = In::mfma(rows[KSTEPS + t], vreg[x][t], t == 0 ? c : dp[x]);
           }
         }
-        if (kFull && t == 1) mfma_read(c);
-        if (kFull && t == LATE) mfma_settle(s);
+        if (kOwn && t == 1) mfma_read(c);
+        if (kOwn && t == LATE) mfma_settle(s);
         if (t >= LATE) {
 #pragma unroll
           for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * KB; ++e)
             s[e / 16][e % 16] = __builtin_amdgcn_exp2f(s[e / 16][e % 16] * scale_log2);
         }
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
-      if constexpr (kFull) mfma_settle(dp);
+      if constexpr (kOwn) mfma_settle(dp);
       // rows past the end are zero and P = 2^-inf, but not where K or V of the lane's key is
       // infinite or NaN: they are hidden too
       if ((CAUSAL && i0 < kw + 32 * KB - 1) || i0 + 32 > sq) {
@@ -726,7 +726,7 @@ __device__ __forceinline__ void attention_bwd_kv(
       for (int x = 0; x < KB; ++x)
 #pragma unroll
         for (int w = 0; w < 4; ++w) pack_p(x, w);
-      if constexpr (kFull) step_end();
+      if constexpr (kOwn) step_end();
       // dV; beside it the rest of P, then dS
       constexpr int WORDS_STEP = (4 * KB + DBLK - 1) / DBLK, LATER = (8 * KB + DBLK - 1) / DBLK;
 #pragma unroll
@@ -743,7 +743,7 @@ __device__ __forceinline__ void attention_bwd_kv(
 #pragma unroll
           for (int w = (n - DBLK) * LATER; w < (n - DBLK + 1) * LATER && w < 8 * KB; ++w) pack_ds(w / 8, w % 8);
         }
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
 #pragma unroll
       for (int n = 0; n < 2 * DBLK; ++n) {
@@ -751,7 +751,7 @@ __device__ __forceinline__ void attention_bwd_kv(
 #pragma unroll
         for (int x = 0; x < KB; ++x)
           dka[x][n % DBLK] = In::mfma(columns[2 * DBLK + n], packed_operand<T>(dk2[x], n / DBLK), dka[x][n % DBLK]);
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
     }
   };
@@ -844,7 +844,7 @@ __device__ __forceinline__ void attention_bwd_q(
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
   constexpr int TILE = kBwdTile * D * 2;
   constexpr bool kScaled = BwdIn<T>::kScaled;
-  constexpr bool kFull = D * QB >= 256;              // more than 256 registers
+  constexpr bool kOwn = D * QB >= 128;              // more than 256 registers
   unsigned char *const kbuf0 = bwd_tile<TILE, 0>(), *const kbuf1 = bwd_tile<TILE, 1>(),
                 *const vbuf0 = bwd_tile<TILE, 2>(), *const vbuf1 = bwd_tile<TILE, 3>();
 
@@ -887,7 +887,7 @@ __device__ __forceinline__ void attention_bwd_q(
       }
     }
   }
-  if constexpr (kFull) {
+  if constexpr (kOwn) {
 #pragma unroll
     for (int x = 0; x < QB; ++x)
 #pragma unroll
@@ -938,14 +938,14 @@ __device__ __forceinline__ void attention_bwd_q(
         read_step(t + kAhead);
 #pragma unroll
         for (int x = 0; x < QB; ++x) {
-          if constexpr (kFull) {
+          if constexpr (kOwn) {
             if (t == 0) s[x] = mfma_vgpr_zero<T, false>(rows[t], qreg[x][t]);
             else mfma_vgpr<T, false>(rows[t], qreg[x][t], s[x]);
           } else {
             s[x] = In::mfma(rows[t], qreg[x][t], t == 0 ? f32x16{} : s[x]);
           }
         }
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
       // P of the first elements while the products of dP go on
       constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 * QB + KSTEPS - LATE - 1) / (KSTEPS - LATE);
@@ -954,23 +954,23 @@ __device__ __forceinline__ void attention_bwd_q(
         read_step(KSTEPS + t + kAhead);
 #pragma unroll
         for (int x = 0; x < QB; ++x) {
-          if constexpr (kFull) {
+          if constexpr (kOwn) {
             if (t == 0) dp[x] = mfma_vgpr_zero<T, true>(rows[KSTEPS + t], greg[x][t]);
             else mfma_vgpr<T, true>(rows[KSTEPS + t], greg[x][t], dp[x]);
           } else {
             dp[x] = In::mfma(rows[KSTEPS + t], greg[x][t], t == 0 ? f32x16{} : dp[x]);
           }
         }
-        if (kFull && t == LATE) mfma_settle(s);
+        if (kOwn && t == LATE) mfma_settle(s);
         if (t >= LATE) {
 #pragma unroll
           for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * QB; ++e)
             s[e / 16][e % 16] =
                 __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], scale_log2, shift[e / 16]));
         }
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
-      if constexpr (kFull) mfma_settle(dp);
+      if constexpr (kOwn) mfma_settle(dp);
       const bool masked = (CAUSAL && j0 + 31 > qw) || j0 + 32 > sk;
       if (masked) {
         if (CAUSAL) bad |= rd.nonfinite(kt, sub);
@@ -995,7 +995,7 @@ __device__ __forceinline__ void attention_bwd_q(
       for (int x = 0; x < QB; ++x)
 #pragma unroll
         for (int w = 0; w < 4; ++w) pack_ds(x, w);
-      if constexpr (kFull) step_end();
+      if constexpr (kOwn) step_end();
       constexpr int WORDS_STEP = (4 * QB + DBLK - 1) / DBLK;
 #pragma unroll
       for (int n = 0; n < 2 * DBLK; ++n) {
@@ -1007,7 +1007,7 @@ __device__ __forceinline__ void attention_bwd_q(
 #pragma unroll
           for (int w = n * WORDS_STEP; w < (n + 1) * WORDS_STEP && w < 4 * QB; ++w) pack_ds(w / 4, 4 + w % 4);
         }
-        if constexpr (kFull) step_end();
+        if constexpr (kOwn) step_end();
       }
     }
   };
