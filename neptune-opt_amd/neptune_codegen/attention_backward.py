@@ -107,12 +107,14 @@ def _operand(t):
     return t, (sb, sh, ss)
 
 
-# What `_plan` prices a launch with, in us on MI355X (fits of timings over sixteen shapes): a workgroup's
+# What `_plan` prices a launch with, in us on MI355X (fits of timings over twenty shapes): a workgroup's
 # pass over a 64-row tile with few workgroups on the chip, and a CU's with the chip full (the clock and
-# the caches are shared; head dim 64 has two workgroups on a CU), and a workgroup's start and end.
-TILE_US = {("kv", 64, 1): (1.0, 0.9, 4.0), ("kv", 128, 1): (1.6, 1.68, 9.0), ("kv", 128, 2): (2.85, 2.85, 28.0),
-           ("kv", 256, 1): (3.3, 3.57, 12.0), ("q", 64, 1): (1.0, 0.82, 3.0), ("q", 128, 1): (1.45, 1.44, 7.0),
-           ("q", 128, 2): (2.33, 2.33, 21.0), ("q", 256, 1): (2.4, 2.62, 8.0)}
+# the caches are shared; head dim 64 has two workgroups on a CU); and a workgroup's start and end, without
+# the mask and with it (its waves then wait for each other on the diagonal).
+TILE_US = {("kv", 64, 1): (1.0, 0.9, 4.0, 4.0), ("q", 64, 1): (1.0, 0.82, 3.0, 3.0),
+           ("kv", 128, 1): (1.6, 1.7, 7.0, 8.0), ("q", 128, 1): (1.45, 1.45, 7.0, 8.0),
+           ("kv", 128, 2): (2.9, 3.07, 11.0, 22.0), ("q", 128, 2): (2.4, 2.45, 11.5, 19.0),
+           ("kv", 256, 1): (3.3, 3.57, 12.0, 12.0), ("q", 256, 1): (2.4, 2.62, 8.0, 8.0)}
 # A split's further launch and its fp32 sums, written and read (through the caches).
 JOIN_US, SUM_BYTES_PER_US, MAX_SUM_BYTES = 4.0, 7e6, 256 << 20
 CUS = 256
@@ -151,7 +153,8 @@ def _launch_cost(works, head_dim, causal, blocks):
     items = sum(w[0] for w in works.values())
     busy = longest = joins = 0.0
     for stage, (n, tiles, most, sums) in works.items():
-        few, full, ends = TILE_US[stage, head_dim, blocks]
+        few, full, *ends = TILE_US[stage, head_dim, blocks]
+        ends = ends[causal]
         # two workgroups on a CU take turns
         tile = 1.7 * full if head_dim == 64 and items > CUS else few
         longest = max(longest, most * tile + ends)
@@ -192,8 +195,8 @@ def _plan_tiles(units, q_tiles, k_tiles, head_dim, causal):
 def _plan(units, sq, sk, head_dim, causal):
     """(kv blocks, kv parts, q blocks, q parts) of a call, the cheapest by TILE_US; searched once for the
     same tile counts.  Two blocks a wave (head dim 128) read each tile half as often and pass twice the rows
-    in 1.6 to 1.7 times the time, but a workgroup starts and ends three times as long: bf16 causal
-    4x32x4096x128 1861 us by two, 1900 by one; full 2x16x4096x128 800 and 875; causal 8x32x1024x128 398 and
+    in 1.7 to 1.8 times the time, with a longer start and end: bf16 causal 4x32x4096x128 1861 us by two,
+    2072 by one; full 2x16x4096x128 800 and 875, 8x32x1024x128 469 and 555; but causal 8x32x1024x128 398 and
     375, 2x8x300x128 59 and 20."""
     return _plan_tiles(units, -(-sq // ATTN_BWD_TILE), -(-sk // ATTN_BWD_TILE), head_dim, causal)
 
