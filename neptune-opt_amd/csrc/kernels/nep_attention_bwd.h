@@ -25,9 +25,11 @@
 // not overlapped, there being one to a CU.  Head dim 64 (fp16 full 8x12x777: 69 us for both stages) passes
 // as many LDS reads and exponentials for half the products, and 7% of rows past the end.
 //
-// Inside a tile the S products stand alone, P is computed beside those of dP, dS beside those of dV (in
-// attention_bwd_q beside the first half of dQ's), each LDS read two steps before its MFMAs: causal
-// 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1867 so; full 2x16x4096x128 874 and 774.
+// Inside a tile P is computed beside the products of dP, dS beside those of dV (in attention_bwd_q P of one
+// block beside the next block's S, and dS beside the first half of dQ's products), each LDS read two steps
+// before its MFMAs: causal 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1862 so; full
+// 2x16x4096x128 874 and 770.  (The same order of blocks in attention_bwd_kv keeps the tile's rows and spills:
+// 1009 us, 1065.)
 //
 // Mapping (v_mfma_f32_32x32x16): attention_bwd_kv computes S[i][j] with A = Q rows from LDS and
 // B = K rows in registers, so lane l holds key l % 32 and registers hold queries
@@ -440,7 +442,7 @@ __device__ void attention_bwd_exact_q(const T* __restrict__ qp, const T* __restr
 // which there are 256: the gradients take them (all, for dK and dV from head dim 128 up), S and dP beside
 // them would spill, and each of their values would cost a move before its exponential.  (`mfma_settle`
 // stands between the last of a chain and the first other use of d: the wait states are the program's here,
-// 12 after an MFMA of 8 passes, as the compiler leaves after its own.)
+// 12 after an MFMA of 8 passes, as the compiler leaves after its own; the MFMAs between are among them.)
 // B_AGPR: b is kept in AGPRs.
 template <typename T, bool B_AGPR>
 __device__ __forceinline__ void mfma_vgpr(typename AttnIn<T>::vec8 a, typename AttnIn<T>::vec8 b,
@@ -475,11 +477,17 @@ __device__ __forceinline__ f32x16 mfma_vgpr_zero(typename AttnIn<T>::vec8 a, typ
   }
   return d;
 }
-template <int N>
-__device__ __forceinline__ void mfma_settle(f32x16 (&c)[N]) {
-  static_assert(N == 1 || N == 2, "one or two");
-  if constexpr (N == 1) asm volatile("s_nop 15" : "+v"(c[0]));
-  else asm volatile("s_nop 15" : "+v"(c[0]), "+v"(c[1]));
+template <int STATES>
+__device__ __forceinline__ void mfma_settle(f32x16& c) {
+  asm volatile("s_nop %1" : "+v"(c) : "n"(STATES - 1));
+}
+template <int STATES>
+__device__ __forceinline__ void mfma_settle(f32x16 (&c)[1]) {
+  mfma_settle<STATES>(c[0]);
+}
+template <int STATES>
+__device__ __forceinline__ void mfma_settle(f32x16 (&c)[2]) {
+  asm volatile("s_nop %2" : "+v"(c[0]), "+v"(c[1]) : "n"(STATES - 1));
 }
 // Nothing moves across: the steps of the loops below stand in the order they were written, each with the
 // next step's LDS reads in flight and vector operations beside its MFMAs.
@@ -688,7 +696,7 @@ __device__ __forceinline__ void attention_bwd_kv(
           }
         }
         if (kOwn && t == 1) mfma_read(c);
-        if (kOwn && t == LATE) mfma_settle(s);
+        if (kOwn && t == LATE) mfma_settle<12 - LATE>(s);
         if (t >= LATE) {
 #pragma unroll
           for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * KB; ++e)
@@ -696,7 +704,7 @@ __device__ __forceinline__ void attention_bwd_kv(
         }
         if constexpr (kOwn) step_end();
       }
-      if constexpr (kOwn) mfma_settle(dp);
+      if constexpr (kOwn) mfma_settle<12>(dp);
       // rows past the end are zero and P = 2^-inf, but not where K or V of the lane's key is
       // infinite or NaN: they are hidden too
       if ((CAUSAL && i0 < kw + 32 * KB - 1) || i0 + 32 > sq) {
@@ -920,40 +928,43 @@ __device__ __forceinline__ void attention_bwd_q(
       const int j0 = tile * kBwdTile + sub;
       if (CAUSAL && j0 > qw + 32 * QB - 1) continue;   // every pair hidden
       if (j0 >= sk) continue;
-      // every step's operands, read kAhead steps before
-      vec8 rows[2 * KSTEPS + kAhead], columns[2 * DBLK + kAhead];
+      // the operands of every step, read kAhead steps before
+      constexpr int ROWS_STEPS = 2 * QB * KSTEPS;
+      vec8 rows[2 * KSTEPS], columns[2 * DBLK];
       auto read_step = [&](int n) {
-        if (n < 2 * KSTEPS) {
-          rows[n] = n < KSTEPS ? rd.row(kt, sub, n) : rd.row(vt, sub, n - KSTEPS);
-        } else {
-          const int m = n - 2 * KSTEPS;
-          if (m < 2 * DBLK) columns[m] = rd.column(kt, sub, m / DBLK, m % DBLK);
+        if (n < ROWS_STEPS) {
+          const int x = n / KSTEPS % QB, t = n % KSTEPS;
+          if (x == 0) {
+            if (n < KSTEPS) rows[t] = rd.row(kt, sub, t);
+            else rows[KSTEPS + t] = rd.row(vt, sub, t);
+          }
+        } else if (n < ROWS_STEPS + 2 * DBLK) {
+          const int m = n - ROWS_STEPS;
+          columns[m] = rd.column(kt, sub, m / DBLK, m % DBLK);
         }
       };
       f32x16 s[QB], dp[QB];
+      auto exponentials = [&](int x, int from, int to) {
+#pragma unroll
+        for (int r = from; r < to && r < 16; ++r)
+          s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], scale_log2, shift[x]));
+      };
+      // S of one block of queries after the other, and then dP; P of a block beside the products behind its S
+      constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 + KSTEPS - LATE - 1) / (KSTEPS - LATE);
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) read_step(n);
 #pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        read_step(t + kAhead);
-#pragma unroll
-        for (int x = 0; x < QB; ++x) {
+      for (int n = 0; n < 2 * QB * KSTEPS; ++n) {
+        const int x = n / KSTEPS % QB, t = n % KSTEPS, chain = n / KSTEPS;
+        read_step(n + kAhead);
+        if (chain < QB) {
           if constexpr (kOwn) {
             if (t == 0) s[x] = mfma_vgpr_zero<T, false>(rows[t], qreg[x][t]);
             else mfma_vgpr<T, false>(rows[t], qreg[x][t], s[x]);
           } else {
             s[x] = In::mfma(rows[t], qreg[x][t], t == 0 ? f32x16{} : s[x]);
           }
-        }
-        if constexpr (kOwn) step_end();
-      }
-      // P of the first elements while the products of dP go on
-      constexpr int LATE = KSTEPS > 4 ? 2 : 1, PER_STEP = (16 * QB + KSTEPS - LATE - 1) / (KSTEPS - LATE);
-#pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        read_step(KSTEPS + t + kAhead);
-#pragma unroll
-        for (int x = 0; x < QB; ++x) {
+        } else {
           if constexpr (kOwn) {
             if (t == 0) dp[x] = mfma_vgpr_zero<T, true>(rows[KSTEPS + t], greg[x][t]);
             else mfma_vgpr<T, true>(rows[KSTEPS + t], greg[x][t], dp[x]);
@@ -961,16 +972,13 @@ __device__ __forceinline__ void attention_bwd_q(
             dp[x] = In::mfma(rows[KSTEPS + t], greg[x][t], t == 0 ? f32x16{} : dp[x]);
           }
         }
-        if (kOwn && t == LATE) mfma_settle(s);
-        if (t >= LATE) {
-#pragma unroll
-          for (int e = (t - LATE) * PER_STEP; e < (t - LATE + 1) * PER_STEP && e < 16 * QB; ++e)
-            s[e / 16][e % 16] =
-                __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], scale_log2, shift[e / 16]));
+        if (chain >= 1 && chain <= QB && t >= LATE) {
+          if (kOwn && t == LATE) mfma_settle<12 - LATE>(s[chain - 1]);
+          exponentials(chain - 1, (t - LATE) * PER_STEP, (t - LATE + 1) * PER_STEP);
         }
         if constexpr (kOwn) step_end();
       }
-      if constexpr (kOwn) mfma_settle(dp);
+      if constexpr (kOwn) mfma_settle<12>(dp[QB - 1]);
       const bool masked = (CAUSAL && j0 + 31 > qw) || j0 + 32 > sk;
       if (masked) {
         if (CAUSAL) bad |= rd.nonfinite(kt, sub);
@@ -999,7 +1007,7 @@ __device__ __forceinline__ void attention_bwd_q(
       constexpr int WORDS_STEP = (4 * QB + DBLK - 1) / DBLK;
 #pragma unroll
       for (int n = 0; n < 2 * DBLK; ++n) {
-        read_step(2 * KSTEPS + n + kAhead);
+        read_step(ROWS_STEPS + n + kAhead);
 #pragma unroll
         for (int x = 0; x < QB; ++x)
           dqa[x][n % DBLK] = In::mfma(columns[n], packed_operand<T>(pk[x], n / DBLK), dqa[x][n % DBLK]);
