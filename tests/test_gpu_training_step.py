@@ -91,8 +91,9 @@ PLAIN = {"norm": plain_norm, "rotary": plain_rotary, "attention": plain_attentio
 
 def operators():
     norm, attention, distill = CG.as_residual_norm_op(0.5), CG.as_attention_grad_op(), CG.as_distill_op(2.0)
+    halves, pairs = CG.as_rotary_op(), CG.as_rotary_op(interleaved=True)
     return {"norm": lambda *a: norm(*a)[:2], "attention": lambda *a: attention(*a)[0],
-            "rotary": lambda q, k, positions, turns, i: CG.as_rotary_op(interleaved=i)(q, k, positions, turns),
+            "rotary": lambda q, k, positions, turns, i: (pairs if i else halves)(q, k, positions, turns),
             "distill": lambda *a: distill(*a)[0]}
 
 
@@ -221,3 +222,37 @@ def test_a_padded_batch_leaves_the_rows_behind_alone():
     for a, b in zip(got[:3], want):                  # loss, dx, dy
         assert torch.equal(a[0], b[0]) and torch.equal(a[1, :90], b[1, :90])
         assert not a[1, 90:].float().abs().any()
+
+
+def test_operators_keep_the_registration_contracts():
+    # schema, fake outputs, autograd registration and traced gradients, by torch's own checker
+    dev = _dev()
+    g = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev).requires_grad_()  # noqa: E731
+    turns, _ = CG.rotary_frequencies(64, device=dev)
+    heads = [r(2, 3, 40, 64) for _ in range(3)]
+    x, y, gamma, gate = r(2, 9, 96), r(2, 9, 96), r(96), r(2, 1, 96)
+    calls = [(CG.as_attention_grad_op(), heads), (CG.as_rotary_op(), (*heads[:2], torch.arange(40, device=dev), turns)),
+             (CG.as_residual_norm_op(), (x, y, gamma, gamma.detach().clone().requires_grad_(), gate)),
+             (CG.as_residual_norm_op(), (x, y, None, gamma, None)),
+             (CG.as_distill_op(), (r(6, 50), torch.randn(6, 4, generator=g).to(dev),
+                                   torch.randint(0, 50, (6, 4), generator=g).to(dev)))]
+    for op, args in calls:
+        print(f"contracts of {op}", flush=True)
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_autograd_registration", "test_faketensor",
+                                                    "test_aot_dispatch_static"))
+
+
+def test_a_traced_layer_gives_the_same_bits():
+    dev = _dev()
+    p, fixed = parameters(2, 33, 3, 64, 130, 8, seed=3)
+    turns, _ = CG.rotary_frequencies(64, device=dev)
+    here = {n: t.to(dev) for n, t in fixed.items()}
+    ops = operators()
+    print("traced layer", flush=True)
+    results = []
+    for wrap in (lambda f: f, lambda f: torch.compile(f, backend="aot_eager", fullgraph=True)):
+        mine = {n: t.to(dev).requires_grad_() for n, t in p.items()}
+        loss = wrap(lambda q: layer(q, here, turns, 3, False, ops))(mine)
+        results.append([loss.detach(), *torch.autograd.grad(loss.sum(), list(mine.values()))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
