@@ -14,15 +14,16 @@
 //    every AGPR) and walks the query tiles (dK and dV stay in registers, four products per pair).
 //  * attention_bwd_q: a workgroup keeps Q and dO of its queries and walks the key tiles (three
 //    products per pair).
-// The last two share a launch where a wave has registers for either (head dim 64, and 128 with one block a
-// wave).  Five products instead of seven, with one stage, would add dQ across key blocks: fp32 atomics,
-// whose order changes results, or an fp32 copy of dQ per key block.
+// The last two share a launch, dQ's workgroups behind the others: apart and together, causal 2x8x1500x128
+// 97 and 57 us, 2x16x2048x128 198 and 146, 7x4x576x256 88 and 55, 1x4x8192x128 438 and 284, full
+// 8x12x777x64 95 and 90, causal 4x32x4096x128 1854 and 1842.  (Long calls of head dim 64 lose 1%, dQ's
+// workgroups being three to a CU alone.)  Five products instead of seven, with one stage, would add dQ
+// across key blocks: fp32 atomics, whose order changes results, or an fp32 copy of dQ per key block.
 //
 // Bound by the matrix cores at the rate that this card's power allows a product: full bf16 2x16x4096x128
-// runs 550 GFLOP of kv in 422 us (1300 TFLOP/s) and 412 of q in 340 (1210), a library product of 8192^3
-// 1165 to 1220.  Causal 4x32x4096x128: 1003 and 802 us, with the tiles on the diagonal passed whole by
-// the waves that need them and a workgroup's start and end (14 and 9 us: its K and V rows, its gradients)
-// not overlapped, there being one to a CU.  Head dim 64 (fp16 full 8x12x777: 69 us for both stages) passes
+// runs 962 GFLOP in 745 us (1290 TFLOP/s), a library product of 8192^3 1165 to 1350.  Causal 4x32x4096x128:
+// 962 GFLOP and the pairs hidden in tiles on the diagonal in 1795 us; a workgroup's start and end (11 us:
+// its rows, its gradients; one to a CU) and its waves' waits on the diagonal weigh twice as much there.  Head dim 64 (fp16 full 8x12x777: 69 us for both stages) passes
 // as many LDS reads and exponentials for half the products, and 7% of rows past the end.
 //
 // Inside a tile P is computed beside the products of dP, dS beside those of dV (in attention_bwd_q P of one
@@ -850,7 +851,8 @@ __device__ __forceinline__ void attention_bwd_q(
   typedef typename In::vec8 vec8;
   constexpr int BM = 32 * QB * W;
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
-  constexpr int TILE = kBwdTile * D * 2;
+  constexpr int ROWS = D <= 128 ? kBwdTile : 32;     // keys per staged tile, as attention_bwd_kv's
+  constexpr int TILE = ROWS * D * 2;
   constexpr bool kScaled = BwdIn<T>::kScaled;
   constexpr bool kOwn = D * QB >= 128;              // more than 256 registers
   unsigned char *const kbuf0 = bwd_tile<TILE, 0>(), *const kbuf1 = bwd_tile<TILE, 1>(),
@@ -873,11 +875,12 @@ __device__ __forceinline__ void attention_bwd_q(
   const T* gp = go + b * gsb + h * gsh;
   const float* st = start + (i64)bh * nq * kBwdTile;
   const float* nd = ndelta + (i64)bh * nq * kBwdTile;
-  const int last = CAUSAL ? min(nk, (q0 + BM + kBwdTile - 1) / kBwdTile) : nk;
-  const int t0 = PARTS ? part * per : 0;
-  const int t1 = PARTS ? min(last, t0 + per) : last;
+  constexpr int PER = kBwdTile / ROWS;
+  const int tiles = (sk + ROWS - 1) / ROWS, last = CAUSAL ? min(tiles, (q0 + BM + ROWS - 1) / ROWS) : tiles;
+  const int t0 = PARTS ? part * per * PER : 0;
+  const int t1 = PARTS ? min(last, t0 + per * PER) : last;
   if (PARTS && part > 0 && t0 >= last) return;       // the block has fewer parts
-  const bool whole = !PARTS || last <= per;
+  const bool whole = !PARTS || last <= per * PER;
 
   vec8 qreg[QB][KSTEPS], greg[QB][KSTEPS];
   float shift[QB], minus[QB];
@@ -908,11 +911,11 @@ __device__ __forceinline__ void attention_bwd_q(
 #pragma unroll
   for (int x = 0; x < QB; ++x) shift[x] += (float)lift;   // P times the power of two of dS
 
-  const BwdTile<D, W> kdma(wave, lane, kss), vdma(wave, lane, vss);
+  const BwdTile<D, W, ROWS> kdma(wave, lane, kss), vdma(wave, lane, vss);
   const BwdRead<T, D> rd(lane);
   auto issue = [&](int tile, unsigned char* kd, unsigned char* vd) {
-    kdma.load(kp, kss, tile * kBwdTile, sk, wave, kd);
-    vdma.load(vp, vss, tile * kBwdTile, sk, wave, vd);
+    kdma.load(kp, kss, tile * ROWS, sk, wave, kd);
+    vdma.load(vp, vss, tile * ROWS, sk, wave, vd);
   };
 
   f32x16 dqa[QB][DBLK];
@@ -924,8 +927,8 @@ __device__ __forceinline__ void attention_bwd_q(
 
   auto body = [&](int tile, const unsigned char* kt, const unsigned char* vt) {
 #pragma unroll
-    for (int sub = 0; sub < kBwdTile; sub += 32) {
-      const int j0 = tile * kBwdTile + sub;
+    for (int sub = 0; sub < ROWS; sub += 32) {
+      const int j0 = tile * ROWS + sub;
       if (CAUSAL && j0 > qw + 32 * QB - 1) continue;   // every pair hidden
       if (j0 >= sk) continue;
       // the operands of every step, read kAhead steps before
@@ -1049,8 +1052,8 @@ __device__ __forceinline__ void attention_bwd_q(
   };
   if constexpr (CAUSAL) {
     if (__syncthreads_or(bad)) {
-      attention_bwd_exact_q<T, D, CAUSAL, W>(qp, kp, vp, gp, st, nd, q0, BM, sq, t0 * kBwdTile,
-                                             min(sk, t1 * kBwdTile), qss, kss, vss, gss, scale,
+      attention_bwd_exact_q<T, D, CAUSAL, W>(qp, kp, vp, gp, st, nd, q0, BM, sq, t0 * ROWS,
+                                             min(sk, t1 * ROWS), qss, kss, vss, gss, scale,
                                              scale_log2, store);
       return;
     }

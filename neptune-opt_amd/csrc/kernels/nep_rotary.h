@@ -103,9 +103,12 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
   const u32 b = token / seq, s = token - b * seq;
   const int half = part / 2;
   const bool turn = slot < turned;
-  // first element, elements of the slot, and for the half layout the distance to their partners
-  const int e = turn ? (int)slot * VEC : part + (int)(slot - turned) * VEC;
-  const int count = (turn ? (LAYOUT == kHalves ? half : part) : dim) - e;
+  // first element, elements of the slot, and for the half layout the distance to their partners; of a
+  // run that is no multiple of VEC the last slot overlaps its neighbour (both write the same values)
+  const int run = turn ? (LAYOUT == kHalves ? half : part) : dim - part;
+  const int at = (int)(turn ? slot : slot - turned) * VEC, back = run - VEC;
+  const int e = (turn ? 0 : part) + (ANY && at > back ? (back > 0 ? back : 0) : at);
+  const int count = run;
   float cs[PAIRS], sn[PAIRS];
   if (turn) {
     const double at = (double)positions[b * psb + s * pss];

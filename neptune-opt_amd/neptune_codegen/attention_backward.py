@@ -33,8 +33,6 @@ _lock = threading.Lock()
 
 _ROWS_ARGS = (hip.PTR,) * 8 + (hip.I32,) * 4 + (hip.I64,) * 9 + (hip.F32,)
 _OPERAND_ARGS = (hip.I32,) * 4 + (hip.I64,) * 12 + (hip.F32,) * 2 + (hip.I32,)
-_KV_ARGS = (hip.PTR,) * 10 + _OPERAND_ARGS
-_Q_ARGS = (hip.PTR,) * 9 + _OPERAND_ARGS
 _KVQ_ARGS = (hip.PTR,) * 12 + _OPERAND_ARGS + (hip.I32,) * 2
 _THREADS = 64 * ATTN_BWD_WAVES
 _JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64,) + (hip.I32,) * 5
@@ -57,17 +55,15 @@ def unit_kinds(head_dim):
     """(stage, blocks per wave, parts) of the units a call at this head dim may launch."""
     yield "rows", 1, False
     for blocks in range(1, attention_backward_blocks(head_dim) + 1):
-        for stage in ("kvq",) if _joint(head_dim, blocks) else ("kv", "q"):
-            yield stage, blocks, False
-            yield stage, blocks, True
+        yield "kvq", blocks, False
+        yield "kvq", blocks, True
 
 
 def _kernel(stage, device, head_dim, causal, dtype, blocks=1, parts=False) -> hip.Kernel:
     key = (stage, device, head_dim, causal, dtype, blocks, parts)
     found = _KERNELS.get(key)
     if found is None:
-        args, threads = {"rows": (_ROWS_ARGS, 256), "kv": (_KV_ARGS, _THREADS), "q": (_Q_ARGS, _THREADS),
-                         "kvq": (_KVQ_ARGS, _THREADS),
+        args, threads = {"rows": (_ROWS_ARGS, 256), "kvq": (_KVQ_ARGS, _THREADS),
                          "kv_join": (_JOIN_ARGS, 256), "q_join": (_JOIN_ARGS, 256)}[stage]
         prog = _program("rows" if stage.endswith("join") else stage, head_dim, causal, dtype, blocks, parts)
         found = _KERNELS[key] = prog.kernel(
@@ -121,14 +117,6 @@ CUS = 256
 PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32)
 
 
-def _joint(head_dim, blocks):
-    """Whether one launch holds both stages: where a wave's accumulators leave registers for either.  The
-    second stage's workgroups then run beside the last of the first: causal 2x8x1500x128 97 us apart, 57
-    together; 1x4x8192x128 438 and 284; 2x4x77x64 16.4 and 10.9; full 8x12x777x64 95 and 90.  (Long calls
-    of head dim 64 lose a little, their dQ workgroups being three to a CU alone: causal 4x32x4096 964, 977.)"""
-    return head_dim * blocks < 256
-
-
 def _stage_work(stage, units, own, other, head_dim, causal, blocks, per):
     """(items, tiles, longest item's tiles, bytes of split sums) of a stage with blocks of `own` rows
     walking the tiles of the `other` rows in parts of `per`."""
@@ -149,24 +137,22 @@ def _stage_work(stage, units, own, other, head_dim, causal, blocks, per):
 
 
 def _launch_cost(works, head_dim, causal, blocks):
-    """us of a launch of `works`, {stage: _stage_work(...)}, and of the joins of what it splits."""
+    """us of the launch of both stages, {stage: _stage_work(...)} in their order, and of the joins of what it
+    splits."""
     items = sum(w[0] for w in works.values())
-    busy = longest = joins = 0.0
+    busy = longest = joins = last = 0.0
     for stage, (n, tiles, most, sums) in works.items():
         few, full, *ends = TILE_US[stage, head_dim, blocks]
-        ends = ends[causal]
         # two workgroups on a CU take turns
         tile = 1.7 * full if head_dim == 64 and items > CUS else few
-        longest = max(longest, most * tile + ends)
-        busy += (tiles * full + n * ends) / CUS
+        last = most * tile + ends[causal]
+        late, longest = last > longest, max(longest, last)
+        busy += (tiles * full + n * ends[causal]) / CUS
         joins += JOIN_US + sums / SUM_BYTES_PER_US if sums else 0.0
     if items <= CUS:
         return longest + joins
-    if not causal and len(works) == 1:               # equal items: whole rounds
-        return -(-items // CUS) * (most * full + ends) + joins
-    # the heaviest start first, and the last to end are short, unless those of the second stage are longer
-    late = list(works.values())[-1][2] > 2 * list(works.values())[0][2]
-    return max(longest, busy + longest / (2 if late else 8)) + joins
+    # the heaviest of a stage start first; what ends last is short, unless the second stage's are longer
+    return max(longest, busy + longest / (2 if late else 4 if causal else 8)) + joins
 
 
 @functools.lru_cache(maxsize=4096)
@@ -179,22 +165,15 @@ def _plan_tiles(units, q_tiles, k_tiles, head_dim, causal):
             found[stage] = [(p, _stage_work(stage, units, own, other, head_dim, causal, blocks, -(-tiles // p)))
                             for p in PARTS
                             if p == 1 or p <= tiles // 2 and 4 * p * units * own * width <= MAX_SUM_BYTES]
-        if _joint(head_dim, blocks):
-            cost, kv, q = min((_launch_cost({"kv": kv, "q": q}, head_dim, causal, blocks), i, j)
-                              for i, kv in found["kv"] for j, q in found["q"])
-        else:
-            (kv_cost, kv), (q_cost, q) = (
-                min((_launch_cost({stage: w}, head_dim, causal, blocks), p) for p, w in found[stage])
-                for stage in ("kv", "q"))
-            cost = kv_cost + q_cost
-        if best is None or cost < best[0]:
-            best = (cost, (blocks, kv, blocks, q))
-    return best[1]
+        cheapest = min((_launch_cost({"kv": kv, "q": q}, head_dim, causal, blocks), blocks, i, j)
+                       for i, kv in found["kv"] for j, q in found["q"])
+        best = cheapest if best is None else min(best, cheapest)
+    return best[1:]
 
 
 def _plan(units, sq, sk, head_dim, causal):
-    """(kv blocks, kv parts, q blocks, q parts) of a call, the cheapest by TILE_US; searched once for the
-    same tile counts.  Two blocks a wave (head dim 128) read each tile half as often and pass twice the rows
+    """(blocks per wave, kv parts, q parts) of a call, the cheapest by TILE_US; searched once for the same
+    tile counts.  Two blocks a wave (head dim 128) read each tile half as often and pass twice the rows
     in 1.7 to 1.8 times the time, with a longer start and end: bf16 causal 4x32x4096x128 1861 us by two,
     2072 by one; full 2x16x4096x128 800 and 875, 8x32x1024x128 469 and 555; but causal 8x32x1024x128 398 and
     375, 2x8x300x128 59 and 20."""
@@ -207,11 +186,11 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
 
     B, H, Sq, D = q.shape
     Sk, units, device = k.shape[2], B * H, calls.device_index(q)
-    kv_blocks, kv_parts, q_blocks, q_parts = plan or _plan(units, Sq, Sk, D, causal)
+    blocks, kv_parts, q_parts = plan or _plan(units, Sq, Sk, D, causal)
     nq, nk = -(-Sq // ATTN_BWD_TILE), -(-Sk // ATTN_BWD_TILE)
     kv_per, q_per = -(-nq // kv_parts), -(-nk // q_parts)
     kv_parts, q_parts = -(-nq // kv_per), -(-nk // q_per)
-    kv_rows, q_rows = 32 * ATTN_BWD_WAVES * kv_blocks, 32 * ATTN_BWD_WAVES * q_blocks
+    rows = 32 * ATTN_BWD_WAVES * blocks              # of a workgroup
     kind = (device, D, causal, q.dtype)
     # scratch: start values and deltas of every padded query row; fp16's bounds; the parts' fp32 sums
     stats = 4 * units * nq * ATTN_BWD_TILE
@@ -226,28 +205,20 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
     qs, ks, vs, gs, os = strides
     sizes, steps = (units, H, Sq, Sk), qs + ks + vs + gs + (scale, scale * LOG2E)
     groups = units * (nq + (nk if q.dtype == torch.float16 else 0))
-    joint = kv_blocks == q_blocks == 1 and _joint(D, 1)
-    kv_groups, q_groups = units * kv_parts * -(-Sk // kv_rows), units * q_parts * -(-Sq // q_rows)
-    read = (tq, tk, tv, grad, start, ndelta, limit)
-    launches = [(_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start,
-                                                     ndelta, limit, H, Sq, Sk, units) + os + gs + vs + (scale,))]
-    if joint:
-        qpart = calls.buffer(3, 2 * stats + bounds + kv_sums)
-        launches.append((_kernel("kvq", *kind, 1, kv_parts > 1 or q_parts > 1), (kv_groups + q_groups,),
-                         read + (dk, dv, dq, part, qpart) + sizes + steps + (kv_per, q_per, kv_groups)))
-    else:
-        qpart = part
-        launches.append((_kernel("kv", *kind, kv_blocks, kv_parts > 1), (kv_groups,),
-                         read + (dk, dv, part) + sizes + steps + (kv_per,)))
+    kv_groups, q_groups = units * kv_parts * -(-Sk // rows), units * q_parts * -(-Sq // rows)
+    qpart = calls.buffer(3, 2 * stats + bounds + kv_sums)
+    launches = [
+        (_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start, ndelta,
+                                             limit, H, Sq, Sk, units) + os + gs + vs + (scale,)),
+        (_kernel("kvq", *kind, blocks, kv_parts > 1 or q_parts > 1), (kv_groups + q_groups,),
+         (tq, tk, tv, grad, start, ndelta, limit, dk, dv, dq, part, qpart) + sizes + steps
+         + (kv_per, q_per, kv_groups))]
     if kv_parts > 1:
         launches.append((_kernel("kv_join", *kind), (-(-units * 2 * Sk * D // 1024),),
-                         (part, dk, dv, units * Sk, Sk, Sq, kv_rows, kv_per, int(causal))))
-    if not joint:
-        launches.append((_kernel("q", *kind, q_blocks, q_parts > 1), (q_groups,),
-                         read + (dq, part) + sizes + steps + (q_per,)))
+                         (part, dk, dv, units * Sk, Sk, Sq, rows, kv_per, int(causal))))
     if q_parts > 1:
         launches.append((_kernel("q_join", *kind), (-(-units * Sq * D // 1024),),
-                         (qpart, dq, 0, units * Sq, Sq, Sk, q_rows, q_per, int(causal))))
+                         (qpart, dq, 0, units * Sq, Sq, Sk, rows, q_per, int(causal))))
     return calls.Plan(device, 7, buffers, (0, 1, 2), launches)
 
 

@@ -715,10 +715,9 @@ def attention_backward_blocks(head_dim: int) -> int:
 
 def attention_backward_kernel_name(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
                                    blocks: int = 1, parts: bool = False) -> str:
-    """Symbol of one stage of attention's gradients: "rows", "kv", "q", "kvq", "kv_join" or
-    "q_join"."""
+    """Symbol of one stage of attention's gradients: "rows", "kvq", "kv_join" or "q_join"."""
     tag, _ = _attn_dtype(dtype)
-    if stage not in ("kv", "q", "kvq"):
+    if stage != "kvq":
         return f"attention_bwd_{stage}_{tag}_d{head_dim}"
     return (f"attention_bwd_{stage}_{tag}_d{head_dim}_{'causal' if causal else 'full'}_b{blocks}"
             f"{'_parts' if parts else ''}")
@@ -727,9 +726,8 @@ def attention_backward_kernel_name(stage: str, head_dim: int, causal: bool, dtyp
 def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtype="bfloat16",
                                    blocks: int = 1, parts: bool = False) -> str:
     """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics with the joins
-    of split ranges ("rows"; the mask does not matter), dK and dV ("kv"), dQ ("q"), or the last two in one
-    launch ("kvq": its first `groups` workgroups take dK and dV).  At head dim 64 two workgroups share a
-    CU, and so a SIMD's 512 registers."""
+    of split ranges ("rows"; the mask does not matter), or dK and dV, by the first `groups` workgroups, and
+    dQ, by the others ("kvq").  At head dim 64 two workgroups share a CU, and so a SIMD's 512 registers."""
     if head_dim not in ATTN_HEAD_DIMS:
         raise NotImplementedError("attention fold supports head_dim 64, 128 and 256")
     if not 1 <= blocks <= attention_backward_blocks(head_dim):
@@ -757,29 +755,24 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
                 f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, "
                 "rows, len, other, block, per, causal);\n}\n")
         return "\n".join(units)
-    outs = {"kv": "void* dk, void* dv", "q": "void* dq", "kvq": "void* dk, void* dv, void* dq"}[stage]
-    sums = "float* sums" + (", float* qsums" if stage == "kvq" else "")
-    pers = "int per" + (", int qper, int groups" if stage == "kvq" else "")
 
-    def call(which, total, per, group):
-        args = f"({ctype}*)dk, ({ctype}*)dv" if which == "kv" else f"({ctype}*)dq"
+    def call(which, outs, sums, per, group):
         return (f"nep::attention_bwd_{which}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
-                f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {args}, {total}, units, heads, sq, sk, qsb, "
+                f"{c}q, {c}k, {c}v, {c}go, start, ndelta, bounds, {outs}, {sums}, units, heads, sq, sk, qsb, "
                 "qsh, qss, ksb, ksh, kss, vsb, vsh, vss, gsb, gsh, gss, scale, scale_log2, "
                 f"{per}, {group});\n")
 
-    body = f"  {call(stage, 'sums', 'per', 'blockIdx.x')}"
-    if stage == "kvq":
-        body = ("  if ((int)blockIdx.x < groups) " + call("kv", "sums", "per", "blockIdx.x")
-                + "  else " + call("q", "qsums", "qper", "(int)blockIdx.x - groups"))
     return "\n".join([
         head,
         f'extern "C" __global__ void __launch_bounds__({threads}, {2 if head_dim == 64 else 1}) {name}('
-        f"const void* q, const void* k, const void* v, const void* go, const float* start, const float* ndelta, const float* bounds, {outs}, "
-        f"{sums}, int units, int heads, int sq, int sk, long long qsb, long long qsh, long long qss, "
-        "long long ksb, long long ksh, long long kss, long long vsb, long long vsh, long long vss, "
-        f"long long gsb, long long gsh, long long gss, float scale, float scale_log2, {pers}) {{\n"
-        + body + "}\n"])
+        "const void* q, const void* k, const void* v, const void* go, const float* start, const float* ndelta, "
+        "const float* bounds, void* dk, void* dv, void* dq, float* sums, float* qsums, int units, int heads, "
+        "int sq, int sk, long long qsb, long long qsh, long long qss, long long ksb, long long ksh, "
+        "long long kss, long long vsb, long long vsh, long long vss, long long gsb, long long gsh, "
+        "long long gss, float scale, float scale_log2, int per, int qper, int groups) {\n"
+        "  if ((int)blockIdx.x < groups) "
+        + call("kv", f"({ctype}*)dk, ({ctype}*)dv", "sums", "per", "blockIdx.x")
+        + "  else " + call("q", f"({ctype}*)dq", "qsums", "qper", "(int)blockIdx.x - groups") + "}\n"])
 
 
 # ---------------------------------------------------------------- distillation from top logits

@@ -49,21 +49,22 @@ def test_metadata_calls():
 
 def test_launch_choice_follows_the_measured_shapes():
     # (units, sq, sk, head dim, causal): the cheapest of the sweep or within a few percent of it
-    assert AB._plan(128, 4096, 4096, 128, True) == (2, 1, 2, 1)
-    assert AB._plan(96, 777, 777, 64, False) == (1, 1, 1, 1)
-    assert AB._plan(8, 77, 77, 64, True) == (1, 1, 1, 1)
-    assert AB._plan(64, 512, 512, 128, True) == (1, 1, 1, 1)
+    assert AB._plan(128, 4096, 4096, 128, True) == (2, 1, 1)
+    assert AB._plan(96, 777, 777, 64, False) == (1, 1, 1)
+    assert AB._plan(8, 77, 77, 64, True) == (1, 1, 1)
+    assert AB._plan(64, 512, 512, 128, True) == (1, 1, 1)
+    assert AB._plan(28, 576, 576, 256, True) == (1, 1, 1)
     assert AB._plan(16, 8000, 77, 64, False)[1] >= 8          # few keys: the queries are split
-    assert AB._plan(16, 16, 8000, 128, False)[3] >= 4         # few queries: the keys are split
+    assert AB._plan(16, 16, 8000, 128, False)[2] >= 4         # few queries: the keys are split
     for units in (1, 7, 300):
         for sq in (1, 64, 65, 5000):
             for sk in (1, 1000):
                 for dim in (64, 128, 256):
                     for causal in (True, False):
-                        kb, kp, qb, qp = AB._plan(units, sq, sk, dim, causal)
+                        blocks, kp, qp = AB._plan(units, sq, sk, dim, causal)
                         assert 1 <= kp <= max(1, -(-sq // 64)) and 1 <= qp <= max(1, -(-sk // 64))
                         assert 8 * kp * units * sk * dim <= AB.MAX_SUM_BYTES or kp == 1
-                        assert kb == qb == 1 or kb == qb == 2 and dim == 128
+                        assert blocks == 1 or blocks == 2 and dim == 128
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
