@@ -12,9 +12,9 @@
 //
 // HBM-bound: every element is read once and written once.  A lane owns one 16-byte slot of a token,
 // computes its angles once and walks `per` heads with them, queries and keys alike; consecutive lanes are
-// consecutive slots, then tokens.  In the half layout a lane has the two slots of its pairs, half a part
-// apart; where a head's slots are a power of two and all turned, each lane has one slot instead and the
-// two of a pair exchange their words, so that a wavefront reads whole rows of a head.
+// consecutive slots, then tokens.  In the half layout the two lanes of a pair of slots exchange their words
+// (each half's lanes a power of two, some idle), so that a wavefront reads whole rows of a head; halves
+// shorter than a word, or of more lanes than a wavefront has, are read by one lane as two slots.
 #pragma once
 
 namespace nep {
@@ -95,30 +95,31 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
                                        i64 psb, i64 pss, float sign, float magnitude) {
   typedef typename St::T T;
   constexpr int VEC = St::kVec, PAIRS = LAYOUT == kPairs ? VEC / 2 : VEC;
-  static_assert(LAYOUT != kExchanged || !ANY, "whole words");
   constexpr int AHEAD = 4;                          // heads in flight per lane
   const u32 id = blockIdx.x * 256u + threadIdx.x;
   const u32 token = id / slots, slot = id - token * slots;
   if (token >= tokens) return;
   const u32 b = token / seq, s = token - b * seq;
   const int half = part / 2;
-  const bool turn = slot < turned;
-  // first element, elements of the slot, and for the half layout the distance to their partners; of a
-  // run that is no multiple of VEC the last slot overlaps its neighbour (both write the same values)
-  const int run = turn ? (LAYOUT == kHalves ? half : part) : dim - part;
-  const int at = (int)(turn ? slot : slot - turned) * VEC, back = run - VEC;
-  const int e = (turn ? 0 : part) + (ANY && at > back ? (back > 0 ? back : 0) : at);
+  const bool turn = slot < turned, second = LAYOUT == kExchanged && turn && slot >= turned / 2;
+  // first element and elements of the slot, whose run starts at `from`; of a run that is no multiple of VEC
+  // the last slot overlaps its neighbour (both write the same values)
+  const int from = !turn ? part : second ? half : 0;
+  const int run = !turn ? dim - part : LAYOUT == kPairs ? part : half;
+  const int at = (int)(!turn ? slot - turned : second ? slot - turned / 2 : slot) * VEC, back = run - VEC;
+  if (at >= run) return;                             // (its partner has none either)
+  const int e = from + (ANY && at > back ? (back > 0 ? back : 0) : at);
   const int count = run;
   float cs[PAIRS], sn[PAIRS];
   if (turn) {
     const double at = (double)positions[b * psb + s * pss];
-    const int first = LAYOUT == kPairs ? e / 2 : LAYOUT == kExchanged && e >= half ? e - half : e;
+    const int first = LAYOUT == kPairs ? e / 2 : e - from;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       const double t = first + i < half ? at * turns[first + i] : 0.0;
       sincos_turns(t, sn[i], cs[i]);
       // (exchanged: the second half's slot is b, and b' = b cos + a sin)
-      sn[i] *= LAYOUT == kExchanged && e < half ? -(sign * magnitude) : sign * magnitude;
+      sn[i] *= LAYOUT == kExchanged && !second ? -(sign * magnitude) : sign * magnitude;
       cs[i] *= magnitude;
     }
   }
@@ -145,7 +146,7 @@ __device__ __forceinline__ void rotary(const typename St::T* __restrict__ q,
         if constexpr (LAYOUT == kExchanged) {
           float own[VEC], other[VEC];
           St::unpack(w0[i], own);
-          St::unpack(exchanged(w0[i], half / VEC), other);
+          St::unpack(exchanged(w0[i], (int)turned / 2), other);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) own[j] = __builtin_fmaf(other[j], sn[j], own[j] * cs[j]);
           w0[i] = St::pack(own);

@@ -138,7 +138,7 @@ def _rotary_programs():
     return [_program(dtype, index, layout, any_rows)
             for dtype in ("bfloat16", "float16", "float32") for index in ("int32", "int64")
             for layout, any_rows in (("halves", False), ("halves", True), ("pairs", False), ("pairs", True),
-                                     ("exchanged", False))]
+                                     ("exchanged", False), ("exchanged", True))]
 
 
 def programs():

@@ -137,10 +137,16 @@ def _run(q, k, positions, turns, magnitude, interleaved, sign):
                     or any(t is not None and (t.data_ptr() % 16 or any(s % vec for s in t.stride()[:3]))
                            for t in used[:2]))
     turned, rest = -(-run // vec), -(-(dim - part) // vec)
-    layout = "pairs" if interleaved else "halves"
-    if not (interleaved or any_rows or rest) and turned & (turned - 1) == 0 and turned <= 32:
-        layout, turned = "exchanged", 2 * turned
-    slots, heads, tokens = turned + rest, heads_q + heads_k, batch * seq
+    layout, slots = "pairs" if interleaved else "halves", turned + rest
+    # one slot a lane and an exchange within a pair, or both slots: bf16 8 x 2048 tokens of 16 + 16 heads of 100
+    # 43 and 80 us, of 96 42 and 61; 4 x 4096 of 32 + 32 heads of 128 95 and 105, 32 + 8 heads 64 of 128 59
+    # and 66; (16 + 8 heads, 128 of 256, 75 and 71).  The lanes of a half, and of a token, are a power of two,
+    # so that its pairs are in one wavefront.
+    lane_run = 2 * (1 << (turned - 1).bit_length())
+    lanes = 1 << (lane_run + rest - 1).bit_length()
+    if not interleaved and run >= vec and lanes <= 64:
+        layout, slots, turned = "exchanged", lanes, lane_run
+    heads, tokens = heads_q + heads_k, batch * seq
     if tokens >= 1 << 31:
         raise NotImplementedError("rotary takes less than 2^31 tokens")
     per = _heads_per_lane(tokens, slots, heads)
