@@ -270,7 +270,8 @@ __device__ __forceinline__ void distill_forward(const typename St::T* __restrict
   }
 }
 
-// Gradient of each row.  The row is written as T g q first; the list's columns are then written
+// Gradient of each row, its columns in gridDim.y parts of `per` (a multiple of a word's; the state is given,
+// so a part needs nothing of the others).  The part is written as T g q first; the list's columns are then written
 // again, whole, by the lanes that hold their entries, after a barrier behind which the first writes
 // are complete.  An index that comes twice is found by a hash of LDS bits (never missed; a false
 // alarm costs the search): each of its entries then sums p over the list in the list's order, so
@@ -283,7 +284,8 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
                                                  const float* __restrict__ stats,
                                                  typename St::T* __restrict__ dz, i64 rows, i64 n,
                                                  i64 stride_g, i64 stride_z, i64 stride_t,
-                                                 i64 stride_i, int count, float c, float temperature) {
+                                                 i64 stride_i, int count, float c, float temperature,
+                                                 i64 per) {
   typedef RowLanes<TPR> R;
   typedef Span<St, TPR, ACCESS> Sp;
   constexpr int VEC = St::kVec, STEP = TPR * VEC, RPW = WG / TPR;
@@ -297,7 +299,8 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   const bool live = row < rows;
   const typename St::T* rp = z + (live ? row : 0) * stride_z;
   typename St::T* op = dz + (live ? row : 0) * n;
-  const Sp sp(rp, 0, live ? n : 0);
+  const i64 c0 = blockIdx.y * per, c1 = c0 + per < n ? c0 + per : n;
+  const Sp sp(rp, c0, live ? c1 : c0);
   const RowWords<St, Sp, (TPR > 64)> row_words(rp, sp);
   const int words = row_words.words;
   TeacherList<St, Lt, Ix, TPR, EPL> list;
@@ -369,7 +372,7 @@ __device__ __forceinline__ void distill_backward(const float* __restrict__ grad,
   if (list.empty || list.bad) return;
 #pragma unroll
   for (int k = 0; k < EPL; ++k) {
-    if (list.at[k] < 0) continue;
+    if (list.at[k] < c0 || list.at[k] >= c1) continue;   // absent, or another part's
     float p = list.e[k];
     if (twice) {
       p = 0.0f;

@@ -30,7 +30,7 @@ _FORWARD, _BACKWARD = calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _FORWARD_ARGS = (hip.PTR,) * 5 + (hip.I64,) * 5 + (hip.I32,) + (hip.F32,) * 3
-_BACKWARD_ARGS = (hip.PTR,) * 6 + (hip.I64,) * 6 + (hip.I32,) + (hip.F32,) * 2
+_BACKWARD_ARGS = (hip.PTR,) * 6 + (hip.I64,) * 6 + (hip.I32,) + (hip.F32,) * 2 + (hip.I64,)
 
 
 def _program(stage: str, var: DistillVariant) -> hip.Program:
@@ -108,10 +108,9 @@ def _variant(z, stride: int, top, index, rows: int, n: int, count: int, stage: s
         tpr = 64 if slots <= alone and count <= 256 else 1024 if rows <= 512 and slots > 1024 else 256
         most = 8 if rows >= 1024 else 4
     else:
-        tpr = 64 if slots <= 256 and count <= 256 else 256 if slots < 2048 else 1024
-        if rows <= 512 and slots > 1024:
-            tpr = 1024
-        most = 4
+        parts = _column_parts(rows, slots)
+        tpr = 64 if slots <= 256 and count <= 256 else 256 if slots < 2048 or parts > 1 else 1024
+        most, slots = 4, -(-slots // parts)
     half = tpr == (64 if stage == "forward" else 256)
     unroll, widest = 1, slots // 2 if half else slots
     while unroll < most and tpr * unroll * 2 <= widest:
@@ -125,6 +124,13 @@ def _variant(z, stride: int, top, index, rows: int, n: int, count: int, stage: s
     return DistillVariant(name(z), name(top), name(index), not aligned, tpr, unroll, entries)
 
 
+def _column_parts(rows: int, slots: int) -> int:
+    """Parts of a row's columns in the gradient, where rows alone leave CUs idle: eight workgroups of 256
+    lanes for each CU, of a slot a lane at least.  bf16 64 rows of 128256 11.9 us, 18.7 whole; one row 5.6, 11.1;
+    500 of 50257 23.7, 26.1; fp32 7 of 181248 6.8, 26.0; from 512 rows on nothing is gained."""
+    return max(1, min(slots // 256, 2048 // rows)) if rows < 512 and slots > 1024 else 1
+
+
 def _launch(stage, z, top, index, strides, args, ends):
     """(kernel, grid, arguments) of a stage; `args` are its pointers, `ends` what follows the strides."""
     rows, n, count = z.numel() // z.shape[-1], z.shape[-1], top.shape[-1]
@@ -132,7 +138,12 @@ def _launch(stage, z, top, index, strides, args, ends):
     kernel = _program(stage, var).kernel(distill_kernel_name(stage, var),
                                          _FORWARD_ARGS if stage == "forward" else _BACKWARD_ARGS,
                                          var.wg, calls.device_index(z))
-    return kernel, (-(-rows // var.rows),), args + (rows, n) + strides + (count,) + ends
+    grid = (-(-rows // var.rows),)
+    if stage == "backward":
+        vec = 16 // z.element_size()
+        per = -(-n // (64 * vec * _column_parts(rows, -(-n // vec)))) * 64 * vec
+        grid, ends = grid + (-(-n // per),), ends + (per,)
+    return kernel, grid, args + (rows, n) + strides + (count,) + ends
 
 
 def run_distill(logits, top_logits, top_index, *, temperature: float = 1.0, return_stats: bool = False):

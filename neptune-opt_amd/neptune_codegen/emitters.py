@@ -824,9 +824,9 @@ def emit_distill_source(stage: str, var: DistillVariant) -> str:
     return (f"{head}\n{bound}(const float* grad, const void* z, const void* t, const void* ix, "
             "const float* stats, void* dz, long long rows, long long n, long long stride_g, "
             "long long stride_z, long long stride_t, long long stride_i, int count, float c, "
-            "float temperature) {\n"
+            "float temperature, long long per) {\n"
             f"  nep::distill_backward{targs}(grad, (const {st}::T*)z, (const {lt}::T*)t, (const {ix}*)ix, "
-            f"stats, ({st}::T*)dz, rows, n, stride_g, stride_z, stride_t, stride_i, count, c, temperature);\n}}\n")
+            f"stats, ({st}::T*)dz, rows, n, stride_g, stride_z, stride_t, stride_i, count, c, temperature, per);\n}}\n")
 
 
 # ---------------------------------------------------------------- residual norm
