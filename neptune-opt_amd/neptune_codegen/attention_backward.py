@@ -31,7 +31,7 @@ _OPS: dict = {}
 _TABLE = calls.Table()
 _lock = threading.Lock()
 
-_ROWS_ARGS = (hip.PTR,) * 8 + (hip.I32,) * 4 + (hip.I64,) * 9 + (hip.F32,)
+_ROWS_ARGS = (hip.PTR,) * 10 + (hip.I32,) * 4 + (hip.I64,) * 15 + (hip.F32,) * 2 + (hip.I32,)
 _OPERAND_ARGS = (hip.I32,) * 4 + (hip.I64,) * 12 + (hip.F32,) * 2 + (hip.I32,)
 _KVQ_ARGS = (hip.PTR,) * 12 + _OPERAND_ARGS + (hip.I32,) * 2
 _THREADS = 64 * ATTN_BWD_WAVES
@@ -208,8 +208,9 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
     kv_groups, q_groups = units * kv_parts * -(-Sk // rows), units * q_parts * -(-Sq // rows)
     qpart = calls.buffer(3, 2 * stats + bounds + kv_sums)
     launches = [
-        (_kernel("rows", *kind), (groups,), (out, grad, tv, lse, 0 if grad_lse is None else glse, start, ndelta,
-                                             limit, H, Sq, Sk, units) + os + gs + vs + (scale,)),
+        (_kernel("rows", *kind), (groups,),
+         (tq, tk, out, grad, tv, lse, 0 if grad_lse is None else glse, start, ndelta, limit, H, Sq, Sk, units)
+         + qs + ks + os + gs + vs + (scale, scale * LOG2E, int(causal))),
         (_kernel("kvq", *kind, blocks, kv_parts > 1 or q_parts > 1), (kv_groups + q_groups,),
          (tq, tk, tv, grad, start, ndelta, limit, dk, dv, dq, part, qpart) + sizes + steps
          + (kv_per, q_per, kv_groups))]

@@ -741,12 +741,15 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
     if stage == "rows":
         units = [
             head,
-            f'extern "C" __global__ void __launch_bounds__(256) {name}(const void* o, const void* go, '
-            "const void* v, const float* lse, const float* glse, float* start, float* ndelta, float* bounds, "
-            "int heads, int sq, int sk, int units, long long osb, long long osh, long long oss, long long gsb, "
-            "long long gsh, long long gss, long long vsb, long long vsh, long long vss, float scale) {\n"
-            f"  nep::attention_bwd_rows<{ctype}, {head_dim}>({c}o, {c}go, {c}v, lse, glse, start, ndelta, "
-            "bounds, heads, sq, sk, units, osb, osh, oss, gsb, gsh, gss, vsb, vsh, vss, scale);\n}\n"]
+            f'extern "C" __global__ void __launch_bounds__(256) {name}(const void* q, const void* k, '
+            "const void* o, const void* go, const void* v, const float* lse, const float* glse, float* start, "
+            "float* ndelta, float* bounds, int heads, int sq, int sk, int units, long long qsb, long long qsh, "
+            "long long qss, long long ksb, long long ksh, long long kss, long long osb, long long osh, "
+            "long long oss, long long gsb, long long gsh, long long gss, long long vsb, long long vsh, "
+            "long long vss, float scale, float scale_log2, int causal) {\n"
+            f"  nep::attention_bwd_rows<{ctype}, {head_dim}>({c}q, {c}k, {c}o, {c}go, {c}v, lse, glse, start, "
+            "ndelta, bounds, heads, sq, sk, units, qsb, qsh, qss, ksb, ksh, kss, osb, osh, oss, gsb, gsh, gss, "
+            "vsb, vsh, vss, scale, scale_log2, causal);\n}\n"]
         for join, pair in (("kv_join", "true"), ("q_join", "false")):
             symbol = attention_backward_kernel_name(join, head_dim, causal, dtype)
             units.append(
