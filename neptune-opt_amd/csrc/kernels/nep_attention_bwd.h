@@ -228,8 +228,44 @@ __device__ __forceinline__ void attention_bwd_rows(
   __shared__ float dots[2][kBwdTile];
   const int nq = (sq + kBwdTile - 1) / kBwdTile, nk = (sk + kBwdTile - 1) / kBwdTile;
   const int tid = threadIdx.x, c = tid % LPR;
-  const bool keys = kScaled && (int)blockIdx.x >= units * nq;
-  const int id = keys ? blockIdx.x - units * nq : blockIdx.x, n = keys ? nk : nq;
+  // tiles of a head whose rows see at most 64 keys: the first workgroups', whose chain of loads and products
+  // is longer than the others'
+  const int few = sk <= kBwdTile ? nq : causal ? 1 : 0, group = (int)blockIdx.x - units * few;
+  if (group < 0) {
+    const int id = blockIdx.x, bh = id / few, t = id % few, b = bh / heads, h = bh % heads;
+    // a wave takes 32 queries (its lanes) by 32 keys (its registers); rows past the end are the last
+    const int wave = tid >> 6, l32 = tid & 31, hi = (tid >> 5) & 1, j0 = 32 * (wave >> 1);
+    const int i = t * kBwdTile + 32 * (wave & 1) + l32, qi = min(i, sq - 1), kj = min(j0 + l32, sk - 1);
+    const T* qr = q + b * qsb + h * qsh + (i64)qi * qss + 8 * hi;
+    const T* gr = go + b * gsb + h * gsh + (i64)qi * gss + 8 * hi;
+    const T* kr = k + b * ksb + h * ksh + (i64)kj * kss + 8 * hi;
+    const T* vr = v + b * vsb + h * vsh + (i64)kj * vss + 8 * hi;
+    const float shift = -lse[(i64)bh * sq + qi] * kLog2e;
+    f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+      s = In::mfma(*(const vec8*)(kr + 16 * x), *(const vec8*)(qr + 16 * x), s);
+      dp = In::mfma(*(const vec8*)(vr + 16 * x), *(const vec8*)(gr + 16 * x), dp);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = j0 + 8 * (r >> 2) + 4 * hi + (r & 3);
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, shift));
+      sum += j < sk && (!causal || j <= i) ? p * dp[r] : 0.0f;
+    }
+    u32 lower, upper;
+    pair_u32<32>(as_u32(sum), lower, upper);
+    if (hi == 0) dots[wave >> 1][32 * (wave & 1) + l32] = as_f32(lower) + as_f32(upper);
+    __syncthreads();
+    const int row = t * kBwdTile + tid;
+    if (tid < kBwdTile)
+      ndelta[(i64)bh * nq * kBwdTile + row] =
+          row < sq ? (glse != nullptr ? glse[(i64)bh * sq + row] : 0.0f) - (dots[0][tid] + dots[1][tid]) : 0.0f;
+    return;
+  }
+  const bool keys = kScaled && group >= units * nq;
+  const int id = keys ? group - units * nq : group, n = keys ? nk : nq;
   const int bh = id / n, t = id % n;
   const int b = bh / heads, h = bh % heads;
   float gm = 0.0f, lm = 0.0f;
@@ -247,34 +283,6 @@ __device__ __forceinline__ void attention_bwd_rows(
         gw[i] = load16_cached(gp + (i64)row * gss + 8 * c);
       }
     }
-    const int seen = causal ? min(sk, (t + 1) * kBwdTile) : sk;
-    if (seen <= kBwdTile) {
-      // a wave takes 32 queries (its lanes) by 32 keys (its registers); rows past the end are the last
-      const int wave = tid >> 6, l32 = tid & 31, hi = (tid >> 5) & 1, j0 = 32 * (wave >> 1);
-      const int i = t * kBwdTile + 32 * (wave & 1) + l32, qi = min(i, sq - 1), kj = min(j0 + l32, sk - 1);
-      const T* qr = q + b * qsb + h * qsh + (i64)qi * qss + 8 * hi;
-      const T* gr = gp + (i64)qi * gss + 8 * hi;
-      const T* kr = k + b * ksb + h * ksh + (i64)kj * kss + 8 * hi;
-      const T* vr = v + b * vsb + h * vsh + (i64)kj * vss + 8 * hi;
-      f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) {
-        s = In::mfma(*(const vec8*)(kr + 16 * x), *(const vec8*)(qr + 16 * x), s);
-        dp = In::mfma(*(const vec8*)(vr + 16 * x), *(const vec8*)(gr + 16 * x), dp);
-      }
-      const float shift = -lse[(i64)bh * sq + qi] * kLog2e;
-      float sum = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = j0 + 8 * (r >> 2) + 4 * hi + (r & 3);
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, shift));
-        sum += j < sk && (!causal || j <= i) ? p * dp[r] : 0.0f;
-      }
-      u32 lower, upper;
-      pair_u32<32>(as_u32(sum), lower, upper);
-      if (hi == 0) dots[wave >> 1][32 * (wave & 1) + l32] = as_f32(lower) + as_f32(upper);
-      __syncthreads();
-    }
 #pragma unroll
     for (int i = 0; i < kBwdTile / RPP; ++i) {
       const int row = t * kBwdTile + i * RPP + tid / LPR;
@@ -289,7 +297,6 @@ __device__ __forceinline__ void attention_bwd_rows(
         }
       }
       dot = group_sum<LPR>(dot);
-      if (seen <= kBwdTile) dot = dots[0][row - t * kBwdTile] + dots[1][row - t * kBwdTile];
       float dl = 0.0f;
       if (row < sq && glse != nullptr) dl = glse[(i64)bh * sq + row];
       if constexpr (kScaled) {
@@ -300,7 +307,7 @@ __device__ __forceinline__ void attention_bwd_rows(
       if (c == 0) {
         start[row0 + row] =
             row < sq ? -lse[(i64)bh * sq + row] / scale + BwdIn<T>::kLift / (scale * kLog2e) : -kInf;
-        ndelta[row0 + row] = row < sq ? dl - dot : 0.0f;
+        if (t >= few) ndelta[row0 + row] = row < sq ? dl - dot : 0.0f;
       }
     }
   } else {

@@ -204,7 +204,8 @@ def _call_plan(q, k, strides, grad_lse, scale, causal, plan=None) -> calls.Plan:
     start, ndelta, limit, part = (calls.buffer(3, o) for o in (0, stats, 2 * stats, 2 * stats + bounds))
     qs, ks, vs, gs, os = strides
     sizes, steps = (units, H, Sq, Sk), qs + ks + vs + gs + (scale, scale * LOG2E)
-    groups = units * (nq + (nk if q.dtype == torch.float16 else 0))
+    few = nq if Sk <= ATTN_BWD_TILE else int(causal)     # tiles of rows that see at most a tile of keys
+    groups = units * (nq + (nk if q.dtype == torch.float16 else 0) + few)
     kv_groups, q_groups = units * kv_parts * -(-Sk // rows), units * q_parts * -(-Sq // rows)
     qpart = calls.buffer(3, 2 * stats + bounds + kv_sums)
     launches = [
