@@ -538,7 +538,13 @@ __device__ __forceinline__ void mfma_settle(f32x16 (&c)[2]) {
 // The registers of an MFMA's c are free for other values once the next MFMA has been issued.
 __device__ __forceinline__ void mfma_read(const f32x16& c) { asm volatile("" : : "v"(c)); }
 __device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
-constexpr int kAhead = 2;               // steps that an LDS read is issued before its MFMAs
+// Three workgroups of head dim 64 share a CU without the mask, by 168 registers: K in LDS, and LDS reads one
+// step before their MFMAs instead of two.  fp16 8x12x777 79 us, 87 with two workgroups; 32x12x777 272, 293;
+// bf16 4x16x2048 239, 249.  (The mask's branch takes registers: causal 4x32x4096 1279 us, 1003 with two.)
+template <int D, bool CAUSAL>
+constexpr bool kThree = D == 64 && !CAUSAL;
+template <int D, bool CAUSAL>
+constexpr int kSteps = kThree<D, CAUSAL> ? 1 : 2;   // that an LDS read is issued before its MFMAs
 
 // A wave's 32 output rows (acc holds their transpose) go through its own 32 * D * 2 bytes of LDS,
 // 16-byte chunks XORed by row, and out as whole rows of 16 bytes per lane.  Written from the
@@ -600,7 +606,9 @@ __device__ __forceinline__ void attention_bwd_kv(
   constexpr int ROWS = D <= 128 ? kBwdTile : 32;     // queries per staged tile
   constexpr int TILE = ROWS * D * 2;
   constexpr bool kOwn = D * KB >= 128;               // more than 256 registers
-  constexpr bool kKeysInLds = D * KB >= 256;         // dK and dV take every AGPR, and K no vector register
+  // K takes no vector register where dK and dV take every AGPR, or three workgroups a CU
+  constexpr bool kKeysInLds = D * KB >= 256 || kThree<D, CAUSAL>;
+  constexpr int kAhead = kSteps<D, CAUSAL>;
   constexpr bool kScaled = BwdIn<T>::kScaled;
   unsigned char *const qbuf0 = bwd_tile<TILE, 0>(), *const qbuf1 = bwd_tile<TILE, 1>(),
                 *const gbuf0 = bwd_tile<TILE, 2>(), *const gbuf1 = bwd_tile<TILE, 3>();
@@ -897,6 +905,7 @@ __device__ __forceinline__ void attention_bwd_q(
   constexpr int ROWS = D <= 128 ? kBwdTile : 32;     // keys per staged tile, as attention_bwd_kv's
   constexpr int TILE = ROWS * D * 2;
   constexpr bool kScaled = BwdIn<T>::kScaled;
+  constexpr int kAhead = kSteps<D, CAUSAL>;
   constexpr bool kOwn = D * QB >= 128;              // more than 256 registers
   unsigned char *const kbuf0 = bwd_tile<TILE, 0>(), *const kbuf1 = bwd_tile<TILE, 1>(),
                 *const vbuf0 = bwd_tile<TILE, 2>(), *const vbuf1 = bwd_tile<TILE, 3>();

@@ -727,7 +727,8 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
                                    blocks: int = 1, parts: bool = False) -> str:
     """hiprtc unit of attention's gradients (nep_attention_bwd.h): the rows' statistics with the joins
     of split ranges ("rows"; the mask does not matter), or dK and dV, by the first `groups` workgroups, and
-    dQ, by the others ("kvq").  At head dim 64 two workgroups share a CU, and so a SIMD's 512 registers."""
+    dQ, by the others ("kvq").  At head dim 64 two workgroups share a CU, and so a SIMD's 512 registers, or
+    three without the mask and whole (parts are for few workgroups)."""
     if head_dim not in ATTN_HEAD_DIMS:
         raise NotImplementedError("attention fold supports head_dim 64, 128 and 256")
     if not 1 <= blocks <= attention_backward_blocks(head_dim):
@@ -758,6 +759,7 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
                 f"  nep::attention_bwd_join<{ctype}, {head_dim}, {pair}>(sums, ({ctype}*)a, ({ctype}*)b, "
                 "rows, len, other, block, per, causal);\n}\n")
         return "\n".join(units)
+    groups = 1 if head_dim > 64 else 2 if causal or parts else 3
 
     def call(which, outs, sums, per, group):
         return (f"nep::attention_bwd_{which}<{ctype}, {head_dim}, {cz}, {waves}, {blocks}, {str(parts).lower()}>("
@@ -767,7 +769,7 @@ def emit_attention_backward_source(stage: str, head_dim: int, causal: bool, dtyp
 
     return "\n".join([
         head,
-        f'extern "C" __global__ void __launch_bounds__({threads}, {2 if head_dim == 64 else 1}) {name}('
+        f'extern "C" __global__ void __launch_bounds__({threads}, {groups}) {name}('
         "const void* q, const void* k, const void* v, const void* go, const float* start, const float* ndelta, "
         "const float* bounds, void* dk, void* dv, void* dq, float* sums, float* qsums, int units, int heads, "
         "int sq, int sk, long long qsb, long long qsh, long long qss, long long ksb, long long ksh, "
