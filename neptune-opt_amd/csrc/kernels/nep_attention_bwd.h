@@ -10,8 +10,8 @@
 //
 // Three stages per call, none with an atomic: results do not depend on the order of workgroups.
 //  * attention_bwd_rows: delta of every query row, and the rows' start values -lse/scale.
-//  * attention_bwd_kv: a workgroup keeps K and V of its keys (in registers, K in LDS where dK and dV take
-//    every AGPR) and walks the query tiles (dK and dV stay in registers, four products per pair).
+//  * attention_bwd_kv: a workgroup keeps K and V of its keys (in registers, or K in LDS) and walks the query
+//    tiles (dK and dV stay in registers, four products per pair).
 //  * attention_bwd_q: a workgroup keeps Q and dO of its queries and walks the key tiles (three
 //    products per pair).
 // The last two share a launch, dQ's workgroups behind the others: apart and together, causal 2x8x1500x128
@@ -23,13 +23,14 @@
 // Bound by the matrix cores at the rate that this card's power allows a product: full bf16 2x16x4096x128
 // runs 962 GFLOP in 745 us (1290 TFLOP/s), a library product of 8192^3 1165 to 1350.  Causal 4x32x4096x128:
 // 962 GFLOP and the pairs hidden in tiles on the diagonal in 1795 us; a workgroup's start and end (11 us:
-// its rows, its gradients; one to a CU) and its waves' waits on the diagonal weigh twice as much there.  Head dim 64 (fp16 full 8x12x777: 69 us for both stages) passes
-// as many LDS reads and exponentials for half the products, and 7% of rows past the end.
+// its rows, its gradients; one to a CU) and its waves' waits on the diagonal weigh twice as much there.
+// Head dim 64 (fp16 full 8x12x777: 66 to 72 us for both stages) passes as many LDS reads and exponentials for
+// half the products, and 7% of rows past the end; its last workgroups leave CUs idle.
 //
 // Inside a tile P is computed beside the products of dP, dS beside those of dV (in attention_bwd_q P of one
 // block beside the next block's S, and dS beside the first half of dQ's products), each LDS read two steps
-// before its MFMAs: causal 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1862 so; full
-// 2x16x4096x128 874 and 770.  (The same order of blocks in attention_bwd_kv keeps the tile's rows and spills:
+// before its MFMAs: causal 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1854 so; full
+// 2x16x4096x128 874 and 768.  (The same order of blocks in attention_bwd_kv keeps the tile's rows and spills:
 // 1009 us, 1065.)
 //
 // Mapping (v_mfma_f32_32x32x16): attention_bwd_kv computes S[i][j] with A = Q rows from LDS and

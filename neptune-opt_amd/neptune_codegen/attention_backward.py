@@ -105,7 +105,7 @@ def _operand(t):
 
 # What `_plan` prices a launch with, in us on MI355X (fits of timings over twenty shapes): a workgroup's
 # pass over a 64-row tile with few workgroups on the chip, and a CU's with the chip full (the clock and
-# the caches are shared; head dim 64 has two workgroups on a CU); and a workgroup's start and end, without
+# the caches are shared; head dim 64 has two or three workgroups on a CU); and a workgroup's start and end, without
 # the mask and with it (its waves then wait for each other on the diagonal).
 TILE_US = {("kv", 64, 1): (1.0, 0.9, 4.0, 4.0), ("q", 64, 1): (1.0, 0.82, 3.0, 3.0),
            ("kv", 128, 1): (1.6, 1.7, 7.0, 8.0), ("q", 128, 1): (1.45, 1.45, 7.0, 8.0),
@@ -143,7 +143,7 @@ def _launch_cost(works, head_dim, causal, blocks):
     busy = longest = joins = last = 0.0
     for stage, (n, tiles, most, sums) in works.items():
         few, full, *ends = TILE_US[stage, head_dim, blocks]
-        # two workgroups on a CU take turns
+        # head dim 64: a CU's workgroups take turns
         tile = 1.7 * full if head_dim == 64 and items > CUS else few
         last = most * tile + ends[causal]
         late, longest = last > longest, max(longest, last)
