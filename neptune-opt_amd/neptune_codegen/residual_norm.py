@@ -113,7 +113,9 @@ def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, b
     """Lanes and slots of a row.  The forward pass takes two slots a lane once the rows fill the chip (bf16
     16384 x 4096 93-95 us with one, two or four; 3000 x 3001 17 us, one 20).  The gradient takes one, on
     workgroups of 512 lanes (1024 would hold its state in 128 registers: bf16 16384 x 4096 gated by sequence
-    174 us, 512 lanes 145; two slots on 256 lanes 209), or of 1024 where a row needs them."""
+    174 us, 512 lanes 145; two slots on 256 lanes 209), or of 1024 where a row needs them; a 16-bit row of
+    1025 to 1536 slots takes three on 512 lanes, whose state fits their 256 registers (gated 16384 x 12288 544
+    us, 644 by two on 1024 lanes; 1088 x 11100 81, 116; four spill: 16384 columns 245, 240)."""
     vec = 16 // x.element_size()
     slots = -(-n // vec)
     nv = 1
@@ -122,6 +124,8 @@ def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, b
     tpr = 1 << max(0, (-(-slots // nv) - 1).bit_length())
     while tpr > 1024:
         tpr, nv = tpr // 2, nv * 2
+    if backward and vec == 8 and 1024 < slots <= 1536:
+        tpr, nv = 512, 3
     wg = max(512 if backward else 256, tpr)
     access = "few" if n < vec else "words" if aligned else "any"
     return ResidualNormVariant(str(x.dtype).replace("torch.", ""), access, tpr, nv, wg, after, gate_kind)

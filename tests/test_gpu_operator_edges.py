@@ -7,6 +7,7 @@ import torch
 
 import neptune_codegen as CG
 from test_gpu_distill import check as check_distill, make as make_distill
+from test_gpu_residual_norm import check as check_norm, make as make_norm
 from test_gpu_rotary import heads, near
 
 pytestmark = pytest.mark.gpu
@@ -36,6 +37,16 @@ def test_rotary_halves_a_power_of_two_apart(part, dtype):
         q = heads(*lead, 4, part, dtype, dev, "bshd", part)
         for run, sign in ((CG.run_rotary, 1), (CG.run_rotary_backward, -1)):
             near(run(q, q, positions, turns)[1], q, positions, turns, 1.0, False, sign)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lead,n,after,gate", [((3, 7), 8193, True, (3, 1)), ((2, 5), 12288, False, None),
+                                               ((11,), 10240, True, (11,)), ((2, 3), 12289, True, ()),
+                                               ((300,), 9000, True, None)])
+def test_norms_of_wide_rows(lead, n, after, gate, dtype):
+    dev = _dev()
+    print(f"residual norm {lead}x{n} {dtype} after={after} gate={gate}", flush=True)
+    check_norm(make_norm(lead, n, dtype, after, gate), 0.5, dev)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
