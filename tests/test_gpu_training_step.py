@@ -225,7 +225,7 @@ def test_a_padded_batch_leaves_the_rows_behind_alone():
 
 
 def test_operators_keep_the_registration_contracts():
-    # schema, fake outputs, autograd registration and traced gradients, by torch's own checker
+    # schema, fake outputs, autograd registration and traced gradients (torch.library.opcheck)
     dev = _dev()
     g = torch.Generator().manual_seed(11)
     r = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev).requires_grad_()  # noqa: E731
