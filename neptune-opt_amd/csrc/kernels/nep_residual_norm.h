@@ -328,6 +328,9 @@ __device__ __forceinline__ void residual_norm_backward(
   constexpr int VEC = St::kVec, RPW = WG / TPR, COLS = Row::COLS;
   constexpr bool kLean = NV * VEC >= 16;
   constexpr int SHARED = kLean ? (AFTER + (GATE == kGateGroup)) * COLS : RPW > 1 ? RPW * COLS : 0;
+  static_assert(!kLean || RPW == 1, "sums of 16 columns a lane are the lane's own");
+  static_assert(SHARED >= (kLean && AFTER ? COLS : 0) + (kLean && GATE == kGateGroup ? COLS : 0) &&
+                    SHARED >= (RPW > 1 ? RPW * COLS : 0), "the sums' LDS");
   __shared__ __attribute__((aligned(16))) float lds[SHARED ? SHARED : 4];
   __shared__ float sums3[2][3 * (WG / 64)];
   const int t = threadIdx.x % TPR;
@@ -335,8 +338,10 @@ __device__ __forceinline__ void residual_norm_backward(
   const int slot = lane.first + lane.local;
   const float mean = 1.0f / (float)n;
   const i64 chunks = gridDim.x;
-  ColumnSums<St, TPR, NV, WG, kLean> da(lds, AFTER ? t : 0);
-  ColumnSums<St, TPR, NV, WG, kLean && GATE == kGateGroup> dg(lds + (kLean && AFTER ? COLS : 0), t);
+  // sums that a form has not (da without AFTER, dg without a group's gate) stay out of LDS: no part of it is theirs
+  ColumnSums<St, TPR, NV, WG, kLean && AFTER> da(lds, t);
+  constexpr int GATE_AT = kLean && AFTER ? COLS : 0;
+  ColumnSums<St, TPR, NV, WG, kLean && GATE == kGateGroup> dg(lds + GATE_AT, t);
   ColumnSums<St, TPR, NV, WG, false> db(lds, t);
 
   // words of gamma_after, gamma_before and the group's gate
