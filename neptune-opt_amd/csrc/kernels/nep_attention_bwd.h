@@ -46,9 +46,14 @@
 //
 // P and dS are rounded to the input type for their products (half a step, bf16 2^-8, fp16 2^-11
 // relative; the sums are fp32), the rounding that Q, K, V and dO themselves carry.  fp16 holds
-// 2^8 P (P alone would be subnormal below 2^-14) and dS times a power of two per head, from
-// bounds on |dO_i| and |v_j|, that keeps it below 2^15 and out of the subnormals; both are divided
-// out of the fp32 sums exactly.
+// 2^8 P (P alone would be subnormal below 2^-14) and dS times a power of two that keeps it below 2^15;
+// both are divided out of the fp32 sums exactly.  By Cauchy-Schwarz (delta_i + dlse_i averages the dP_ij)
+//   |dP_ij - delta_i| <= |dO_i| max|v| + |delta_i| <= 2 |dO_i| max|v| + |dlse_i|
+// For dQ_i the power is the query's own, from the first bound.  For dK_j, a sum over queries, the words of
+// all of them share one, from the second: of the queries that a wave's keys are walked with, under the mask
+// from the tile of its first key on.  A dS below 2^-29 of that bound is a subnormal there, off by up to
+// 2^-39 of the bound: it weighs only where every query that a key matters to has a gradient as much
+// smaller than another of those queries'.
 #pragma once
 
 namespace nep {
@@ -188,27 +193,25 @@ __device__ __forceinline__ typename AttnIn<T>::vec8 packed_operand(const u32* pk
   return __builtin_bit_cast(typename AttnIn<T>::vec8, w);
 }
 
-// The head's power of two on fp16 dS: |dP_ij - delta_i| <= 2 max|dO_i| max|v_j| + max|dlse_i|
-// (Cauchy-Schwarz; delta_i + dlse_i averages the dP_ij), below 2^e; 2^8 P dS 2^(7 - e) stays below
-// 2^15.  Returns 7 - e.  bounds: per 64 rows of queries (|dO|, |dlse|), then per 64 keys |v|.
-__device__ __forceinline__ int bwd_exponent(const float* __restrict__ rows, int nq,
-                                            const float* __restrict__ keys, int nk, int lane) {
-  float g = 0.0f, l = 0.0f, v = 0.0f;
-  for (int i = lane; i < nq; i += 64) {
-    g = __builtin_fmaxf(g, rows[2 * i]);
-    l = __builtin_fmaxf(l, rows[2 * i + 1]);
-  }
-  for (int i = lane; i < nk; i += 64) v = __builtin_fmaxf(v, keys[i]);
-  const float bound = 2.0f * group_max<64>(g) * group_max<64>(v) + group_max<64>(l);
-  const int e = (int)(as_u32(bound) >> 23) - 126;   // bound < 2^e
+// fp16's power of two on dS for a bound on |dP_ij - delta_i|: with bound < 2^e, 2^8 P dS 2^(7 - e) stays
+// below 2^15.  Returns 7 - e.
+__device__ __forceinline__ int bwd_exponent(float bound) {
+  const int e = (int)(as_u32(bound) >> 23) - 126;
   return 7 - min(max(e, -100), 100);
+}
+// The most of `n` bounds that are `step` apart (the wave's).
+__device__ __forceinline__ float bwd_most(const float* __restrict__ bounds, int step, int n, int lane) {
+  float m = 0.0f;
+  for (int i = lane; i < n; i += 64) m = __builtin_fmaxf(m, bounds[step * i]);
+  return group_max<64>(m);
 }
 
 // delta_i and the start values of every query row, and fp16's bounds.  start[bh][sqp] holds
 // -lse/scale + lift (with rows from sq to sqp, a multiple of 64, at -inf: their P is 0), and
 // ndelta[bh][sqp] -delta_i (0 there).  A workgroup of 256 threads takes 64 query rows, D/8 lanes a
-// row; with fp16 the workgroups behind them take 64 keys each and bound |v|.  Rows with an infinity
-// or NaN are left out of the bounds: what they reach is not finite whatever the scale.
+// row; with fp16 the workgroups behind them take 64 keys each and bound |v|.  bounds: per 64 rows of queries
+// (|dO|, |dlse|), then per 64 keys |v|.  Rows with an infinity or NaN are left out of the bounds: what they
+// reach is not finite whatever the scale.
 // Rows that see at most 64 keys (the first tile under the causal mask) take delta + dlse as the sum of
 // P_ij dP_ij over their keys instead: with few keys O is as large as a row of V, and its rounding, times
 // dO, weighs on every dS of the row (relative 2-norm errors of dQ and dK, bf16 causal 2x4x77x64, are 1.61
@@ -655,10 +658,14 @@ __device__ __forceinline__ void attention_bwd_kv(
     }
   }
   int lift = 0;
-  if constexpr (kScaled)
-    lift = bwd_exponent(bounds + 2 * (i64)bh * nq, nq,
-                        bounds + 2 * (i64)units * nq + (i64)bh * ((sk + kBwdTile - 1) / kBwdTile),
-                        (sk + kBwdTile - 1) / kBwdTile, lane);
+  if constexpr (kScaled) {
+    const int nk = (sk + kBwdTile - 1) / kBwdTile;
+    const int from = max(t0 / PER, CAUSAL ? kw / kBwdTile : 0), to = (t1 + PER - 1) / PER;
+    const float* rows = bounds + 2 * ((i64)bh * nq + from);
+    lift = bwd_exponent(2.0f * bwd_most(rows, 2, to - from, lane) *
+                            bwd_most(bounds + 2 * (i64)units * nq + (i64)bh * nk, 1, nk, lane) +
+                        bwd_most(rows + 1, 2, to - from, lane));
+  }
   const float ds_mul = exp2_int(lift);
 
   const BwdTile<D, W, ROWS> qdma(wave, lane, qss), gdma(wave, lane, gss);
@@ -951,19 +958,34 @@ __device__ __forceinline__ void attention_bwd_q(
       }
     }
   }
+  int lift[QB];                                      // a query's power of two on dS
+  float most = 0.0f;                                 // |v|
+  if constexpr (kScaled) most = bwd_most(bounds + 2 * (i64)units * nq + (i64)bh * nk, 1, nk, lane);
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    lift[x] = 0;
+    if constexpr (kScaled) {
+      float g2 = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = (float)greg[x][s][j];
+          g2 = __builtin_fmaf(w, w, g2);
+        }
+      u32 lower, upper;
+      pair_u32<32>(as_u32(g2), lower, upper);
+      lift[x] = bwd_exponent(__builtin_sqrtf(as_f32(lower) + as_f32(upper)) * 1.001f * most +
+                             __builtin_fabsf(minus[x]));
+      shift[x] += (float)lift[x];                    // on P
+    }
+  }
   if constexpr (kOwn) {
 #pragma unroll
     for (int x = 0; x < QB; ++x)
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) asm("" : "+a"(greg[x][s]));
   }
-  int lift = 0;
-  if constexpr (kScaled)
-    lift = bwd_exponent(bounds + 2 * (i64)bh * nq, nq, bounds + 2 * (i64)units * nq + (i64)bh * nk,
-                        nk, lane);
-#pragma unroll
-  for (int x = 0; x < QB; ++x) shift[x] += (float)lift;   // P times the power of two of dS
-
   const BwdTile<D, W, ROWS> kdma(wave, lane, kss), vdma(wave, lane, vss);
   const BwdRead<T, D> rd(lane);
   auto issue = [&](int tile, unsigned char* kd, unsigned char* vd) {
@@ -1111,14 +1133,16 @@ __device__ __forceinline__ void attention_bwd_q(
       return;
     }
   }
-  const float sf = scale * exp2_int(-(int)BwdIn<T>::kLift) * exp2_int(-lift);
+  float sf[QB];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) sf[x] = scale * exp2_int(-(int)BwdIn<T>::kLift) * exp2_int(-lift[x]);
   if (whole) {
     if constexpr (!CAUSAL) __syncthreads();          // every wave is done with the tiles
     static_assert(W <= 4, "one tile buffer for each wave");
     unsigned char* stage = wave == 0 ? kbuf0 : wave == 1 ? kbuf1 : wave == 2 ? vbuf0 : vbuf1;
 #pragma unroll
     for (int x = 0; x < QB; ++x)
-      bwd_store_rows<T, D>(stage, dqa[x], sf, dq + row0 * D, qw + 32 * x, sq, lane);
+      bwd_store_rows<T, D>(stage, dqa[x], sf[x], dq + row0 * D, qw + 32 * x, sq, lane);
   } else {
 #pragma unroll
     for (int x = 0; x < QB; ++x) {
@@ -1128,8 +1152,8 @@ __device__ __forceinline__ void attention_bwd_q(
       for (int a = 0; a < DBLK; ++a)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          store(i, 32 * a + 8 * g + 4 * hi, dqa[x][a][4 * g] * sf, dqa[x][a][4 * g + 1] * sf,
-                dqa[x][a][4 * g + 2] * sf, dqa[x][a][4 * g + 3] * sf);
+          store(i, 32 * a + 8 * g + 4 * hi, dqa[x][a][4 * g] * sf[x], dqa[x][a][4 * g + 1] * sf[x],
+                dqa[x][a][4 * g + 2] * sf[x], dqa[x][a][4 * g + 3] * sf[x]);
     }
   }
 }
