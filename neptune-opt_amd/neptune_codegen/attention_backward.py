@@ -91,6 +91,14 @@ def validate_attention_backward_inputs(grad, q, k, v, out, lse, grad_lse=None, *
     return shape
 
 
+def _scale(scale, head_dim: int = 64) -> float:
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    # (the kernels hold lse / scale in fp32)
+    if not 2.0 ** -100 <= scale <= calls.MOST_FLOAT:
+        raise ValueError("attention scale must be finite and positive, from 2^-100 to 2^125")
+    return scale
+
+
 def _operand(t):
     """(t, or its contiguous copy where a kernel cannot read its rows; batch, head, row strides).
     Rows that overlap (an expanded sequence) are copied too: a tile's rows past the end must read as
@@ -243,10 +251,7 @@ def _run(grad, q, k, v, out, lse, grad_lse, scale, causal, plan=None):
     metadata = isinstance(q, torch.Tensor) and calls.is_metadata(q)
     validate_attention_backward_inputs(grad, q, k, v, out, lse, grad_lse, metadata=metadata)
     given, number = (grad, q, k, v, out, lse, grad_lse), scale
-    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-    # (the kernels hold lse / scale in fp32)
-    if not 2.0 ** -100 <= scale <= calls.MOST_FLOAT:
-        raise ValueError("attention scale must be finite and positive, from 2^-100 to 2^125")
+    scale = _scale(scale, q.shape[3])
     if metadata or q.numel() == 0:
         # without a query nothing reaches the keys
         return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
@@ -271,7 +276,7 @@ def as_attention_grad_op(scale: float | None = None, causal: bool = True, lib: s
     from neptune_codegen.attention import run_attention
     from neptune_codegen.autotune import parameter_tag
 
-    params = {"scale": float(scale)} if scale is not None else {}
+    params = {"scale": _scale(scale)} if scale is not None else {}
     causal = bool(causal)
     key = (lib, tuple(sorted(params.items())), causal)
     with _lock:
