@@ -104,8 +104,10 @@ def _operand(t):
     Rows that overlap (an expanded sequence) are copied too: a tile's rows past the end must read as
     zero."""
     sb, sh, ss, sd = t.stride()
-    if not (sd == 1 and sb % 8 == 0 and sh % 8 == 0 and ss % 8 == 0 and ss < K_ROW_STRIDE_MAX
-            and (ss >= t.shape[3] or t.shape[2] == 1) and t.data_ptr() % 16 == 0):
+    if t.shape[2] == 1:
+        ss = t.shape[3]                              # one row has any stride
+    if not (sd == 1 and sb % 8 == 0 and sh % 8 == 0 and ss % 8 == 0 and t.shape[3] <= ss < K_ROW_STRIDE_MAX
+            and t.data_ptr() % 16 == 0):
         t = t.contiguous()
         sb, sh, ss, _ = t.stride()
     return t, (sb, sh, ss)
