@@ -269,6 +269,13 @@ py::object key_of(const std::vector<at::Tensor>& tensors) {
 }
 
 // ---------------------------------------------------------------- direct entry points
+// The error that the Python launch path raises (hip.HipError), for entry points that are called from Python.
+[[noreturn]] void throw_hip_error(const std::string& message) {
+  const py::object type = py::module_::import("neptune_codegen.hip").attr("HipError");
+  PyErr_SetString(type.ptr(), message.c_str());
+  throw py::error_already_set();
+}
+
 // One call layout of an entry point: the buffers it allocates (results first, then scratch) and its
 // launches, whose pointer arguments are each an input, or a buffer at a byte offset.
 class CallPlan {
@@ -353,7 +360,7 @@ class CallPlan {
         }
         const int rc = nep_launch_packed(l.kernel, l.grid[0], l.grid[1], l.grid[2], l.block, l.lds,
                                          stream, image, l.image.size());
-        TORCH_CHECK(rc == NEP_OK, "neptune launch failed: ", nep_last_error());
+        if (rc != NEP_OK) throw_hip_error(std::string("launch: ") + nep_last_error());
       }
     }
     if (bare_) return py::cast(buffers[returns_[0]]);
