@@ -46,7 +46,8 @@
 //
 // P and dS are rounded to the input type for their products (half a step, bf16 2^-8, fp16 2^-11
 // relative; the sums are fp32), the rounding that Q, K, V and dO themselves carry.  fp16 holds
-// 2^8 P (P alone would be subnormal below 2^-14) and dS times a power of two that keeps it below 2^15;
+// 2^14 P (a normal number down to 2^-28; two more bits are left for a P past 1, which large scores' rounding
+// may make) and dS times a power of two that keeps it below 2^15;
 // both are divided out of the fp32 sums exactly.  By Cauchy-Schwarz (delta_i + dlse_i averages the dP_ij)
 //   |dP_ij - delta_i| <= |dO_i| max|v| + |delta_i| <= 2 |dO_i| max|v| + |dlse_i|
 // For dQ_i the power is the query's own, from the first bound.  For dK_j, a sum over queries, the words of
@@ -73,7 +74,7 @@ struct BwdIn<__bf16> {
 template <>
 struct BwdIn<_Float16> {
   static constexpr bool kScaled = true;
-  static constexpr float kLift = 8.0f;
+  static constexpr float kLift = 14.0f;
   static constexpr u32 kExponent = 0x7c007c00u;
 };
 
@@ -193,11 +194,11 @@ __device__ __forceinline__ typename AttnIn<T>::vec8 packed_operand(const u32* pk
   return __builtin_bit_cast(typename AttnIn<T>::vec8, w);
 }
 
-// fp16's power of two on dS for a bound on |dP_ij - delta_i|: with bound < 2^e, 2^8 P dS 2^(7 - e) stays
-// below 2^15.  Returns 7 - e.
+// fp16's power of two on dS for a bound on |dP_ij - delta_i|, behind the one on P: with bound < 2^e,
+// 2^14 P (dP - delta) 2^(1 - e) stays below 2^15.  Returns 1 - e.
 __device__ __forceinline__ int bwd_exponent(float bound) {
   const int e = (int)(as_u32(bound) >> 23) - 126;
-  return 7 - min(max(e, -100), 100);
+  return 1 - min(max(e, -100), 100);
 }
 // The most of `n` bounds that are `step` apart (the wave's).
 __device__ __forceinline__ float bwd_most(const float* __restrict__ bounds, int step, int n, int lane) {

@@ -83,3 +83,22 @@ def test_rows_without_a_gradient():
     got = CG.run_attention_backward(grad, q, k, v, out, lse)
     assert not got[0][:, :, 10:100].any()
     check(got, grad, q, k, v, 128 ** -0.5, True)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_that_every_query_passes_over(dim, causal):
+    """One key takes all but e^-19 of each row, and the gradient is large: the other keys' dV are well above the
+    type's smallest numbers, from P around 2^-27.  P's words hold 2^14 P, so a subnormal one is off by up to 2^-39."""
+    dev = _dev()
+    print(f"attention backward of passed-over keys {dim} causal={causal}", flush=True)
+    q, k, v, grad = inputs((1, 2, 16, dim), 16 if causal else 64, torch.float16, dev, seed=25, grad_scale=2.0 ** 12)
+    q, k = (1 + q / 16).half(), (k / 64).half()
+    k[:, :, 0] = 19 / dim ** 0.5
+    out, lse = CG.run_attention(q, k, v, causal=causal, return_lse=True)
+    _, _, dv = CG.run_attention_backward(grad, q, k, v, out, lse, causal=causal)
+    u = 2.0 ** -11
+    (_, _, want), (_, _, off) = formulas(grad, q, k, v, dim ** -0.5, causal, None, u, 2.0 ** -13)
+    off = off + 2.0 ** -39 * grad.double().cpu().abs().sum(2, keepdim=True)
+    assert 2.0 ** -16 < want[:, :, 1:].abs().median() < 2.0 ** -9
+    assert ((dv.double().cpu() - want).abs() / off).max() <= 1.0
