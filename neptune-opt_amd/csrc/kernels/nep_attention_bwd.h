@@ -16,21 +16,22 @@
 //    products per pair).
 // The last two share a launch, dQ's workgroups behind the others: apart and together, causal 2x8x1500x128
 // 97 and 57 us, 2x16x2048x128 198 and 146, 7x4x576x256 88 and 55, 1x4x8192x128 438 and 284, full
-// 8x12x777x64 95 and 90, causal 4x32x4096x128 1854 and 1842.  (Long calls of head dim 64 lose 1%, dQ's
+// 8x12x777x64 95 and 90; causal 4x32x4096x128 the same within 1%.  (Long calls of head dim 64 lose 1%, dQ's
 // workgroups being three to a CU alone.)  Five products instead of seven, with one stage, would add dQ
 // across key blocks: fp32 atomics, whose order changes results, or an fp32 copy of dQ per key block.
 //
 // Bound by the matrix cores at the rate that this card's power allows a product: full bf16 2x16x4096x128
-// runs 962 GFLOP in 745 us (1290 TFLOP/s), a library product of 8192^3 1165 to 1350.  Causal 4x32x4096x128:
-// 962 GFLOP and the pairs hidden in tiles on the diagonal in 1795 us; a workgroup's start and end (11 us:
-// its rows, its gradients; one to a CU) and its waves' waits on the diagonal weigh twice as much there.
-// Head dim 64 (fp16 full 8x12x777: 66 to 72 us for both stages) passes as many LDS reads and exponentials for
+// takes 760 to 770 us for the call's 962 GFLOP (1260 TFLOP/s), a library product of 8192^3 1165 to 1350.  Causal
+// 4x32x4096x128: 1924 GFLOP, and the pairs hidden in tiles on the diagonal, in 1810 to 1940 us from card to card;
+// a workgroup's start and end (11 us: its rows, its gradients; one to a CU) are as long for half the tiles, and
+// on the diagonal its waves wait for each other (with that, 19 to 22 us).
+// Head dim 64 (fp16 full 8x12x777: 69 to 80 us the call) passes as many LDS reads and exponentials for
 // half the products, and 7% of rows past the end; its last workgroups leave CUs idle.
 //
 // Inside a tile P is computed beside the products of dP, dS beside those of dV (in attention_bwd_q P of one
 // block beside the next block's S, and dS beside the first half of dQ's products), each LDS read two steps
-// before its MFMAs: causal 4x32x4096x128 1994 us in the order S, dP, P, dS, products and 1854 so; full
-// 2x16x4096x128 874 and 768.  (The same order of blocks in attention_bwd_kv keeps the tile's rows and spills:
+// before its MFMAs: causal 4x32x4096x128 7% less than in the order S, dP, P, dS, products; full
+// 2x16x4096x128 874 us so and 768.  (The same order of blocks in attention_bwd_kv keeps the tile's rows and spills:
 // 1009 us, 1065.)
 //
 // Mapping (v_mfma_f32_32x32x16): attention_bwd_kv computes S[i][j] with A = Q rows from LDS and
@@ -543,8 +544,8 @@ __device__ __forceinline__ void mfma_settle(f32x16 (&c)[2]) {
 // The registers of an MFMA's c are free for other values once the next MFMA has been issued.
 __device__ __forceinline__ void mfma_read(const f32x16& c) { asm volatile("" : : "v"(c)); }
 __device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); }
-// Three workgroups of head dim 64 share a CU without the mask, by 168 registers: K in LDS, and LDS reads one
-// step before their MFMAs instead of two.  fp16 8x12x777 79 us, 87 with two workgroups; 32x12x777 272, 293;
+// Three workgroups of head dim 64 share a CU without the mask, by 168 registers (6 spilled in bf16, 9 in fp16): K
+// in LDS, and LDS reads one step before their MFMAs instead of two.  fp16 8x12x777 79 us, 87 with two workgroups; 32x12x777 272, 293;
 // bf16 4x16x2048 239, 249.  (The mask's branch takes registers: causal 4x32x4096 1279 us, 1003 with two.)
 template <int D, bool CAUSAL>
 constexpr bool kThree = D == 64 && !CAUSAL;
@@ -588,11 +589,12 @@ __device__ __forceinline__ unsigned char* bwd_tile() {
   return tile;
 }
 
-// dK and dV.  W waves of 32 KB keys each; a wave's K and V rows and its dK^T and dV^T stay in
-// registers, the workgroup's Q and dO tiles are staged for all of its waves.  One wave per SIMD:
-// at KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1
-// (at 32 keys a wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock: full
-// 2x16x4096x128 955 us, 907 with two blocks).
+// dK and dV.  W waves of 32 KB keys each; a wave's V rows and its dK^T and dV^T stay in registers, its K
+// rows too (in LDS where dK and dV take every AGPR, D KB = 256, and where three workgroups share a CU); the
+// workgroup's Q and dO tiles are staged for all of its waves.  From head dim 128 on a SIMD has one wave: at
+// KB = 2 every operand read from LDS feeds two MFMAs, which halves the LDS traffic of KB = 1 (at 32 keys a
+// wave the four SIMDs' operand reads alone fill the LDS's 128 bytes a clock: full 2x16x4096x128 872 to 881
+// us, 770 with two blocks).  Under the mask two blocks of head dim 128, and 256, spill 9 to 40 registers a lane.
 // PARTS: each block's query tiles are taken in parts of `per` (64-row tiles, from the block's first);
 // of a block with more than one, each part's fp32 sums go to `sums` [part][bh][key][dK, dV][D] for
 // attention_bwd_join.

@@ -19,7 +19,8 @@
 // HBM-bound: the forward pass reads x and y and writes r and h, the gradient reads x, y, dr and dh and
 // writes dx and dy, once each; rows stay in registers as packed words.  Forward bf16 16384 x 4096 91-95 us
 // (5.7-5.9 TB/s; one slot a lane, two and four within 4%), 65536 x 256 24 us; gradient 143-146 us, fp32
-// 8192 x 4096 138, bf16 16384 x 8192 280; 16384 columns 180-250 us per 0.8 GB, where registers run out.
+// 8192 x 4096 138, bf16 16384 x 8192 280; 16384 columns 144-204 us per 0.8 GB (of any
+// alignment 192-320), where registers run out.
 #pragma once
 
 namespace nep {
@@ -306,9 +307,12 @@ struct ColumnSums {
 // A workgroup of WG lanes walks a chunk of rows, WG / TPR at a time, and keeps the column sums, one
 // partial row per workgroup and quantity (256 workgroups: 3% of the bytes at 16384 x 4096).  With up to 8
 // columns a lane the next rows' words are in flight under the arithmetic of these, the gammas and the
-// gate stay in registers in fp32, and an element's terms are kept from the sums to the results; with 16
-// there are no registers for that, and sums but dgamma_before's are in LDS.
-//   `per_group` workgroups share each group of `group` rows, or (per_group 0) each takes whole groups.
+// gate stay in registers as packed words, and an element's terms are kept from the sums to the results; with 16
+// there are no registers for that: a row's words and the gammas are read when it is begun, and the sums of
+// dgamma_after and of a group's gate are in LDS.
+//   `per_group` workgroups share each group of `group` rows, or (per_group 0) each takes whole groups: between
+//   129 and 255 groups, and a little above 256, that leaves CUs idle (bf16 16384 x 4096 in 128 groups 159 us,
+//   129 263, 200 174, 256 158, 257 248, 512 157).
 //   Rows and groups are dealt in turn, so that the workgroups walk through memory together: in
 //   contiguous chunks, 512 KB apart at bf16 16384 x 4096, they meet in the same memory channels (160-166
 //   us; in turn 148-150; with exact waits, above, 143-146, 5.6 TB/s).

@@ -113,7 +113,8 @@ def _operand(t):
     return t, (sb, sh, ss)
 
 
-# What `_plan` prices a launch with, in us on MI355X (fits of timings over twenty shapes): a workgroup's
+# What `_plan` prices a launch with, in us on MI355X (fits of timings over 34 shapes; of the plans within 1.5 times its
+# price the chosen one is within 4% of the fastest in 33 of them, and 10% in causal 1x8x2000x256): a workgroup's
 # pass over a 64-row tile with few workgroups on the chip, and a CU's with the chip full (the clock and
 # the caches are shared; head dim 64 has two or three workgroups on a CU); and a workgroup's start and end, without
 # the mask and with it (its waves then wait for each other on the diagonal).
@@ -184,9 +185,9 @@ def _plan_tiles(units, q_tiles, k_tiles, head_dim, causal):
 def _plan(units, sq, sk, head_dim, causal):
     """(blocks per wave, kv parts, q parts) of a call, the cheapest by TILE_US; searched once for the same
     tile counts.  Two blocks a wave (head dim 128) read each tile half as often and pass twice the rows
-    in 1.7 to 1.8 times the time, with a longer start and end: bf16 causal 4x32x4096x128 1861 us by two,
-    2072 by one; full 2x16x4096x128 800 and 875, 8x32x1024x128 469 and 555; but causal 8x32x1024x128 398 and
-    375, 2x8x300x128 59 and 20."""
+    in 1.7 to 1.8 times the time, with a longer start and end: bf16 causal 4x32x4096x128 1858 us by two,
+    2055 by one; full 2x16x4096x128 770 and 876, 8x32x1024x128 476 and 566; but causal 8x32x1024x128 395 and
+    383, 2x8x300x128 39 and 22."""
     return _plan_tiles(units, -(-sq // ATTN_BWD_TILE), -(-sk // ATTN_BWD_TILE), head_dim, causal)
 
 

@@ -114,8 +114,12 @@ def _variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, b
     16384 x 4096 93-95 us with one, two or four; 3000 x 3001 17 us, one 20).  The gradient takes one, on
     workgroups of 512 lanes (1024 would hold its state in 128 registers: bf16 16384 x 4096 gated by sequence
     174 us, 512 lanes 145; two slots on 256 lanes 209), or of 1024 where a row needs them; a 16-bit row of
-    1025 to 1536 slots takes three on 512 lanes, whose state fits their 256 registers (gated 16384 x 12288 544
-    us, 644 by two on 1024 lanes; 1088 x 11100 81, 116; four spill: 16384 columns 245, 240)."""
+    1025 to 1536 slots takes three on 512 lanes, whose state fits their 256 registers but for rows of any alignment
+    with gamma_after and a group's gate, which spill 20 (fp16) and 26 (gated 16384 x 12288 541 us, 644 by two on 1024
+    lanes; 1088 x 11100 81, 116; four spill: 16384 columns 245, 240).  On 1024 lanes with 128 registers the forms
+    of one 16-byte slot fit but for 8192 16-bit columns with gamma_after and a gate (up to 23 spilled); of two and
+    four most gated forms spill (fp32 8192 columns up to 52, 16384 up to 138): fp32 4096 x 8192 149 us bare, 250
+    with gamma_after and a gate per sequence; 16-bit 8192 x 16384 288 and 408."""
     vec = 16 // x.element_size()
     slots = -(-n // vec)
     nv = 1
