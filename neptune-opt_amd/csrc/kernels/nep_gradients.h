@@ -1,0 +1,175 @@
+// nep_gradients.h -- the 2-norm of many tensors together, and their scaling to a largest norm (gfx950).
+//
+//   norm = sqrt(sum over all elements of g^2)          out = g * min(1, max_norm / norm)
+// Squares and sums are fp64: the square of an fp32 number neither overflows nor vanishes there, and the
+// conversion and the FMA are hidden behind the loads.  The norm is rounded to fp32 once and the factor comes
+// from the rounded norm, so that a norm computed before gives the same bits.  A norm that is an infinity or
+// NaN has no factor: the elements stay as they are.
+//
+// A launch takes up to kTensors tensors by value, in its arguments: nothing is copied to the device, and a
+// captured launch keeps its own list.  Their elements are dealt to the workgroups in turn, in pieces of
+// `piece` elements that do not cross tensors; a workgroup finds a piece's tensor by bisection (scalar loads
+// from the arguments).  Scaling walks the pieces from the last to the first: what the norm read last is still
+// in the memory-side cache.
+#pragma once
+
+namespace nep {
+
+constexpr int kTensors = 112;                        // 3584 bytes; all arguments stay below 4096
+constexpr int kSumLanes = 1024;
+
+struct TensorEntry {
+  const void* in;
+  void* out;
+  u64 count;                                         // elements, at least one
+  u32 first;                                         // number of its first piece
+  u32 kind;                                          // types of in and out, see visit
+};
+struct TensorList {
+  TensorEntry entry[kTensors];
+};
+
+// in and out
+constexpr u32 kF32 = 0, kBF16 = 1, kF16 = 2, kBF16ToF32 = 3, kF16ToF32 = 4;
+
+// The entry that piece p belongs to; entries [0, count) with ascending first pieces.
+__device__ __forceinline__ const TensorEntry& entry_of(const TensorList& list, int count, u32 p) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list.entry[mid].first <= p) lo = mid;
+    else hi = mid;
+  }
+  return list.entry[lo];
+}
+
+// Sum over the workgroup of kSumLanes lanes, the same in every lane.  (lds: a double per wavefront)
+__device__ __forceinline__ double workgroup_sum(double v, double* lds) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    const int from = (lane ^ d) * 4;
+    const u64 lo = (u32)__builtin_amdgcn_ds_bpermute(from, (int)(u32)b);
+    const u64 hi = (u32)__builtin_amdgcn_ds_bpermute(from, (int)(u32)(b >> 32));
+    v += __builtin_bit_cast(double, lo | hi << 32);
+  }
+  if (lane == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double total = 0.0;
+#pragma unroll
+  for (int w = 0; w < kSumLanes / 64; ++w) total += lds[w];
+  return total;
+}
+
+// Squares of elements [first, end) of p, added to acc.
+template <class St>
+__device__ __forceinline__ void add_squares(const typename St::T* p, i64 first, i64 end, double& acc) {
+  constexpr int VEC = St::kVec, FLIGHT = 4;
+  const i64 words = (end - first) / VEC;
+  p += first;
+  for (i64 w0 = 0; w0 < words; w0 += kSumLanes * FLIGHT) {
+    u32x4 w[FLIGHT];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      w[f] = i < words ? load16_any(p + i * VEC) : u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      float v[VEC];
+      St::unpack(w[f], v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc = __builtin_fma((double)v[j], (double)v[j], acc);
+    }
+  }
+  const i64 rest = words * VEC + threadIdx.x;
+  if (rest < end - first) {
+    const double v = (double)St::load(p + rest);
+    acc = __builtin_fma(v, v, acc);
+  }
+}
+
+__device__ __forceinline__ void gradient_sums(const TensorList& list, int count, u32 pieces, int piece,
+                                              double* __restrict__ sums) {
+  __shared__ double lds[kSumLanes / 64];
+  double acc = 0.0;
+  for (u32 p = blockIdx.x; p < pieces; p += gridDim.x) {
+    const TensorEntry& e = entry_of(list, count, p);
+    const i64 first = (i64)(p - e.first) * piece;
+    const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
+    if (e.kind == kF32) add_squares<F32>((const float*)e.in, first, end, acc);
+    else if (e.kind == kBF16 || e.kind == kBF16ToF32) add_squares<BF16>((const u16*)e.in, first, end, acc);
+    else add_squares<F16>((const _Float16*)e.in, first, end, acc);
+  }
+  const double total = workgroup_sum(acc, lds);
+  if (threadIdx.x == 0) sums[blockIdx.x] = total;
+}
+
+// The norm from the workgroups' sums.
+__device__ __forceinline__ float norm_of(const double* __restrict__ sums, int count) {
+  __shared__ double lds[kSumLanes / 64];
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < count; i += kSumLanes) acc += sums[i];
+  return (float)__builtin_sqrt(workgroup_sum(acc, lds));
+}
+
+__device__ __forceinline__ void gradient_norm(const double* __restrict__ sums, int count, float* __restrict__ norm) {
+  const float v = norm_of(sums, count);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+template <class St, class Ot>
+__device__ __forceinline__ void scale_elements(const typename St::T* p, typename Ot::T* q, i64 first, i64 end,
+                                               float factor) {
+  constexpr int VEC = St::kVec, FLIGHT = 4;
+  const i64 words = (end - first) / VEC;
+  p += first;
+  q += first;
+  for (i64 w0 = 0; w0 < words; w0 += kSumLanes * FLIGHT) {
+    u32x4 w[FLIGHT];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      if (i < words) w[f] = load16_any(p + i * VEC);
+    }
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      if (i >= words) continue;
+      float v[VEC];
+      St::unpack(w[f], v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] *= factor;
+#pragma unroll
+      for (int j = 0; j < VEC; j += Ot::kVec) store16_any(q + i * VEC + j, Ot::pack(v + j));
+    }
+  }
+  const i64 rest = words * VEC + threadIdx.x;
+  if (rest < end - first) Ot::store(q + rest, St::load(p + rest) * factor);
+}
+
+// `sums` null: the norm is given.  `copies`: whether an entry's out is not its in.
+__device__ __forceinline__ void gradient_scale(const TensorList& list, int count, u32 pieces, int piece,
+                                               const double* __restrict__ sums, int n_sums,
+                                               const float* __restrict__ given, float* __restrict__ norm_out,
+                                               float max_norm, int copies) {
+  const float norm = sums != nullptr ? norm_of(sums, n_sums) : *given;
+  if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  const float factor = is_finite(norm) && norm > max_norm ? div_rn(max_norm, norm) : 1.0f;
+  if (factor == 1.0f && !copies) return;
+  for (u32 i = blockIdx.x; i < pieces; i += gridDim.x) {
+    const u32 p = pieces - 1 - i;
+    const TensorEntry& e = entry_of(list, count, p);
+    if (factor == 1.0f && e.in == e.out) continue;
+    const i64 first = (i64)(p - e.first) * piece;
+    const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
+    if (e.kind == kF32) scale_elements<F32, F32>((const float*)e.in, (float*)e.out, first, end, factor);
+    else if (e.kind == kBF16) scale_elements<BF16, BF16>((const u16*)e.in, (u16*)e.out, first, end, factor);
+    else if (e.kind == kF16) scale_elements<F16, F16>((const _Float16*)e.in, (_Float16*)e.out, first, end, factor);
+    else if (e.kind == kBF16ToF32) scale_elements<BF16, F32>((const u16*)e.in, (float*)e.out, first, end, factor);
+    else scale_elements<F16, F32>((const _Float16*)e.in, (float*)e.out, first, end, factor);
+  }
+}
+
+}  // namespace nep

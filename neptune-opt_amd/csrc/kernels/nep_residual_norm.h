@@ -160,13 +160,123 @@ __device__ __forceinline__ void row_sums(float* v, float* lds) {
   }
 }
 
-template <class St, int TPR, int NV, int ACCESS, bool AFTER, int GATE, int WG>
+// ---------------------------------------------------------------- an 8-bit output
+// h in 8 bits, h ~ scale q: blocks of GROUP columns (of the whole row, 0) have an fp32 scale each,
+//   scale = max|h| / M, M the format's largest value, or the least power of two that is no less (POWER),
+// and at least 2^-126, the least normal number; q = h / scale rounded to the format, half to even.  A block
+// with an infinity or NaN has that for a scale, so that scale q is not finite in any of its columns.
+constexpr int kSameType = 0, kE4M3 = 1, kE5M2 = 2, kInt8 = 3;
+
+template <int FORMAT>
+struct Format;
+template <>
+struct Format<kE4M3> {
+  static constexpr float kMost = 448.0f;             // 1.75 2^8
+  static constexpr u32 kExponent = 8, kFraction = 0x600000u;
+  __device__ static __forceinline__ u32 pack(const float* v) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+  }
+};
+template <>
+struct Format<kE5M2> {
+  static constexpr float kMost = 57344.0f;           // 1.75 2^15
+  static constexpr u32 kExponent = 15, kFraction = 0x600000u;
+  __device__ static __forceinline__ u32 pack(const float* v) {
+    const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(v[0], v[1], 0, false);
+    return (u32)__builtin_amdgcn_cvt_pk_bf8_f32(v[2], v[3], lo, true);
+  }
+};
+template <>
+struct Format<kInt8> {
+  static constexpr float kMost = 127.0f;             // (1 + 63/64) 2^6
+  static constexpr u32 kExponent = 6, kFraction = 0x7e0000u;
+  __device__ static __forceinline__ u32 pack(const float* v) {
+    u32 w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float r = __builtin_rintf(v[j]);         // (NaN becomes -127)
+      const int i = (int)__builtin_fminf(__builtin_fmaxf(r, -127.0f), 127.0f);
+      w |= ((u32)i & 0xffu) << (8 * j);
+    }
+    return w;
+  }
+};
+
+// The scale of a block whose largest magnitude has the bits `most` (a NaN's are above an infinity's).
+template <int FORMAT, bool POWER>
+__device__ __forceinline__ float block_scale(u32 most) {
+  typedef Format<FORMAT> F;
+  if (most >= 0x7f800000u) return as_f32(most);
+  if constexpr (POWER) {
+    // up to the next exponent where the fraction is above that of M
+    const int b = (int)((most + (0x7fffffu - F::kFraction)) & 0x7f800000u) - (int)(F::kExponent << 23);
+    return as_f32((u32)(b > 0x00800000 ? b : 0x00800000));
+  }
+  return __builtin_fmaxf(div_rn(as_f32(most), F::kMost), 0x1p-126f);
+}
+
+template <int G>
+__device__ __forceinline__ u32 group_most(u32 v) {
+  auto up = [](u32 a, u32 b) { return a > b ? a : b; };
+  if constexpr (G >= 2) v = up(v, partner_u32<1>(v));
+  if constexpr (G >= 4) v = up(v, partner_u32<2>(v));
+  if constexpr (G >= 8) v = up(v, partner_u32<4>(v));
+  if constexpr (G >= 16) v = up(v, partner_u32<8>(v));
+  if constexpr (G >= 32) v = up(v, partner_u32<16>(v));
+  if constexpr (G >= 64) v = up(v, partner_u32<32>(v));
+  return v;
+}
+// over the TPR lanes of a row; `lds` holds a word per wave
+template <int TPR>
+__device__ __forceinline__ u32 row_most(u32 v, u32* lds) {
+  v = group_most<(TPR < 64 ? TPR : 64)>(v);
+  if constexpr (TPR > 64) {
+    constexpr int WPR = TPR / 64;
+    const int wave = threadIdx.x >> 6, first = (wave / WPR) * WPR;
+    if (lane_id() == 0) lds[wave] = v;
+    __syncthreads();
+    v = group_most<WPR>(lds[first + lane_id() % WPR]);
+  }
+  return v;
+}
+
+// Columns (u TPR + t) VEC ... of the row `local` behind row0: VEC values in 8 bits.
+template <int FORMAT, int VEC, int ACCESS>
+__device__ __forceinline__ void store_8bit(unsigned char* p, i64 row0, int local, bool live, int e, int n,
+                                           const float* v) {
+  typedef u32 u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+  typedef u32 u32_any __attribute__((aligned(1)));
+  u32 w[VEC / 4];
+#pragma unroll
+  for (int j = 0; j < VEC / 4; ++j) w[j] = Format<FORMAT>::pack(v + 4 * j);
+  if constexpr (ACCESS == kWords) {
+    const u32 off = live && e < n ? (u32)(local * n + e) : kNowhere;
+    const __amdgpu_buffer_rsrc_t r = buffer_at(p + row0 * n);
+    if constexpr (VEC == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w[0], w[1]}, r, off, 0, 2);
+    else __builtin_amdgcn_raw_buffer_store_b32(w[0], r, off, 0, 2);
+  } else if (live) {
+    unsigned char* q = p + (row0 + local) * n + e;
+    if (e + VEC <= n) {
+      if constexpr (VEC == 8) *(u32x2_any*)q = u32x2{w[0], w[1]};
+      else *(u32_any*)q = w[0];
+    } else if (e < n) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (e + j < n) q[j] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+    }
+  }
+}
+
+// (FORMAT other than kSameType: `normed` is in that format, `scales` has a number per block)
+template <class St, int TPR, int NV, int ACCESS, bool AFTER, int GATE, int WG, int FORMAT = kSameType,
+          int GROUP = 0, bool POWER = false>
 __device__ __forceinline__ void residual_norm_forward(
     const typename St::T* __restrict__ x, const typename St::T* __restrict__ y,
     const typename St::T* __restrict__ gate, const typename St::T* __restrict__ after,
     const typename St::T* __restrict__ before, typename St::T* __restrict__ residual,
-    typename St::T* __restrict__ normed, float* __restrict__ stats, i64 rows, int n, i64 stride_x,
-    i64 stride_y, i64 group, float scale, float eps) {
+    void* __restrict__ normed, float* __restrict__ stats, i64 rows, int n, i64 stride_x,
+    i64 stride_y, i64 group, float scale, float eps, float* __restrict__ scales = nullptr) {
   typedef NormRow<St, TPR, NV, ACCESS> Row;
   constexpr int VEC = St::kVec;
   __shared__ float lds[2][WG / 64];
@@ -223,14 +333,58 @@ __device__ __forceinline__ void residual_norm_forward(
   }
   row_sums<TPR, 1>(&total, lds[1]);
   const float rate_r = frsq(__builtin_fmaf(total, mean, eps));
+  if constexpr (FORMAT == kSameType) {
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    float b[VEC], h[VEC];
-    St::unpack(bw[u], b);
+    for (int u = 0; u < NV; ++u) {
+      float b[VEC], h[VEC];
+      St::unpack(bw[u], b);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) h[j] = r[u][j] * rate_r * b[j];
-    Row::store(residual, row0, lane.local, live, u, n, t, r[u]);
-    Row::store(normed, row0, lane.local, live, u, n, t, h);
+      for (int j = 0; j < VEC; ++j) h[j] = r[u][j] * rate_r * b[j];
+      Row::store(residual, row0, lane.local, live, u, n, t, r[u]);
+      Row::store((typename St::T*)normed, row0, lane.local, live, u, n, t, h);
+    }
+  } else {
+    // the lanes of a block are neighbours: its columns are a power of two, and so many lanes hold a row or
+    // several blocks of one slot
+    constexpr int LANES = GROUP == 0 ? TPR : GROUP / VEC < TPR ? GROUP / VEC : TPR;
+    static_assert(GROUP == 0 || LANES <= 64, "a block is in one wavefront");
+    static_assert(GROUP == 0 || NV == 1 || TPR * VEC % GROUP == 0, "a slot holds whole blocks");
+    __shared__ u32 lds_most[WG / 64];
+    u32 most[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      float b[VEC];
+      St::unpack(bw[u], b);
+      Row::store(residual, row0, lane.local, live, u, n, t, r[u]);
+      most[u] = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        r[u][j] = r[u][j] * rate_r * b[j];
+        const u32 bits = as_u32(r[u][j]) & 0x7fffffffu;
+        most[u] = bits > most[u] ? bits : most[u];
+      }
+      if constexpr (GROUP > 0) most[u] = group_most<LANES>(most[u]);
+      else if (u > 0) most[0] = most[u] > most[0] ? most[u] : most[0];
+    }
+    if constexpr (GROUP == 0) most[0] = row_most<TPR>(most[0], lds_most);
+    const int blocks = GROUP == 0 ? 1 : (n + GROUP - 1) / GROUP;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int e = Row::at(u, t);
+      const float s = block_scale<FORMAT, POWER>(most[GROUP == 0 ? 0 : u]);
+      const float inverse = is_finite(s) ? div_rn(1.0f, s) : 0.0f;
+      float h[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        // the quotient, by one step from the product: without it twice as many values land on the other side of
+        // a rounding as with a division
+        h[j] = r[u][j] * inverse;
+        if constexpr (!POWER) h[j] = __builtin_fmaf(__builtin_fmaf(-h[j], s, r[u][j]), inverse, h[j]);
+      }
+      store_8bit<FORMAT, VEC, ACCESS>((unsigned char*)normed, row0, lane.local, live, e, n, h);
+      if (live && e < n && (GROUP == 0 ? u == 0 && t == 0 : t % LANES == 0))
+        scales[row * blocks + (GROUP == 0 ? 0 : e / GROUP)] = s;
+    }
   }
   if (stats != nullptr && t == 0 && live) {
     stats[2 * row] = rate_y;

@@ -21,7 +21,8 @@
 //
 // The training operators' direct entry points (neptune_codegen/calls.py) keep their calls here too:
 // CallPlan is one call layout's buffers and launches, CallTable finds it again by the layout of the
-// tensors and the numbers of a call.
+// tensors and the numbers of a call.  GradientCalls runs the operators that take a list of tensors
+// (neptune_codegen/gradients.py), whose launches hold the tensors' addresses by value.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
@@ -30,6 +31,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -453,6 +455,263 @@ class CallTable {
   std::unordered_map<Key, std::shared_ptr<CallPlan>, KeyHash> plans_;
 };
 
+// The norm of many tensors and their scaling (csrc/kernels/nep_gradients.h), on one device.
+class GradientCalls {
+ public:
+  // kernels' handles, tensors a launch takes, lanes of a workgroup, workgroups of a launch at most
+  GradientCalls(uint64_t sums, uint64_t norm, uint64_t scale, int tensors, int lanes, int workgroups)
+      : sums_(sums), norm_(norm), scale_(scale), tensors_(tensors), lanes_(lanes), workgroups_(workgroups) {
+    TORCH_CHECK(sums != 0 && norm != 0 && scale != 0 && tensors > 0 && lanes > 0 && workgroups > 0,
+                "GradientCalls: bad kernels");
+  }
+
+  // The tensors' norm (fp32, no dimensions), or None for a list that this does not take.
+  py::object norm(const py::handle& tensors) const {
+    std::vector<at::Tensor> in;
+    if (!collect(tensors, in)) return py::none();
+    const c10::Device device = in[0].device();
+    const c10::DeviceGuard guard(device);
+    hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
+    std::vector<Entry> entries;
+    for (const at::Tensor& t : in) add(entries, t, t);
+    const Pieces pieces = deal(entries);
+    at::Tensor out = at::empty({}, at::TensorOptions().device(device).dtype(at::kFloat));
+    launch_norm(entries, pieces, device, stream, static_cast<float*>(out.data_ptr()));
+    return py::cast(out);
+  }
+
+  // `out`: None (in place) or a list.  `given`: None or the norm.  The norm, or None for lists that this does
+  // not take.
+  py::object clip(const py::handle& tensors, const py::handle& out, const py::handle& given, float max_norm) const {
+    std::vector<at::Tensor> in, made;
+    if (!collect(tensors, in)) return py::none();
+    const bool in_place = out.is_none();
+    if (!in_place && (!collect(out, made) || made.size() != in.size())) return py::none();
+    const std::vector<at::Tensor>& to = in_place ? in : made;
+    const c10::Device device = in[0].device();
+    for (size_t i = 0; i < in.size(); ++i) {
+      const at::Tensor &a = in[i], &b = to[i];
+      if (b.requires_grad() || b.device() != device || !same_order(a, b) ||
+          (b.scalar_type() != a.scalar_type() && b.scalar_type() != at::kFloat))
+        return py::none();
+    }
+    if (!separate(in, to)) return py::none();
+    const float* known = nullptr;
+    at::Tensor norm;
+    if (!given.is_none()) {
+      if (!THPVariable_CheckExact(given.ptr())) return py::none();
+      norm = THPVariable_Unpack(given.ptr());
+      if (!plain(norm) || norm.device() != device || norm.scalar_type() != at::kFloat || norm.dim() != 0 ||
+          inside(norm, to))
+        return py::none();
+      known = static_cast<const float*>(norm.data_ptr());
+    }
+    const c10::DeviceGuard guard(device);
+    hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
+    std::vector<Entry> entries;
+    for (size_t i = 0; i < in.size(); ++i) add(entries, in[i], to[i]);
+    const Pieces pieces = deal(entries);
+    if (known == nullptr) norm = at::empty({}, at::TensorOptions().device(device).dtype(at::kFloat));
+    if (entries.empty()) {                           // nothing but its norm, 0
+      if (known == nullptr) launch_norm(entries, pieces, device, stream, static_cast<float*>(norm.data_ptr()));
+      return py::cast(norm);
+    }
+    at::Tensor sums;
+    if (known == nullptr) sums = launch_sums(entries, pieces, device, stream);
+    int copies = 0;
+    for (const Entry& e : entries) copies |= e.in != e.out;
+    // from the last list to the first, as the pieces of each
+    for (size_t i = pieces.launches.size(); i-- > 0;) {
+      const Part& part = pieces.launches[i];
+      Image image(entries, part, tensors_, pieces.piece);
+      image.put(known == nullptr ? sums.data_ptr() : nullptr);
+      image.put(static_cast<int32_t>(known == nullptr ? sums.numel() : 0));
+      image.align(8);
+      image.put(static_cast<const void*>(known));
+      image.put(known == nullptr && i + 1 == pieces.launches.size() ? norm.data_ptr() : nullptr);
+      image.put(max_norm);
+      image.put(static_cast<int32_t>(copies));
+      launch(scale_, grid(part), image, stream);
+    }
+    for (const at::Tensor& t : to)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return py::cast(norm);
+  }
+
+ private:
+  struct Entry {                                     // TensorEntry of nep_gradients.h
+    const void* in;
+    void* out;
+    uint64_t count;
+    uint32_t first, kind;
+  };
+  static_assert(sizeof(Entry) == 32, "the kernels' layout");
+  struct Part {
+    size_t begin, end;                               // entries of one launch
+    uint32_t pieces;
+  };
+  struct Pieces {
+    int32_t piece;
+    std::vector<Part> launches;
+  };
+
+  // A launch's arguments: its entries, their number, pieces and elements of a piece, then the rest.
+  struct Image {
+    Image(const std::vector<Entry>& entries, const Part& part, int tensors, int32_t piece) {
+      bytes.resize(tensors * sizeof(Entry));
+      if (part.end > part.begin)
+        std::memcpy(bytes.data(), &entries[part.begin], (part.end - part.begin) * sizeof(Entry));
+      put(static_cast<int32_t>(part.end - part.begin));
+      put(part.pieces);
+      put(piece);
+      align(8);
+    }
+    template <class T>
+    void put(T value) {
+      const size_t at = bytes.size();
+      bytes.resize(at + sizeof(T));
+      std::memcpy(bytes.data() + at, &value, sizeof(T));
+    }
+    void align(size_t n) { bytes.resize((bytes.size() + n - 1) / n * n); }
+    std::vector<uint8_t> bytes;
+  };
+
+  static bool plain(const at::Tensor& t) {
+    return t.defined() && t.device().is_cuda() && t.layout() == c10::kStrided && !t.is_neg() && !t.is_conj() &&
+           !t.key_set().has(c10::DispatchKey::Python);
+  }
+
+  // The tensors of a list or tuple that is not empty: of the three types, on one device, without gaps.
+  static bool collect(const py::handle& list, std::vector<at::Tensor>& out) {
+    if (!PyList_CheckExact(list.ptr()) && !PyTuple_CheckExact(list.ptr())) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+    if (n == 0) return false;
+    out.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PySequence_Fast_GET_ITEM(list.ptr(), i);
+      if (!THPVariable_CheckExact(o)) return false;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!plain(t) || (!out.empty() && t.device() != out[0].device()) || !t.is_non_overlapping_and_dense())
+        return false;
+      if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf)
+        return false;
+      out.push_back(t);
+    }
+    return true;
+  }
+
+  // Whether the elements of two tensors without gaps lie in one order.
+  static bool same_order(const at::Tensor& a, const at::Tensor& b) {
+    if (a.sizes() != b.sizes()) return false;
+    for (int64_t d = 0; d < a.dim(); ++d)
+      if (a.size(d) != 1 && a.numel() != 0 && a.stride(d) != b.stride(d)) return false;
+    return true;
+  }
+
+  static void add(std::vector<Entry>& entries, const at::Tensor& in, const at::Tensor& out) {
+    if (in.numel() == 0) return;
+    const bool wider = in.scalar_type() != at::kFloat && out.scalar_type() == at::kFloat;
+    const uint32_t kind = in.scalar_type() == at::kFloat ? 0 : (in.scalar_type() == at::kBFloat16 ? 1 : 2) + 2 * wider;
+    entries.push_back({in.data_ptr(), out.data_ptr(), static_cast<uint64_t>(in.numel()), 0, kind});
+  }
+
+  // Whether what is written overlaps nothing else that is written or read, but for a tensor that is written
+  // where it is read.
+  static bool separate(const std::vector<at::Tensor>& in, const std::vector<at::Tensor>& out) {
+    struct Range {
+      uintptr_t begin, end;
+      bool written;
+    };
+    std::vector<Range> ranges;
+    auto range = [&](const at::Tensor& t, bool written) {
+      if (t.numel() == 0) return;
+      const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+      ranges.push_back({begin, begin + t.numel() * t.element_size(), written});
+    };
+    for (size_t i = 0; i < in.size(); ++i) {
+      range(out[i], true);
+      if (out[i].data_ptr() != in[i].data_ptr() || out[i].scalar_type() != in[i].scalar_type()) range(in[i], false);
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;                  // ends of the ranges so far
+    for (const Range& r : ranges) {
+      if (r.begin < (r.written ? any : written)) return false;
+      any = std::max(any, r.end);
+      if (r.written) written = std::max(written, r.end);
+    }
+    return true;
+  }
+
+  static bool inside(const at::Tensor& t, const std::vector<at::Tensor>& all) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    for (const at::Tensor& a : all) {
+      const auto begin = reinterpret_cast<uintptr_t>(a.data_ptr());
+      if (at + 4 > begin && at < begin + a.numel() * a.element_size()) return true;
+    }
+    return false;
+  }
+
+  // Elements of a piece, and the lists' pieces.  At least one load of each lane, four where the pieces are
+  // many for the workgroups.
+  Pieces deal(std::vector<Entry>& entries) const {
+    Pieces p;
+    uint64_t total = 0;
+    for (const Entry& e : entries) total += e.count;
+    p.piece = lanes_ * 8;
+    while (p.piece < lanes_ * 32 && total / p.piece >= 16ull * workgroups_) p.piece *= 2;
+    for (size_t begin = 0; begin < entries.size(); begin += tensors_) {
+      Part part{begin, std::min(entries.size(), begin + tensors_), 0};
+      uint64_t pieces = 0;
+      for (size_t i = part.begin; i < part.end; ++i) {
+        entries[i].first = static_cast<uint32_t>(pieces);
+        pieces += (entries[i].count + p.piece - 1) / p.piece;
+      }
+      TORCH_CHECK_NOT_IMPLEMENTED(pieces < (1ull << 31), "gradients of more than 2^31 pieces of ", p.piece, " elements");
+      part.pieces = static_cast<uint32_t>(pieces);
+      p.launches.push_back(part);
+    }
+    return p;
+  }
+
+  uint32_t grid(const Part& part) const { return std::min<uint32_t>(part.pieces, workgroups_); }
+
+  void launch(uint64_t kernel, uint32_t workgroups, const Image& image, hipStream_t stream) const {
+    const int rc = nep_launch_packed(kernel, workgroups, 1, 1, lanes_, 0, stream, image.bytes.data(), image.bytes.size());
+    if (rc != NEP_OK) throw_hip_error(std::string("launch: ") + nep_last_error());
+  }
+
+  // One sum for each workgroup of all launches.
+  at::Tensor launch_sums(const std::vector<Entry>& entries, const Pieces& pieces, c10::Device device,
+                         hipStream_t stream) const {
+    int64_t count = 0;
+    for (const Part& part : pieces.launches) count += grid(part);
+    at::Tensor sums = at::empty({count}, at::TensorOptions().device(device).dtype(at::kDouble));
+    double* at = static_cast<double*>(sums.data_ptr());
+    for (const Part& part : pieces.launches) {
+      Image image(entries, part, tensors_, pieces.piece);
+      image.put(at);
+      launch(sums_, grid(part), image, stream);
+      at += grid(part);
+    }
+    return sums;
+  }
+
+  void launch_norm(const std::vector<Entry>& entries, const Pieces& pieces, c10::Device device, hipStream_t stream,
+                   float* out) const {
+    const at::Tensor sums = launch_sums(entries, pieces, device, stream);
+    Image image({}, Part{0, 0, 0}, 0, 0);
+    image.bytes.clear();
+    image.put(sums.data_ptr());
+    image.put(static_cast<int32_t>(sums.numel()));
+    image.align(8);
+    image.put(out);
+    launch(norm_, 1, image, stream);
+  }
+
+  const uint64_t sums_, norm_, scale_;
+  const int tensors_, lanes_, workgroups_;
+};
+
 int64_t dtype_code(const at::Tensor& t) { return static_cast<int64_t>(t.scalar_type()); }
 
 bool installed(const std::string& qualname) {
@@ -475,6 +734,11 @@ PYBIND11_MODULE(_neptune_dispatch, m) {
       .def(py::init<int, const py::tuple&, std::vector<int>, bool, const py::tuple&>(), py::arg("n_inputs"),
            py::arg("buffers"), py::arg("returns"), py::arg("bare"), py::arg("launches"))
       .def("run", &CallPlan::run, py::arg("tensors"));
+  py::class_<GradientCalls>(m, "GradientCalls")
+      .def(py::init<uint64_t, uint64_t, uint64_t, int, int, int>(), py::arg("sums"), py::arg("norm"),
+           py::arg("scale"), py::arg("tensors"), py::arg("lanes"), py::arg("workgroups"))
+      .def("norm", &GradientCalls::norm, py::arg("tensors"))
+      .def("clip", &GradientCalls::clip, py::arg("tensors"), py::arg("out"), py::arg("given"), py::arg("max_norm"));
   py::class_<CallTable>(m, "CallTable")
       .def(py::init<>())
       .def("run", &CallTable::run, py::arg("tensors"), py::arg("numbers"))

@@ -21,11 +21,15 @@ from neptune_codegen.attention import (as_attention_op, attention_fold, exact_pa
 from neptune_codegen.attention_backward import as_attention_grad_op, run_attention_backward
 from neptune_codegen.autotune import best_config, machine_key, op_key, parameter_tag
 from neptune_codegen.distill import as_distill_op, run_distill, run_distill_backward
+from neptune_codegen.embedding import as_embedding_op, run_embedding, run_embedding_backward
 from neptune_codegen.emitters import (check_supported, derived_producer_expr, emit_fold_policy,
                                       emit_kernel_source, emit_rms_state_source,
                                       emit_segment_source, param_bindings)
-from neptune_codegen.residual_norm import (as_residual_norm_op, run_residual_norm,
-                                           run_residual_norm_backward)
+from neptune_codegen.gradients import (as_clip_gradients_op, as_gradient_norm_op, run_clip_gradients,
+                                       run_gradient_norm)
+from neptune_codegen.residual_norm import (as_residual_norm_op, as_residual_norm_quantized_op,
+                                           run_residual_norm, run_residual_norm_backward,
+                                           run_residual_norm_quantized)
 from neptune_codegen.rotary import as_rotary_op, rotary_frequencies, run_rotary, run_rotary_backward
 from neptune_codegen.skeleton import (NEGATIVE_CONTROLS, SKELETONS, STATE_REDUCTIONS,
                                       NumericalContract, Skeleton, StateField, StateReduction,
@@ -72,8 +76,11 @@ __all__ = [
     "run_attention", "attention_fold", "as_attention_op", "launch_attention", "exact_path_taken",
     "run_attention_backward", "as_attention_grad_op",
     "run_rotary", "run_rotary_backward", "rotary_frequencies", "as_rotary_op",
+    "run_embedding", "run_embedding_backward", "as_embedding_op",
+    "run_gradient_norm", "run_clip_gradients", "as_gradient_norm_op", "as_clip_gradients_op",
     "run_distill", "run_distill_backward", "as_distill_op",
     "run_residual_norm", "run_residual_norm_backward", "as_residual_norm_op",
+    "run_residual_norm_quantized", "as_residual_norm_quantized_op",
     "compile_readout", "run_readout", "run_log_softmax", "as_readout_op", "readout_op_handle",
     "best_config", "machine_key", "op_key", "parameter_tag", "prebuilt_programs",
     # internals the reference package also exports: the algebra's quotient-power marker and

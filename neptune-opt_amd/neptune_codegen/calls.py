@@ -169,6 +169,26 @@ def check_tensor(t, name: str, *, metadata: bool) -> None:
         raise ValueError(f"{name} is on {t.device}; execution requires a ROCm (cuda) device")
 
 
+def overlap(a, b) -> bool:
+    """Whether the memory between two tensors' first and last elements overlaps."""
+    def ends(t):
+        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        return t.data_ptr(), t.data_ptr() + span * t.element_size()
+
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
+def written(t) -> None:
+    """Tells autograd that a kernel has written `t` in place."""
+    import torch
+
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def check_grid(grid, threads: int, name: str) -> None:
     if grid[0] * threads > MOST_THREADS or any(n > 65535 for n in grid[1:]):
         raise NotImplementedError(f"{name}: the call needs a grid of {tuple(grid)} workgroups of {threads} "

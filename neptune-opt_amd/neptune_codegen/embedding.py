@@ -1,0 +1,313 @@
+"""Embedding lookup with a scale, and the table's gradient.
+
+There is no reference function for this path:
+
+    out[i] = scale * table[token i]          dtable[v] = scale * sum over i with token i = v of grad[i]
+
+Layout contract: tokens [...] in int32 or int64, a table [vocab, n] in float32, bfloat16 or float16, the
+output [..., n] in its dtype.  A negative token stands for none: a row of zeros, and no gradient.  A token of
+vocab or more has a row of NaN and no gradient; it is never read through.  The arithmetic is fp32 with one
+rounding; the gradient's rows are added in the order of their positions, without atomics.  Formulas and
+mapping are in csrc/kernels/nep_embedding.h.
+"""
+from __future__ import annotations
+
+import threading
+
+from neptune_codegen import calls, hip
+from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_sort_name, embedding_sums_name,
+                                      emit_embedding_sort_source, emit_embedding_source,
+                                      emit_embedding_sums_source)
+
+PER_LANE = 4             # tokens that a lane sorts
+MOST_DIGIT = 9           # bits that one pass of the sort takes
+_PROGRAMS: dict = {}
+_OPS: dict = {}
+_FORWARD, _BACKWARD = calls.Table(), calls.Table()
+_lock = threading.Lock()
+
+_LOOKUP_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,)
+_SORT_ARGS = (hip.PTR,) * 4 + (hip.I64,) * 4 + (hip.I32,) * 3
+_MERGE_ARGS = (hip.PTR,) * 4 + (hip.I64, hip.I32)
+_SUMS_ARGS = (hip.PTR,) * 5 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.I32, hip.F32)
+_JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 2 + (hip.I32,) * 2 + (hip.I64, hip.F32)
+
+
+def _program(name: str, emit, *args) -> hip.Program:
+    with _lock:
+        prog = _PROGRAMS.get(name)
+        if prog is None:
+            prog = _PROGRAMS[name] = hip.Program(emit(*args), f"{name}.hip", BASE_OPTIONS)
+        return prog
+
+
+def _lookup_program(var: EmbeddingVariant) -> hip.Program:
+    return _program(var.name, emit_embedding_source, var)
+
+
+def _sort_program(index: str, threads: int) -> hip.Program:
+    return _program(embedding_sort_name("sort", index, threads), emit_embedding_sort_source, index, threads)
+
+
+def _sums_program(dtype, out, access: str, add: bool) -> hip.Program:
+    return _program(embedding_sums_name("sums", dtype, out, access, add), emit_embedding_sums_source, dtype, out,
+                    access, add)
+
+
+def _scale(scale) -> float:
+    if type(scale) not in (int, float) or not abs(scale) <= calls.MOST_FLOAT:
+        raise ValueError("embedding needs a scale that is finite in fp32")
+    return float(scale)
+
+
+def _check_rows(t, name: str, *, metadata: bool) -> None:
+    import torch
+
+    calls.check_tensor(t, f"embedding {name}", metadata=metadata)
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"embedding takes float32, bfloat16 and float16, got {t.dtype} for {name}")
+
+
+def _check_tokens(tokens, device, *, metadata: bool) -> None:
+    import torch
+
+    calls.check_tensor(tokens, "embedding tokens", metadata=metadata)
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding tokens must be int32 or int64, got {tokens.dtype}")
+    if tokens.device != device:
+        raise ValueError("embedding tensors must be on the same device")
+
+
+def _check_sizes(tokens, vocab: int, n: int) -> None:
+    if tokens.numel() >= 1 << 31 or vocab >= 1 << 31 or n >= 1 << 28:
+        raise NotImplementedError("embedding takes less than 2^31 tokens and rows, and rows of less than 2^28")
+
+
+def validate_embedding_inputs(tokens, table, *, metadata: bool = False) -> None:
+    _check_rows(table, "table", metadata=metadata)
+    if table.ndim != 2 or not table.numel():
+        raise ValueError(f"embedding table must be [vocab, n] with both at least 1, got {tuple(table.shape)}")
+    _check_tokens(tokens, table.device, metadata=metadata)
+    _check_sizes(tokens, *table.shape)
+
+
+def validate_embedding_gradient_inputs(grad, tokens, vocab, into=None, *, metadata: bool = False) -> None:
+    import torch
+
+    _check_rows(grad, "grad", metadata=metadata)
+    _check_tokens(tokens, grad.device, metadata=metadata)
+    if type(vocab) is not int or vocab < 1:
+        raise ValueError("embedding needs a vocab of at least 1")
+    if not grad.ndim or grad.shape[:-1] != tokens.shape or not grad.shape[-1]:
+        raise ValueError(f"embedding grad {tuple(grad.shape)} must be [..., n] with tokens of the leading sizes, "
+                         f"got {tuple(tokens.shape)}")
+    n = grad.shape[-1]
+    _check_sizes(tokens, vocab, n)
+    if into is None:
+        return
+    calls.check_tensor(into, "embedding into", metadata=metadata)
+    if into.shape != (vocab, n) or into.device != grad.device:
+        raise ValueError(f"embedding into must be [{vocab}, {n}] on the gradient's device, got {tuple(into.shape)}")
+    if into.dtype not in (grad.dtype, torch.float32):
+        raise TypeError(f"embedding into must be float32 or {grad.dtype}, got {into.dtype}")
+    if into.requires_grad:
+        raise ValueError("embedding into is written in place and must not require grad")
+    if (n > 1 and into.stride(1) != 1) or (vocab > 1 and into.stride(0) < n):
+        raise ValueError("embedding into must have unit column stride and rows that do not overlap")
+
+
+def _apart(grad, into) -> bool:
+    import torch
+
+    return not isinstance(grad, torch.Tensor) or calls.is_metadata(grad) or calls.is_metadata(into) or \
+        not calls.overlap(grad, into)
+
+
+def _access(n: int, *tensors) -> str:
+    """`tensors`: (tensor, row stride)."""
+    vec = 16 // tensors[0][0].element_size()
+    if n < vec:
+        return "few"
+    return "words" if n % vec == 0 and all(t.data_ptr() % 16 == 0 and s % (16 // t.element_size()) == 0
+                                           for t, s in tensors) else "any"
+
+
+def _name(t) -> str:
+    return str(t.dtype).replace("torch.", "")
+
+
+def _flat(tokens):
+    """Tokens whose elements have one stride, and that stride."""
+    used, stride = calls.rows_of(tokens.unsqueeze(-1))
+    return (tokens if used.data_ptr() == tokens.data_ptr() else used), stride
+
+
+def _lookup_variant(table, tokens, access: str, n: int) -> EmbeddingVariant:
+    slots = -(-n // (16 // table.element_size()))
+    tpr = min(256, 1 << max(0, (slots - 1).bit_length()))
+    return EmbeddingVariant(_name(table), _name(tokens), access, tpr, 2 if slots >= 512 else 1)
+
+
+def run_embedding(tokens, table, *, scale: float = 1.0):
+    """Rows [..., n] of the table for tokens [...], times `scale`, in the table's dtype, on the current
+    stream.  A call whose tensor layouts and scale were seen before reuses that call's kernel and launch
+    shape."""
+    import torch
+
+    given = (tokens, table)
+    found = _FORWARD.run(given, (scale,))
+    if found is not None:
+        return found
+    metadata = isinstance(table, torch.Tensor) and calls.is_metadata(table)
+    validate_embedding_inputs(*given, metadata=metadata)
+    number, scale = scale, _scale(scale)
+    (vocab, n), rows = table.shape, tokens.numel()
+    shape = (*tokens.shape, n)
+    if metadata or rows == 0:
+        return torch.empty(shape, dtype=table.dtype, device=table.device)
+    (flat, si), (used, st) = _flat(tokens), calls.rows_of(table)
+    var = _lookup_variant(table, tokens, _access(n, (used, st)), n)
+    slots = -(-n // (16 // table.element_size()))
+    device = calls.device_index(table)
+    kernel = _lookup_program(var).kernel(var.name, _LOOKUP_ARGS, 256, device)
+    launch = (kernel, (-(-rows // (256 // var.tpr)), min(65535, -(-slots // (var.tpr * var.unroll)))),
+              (calls.tensor(0), calls.tensor(1), calls.buffer(0), rows, n, vocab, si, st, scale))
+    plan = calls.Plan(device, 2, [(shape, table.dtype)], (0,), [launch], bare=True)
+    if calls.same(given, (flat, used)):
+        _FORWARD.keep(given, (number,), plan)
+    return plan.run((flat, used))
+
+
+def _digits(vocab: int) -> tuple[int, int]:
+    """(bits of a digit, digits) of a sort of keys from 0 to vocab."""
+    bits = vocab.bit_length()
+    passes = -(-bits // MOST_DIGIT)
+    return -(-bits // passes), passes
+
+
+def _chunk(count: int, words: int) -> int:
+    """Sorted entries that a wavefront adds."""
+    chunk = 16
+    while chunk < 256 and -(-count // (2 * chunk)) * -(-words // 64) >= 4096:
+        chunk *= 2
+    return chunk
+
+
+def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into=None):
+    """Gradient [vocab, n] of the table for the output's gradient `grad` [..., n], in its dtype; or, with
+    `into` [vocab, n] in that dtype or float32, the gradient added to `into` in place (one rounding for each
+    row that a token names, the others untouched), and `into`."""
+    import torch
+
+    given, add = (grad, tokens, into), into is not None
+    # (what the layout of the tensors does not say; refused below)
+    apart = not add or (isinstance(into, torch.Tensor) and not into.requires_grad and _apart(grad, into))
+    found = _BACKWARD.run(given, (vocab, scale)) if apart else None
+    if found is not None:
+        if not add:
+            return found[0]
+        calls.written(into)
+        return into
+    metadata = isinstance(grad, torch.Tensor) and calls.is_metadata(grad)
+    validate_embedding_gradient_inputs(grad, tokens, vocab, into, metadata=metadata)
+    if not metadata and not apart:
+        raise ValueError("embedding into must not overlap the gradient that is added to it")
+    number, scale = scale, _scale(scale)
+    n, count = grad.shape[-1], tokens.numel()
+    if metadata or count == 0:
+        return torch.zeros((vocab, n), dtype=grad.dtype, device=grad.device) if into is None else into
+    (g, sg), (flat, si) = calls.rows_of(grad), _flat(tokens)
+    used, device = (g, flat, into), calls.device_index(grad)
+    st = n if into is None else into.stride(0) if vocab > 1 else n
+    out = grad.dtype if into is None else into.dtype
+    words = -(-n // (16 // grad.element_size()))
+    access = _access(n, (g, sg), *([(into, st)] if add else []))
+    threads = 1024 if count > 256 * PER_LANE else 256
+    piece = threads * PER_LANE
+    pieces = -(-count // piece)
+    width, passes = _digits(vocab)
+    chunk = _chunk(count, words)
+    chunks, columns = -(-count // chunk), -(-words // 256)
+    lanes = 256 * columns
+    # result; keys and positions, in pieces and merged; parts of runs over several chunks
+    buffers = [] if add else [((vocab, n), out)]
+    keys, positions = calls.buffer(len(buffers)), calls.buffer(len(buffers) + 1)
+    buffers += [((pieces * piece,), torch.int32)] * 2
+    table = calls.tensor(2) if add else calls.buffer(0)
+    size = 0 if add else vocab * n * grad.element_size()
+    clear = min(2048, -(-size // (threads * 64)))
+    prog = _sort_program(_name(tokens), threads)
+    launches = [(prog.kernel(embedding_sort_name("sort", _name(tokens), threads), _SORT_ARGS, threads, device),
+                 (pieces + clear,), (calls.tensor(1), keys, positions, table, count, vocab, si, size, width, passes,
+                                     pieces))]
+    if pieces > 1:
+        merged = calls.buffer(len(buffers)), calls.buffer(len(buffers) + 1)
+        buffers += [((count,), torch.int32)] * 2
+        launches.append((prog.kernel(embedding_sort_name("merge", _name(tokens), threads), _MERGE_ARGS, 256, device),
+                         (pieces * threads // 256,), (keys, positions, *merged, count, pieces)))
+        keys, positions = merged
+    parts = calls.buffer(len(buffers))
+    buffers.append(((chunks * 2 * lanes * (16 // grad.element_size()),), torch.float32))
+    prog = _sums_program(_name(grad), str(out), access, add)
+    tag = (_name(grad), str(out), access, add)
+    launches.append((prog.kernel(embedding_sums_name("sums", *tag), _SUMS_ARGS, 256, device), (chunks, columns),
+                     (calls.tensor(0), keys, positions, table, parts, count, n, vocab, sg, st, chunk, scale)))
+    if chunks > 1:
+        launches.append((prog.kernel(embedding_sums_name("join", *tag), _JOIN_ARGS, 512, device),
+                         (chunks, -(-words // 64)),
+                         (keys, parts, table, count, n, vocab, st, chunk, chunks, lanes, scale)))
+    plan = calls.Plan(device, 3, buffers, () if add else (0,), launches)
+    if calls.same(given, used):
+        _BACKWARD.keep(given, (vocab, number), plan)
+    made = plan.run(used)
+    if add:
+        calls.written(into)
+        return into
+    return made[0]
+
+
+def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
+    """Differentiable custom op `(Tensor tokens, Tensor table) -> Tensor` with the scale in its name; the
+    gradient is the table's."""
+    import torch
+
+    from neptune_codegen.autotune import parameter_tag
+
+    scale = _scale(scale)
+    key = (lib, scale)
+    with _lock:
+        if key in _OPS:
+            return _OPS[key]
+    name = f"embedding{parameter_tag({'scale': scale})}"
+
+    def _forward(tokens, table):
+        return run_embedding(tokens, table, scale=scale)
+
+    def _forward_fake(tokens, table):
+        validate_embedding_inputs(tokens, table, metadata=True)
+        return torch.empty((*tokens.shape, table.shape[1]), dtype=table.dtype, device=table.device)
+
+    def _backward(grad, tokens, vocab):
+        return run_embedding_backward(grad, tokens, vocab, scale=scale)
+
+    def _backward_fake(grad, tokens, vocab):
+        return torch.empty((vocab, grad.shape[-1]), dtype=grad.dtype, device=grad.device)
+
+    define = torch.library.custom_op
+    op = define(f"{lib}::{name}", mutates_args=(), schema="(Tensor tokens, Tensor table) -> Tensor")(_forward)
+    op.register_fake(_forward_fake)
+    back = define(f"{lib}::{name}_backward", mutates_args=(),
+                  schema="(Tensor grad, Tensor tokens, SymInt vocab) -> Tensor")(_backward)
+    back.register_fake(_backward_fake)
+
+    def _setup(ctx, inputs, output):
+        ctx.save_for_backward(inputs[0])
+        ctx.vocab = inputs[1].shape[0]
+
+    def _grad(ctx, grad):
+        return None, back(grad, ctx.saved_tensors[0], ctx.vocab)
+
+    op.register_autograd(_grad, setup_context=_setup)
+    with _lock:
+        _OPS[key] = op
+    return op

@@ -846,10 +846,14 @@ class ResidualNormVariant:
     wg: int             # lanes per workgroup
     after: bool         # a norm behind the block
     gate: str           # "none", "rows" (one per row) or "group" (one per group of rows)
+    out: str = ""       # the 8-bit type of "quantized"
+    block: int = 0      # columns that share a scale, 0 for a row
+    power_of_two: bool = False
 
     def tag(self) -> str:
         return (f"{dtype_tag(self.dtype)[0]}_{self.access}{self.tpr}n{self.nv}w{self.wg}"
-                f"{'_after' if self.after else ''}{'' if self.gate == 'none' else '_' + self.gate}")
+                f"{'_after' if self.after else ''}{'' if self.gate == 'none' else '_' + self.gate}"
+                + (f"_{self.out}_{self.block}{'p' if self.power_of_two else ''}" if self.out else ""))
 
 
 def residual_norm_kernel_name(stage: str, var: ResidualNormVariant) -> str:
@@ -859,8 +863,8 @@ def residual_norm_kernel_name(stage: str, var: ResidualNormVariant) -> str:
 
 
 def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
-    """hiprtc unit of the residual norm ("forward") or its gradients with their join ("backward"),
-    nep_residual_norm.h."""
+    """hiprtc unit of the residual norm ("forward"), with an 8-bit output ("quantized") or its gradients with
+    their join ("backward"), nep_residual_norm.h."""
     st = dtype_tag(var.dtype)[1]
     gate = {"none": "nep::kGateNone", "rows": "nep::kGateRows", "group": "nep::kGateGroup"}[var.gate]
     access = {"words": "nep::kWords", "any": "nep::kAnyRows", "few": "nep::kFewColumns"}[var.access]
@@ -877,6 +881,14 @@ def emit_residual_norm_source(stage: str, var: ResidualNormVariant) -> str:
                 f"  nep::residual_norm_forward<{st}, {var.tpr}, {var.nv}, {flags}>({c}x, {c}y, {c}gate, "
                 f"{c}after, {c}before, {m}residual, {m}normed, stats, rows, n, stride_x, stride_y, group, "
                 "scale, eps);\n}\n")
+    if stage == "quantized":
+        fmt = {"float8_e4m3fn": "nep::kE4M3", "float8_e5m2": "nep::kE5M2", "int8": "nep::kInt8"}[var.out]
+        return (f"{head}\n{bound}(const void* x, const void* y, const void* gate, const void* after, "
+                "const void* before, void* residual, void* normed, float* stats, long long rows, int n, "
+                "long long stride_x, long long stride_y, long long group, float scale, float eps, float* scales) {\n"
+                f"  nep::residual_norm_forward<{st}, {var.tpr}, {var.nv}, {flags}, {fmt}, {var.block}, "
+                f"{str(var.power_of_two).lower()}>({c}x, {c}y, {c}gate, {c}after, {c}before, {m}residual, normed, "
+                "stats, rows, n, stride_x, stride_y, group, scale, eps, scales);\n}\n")
     return (f"{head}\n{bound}(const void* dres, const void* dnormed, const void* x, const void* y, "
             "const void* gate, const void* after, const void* before, const float* stats, void* dx, void* dy, "
             "void* dgate, void* dafter, void* dbefore, float* sums, long long rows, int n, "
@@ -917,3 +929,99 @@ def emit_rotary_source(dtype, index: str, layout: str, any_rows: bool) -> str:
             f"(const {px}*)positions, turns, {m}qo, {m}ko, (nep::u32)tokens, (nep::u32)seq, dim, part, "
             "(nep::u32)slots, (nep::u32)turned, heads_q, heads_k, per, qsb, qsh, qss, ksb, ksh, kss, psb, pss, "
             "sign, magnitude);\n}\n")
+
+
+# ---------------------------------------------------------------- embedding
+EMBEDDING_ACCESS = {"words": "nep::kRowWords", "any": "nep::kRowAny", "few": "nep::kRowFew"}
+_INDEX_TYPES = {"int32": "int", "int64": "long long"}
+
+
+@dataclasses.dataclass(frozen=True)
+class EmbeddingVariant:
+    """One launch shape of the embedding lookup."""
+
+    dtype: str
+    index: str          # the tokens' dtype
+    access: str         # rows of whole 16-byte "words", of "any" alignment and width, of "few" columns
+    tpr: int            # lanes per row
+    unroll: int         # 16-byte words of a lane in flight
+
+    @property
+    def name(self) -> str:
+        return (f"embedding_{dtype_tag(self.dtype)[0]}_{self.index[0]}{self.index[3:]}_{self.access}"
+                f"{self.tpr}u{self.unroll}")
+
+
+def emit_embedding_source(var: EmbeddingVariant) -> str:
+    """hiprtc unit of the embedding lookup, nep_embedding.h."""
+    st, ix = dtype_tag(var.dtype)[1], _INDEX_TYPES[var.index]
+    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding lookup\n"
+            + kernel_header("nep_device.h", "nep_embedding.h")
+            + f'\nextern "C" __global__ void __launch_bounds__(256) {var.name}(const void* tokens, '
+            "const void* table, void* out, long long rows, int n, long long vocab, long long stride_i, "
+            "long long stride_t, float scale) {\n"
+            f"  nep::embedding<{st}, {ix}, {var.tpr}, {var.unroll}, {EMBEDDING_ACCESS[var.access]}>("
+            f"(const {ix}*)tokens, (const {st}::T*)table, ({st}::T*)out, rows, n, vocab, stride_i, stride_t, "
+            "scale);\n}\n")
+
+
+def embedding_sort_name(stage: str, index: str, threads: int) -> str:
+    return f"embedding_{stage}_{index[0]}{index[3:]}_{threads}"
+
+
+def emit_embedding_sort_source(index: str, threads: int) -> str:
+    """hiprtc unit of the tokens' sort in pieces ("sort") and of the pieces' merge ("merge"), nep_embedding.h."""
+    ix = _INDEX_TYPES[index]
+    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: tokens in order\n"
+            + kernel_header("nep_device.h", "nep_embedding.h")
+            + f'\nextern "C" __global__ void __launch_bounds__({threads}) '
+            f"{embedding_sort_name('sort', index, threads)}(const void* tokens, unsigned* keys, "
+            "unsigned* positions, void* table, long long count, long long vocab, long long stride_i, "
+            "long long bytes, int width, int passes, int pieces) {\n"
+            f"  nep::embedding_sort<{ix}, {threads}>((const {ix}*)tokens, keys, positions, (char*)table, count, "
+            "vocab, stride_i, bytes, width, passes, pieces);\n}\n"
+            'extern "C" __global__ void __launch_bounds__(256) '
+            f"{embedding_sort_name('merge', index, threads)}(const unsigned* keys, const unsigned* positions, "
+            "unsigned* keys_out, unsigned* positions_out, long long count, int pieces) {\n"
+            f"  nep::embedding_merge<{threads} * nep::kPerLane>(keys, positions, keys_out, positions_out, count, "
+            "pieces);\n}\n")
+
+
+def embedding_sums_name(stage: str, dtype, out, access: str, add: bool) -> str:
+    return f"embedding_{stage}_{dtype_tag(dtype)[0]}_{dtype_tag(out)[0]}_{access}{'_add' if add else ''}"
+
+
+def emit_embedding_sums_source(dtype, out, access: str, add: bool) -> str:
+    """hiprtc unit of the sums of sorted rows ("sums") and of long runs' parts ("join"), nep_embedding.h."""
+    st, ot = dtype_tag(dtype)[1], dtype_tag(out)[1]
+    targs = f"{st}, {ot}, {EMBEDDING_ACCESS[access]}, {str(add).lower()}"
+    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: rows' sums\n"
+            + kernel_header("nep_device.h", "nep_embedding.h")
+            + '\nextern "C" __global__ void __launch_bounds__(256) '
+            f"{embedding_sums_name('sums', dtype, out, access, add)}(const void* grad, const unsigned* keys, "
+            "const unsigned* positions, void* table, float* parts, long long count, int n, long long vocab, "
+            "long long stride_g, long long stride_t, int chunk, float scale) {\n"
+            f"  nep::embedding_sums<{targs}>((const {st}::T*)grad, keys, positions, ({ot}::T*)table, parts, count, "
+            "n, (nep::u32)vocab, stride_g, stride_t, chunk, scale);\n}\n"
+            'extern "C" __global__ void __launch_bounds__(512) '
+            f"{embedding_sums_name('join', dtype, out, access, add)}(const unsigned* keys, const float* parts, "
+            "void* table, long long count, int n, long long vocab, long long stride_t, int chunk, int chunks, "
+            "long long lanes, float scale) {\n"
+            f"  nep::embedding_join<{targs}, 8>(keys, parts, ({ot}::T*)table, count, n, (nep::u32)vocab, stride_t, "
+            "chunk, chunks, lanes, scale);\n}\n")
+
+
+# ---------------------------------------------------------------- gradients of a whole model
+def emit_gradients_source() -> str:
+    """hiprtc unit of the gradients' sums of squares, norm and scaling, nep_gradients.h."""
+    bound = 'extern "C" __global__ void __launch_bounds__(1024)'
+    listed = "nep::TensorList list, int count, unsigned pieces, int piece"
+    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// gradients' norm and scaling\n"
+            + kernel_header("nep_device.h", "nep_gradients.h")
+            + f"\n{bound} gradient_sums({listed}, double* sums) {{\n"
+            "  nep::gradient_sums(list, count, pieces, piece, sums);\n}\n"
+            f"{bound} gradient_norm(const double* sums, int count, float* norm) {{\n"
+            "  nep::gradient_norm(sums, count, norm);\n}\n"
+            f"{bound} gradient_scale({listed}, const double* sums, int n_sums, const float* given, "
+            "float* norm, float max_norm, int copies) {\n"
+            "  nep::gradient_scale(list, count, pieces, piece, sums, n_sums, given, norm, max_norm, copies);\n}\n")

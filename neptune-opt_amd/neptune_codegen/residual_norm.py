@@ -7,7 +7,8 @@ There is no reference function for this path; it is run_rms_norm twice around th
     normed   = norm(residual; gamma_before)                         (the next block's input)
 
 with norm(v; gamma) = v * rsqrt(mean(v^2) + eps) * gamma over the last dimension.  gamma_after may be
-None (y is added as it is), and so may the gate.  Formulas and mapping are in
+None (y is added as it is), and so may the gate.  run_residual_norm_quantized returns normed in 8 bits
+with scales, for an 8-bit matrix product.  Formulas and mapping are in
 csrc/kernels/nep_residual_norm.h.
 
 Layout contract: x and y [..., n] of one shape and dtype (float32, bfloat16, float16), n up to 16384;
@@ -18,6 +19,7 @@ Column sums (gradients of the gammas and of a broadcast gate) are added in one o
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 import threading
 
@@ -31,10 +33,11 @@ MAX_STRIDE = 1 << 22
 CUS = 256
 _PROGRAMS: dict = {}
 _OPS: dict = {}
-_FORWARD, _BACKWARD = calls.Table(), calls.Table()
+_FORWARD, _QUANTIZED, _BACKWARD = calls.Table(), calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _FORWARD_ARGS = (hip.PTR,) * 8 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,) * 2
+_QUANTIZED_ARGS = _FORWARD_ARGS + (hip.PTR,)
 _BACKWARD_ARGS = (hip.PTR,) * 14 + (hip.I64, hip.I32) + (hip.I64,) * 6 + (hip.F32,)
 _JOIN_ARGS = (hip.PTR,) * 4 + (hip.I32,) + (hip.I64,) * 2
 
@@ -184,6 +187,115 @@ def run_residual_norm(x, y, gamma_after, gamma_before, *, gate=None, residual_sc
     if calls.same(given, used):
         _FORWARD.keep(given, numbers, plan)
     return plan.run(used)
+
+
+# columns that share a scale, and the number that stands for an 8-bit type in a call's key
+BLOCKS = (32, 64, 128)
+_FORMATS = ("float8_e4m3fn", "float8_e5m2", "int8")
+
+
+def _format(dtype) -> str:
+    name = str(dtype).replace("torch.", "")
+    if name not in _FORMATS:
+        raise TypeError(f"residual norm's 8-bit outputs are {', '.join(_FORMATS)}, got {dtype}")
+    return name
+
+
+def _block(group) -> int:
+    if group is not None and (type(group) is not int or group not in BLOCKS):
+        raise ValueError(f"residual norm's scales are one per row (None) or per {BLOCKS} columns, got {group!r}")
+    return group or 0
+
+
+def _quantized_outputs(x, dtype, block: int, return_stats: bool):
+    import torch
+
+    blocks = -(-x.shape[-1] // block) if block else 1
+    return [(x.shape, x.dtype), (x.shape, dtype), ((*x.shape[:-1], blocks), torch.float32)] + (
+        [((*x.shape[:-1], 2), torch.float32)] if return_stats else [])
+
+
+def run_residual_norm_quantized(x, y, gamma_after, gamma_before, *, gate=None, residual_scale: float = 1.0,
+                                eps: float = 1e-6, dtype=None, group: int | None = None,
+                                power_of_two: bool = False, return_stats: bool = False):
+    """(residual, values, scales) on the current stream: run_residual_norm with the second result in 8 bits,
+    for an 8-bit matrix product, normed ~ values * scales, and with `return_stats` the rates as a fourth.
+
+    `dtype` is torch.float8_e4m3fn (the default), float8_e5m2 or int8; `scales` [..., 1] in fp32 has one number
+    per row, or [..., ceil(n / group)] one per `group` (32, 64 or 128) columns: the largest magnitude over the
+    type's largest value, or with `power_of_two` the least power of two that is no less, at least 2^-126 (0
+    stays 0); values are rounded half to even.  Where a row or group holds an infinity or NaN, its scale is not
+    finite.  The gradient is straight through: run_residual_norm_backward, with the rates."""
+    import torch
+
+    given, return_stats, power_of_two = (x, y, gamma_after, gamma_before, gate), bool(return_stats), bool(power_of_two)
+    dtype = torch.float8_e4m3fn if dtype is None else dtype
+    out, block = _format(dtype), _block(group)
+    numbers = (residual_scale, eps, return_stats, _FORMATS.index(out), block, power_of_two)
+    found = _QUANTIZED.run(given, numbers)
+    if found is not None:
+        return found
+    metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
+    groups, group_rows = validate_residual_norm_inputs(*given, metadata=metadata)
+    scale, eps = _scale(residual_scale), _eps(eps)
+    outputs = _quantized_outputs(x, dtype, block, return_stats)
+    if metadata or x.numel() == 0:
+        return tuple(torch.empty(shape, dtype=kind, device=x.device) for shape, kind in outputs)
+    n = x.shape[-1]
+    rows = x.numel() // n
+    used, strides, aligned = _operands((x, y), (gamma_after, gamma_before, gate), n)
+    var = _variant(x, aligned, rows, n, gamma_after is not None, _gate_kind(groups, group_rows), False)
+    var = dataclasses.replace(var, out=out, block=block, power_of_two=power_of_two)
+    device = calls.device_index(x)
+    kernel = _program("quantized", var).kernel(residual_norm_kernel_name("quantized", var), _QUANTIZED_ARGS, var.wg,
+                                               device)
+    tx, ty, after, before, tgate = map(calls.tensor, range(5))
+    launch = (kernel, (-(-rows // (var.wg // var.tpr)),),
+              (tx, ty, tgate, after, before, calls.buffer(0), calls.buffer(1),
+               calls.buffer(3) if return_stats else 0, rows, n) + strides
+              + (max(group_rows, 1), scale, eps, calls.buffer(2)))
+    plan = calls.Plan(device, 5, outputs, range(len(outputs)), [launch])
+    if calls.same(given, used):
+        _QUANTIZED.keep(given, numbers, plan)
+    return plan.run(used)
+
+
+def as_residual_norm_quantized_op(residual_scale: float = 1.0, eps: float = 1e-6, dtype=None,
+                                  group: int | None = None, power_of_two: bool = False, lib: str = "neptune"):
+    """Custom op `(Tensor x, Tensor y, Tensor? gamma_after, Tensor gamma_before, Tensor? gate) -> (Tensor
+    residual, Tensor values, Tensor scales, Tensor stats)` with the numbers in its name.  Its 8-bit results have
+    no gradient in torch: a differentiable product calls run_residual_norm_backward with the stats."""
+    import torch
+
+    from neptune_codegen.autotune import parameter_tag
+
+    scale, eps, block, power_of_two = _scale(residual_scale), _eps(eps), _block(group), bool(power_of_two)
+    dtype = torch.float8_e4m3fn if dtype is None else dtype
+    out = _format(dtype)
+    key = (lib, scale, eps, out, block, power_of_two)
+    with _lock:
+        if key in _OPS:
+            return _OPS[key]
+    name = (f"residual_norm_{out}_{f'blocks{block}' if block else 'rows'}{'_powers' if power_of_two else ''}"
+            f"{parameter_tag({'scale': scale, 'eps': eps})}")
+
+    def _forward(x, y, gamma_after, gamma_before, gate):
+        return run_residual_norm_quantized(x, y, gamma_after, gamma_before, gate=gate, residual_scale=scale, eps=eps,
+                                           dtype=dtype, group=group, power_of_two=power_of_two, return_stats=True)
+
+    def _forward_fake(x, y, gamma_after, gamma_before, gate):
+        validate_residual_norm_inputs(x, y, gamma_after, gamma_before, gate, metadata=True)
+        return tuple(torch.empty(shape, dtype=kind, device=x.device)
+                     for shape, kind in _quantized_outputs(x, dtype, block, True))
+
+    op = torch.library.custom_op(
+        f"{lib}::{name}", mutates_args=(),
+        schema="(Tensor x, Tensor y, Tensor? gamma_after, Tensor gamma_before, Tensor? gate) "
+               "-> (Tensor, Tensor, Tensor, Tensor)")(_forward)
+    op.register_fake(_forward_fake)
+    with _lock:
+        _OPS[key] = op
+    return op
 
 
 def _chunks(rows, groups, group, gate_kind, rpw):

@@ -1,0 +1,76 @@
+"""The embedding without a GPU: refusals, metadata calls, and launches that cover tokens and columns."""
+import math
+
+import pytest
+import torch
+
+import neptune_codegen as CG
+from neptune_codegen import embedding as EM
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+I, T, G = meta(2, 3, dtype=torch.int64), meta(10, 16), meta(2, 3, 16)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((I, meta(10)), {}, ValueError), ((I, meta(0, 16)), {}, ValueError), ((I, meta(10, 0)), {}, ValueError),
+    ((meta(2, 3, dtype=torch.int16), T), {}, TypeError), ((meta(2, 3), T), {}, TypeError),
+    ((I, meta(10, 16, dtype=torch.float64)), {}, TypeError), ((I, None), {}, TypeError), (([1], T), {}, TypeError),
+    ((I, T), {"scale": math.inf}, ValueError), ((I, T), {"scale": math.nan}, ValueError),
+    ((I, T), {"scale": "1"}, ValueError), ((I, T), {"scale": torch.ones(())}, ValueError)])
+def test_refusals(args, kw, error):
+    with pytest.raises(error):
+        CG.run_embedding(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((meta(2, 16), I, 10), {}, ValueError), ((meta(2, 3, 0), I, 10), {}, ValueError), ((G, I, 0), {}, ValueError),
+    ((G, I, True), {}, ValueError), ((G, I, 10.0), {}, ValueError), ((G, I.int().float(), 10), {}, TypeError),
+    ((G.double(), I, 10), {}, TypeError), ((G, I, 10), {"scale": -math.inf}, ValueError),
+    ((G, I, 1 << 31), {}, NotImplementedError),
+    ((G, I, 10), {"into": meta(10, 15)}, ValueError), ((G, I, 10), {"into": meta(11, 16)}, ValueError),
+    ((G, I, 10), {"into": meta(10, 16, dtype=torch.float16)}, TypeError),
+    ((G.float(), I, 10), {"into": meta(10, 16)}, TypeError), ((G, I, 10), {"into": meta(16, 10).T}, ValueError),
+    ((G, I, 10), {"into": meta(1, 16).expand(10, 16)}, ValueError), ((G, I, 10), {"into": [1]}, TypeError),
+    ((G, I, 10), {"into": meta(10, 16).requires_grad_()}, ValueError)])
+def test_gradient_refusals(args, kw, error):
+    with pytest.raises(error):
+        CG.run_embedding_backward(*args, **kw)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError, match="device"):
+        CG.run_embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4))
+    with pytest.raises(ValueError, match="device"):
+        CG.run_embedding_backward(torch.zeros(2, 4), torch.zeros(2, dtype=torch.int64), 3)
+
+
+def test_metadata_calls():
+    assert CG.run_embedding(I, T, scale=4).shape == (2, 3, 16)
+    assert CG.run_embedding(meta(dtype=torch.int32), T).shape == (16,)
+    grad = CG.run_embedding_backward(G, I, 10)
+    assert grad.shape == (10, 16) and grad.dtype == torch.bfloat16
+    into = meta(10, 16, dtype=torch.float32)
+    assert CG.run_embedding_backward(G, I, 10, into=into) is into
+    op = CG.as_embedding_op(2.0)
+    assert op is CG.as_embedding_op(2) and op(I, T).shape == (2, 3, 16)
+
+
+def test_a_sorts_digits_hold_the_keys():
+    for vocab in (1, 2, 7, 511, 512, 513, 32000, 128256, (1 << 27) - 1, 1 << 27, (1 << 31) - 1):
+        width, passes = EM._digits(vocab)
+        assert 1 <= width <= EM.MOST_DIGIT and width * passes >= vocab.bit_length()
+
+
+def test_tokens_have_one_stride():
+    x = torch.arange(24).view(4, 6)
+    for t, stride in ((x, 1), (x[:, ::2], None), (x[:, 1], 6), (x.T, None), (x[0, 0], 0), (x[:1, :1].expand(4, 6), 0)):
+        flat, step = EM._flat(t)
+        assert flat.numel() == t.numel()
+        if stride is not None:
+            assert flat.data_ptr() == t.data_ptr() and step == stride
+        walked = flat.as_strided((t.numel(),), (step,), flat.storage_offset())
+        assert torch.equal(walked, t.reshape(-1))
