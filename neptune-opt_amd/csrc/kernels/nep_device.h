@@ -178,6 +178,9 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 __device__ __forceinline__ u32x4 load16_any(const void* p) {
   return *reinterpret_cast<const u32x4_any*>(p);
 }
+__device__ __forceinline__ u32x4 load16_any_once(const void* p) {    // (not cached)
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+}
 __device__ __forceinline__ void store16_any(void* p, const u32x4& w) {
   __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
 }

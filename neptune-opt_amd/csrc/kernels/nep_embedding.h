@@ -4,13 +4,12 @@
 // A negative token stands for none: a row of zeros, and no gradient.  A token of `vocab` or more has a row
 // of NaN and no gradient; neither is read through.  Products and sums are fp32, rounded once.
 //
-// Gradient.  The tokens are sorted (by token, then by position), so that every row of the table is the sum
-// of one run of sorted entries, added in one order, without atomics:
-//   sort    pieces of the tokens, each by a workgroup in LDS, while the others clear the table
-//   merge   (more than one piece) an entry's place is its own in its piece and those of the other pieces'
-//           entries in front of it, found by bisection
+// Gradient.  The tokens are put in order, equal ones by position, so that every row of the table is the sum of
+// one run of entries, added in one order, without atomics:
+//   order   the tokens' places, by counting
 //   sums    a wavefront adds a chunk of entries over its columns, several rows in flight; runs that end
-//           inside the chunk are written, the others' parts are kept in fp32
+//           inside the chunk are written, the others' parts are kept in fp32; further workgroups clear the
+//           rows that no token names
 //   join    the parts of each run of several chunks, in order
 #pragma once
 
@@ -25,7 +24,7 @@ constexpr int kRowWords = 0, kRowAny = 1, kRowFew = 2;
 template <class St, int ACCESS, bool STREAM>
 __device__ __forceinline__ u32x4 row_word(const typename St::T* p, int n) {
   if constexpr (ACCESS == kRowWords) return STREAM ? load16(p) : load16_cached(p);
-  else if constexpr (ACCESS == kRowAny) return load16_any(p);
+  else if constexpr (ACCESS == kRowAny) return STREAM ? load16_any_once(p) : load16_any(p);
   else {
     float v[St::kVec];
 #pragma unroll
@@ -93,13 +92,12 @@ __device__ __forceinline__ void embedding(const Ix* __restrict__ tokens, const t
   }
 }
 
-// ---------------------------------------------------------------- sorting the tokens
-constexpr int kDigit = 9;                            // bits of a digit at most
-constexpr int kPerLane = 4;                          // entries of a lane
+// ---------------------------------------------------------------- tokens in order
+constexpr int kMostKeys = 1024;                      // rows of the table that a workgroup counts
 
-// Sums of the lanes before each lane, over the workgroup; `lds` holds an int per wavefront.
+// Sums of the lanes before each lane, over the workgroup, and of all; `lds` holds an int per wavefront.
 template <int WAVES>
-__device__ __forceinline__ int exclusive_sum(int v, int* lds) {
+__device__ __forceinline__ int exclusive_sum(int v, int* lds, int& all) {
   const int lane = lane_id(), wave = threadIdx.x >> 6;
   int s = v;
 #pragma unroll
@@ -107,158 +105,156 @@ __device__ __forceinline__ int exclusive_sum(int v, int* lds) {
     const int o = __builtin_amdgcn_ds_bpermute((lane - d) * 4, s);
     s += lane >= d ? o : 0;
   }
+  __syncthreads();                                   // the last sums have been read
   if (lane == 63) lds[wave] = s;
   __syncthreads();
   int before = 0;
+  all = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) before += w < wave ? lds[w] : 0;
+  for (int w = 0; w < WAVES; ++w) {
+    before += w < wave ? lds[w] : 0;
+    all += lds[w];
+  }
   return before + s - v;
 }
 
-// Piece blockIdx.x of THREADS * kPerLane tokens: keys (the token, or `vocab` for an absent one) and
-// positions in order, to its place in `keys` and `positions`.  A stable sort by `passes` digits of `width`
-// bits, from the last: a wavefront's lanes with one digit are found by a ballot for each of its bits.
-template <class Ix, int THREADS>
-__device__ __forceinline__ void sort_tokens(const Ix* __restrict__ tokens, u32* __restrict__ keys,
-                                            u32* __restrict__ positions, i64 count, i64 vocab, i64 stride_i,
-                                            int width, int passes) {
-  constexpr int WAVES = THREADS / 64, PIECE = THREADS * kPerLane, COUNTERS = WAVES << kDigit;
-  constexpr int MINE = COUNTERS / THREADS;           // counters of a lane
-  __shared__ u16 counters[WAVES][1 << kDigit];
-  __shared__ u32 lds_keys[PIECE], lds_positions[PIECE];
+// The tokens by (token mod W, token / W), then by position, W = 2^log_shares workgroups: workgroup w has the
+// tokens that are w mod W, and its places are behind those of the workgroups before it.  Each of its wavefronts
+// walks a run of the positions, counts its tokens (and those of earlier workgroups) and lists them; when the
+// counters have become places, the list goes there.  Every workgroup reads all tokens (from L2, a few
+// instructions for 64 of them), and none waits for another.  Frequent tokens, often neighbours, spread over the
+// workgroups; a wavefront whose list is too short walks its run again.
+// `named` gets a byte for each row of the table: whether a token names it.  Places behind the last token
+// have the key `vocab`.
+template <class Ix, int WAVES>
+__device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u32* __restrict__ keys,
+                                                u32* __restrict__ positions, unsigned char* __restrict__ named,
+                                                i64 count, u32 vocab, i64 stride_i, int log_shares) {
+  constexpr int THREADS = WAVES * 64, BATCHES = 8, GROUP = 64 * BATCHES, LIST = 512;
+  __shared__ int counters[WAVES][kMostKeys];
+  __shared__ u32 list_keys[WAVES][LIST], list_positions[WAVES][LIST];
   __shared__ int sums[WAVES];
-  const int lane = lane_id(), wave = threadIdx.x >> 6, place = wave * 64 * kPerLane + lane;
-  const i64 first = (i64)blockIdx.x * PIECE;
-  u32 key[kPerLane], position[kPerLane];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const u32 share = blockIdx.x, mask = (1u << log_shares) - 1;
+  const int mine = share < vocab ? (int)((vocab - 1 - share) >> log_shares) + 1 : 0;    // keys
+  for (int k = lane; k < mine; k += 64) counters[wave][k] = 0;
+  const i64 run = ((count + THREADS - 1) / THREADS) * 64;
+  const i64 first = wave * run < count ? wave * run : count, end = first + run < count ? first + run : count;
+  const u32 lane_bytes = (u32)lane * (u32)stride_i * (u32)sizeof(Ix);    // (strides are below 2^20)
+  // a group of positions; absent tokens behind the end
+  auto load = [&](i64 i0, Ix* token) {
+    if (i0 + GROUP <= end) {
 #pragma unroll
-  for (int r = 0; r < kPerLane; ++r) {
-    const i64 i = first + place + r * 64;
-    const i64 token = i < count ? (i64)tokens[i * stride_i] : -1;
-    key[r] = (u32)(token >= 0 && token < vocab ? token : vocab);
-    position[r] = (u32)i;
-  }
-  volatile u16* mine = counters[wave];
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * width, digits = 1 << width;
-    for (int d = lane; d < digits; d += 64) mine[d] = 0;
-    int rank[kPerLane];
+      for (int b = 0; b < BATCHES; ++b)
+        token[b] = *(const Ix*)((const char*)(tokens + (i0 + b * 64) * stride_i) + lane_bytes);
+    } else {
 #pragma unroll
-    for (int r = 0; r < kPerLane; ++r) {
-      const u32 digit = (key[r] >> shift) & (digits - 1);
-      u64 same = ~0ull;
-      for (int b = 0; b < width; ++b) {
-        const bool bit = (digit >> b) & 1;
-        const u64 set = __builtin_amdgcn_ballot_w64(bit);
-        same &= bit ? set : ~set;
+      for (int b = 0; b < BATCHES; ++b) {
+        const i64 i = i0 + b * 64 + lane;
+        token[b] = i < end ? tokens[i * stride_i] : (Ix)-1;
       }
-      const int before = __builtin_amdgcn_mbcnt_hi((u32)(same >> 32), __builtin_amdgcn_mbcnt_lo((u32)same, 0));
-      const int base = mine[digit];
-      if (before == 0) mine[digit] = (u16)(base + __builtin_popcountll(same));
-      rank[r] = base + before;
     }
-    __syncthreads();
-    // counters by (digit, wavefront) become the sums of those in front
-    int own[MINE], total = 0;
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const int c = threadIdx.x * MINE + i;
-      own[i] = c < digits * WAVES ? counters[c % WAVES][c / WAVES] : 0;
-      total += own[i];
+  };
+  auto known = [&](Ix token) -> u32 {                // unknown tokens are of no workgroup
+    if constexpr (sizeof(Ix) == 8) {
+      const u64 t = (u64)token;
+      return (u32)(t >> 32) == 0 && (u32)t < vocab ? (u32)t : ~0u;
+    } else {
+      return (u32)token < vocab ? (u32)token : ~0u;
     }
-    int before = exclusive_sum<WAVES>(total, sums);
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const int c = threadIdx.x * MINE + i;
-      if (c < digits * WAVES) counters[c % WAVES][c / WAVES] = (u16)before;
-      before += own[i];
+  };
+  // every group of the wavefront's run, the next one's tokens in flight
+  auto walk = [&](auto each) {
+    Ix a[BATCHES], b[BATCHES];
+    load(first, a);
+    for (i64 i0 = first; i0 < end; i0 += 2 * GROUP) {
+      load(i0 + GROUP, b);
+      each(i0, a);
+      if (i0 + GROUP >= end) break;
+      load(i0 + 2 * GROUP, a);
+      each(i0 + GROUP, b);
     }
-    __syncthreads();
+  };
+  int earlier = 0, listed = 0;
+  walk([&](i64 i0, const Ix* token) {
 #pragma unroll
-    for (int r = 0; r < kPerLane; ++r) {
-      const int to = rank[r] + mine[(key[r] >> shift) & (digits - 1)];
-      lds_keys[to] = key[r];
-      lds_positions[to] = position[r];
+    for (int b = 0; b < BATCHES; ++b) {
+      const u32 key = known(token[b]), of = key & mask;
+      earlier += of < share ? 1 : 0;
+      const bool own = of == share && key != ~0u;
+      const u64 some = __builtin_amdgcn_ballot_w64(own);
+      if (some == 0) continue;
+      const int at = listed + __builtin_amdgcn_mbcnt_hi((u32)(some >> 32), __builtin_amdgcn_mbcnt_lo((u32)some, 0));
+      if (own) {
+        __hip_atomic_fetch_add(&counters[wave][key >> log_shares], 1, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (at < LIST) {
+          list_keys[wave][at] = key;
+          list_positions[wave][at] = (u32)(i0 + b * 64 + lane);
+        }
+      }
+      listed += __builtin_popcountll(some);
     }
-    __syncthreads();
+  });
+  int base;
+  exclusive_sum<WAVES>(earlier, sums, base);         // (its barriers are behind all counts)
+  for (int k0 = 0; k0 < mine; k0 += THREADS) {
+    const int k = k0 + threadIdx.x;
+    int total = 0, all;
+    if (k < mine) {
 #pragma unroll
-    for (int r = 0; r < kPerLane; ++r) {
-      key[r] = lds_keys[place + r * 64];
-      position[r] = lds_positions[place + r * 64];
+      for (int w = 0; w < WAVES; ++w) total += counters[w][k];
     }
-  }
+    int place = base + exclusive_sum<WAVES>(total, sums, all);
+    if (k < mine) {
+      named[((u32)k << log_shares) | share] = total > 0;
 #pragma unroll
-  for (int r = 0; r < kPerLane; ++r) {
-    const i64 i = first + place + r * 64;
-    keys[i] = key[r];
-    positions[i] = position[r];
-  }
-}
-
-// The first `pieces` workgroups sort, the others (if any) write zeros over `bytes` bytes from the 16-byte
-// aligned `table`.
-template <class Ix, int THREADS>
-__device__ __forceinline__ void embedding_sort(const Ix* __restrict__ tokens, u32* __restrict__ keys,
-                                               u32* __restrict__ positions, char* __restrict__ table, i64 count,
-                                               i64 vocab, i64 stride_i, i64 bytes, int width, int passes,
-                                               int pieces) {
-  if ((int)blockIdx.x < pieces) {
-    sort_tokens<Ix, THREADS>(tokens, keys, positions, count, vocab, stride_i, width, passes);
-    return;
-  }
-  const i64 words = bytes / 16, at = (i64)(blockIdx.x - pieces) * THREADS + threadIdx.x;
-  const i64 step = (i64)(gridDim.x - pieces) * THREADS;
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  for (i64 w = at; w < words; w += step) store16(table + w * 16, zero);
-  for (i64 b = words * 16 + at * 2; b < bytes; b += step * 2) *(u16*)(table + b) = 0;
-}
-
-// Entries of `keys[0..size)` (in order) that are less than `key`, or not more.
-__device__ __forceinline__ int count_before(const u32* keys, int size, u32 key, bool or_same) {
-  int lo = 0, n = size;
-  while (n > 0) {
-    const int half = n >> 1;
-    const u32 k = keys[lo + half];
-    const bool up = or_same ? k <= key : k < key;
-    lo = up ? lo + half + 1 : lo;
-    n = up ? n - half - 1 : half;
-  }
-  return lo;
-}
-
-// blockIdx.x: 256 * kPerLane entries of the pieces of PIECE entries.  Entries past `count` have the last
-// places, and are not written.
-template <int PIECE>
-__device__ __forceinline__ void embedding_merge(const u32* __restrict__ keys, const u32* __restrict__ positions,
-                                                u32* __restrict__ keys_out, u32* __restrict__ positions_out,
-                                                i64 count, int pieces) {
-  constexpr int SHARE = 256 * kPerLane;
-  __shared__ u32x4 words[PIECE / 4];
-  const u32* other = (const u32*)words;
-  const int piece = (int)(((i64)blockIdx.x * SHARE) / PIECE);
-  const i64 first = (i64)blockIdx.x * SHARE;
-  u32 key[kPerLane], position[kPerLane];
-  i64 to[kPerLane];
-#pragma unroll
-  for (int r = 0; r < kPerLane; ++r) {
-    const i64 i = first + r * 256 + threadIdx.x;
-    key[r] = keys[i];
-    position[r] = positions[i];
-    to[r] = i - (i64)piece * PIECE;
-  }
-  for (int p = 0; p < pieces; ++p) {
-    if (p == piece) continue;
-    __syncthreads();
-    for (int w = threadIdx.x; w < PIECE / 4; w += 256) words[w] = load16_cached(keys + (i64)p * PIECE + w * 4);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kPerLane; ++r) to[r] += count_before(other, PIECE, key[r], p < piece);
-  }
-#pragma unroll
-  for (int r = 0; r < kPerLane; ++r)
-    if ((i64)position[r] < count && to[r] < count) {
-      keys_out[to[r]] = key[r];
-      positions_out[to[r]] = position[r];
+      for (int w = 0; w < WAVES; ++w) {
+        const int c = counters[w][k];
+        counters[w][k] = place;
+        place += c;
+      }
     }
+    base += all;
+  }
+  __syncthreads();
+  if (share == mask)
+    for (i64 i = base + (int)threadIdx.x; i < count; i += THREADS) keys[i] = vocab;
+  // tokens in order of their positions, to their places
+  const int bits = mine > 1 ? 32 - __builtin_clz(mine - 1) : 0;
+  auto put = [&](bool own, u32 key, u32 position) {
+    const int k = own ? (int)(key >> log_shares) : 0;
+    u64 same = __builtin_amdgcn_ballot_w64(own);
+    for (int b = 0; b < bits; ++b) {
+      const bool bit = (k >> b) & 1;
+      const u64 set = __builtin_amdgcn_ballot_w64(bit);
+      same &= bit ? set : ~set;
+    }
+    const int before = __builtin_amdgcn_mbcnt_hi((u32)(same >> 32), __builtin_amdgcn_mbcnt_lo((u32)same, 0));
+    if (own) {
+      // (the wavefront's own counters: its reads and writes stay in order)
+      volatile int* counter = &counters[wave][k];
+      const int place = *counter + before;
+      if (before == 0) *counter = place + __builtin_popcountll(same);
+      keys[place] = key;
+      positions[place] = position;
+    }
+  };
+  if (listed <= LIST) {
+    for (int l0 = 0; l0 < listed; l0 += 64) {
+      const bool here = l0 + lane < listed;
+      put(here, here ? list_keys[wave][l0 + lane] : 0, here ? list_positions[wave][l0 + lane] : 0);
+    }
+  } else {
+    walk([&](i64 i0, const Ix* token) {
+#pragma unroll
+      for (int b = 0; b < BATCHES; ++b) {
+        const u32 key = known(token[b]);
+        const bool own = (key & mask) == share && key != ~0u;
+        if (__builtin_amdgcn_ballot_w64(own) != 0) put(own, key, (u32)(i0 + b * 64 + lane));
+      }
+    });
+  }
 }
 
 // ---------------------------------------------------------------- sums
@@ -284,31 +280,73 @@ __device__ __forceinline__ void write_row(typename Ot::T* row, const float* acc,
   store_values<Ot, ACCESS, VEC>(row + column, v, n, from);
 }
 
-// Chunk blockIdx.x of `chunk` entries (a multiple of 64 or less than it), columns of the word of lane
-// blockIdx.y * 256 + threadIdx.x.  parts: [chunks][2][lanes][VEC] fp32, of the run that the chunk before
-// began (0), and of the one that begins here and goes on (1).
+// Zeros to the rows that no token names, four words a lane: of rows of up to 64 words, 2^log_lanes lanes each; or of
+// one row, in 2^log_tiles wavefronts.  The wavefronts walk the table's memory in order, 4 KB each, so that few of
+// the memory's pages are open and the wait for `named` is hidden (1.05 GB by workgroups of a wavefront 171 us, by
+// larger ones with four words a lane 182-196, a word a lane 157, but not behind a load).
+template <class St, int ACCESS>
+__device__ __forceinline__ void clear_rows(const unsigned char* __restrict__ named, typename St::T* __restrict__ table,
+                                           u32 block, int n, u32 vocab, int log_lanes, int log_tiles) {
+  constexpr int WORDS = 4;
+  const int lane = lane_id();
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  auto clear = [&](u32 row, int at) {
+    typename St::T* p = table + (i64)row * n + word_column<St, ACCESS>(at, n);
+    if constexpr (ACCESS == kRowWords) *(u32x4*)p = zero;
+    else if constexpr (ACCESS == kRowAny) *(u32x4_any*)p = zero;
+    else
+      for (int j = 0; j < n; ++j) St::store(p + j, 0.0f);
+  };
+  if (log_lanes < 7) {
+    const int rows = 64 >> log_lanes, at = lane & ((1 << log_lanes) - 1);
+    const u32 first = block * (WORDS * rows) + (lane >> log_lanes);
+    bool empty[WORDS];
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) empty[u] = first + u * rows < vocab && !named[first + u * rows];
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u)
+      if (empty[u] && at * St::kVec < n) clear(first + u * rows, at);
+  } else {
+    const u32 row = block >> log_tiles;
+    const int first = (int)(block & ((1u << log_tiles) - 1)) * 64 * WORDS + lane;
+    if (row >= vocab || named[row]) return;
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u)
+      if ((first + u * 64) * St::kVec < n) clear(row, first + u * 64);
+  }
+}
+
+// Workgroup (a wavefront) b < sums: chunk b / columns of `chunk` entries, columns of the word of lane
+// (b % columns) * 64 + lane; the workgroups behind clear the other rows.  parts: [chunks][2][lanes][VEC] fp32,
+// of the run that the chunk before began (0), and of the one that begins here and goes on (1).
 template <class St, class Ot, int ACCESS, bool ADD>
 __device__ __forceinline__ void embedding_sums(const typename St::T* __restrict__ grad,
                                                const u32* __restrict__ keys, const u32* __restrict__ positions,
+                                               const unsigned char* __restrict__ named,
                                                typename Ot::T* __restrict__ table, float* __restrict__ parts,
                                                i64 count, int n, u32 vocab, i64 stride_g, i64 stride_t, int chunk,
-                                               float scale) {
+                                               int columns, u32 sums, int log_lanes, int log_tiles, float scale) {
   constexpr int VEC = St::kVec, FLIGHT = 8;
-  const int lane = lane_id(), at = blockIdx.y * 256 + threadIdx.x;
-  const int wave_at = __builtin_amdgcn_readfirstlane(at - lane);
-  if (wave_at * VEC >= n) return;
+  if constexpr (!ADD) {
+    if (blockIdx.x >= sums) {
+      clear_rows<Ot, ACCESS>(named, table, blockIdx.x - sums, n, vocab, log_lanes, log_tiles);
+      return;
+    }
+  }
+  const u32 number = blockIdx.x / columns;           // of the chunk
+  const int lane = lane_id(), at = (blockIdx.x - number * columns) * 64 + lane;
   const bool active = at * VEC < n;
   const int column = active ? word_column<St, ACCESS>(at, n) : 0;
-  const i64 first = (i64)blockIdx.x * chunk, end = first + chunk < count ? first + chunk : count;
-  const i64 lanes = (i64)gridDim.y * 256;
-  float* part = parts + ((i64)blockIdx.x * 2 * lanes + at) * VEC;
+  const i64 first = (i64)number * chunk, end = first + chunk < count ? first + chunk : count;
+  const i64 lanes = (i64)columns * 64;
+  float* part = parts + ((i64)number * 2 * lanes + at) * VEC;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
   u32 current = keys[first];
+  const u32 last = keys[first > 0 ? first - 1 : 0], next = keys[end < count ? end : count - 1];
   if (current >= vocab) return;                      // absent tokens are last
-  // whether the current run began in front of this chunk
-  bool before = first > 0 && keys[first - 1] == current;
+  bool before = first > 0 && last == current;        // the current run began in front of this chunk
   auto flush = [&](bool goes_on) {
     if (!active) return;
     if (before || goes_on) {
@@ -352,32 +390,32 @@ __device__ __forceinline__ void embedding_sums(const typename St::T* __restrict_
       }
     }
   }
-  flush(end < count && keys[end] == current);
+  flush(end < count && next == current);
 }
 
-// The run that begins in chunk blockIdx.x and goes on behind it, if there is one: its parts, over the
-// columns of the words of the 64 lanes of blockIdx.y.  The parts are dealt to the workgroup's WAVES
-// wavefronts in turn and their sums added in order.
+// The run that begins in chunk blockIdx.x and goes on behind it, if there is one: its parts, over the words of
+// the 64 lanes of blockIdx.y.  The WAVES wavefronts take the parts in turn, and their sums are added in order.
 template <class St, class Ot, int ACCESS, bool ADD, int WAVES>
 __device__ __forceinline__ void embedding_join(const u32* __restrict__ keys, const float* __restrict__ parts,
                                                typename Ot::T* __restrict__ table, i64 count, int n, u32 vocab,
-                                               i64 stride_t, int chunk, int chunks, i64 lanes, float scale) {
-  constexpr int VEC = St::kVec, FLIGHT = 4;
+                                               i64 stride_t, int chunk, int chunks, float scale) {
+  constexpr int VEC = St::kVec, FLIGHT = 8;
   __shared__ float lds[WAVES][64][VEC + 4];
   const i64 first = (i64)blockIdx.x * chunk, end = first + chunk;
   if (end >= count) return;
-  const u32 key = keys[end - 1];
-  if (key >= vocab || keys[end] != key) return;
-  if (first > 0 && keys[first] == key && keys[first - 1] == key) return;    // it began earlier
-  // chunks whose first entry is of this run
-  int lo = (int)blockIdx.x + 1, hi = chunks;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (keys[(i64)mid * chunk] == key) lo = mid;
-    else hi = mid;
+  const u32 key = keys[end - 1], behind = keys[end], begin = keys[first], before = keys[first > 0 ? first - 1 : 0];
+  if (key >= vocab || behind != key) return;
+  if (first > 0 && begin == key && before == key) return;                  // it began earlier
+  const int lane = lane_id();
+  int items = 1;                                     // this chunk's part, and one of each that begins with the run
+  for (int c0 = (int)blockIdx.x + 1; c0 < chunks; c0 += 64) {
+    const bool goes_on = c0 + lane < chunks && keys[(i64)(c0 + lane) * chunk] == key;
+    const u64 ends = ~__builtin_amdgcn_ballot_w64(goes_on);
+    items += ends != 0 ? (int)__builtin_ctzll(ends) : 64;
+    if (ends != 0) break;
   }
-  const int items = hi - (int)blockIdx.x;            // this chunk's part, and one of each behind it
-  const int lane = lane_id(), wave = threadIdx.x >> 6, at = blockIdx.y * 64 + lane;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), at = blockIdx.y * 64 + lane;
+  const i64 lanes = (i64)gridDim.y * 64;
   const float* mine = parts + ((i64)blockIdx.x * 2 * lanes + at) * VEC;
   float acc[VEC];
 #pragma unroll
@@ -401,8 +439,7 @@ __device__ __forceinline__ void embedding_join(const u32* __restrict__ keys, con
   for (int j = 0; j < VEC; ++j) lds[wave][lane][j] = acc[j];
   __syncthreads();
   if (wave > 0 || at * VEC >= n) return;
-  const int waves = items < WAVES ? items : WAVES;
-  for (int w = 1; w < waves; ++w)
+  for (int w = 1; w < WAVES && w < items; ++w)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] += lds[w][lane][j];
   write_row<Ot, ACCESS, ADD, VEC>(table + (i64)key * stride_t, acc, scale, at,

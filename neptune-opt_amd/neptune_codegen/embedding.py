@@ -15,22 +15,21 @@ from __future__ import annotations
 import threading
 
 from neptune_codegen import calls, hip
-from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_sort_name, embedding_sums_name,
-                                      emit_embedding_sort_source, emit_embedding_source,
+from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_order_name, embedding_sums_name,
+                                      emit_embedding_order_source, emit_embedding_source,
                                       emit_embedding_sums_source)
 
-PER_LANE = 4             # tokens that a lane sorts
-MOST_DIGIT = 9           # bits that one pass of the sort takes
+MOST_KEYS = 1024         # rows that a workgroup counts the tokens of (nep_embedding.h kMostKeys)
+MOST_STRIDE = 1 << 20
 _PROGRAMS: dict = {}
 _OPS: dict = {}
 _FORWARD, _BACKWARD = calls.Table(), calls.Table()
 _lock = threading.Lock()
 
 _LOOKUP_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,)
-_SORT_ARGS = (hip.PTR,) * 4 + (hip.I64,) * 4 + (hip.I32,) * 3
-_MERGE_ARGS = (hip.PTR,) * 4 + (hip.I64, hip.I32)
-_SUMS_ARGS = (hip.PTR,) * 5 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.I32, hip.F32)
-_JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 2 + (hip.I32,) * 2 + (hip.I64, hip.F32)
+_ORDER_ARGS = (hip.PTR,) * 4 + (hip.I64,) * 3 + (hip.I32,)
+_SUMS_ARGS = (hip.PTR,) * 6 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.I32,) * 5 + (hip.F32,)
+_JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 2 + (hip.I32,) * 2 + (hip.F32,)
 
 
 def _program(name: str, emit, *args) -> hip.Program:
@@ -45,8 +44,8 @@ def _lookup_program(var: EmbeddingVariant) -> hip.Program:
     return _program(var.name, emit_embedding_source, var)
 
 
-def _sort_program(index: str, threads: int) -> hip.Program:
-    return _program(embedding_sort_name("sort", index, threads), emit_embedding_sort_source, index, threads)
+def _order_program(index: str, waves: int) -> hip.Program:
+    return _program(embedding_order_name(index, waves), emit_embedding_order_source, index, waves)
 
 
 def _sums_program(dtype, out, access: str, add: bool) -> hip.Program:
@@ -139,6 +138,8 @@ def _name(t) -> str:
 def _flat(tokens):
     """Tokens whose elements have one stride, and that stride."""
     used, stride = calls.rows_of(tokens.unsqueeze(-1))
+    if stride >= MOST_STRIDE:                        # (a wavefront's are addressed with 32-bit offsets)
+        used, stride = used.contiguous(), 1
     return (tokens if used.data_ptr() == tokens.data_ptr() else used), stride
 
 
@@ -178,17 +179,19 @@ def run_embedding(tokens, table, *, scale: float = 1.0):
     return plan.run((flat, used))
 
 
-def _digits(vocab: int) -> tuple[int, int]:
-    """(bits of a digit, digits) of a sort of keys from 0 to vocab."""
-    bits = vocab.bit_length()
-    passes = -(-bits // MOST_DIGIT)
-    return -(-bits // passes), passes
+def _shares(vocab: int) -> int:
+    """Workgroups (log 2) that the rows of the table are dealt to for the tokens' order: one a CU, or a row
+    each; more where their counters would not hold the rows."""
+    log = min(8, (vocab - 1).bit_length())
+    while -(-vocab >> log) > MOST_KEYS:
+        log += 1
+    return log
 
 
 def _chunk(count: int, words: int) -> int:
     """Sorted entries that a wavefront adds."""
     chunk = 16
-    while chunk < 256 and -(-count // (2 * chunk)) * -(-words // 64) >= 4096:
+    while chunk < 256 and -(-count // (2 * chunk)) * -(-words // 64) > 1536:
         chunk *= 2
     return chunk
 
@@ -222,40 +225,28 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
     out = grad.dtype if into is None else into.dtype
     words = -(-n // (16 // grad.element_size()))
     access = _access(n, (g, sg), *([(into, st)] if add else []))
-    threads = 1024 if count > 256 * PER_LANE else 256
-    piece = threads * PER_LANE
-    pieces = -(-count // piece)
-    width, passes = _digits(vocab)
+    log, waves = _shares(vocab), 16 if count > 1024 else 4
     chunk = _chunk(count, words)
-    chunks, columns = -(-count // chunk), -(-words // 256)
-    lanes = 256 * columns
-    # result; keys and positions, in pieces and merged; parts of runs over several chunks
+    chunks, columns = -(-count // chunk), -(-words // 64)
+    # result; keys, positions and the rows that are named; parts of runs over several chunks
     buffers = [] if add else [((vocab, n), out)]
-    keys, positions = calls.buffer(len(buffers)), calls.buffer(len(buffers) + 1)
-    buffers += [((pieces * piece,), torch.int32)] * 2
+    keys, positions, named, parts = (calls.buffer(len(buffers) + i) for i in range(4))
+    buffers += [((count,), torch.int32)] * 2 + [((vocab,), torch.uint8)]
+    buffers.append(((chunks * 2 * 64 * columns * (16 // grad.element_size()),), torch.float32))
     table = calls.tensor(2) if add else calls.buffer(0)
-    size = 0 if add else vocab * n * grad.element_size()
-    clear = min(2048, -(-size // (threads * 64)))
-    prog = _sort_program(_name(tokens), threads)
-    launches = [(prog.kernel(embedding_sort_name("sort", _name(tokens), threads), _SORT_ARGS, threads, device),
-                 (pieces + clear,), (calls.tensor(1), keys, positions, table, count, vocab, si, size, width, passes,
-                                     pieces))]
-    if pieces > 1:
-        merged = calls.buffer(len(buffers)), calls.buffer(len(buffers) + 1)
-        buffers += [((count,), torch.int32)] * 2
-        launches.append((prog.kernel(embedding_sort_name("merge", _name(tokens), threads), _MERGE_ARGS, 256, device),
-                         (pieces * threads // 256,), (keys, positions, *merged, count, pieces)))
-        keys, positions = merged
-    parts = calls.buffer(len(buffers))
-    buffers.append(((chunks * 2 * lanes * (16 // grad.element_size()),), torch.float32))
-    prog = _sums_program(_name(grad), str(out), access, add)
     tag = (_name(grad), str(out), access, add)
-    launches.append((prog.kernel(embedding_sums_name("sums", *tag), _SUMS_ARGS, 256, device), (chunks, columns),
-                     (calls.tensor(0), keys, positions, table, parts, count, n, vocab, sg, st, chunk, scale)))
+    order, prog = embedding_order_name(_name(tokens), waves), _sums_program(*tag)
+    # wavefronts that clear: four words a lane, of several short rows or a part of a long one
+    log_lanes, log_tiles = min(7, (words - 1).bit_length()), (-(-words // 256) - 1).bit_length()
+    clear = 0 if add else -(-vocab // (4 * (64 >> log_lanes))) if log_lanes < 7 else vocab << log_tiles
+    launches = [(_order_program(_name(tokens), waves).kernel(order, _ORDER_ARGS, 64 * waves, device), (1 << log,),
+                 (calls.tensor(1), keys, positions, named, count, vocab, si, log)),
+                (prog.kernel(embedding_sums_name("sums", *tag), _SUMS_ARGS, 64, device), (chunks * columns + clear,),
+                 (calls.tensor(0), keys, positions, named, table, parts, count, n, vocab, sg, st, chunk, columns,
+                  chunks * columns, log_lanes, log_tiles, scale))]
     if chunks > 1:
-        launches.append((prog.kernel(embedding_sums_name("join", *tag), _JOIN_ARGS, 512, device),
-                         (chunks, -(-words // 64)),
-                         (keys, parts, table, count, n, vocab, st, chunk, chunks, lanes, scale)))
+        launches.append((prog.kernel(embedding_sums_name("join", *tag), _JOIN_ARGS, 256, device),
+                         (chunks, columns), (keys, parts, table, count, n, vocab, st, chunk, chunks, scale)))
     plan = calls.Plan(device, 3, buffers, () if add else (0,), launches)
     if calls.same(given, used):
         _BACKWARD.keep(given, (vocab, number), plan)

@@ -965,26 +965,20 @@ def emit_embedding_source(var: EmbeddingVariant) -> str:
             "scale);\n}\n")
 
 
-def embedding_sort_name(stage: str, index: str, threads: int) -> str:
-    return f"embedding_{stage}_{index[0]}{index[3:]}_{threads}"
+def embedding_order_name(index: str, waves: int) -> str:
+    return f"embedding_order_{index[0]}{index[3:]}_{waves}"
 
 
-def emit_embedding_sort_source(index: str, threads: int) -> str:
-    """hiprtc unit of the tokens' sort in pieces ("sort") and of the pieces' merge ("merge"), nep_embedding.h."""
+def emit_embedding_order_source(index: str, waves: int) -> str:
+    """hiprtc unit that puts the tokens in order for their rows' sums, nep_embedding.h."""
     ix = _INDEX_TYPES[index]
     return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: tokens in order\n"
             + kernel_header("nep_device.h", "nep_embedding.h")
-            + f'\nextern "C" __global__ void __launch_bounds__({threads}) '
-            f"{embedding_sort_name('sort', index, threads)}(const void* tokens, unsigned* keys, "
-            "unsigned* positions, void* table, long long count, long long vocab, long long stride_i, "
-            "long long bytes, int width, int passes, int pieces) {\n"
-            f"  nep::embedding_sort<{ix}, {threads}>((const {ix}*)tokens, keys, positions, (char*)table, count, "
-            "vocab, stride_i, bytes, width, passes, pieces);\n}\n"
-            'extern "C" __global__ void __launch_bounds__(256) '
-            f"{embedding_sort_name('merge', index, threads)}(const unsigned* keys, const unsigned* positions, "
-            "unsigned* keys_out, unsigned* positions_out, long long count, int pieces) {\n"
-            f"  nep::embedding_merge<{threads} * nep::kPerLane>(keys, positions, keys_out, positions_out, count, "
-            "pieces);\n}\n")
+            + f'\nextern "C" __global__ void __launch_bounds__({64 * waves}) {embedding_order_name(index, waves)}('
+            "const void* tokens, unsigned* keys, unsigned* positions, unsigned char* named, long long count, "
+            "long long vocab, long long stride_i, int log_shares) {\n"
+            f"  nep::embedding_order<{ix}, {waves}>((const {ix}*)tokens, keys, positions, named, count, "
+            "(nep::u32)vocab, stride_i, log_shares);\n}\n")
 
 
 def embedding_sums_name(stage: str, dtype, out, access: str, add: bool) -> str:
@@ -997,18 +991,19 @@ def emit_embedding_sums_source(dtype, out, access: str, add: bool) -> str:
     targs = f"{st}, {ot}, {EMBEDDING_ACCESS[access]}, {str(add).lower()}"
     return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: rows' sums\n"
             + kernel_header("nep_device.h", "nep_embedding.h")
-            + '\nextern "C" __global__ void __launch_bounds__(256) '
+            + '\nextern "C" __global__ void __launch_bounds__(64) '
             f"{embedding_sums_name('sums', dtype, out, access, add)}(const void* grad, const unsigned* keys, "
-            "const unsigned* positions, void* table, float* parts, long long count, int n, long long vocab, "
-            "long long stride_g, long long stride_t, int chunk, float scale) {\n"
-            f"  nep::embedding_sums<{targs}>((const {st}::T*)grad, keys, positions, ({ot}::T*)table, parts, count, "
-            "n, (nep::u32)vocab, stride_g, stride_t, chunk, scale);\n}\n"
-            'extern "C" __global__ void __launch_bounds__(512) '
+            "const unsigned* positions, const unsigned char* named, void* table, float* parts, long long count, int n, "
+            "long long vocab, long long stride_g, long long stride_t, int chunk, int columns, unsigned sums, "
+            "int log_lanes, int log_tiles, float scale) {\n"
+            f"  nep::embedding_sums<{targs}>((const {st}::T*)grad, keys, positions, named, ({ot}::T*)table, parts, "
+            "count, n, (nep::u32)vocab, stride_g, stride_t, chunk, columns, sums, log_lanes, log_tiles, scale);\n}\n"
+            'extern "C" __global__ void __launch_bounds__(256) '
             f"{embedding_sums_name('join', dtype, out, access, add)}(const unsigned* keys, const float* parts, "
             "void* table, long long count, int n, long long vocab, long long stride_t, int chunk, int chunks, "
-            "long long lanes, float scale) {\n"
-            f"  nep::embedding_join<{targs}, 8>(keys, parts, ({ot}::T*)table, count, n, (nep::u32)vocab, stride_t, "
-            "chunk, chunks, lanes, scale);\n}\n")
+            "float scale) {\n"
+            f"  nep::embedding_join<{targs}, 4>(keys, parts, ({ot}::T*)table, count, n, (nep::u32)vocab, stride_t, "
+            "chunk, chunks, scale);\n}\n")
 
 
 # ---------------------------------------------------------------- gradients of a whole model

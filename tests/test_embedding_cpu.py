@@ -59,10 +59,14 @@ def test_metadata_calls():
     assert op is CG.as_embedding_op(2) and op(I, T).shape == (2, 3, 16)
 
 
-def test_a_sorts_digits_hold_the_keys():
-    for vocab in (1, 2, 7, 511, 512, 513, 32000, 128256, (1 << 27) - 1, 1 << 27, (1 << 31) - 1):
-        width, passes = EM._digits(vocab)
-        assert 1 <= width <= EM.MOST_DIGIT and width * passes >= vocab.bit_length()
+def test_the_workgroups_that_order_tokens_count_every_row():
+    for vocab in (1, 2, 7, 255, 256, 257, 32000, 128256, 1 << 18, (1 << 18) + 1, 1 << 27, (1 << 31) - 1):
+        shares = 1 << EM._shares(vocab)
+        assert -(-vocab // shares) <= EM.MOST_KEYS and (shares <= 256 or -(-vocab // (shares // 2)) > EM.MOST_KEYS)
+        # rows of workgroup w, as the kernel counts them
+        mine = [(vocab - 1 - w) // shares + 1 if w < vocab else 0 for w in range(min(shares, 4096))]
+        if shares <= 4096:
+            assert sum(mine) == vocab
 
 
 def test_tokens_have_one_stride():
