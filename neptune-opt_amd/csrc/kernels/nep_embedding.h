@@ -11,6 +11,7 @@
 //           inside the chunk are written, the others' parts are kept in fp32; further workgroups clear the
 //           rows that no token names
 //   join    the parts of each run of several chunks, in order
+// or, of few tokens, by one launch in which each row's first token finds the others.
 #pragma once
 
 namespace nep {
@@ -284,8 +285,9 @@ __device__ __forceinline__ void write_row(typename Ot::T* row, const float* acc,
 // one row, in 2^log_tiles wavefronts.  The wavefronts walk the table's memory in order, 4 KB each, so that few of
 // the memory's pages are open and the wait for `named` is hidden (1.05 GB by workgroups of a wavefront 171 us, by
 // larger ones with four words a lane 182-196, a word a lane 157, but not behind a load).
+// `named` has a byte for each row from `base` on.
 template <class St, int ACCESS>
-__device__ __forceinline__ void clear_rows(const unsigned char* __restrict__ named, typename St::T* __restrict__ table,
+__device__ __forceinline__ void clear_rows(const unsigned char* named, u32 base, typename St::T* __restrict__ table,
                                            u32 block, int n, u32 vocab, int log_lanes, int log_tiles) {
   constexpr int WORDS = 4;
   const int lane = lane_id();
@@ -302,14 +304,14 @@ __device__ __forceinline__ void clear_rows(const unsigned char* __restrict__ nam
     const u32 first = block * (WORDS * rows) + (lane >> log_lanes);
     bool empty[WORDS];
 #pragma unroll
-    for (int u = 0; u < WORDS; ++u) empty[u] = first + u * rows < vocab && !named[first + u * rows];
+    for (int u = 0; u < WORDS; ++u) empty[u] = first + u * rows < vocab && !named[first + u * rows - base];
 #pragma unroll
     for (int u = 0; u < WORDS; ++u)
       if (empty[u] && at * St::kVec < n) clear(first + u * rows, at);
   } else {
     const u32 row = block >> log_tiles;
     const int first = (int)(block & ((1u << log_tiles) - 1)) * 64 * WORDS + lane;
-    if (row >= vocab || named[row]) return;
+    if (row >= vocab || named[row - base]) return;
 #pragma unroll
     for (int u = 0; u < WORDS; ++u)
       if ((first + u * 64) * St::kVec < n) clear(row, first + u * 64);
@@ -329,7 +331,7 @@ __device__ __forceinline__ void embedding_sums(const typename St::T* __restrict_
   constexpr int VEC = St::kVec, FLIGHT = 8;
   if constexpr (!ADD) {
     if (blockIdx.x >= sums) {
-      clear_rows<Ot, ACCESS>(named, table, blockIdx.x - sums, n, vocab, log_lanes, log_tiles);
+      clear_rows<Ot, ACCESS>(named, 0, table, blockIdx.x - sums, n, vocab, log_lanes, log_tiles);
       return;
     }
   }
@@ -444,6 +446,84 @@ __device__ __forceinline__ void embedding_join(const u32* __restrict__ keys, con
     for (int j = 0; j < VEC; ++j) acc[j] += lds[w][lane][j];
   write_row<Ot, ACCESS, ADD, VEC>(table + (i64)key * stride_t, acc, scale, at,
                                   word_column<St, ACCESS>(at, n), n);
+}
+
+// ---------------------------------------------------------------- few tokens
+// Up to 256 tokens in one launch: a lane of the workgroup has a token.  Workgroup b < sums: the row of token
+// b / columns where that is its first, over the words of 64 lanes; its four wavefronts take the row's tokens in turn,
+// and their sums are added in order.  The workgroups behind mark the tokens of the rows that they clear in LDS.
+template <class St, class Ot, class Ix, int ACCESS, bool ADD>
+__device__ __forceinline__ void embedding_few(const Ix* __restrict__ tokens, const typename St::T* __restrict__ grad,
+                                              typename Ot::T* __restrict__ table, int count, int n, u32 vocab,
+                                              i64 stride_i, i64 stride_g, i64 stride_t, int columns, u32 sums,
+                                              int log_lanes, int log_tiles, float scale) {
+  constexpr int VEC = St::kVec, FLIGHT = 8, WAVES = 4;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), tid = threadIdx.x;
+  const i64 token = tid < count ? (i64)tokens[tid * stride_i] : -1;
+  const u32 key = token >= 0 && token < (i64)vocab ? (u32)token : ~0u;
+  if constexpr (!ADD) {
+    __shared__ unsigned char named[1024];
+    if (blockIdx.x >= sums) {
+      const u32 block = blockIdx.x - sums, per = 64 >> (log_lanes < 6 ? log_lanes : 6);
+      const u32 base = log_lanes < 7 ? block * (WAVES * 4 * per) : block * WAVES >> log_tiles;
+      ((u32*)named)[tid] = 0;
+      __syncthreads();
+      if (key - base < 1024) named[key - base] = 1;  // (of at most 16 * 64 rows)
+      __syncthreads();
+      clear_rows<Ot, ACCESS>(named, base, table, block * WAVES + wave, n, vocab, log_lanes, log_tiles);
+      return;
+    }
+  }
+  __shared__ u32 keys[256];
+  __shared__ u16 list[256];
+  __shared__ int found[WAVES];
+  __shared__ float lds[WAVES][64][VEC + 4];
+  const int number = blockIdx.x / columns, at = (blockIdx.x - number * columns) * 64 + lane;
+  keys[tid] = key;
+  __syncthreads();
+  const u32 mine = keys[number];
+  const u64 same = __builtin_amdgcn_ballot_w64(key == mine);
+  if (lane == 0) found[wave] = __builtin_popcountll(same);
+  if (__syncthreads_or(mine == ~0u || (key == mine && tid < number))) return;
+  int place = __builtin_amdgcn_mbcnt_hi((u32)(same >> 32), __builtin_amdgcn_mbcnt_lo((u32)same, 0)), items = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    place += w < wave ? found[w] : 0;
+    items += found[w];
+  }
+  if (key == mine) list[place] = (u16)tid;
+  __syncthreads();
+  const bool active = at * VEC < n;
+  const int column = active ? word_column<St, ACCESS>(at, n) : 0;
+  float acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+  for (int i0 = wave; i0 < items; i0 += WAVES * FLIGHT) {
+    u32x4 w[FLIGHT];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int i = i0 + f * WAVES;
+      const i64 row = (i64)list[i < items ? i : i0] * stride_g;
+      if (active) w[f] = row_word<St, ACCESS, true>(grad + row + column, n);
+    }
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      if (i0 + f * WAVES < items) {
+        float v[VEC];
+        St::unpack(w[f], v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += v[j];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) lds[wave][lane][j] = acc[j];
+  __syncthreads();
+  if (wave > 0 || !active) return;
+  for (int w = 1; w < WAVES && w < items; ++w)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] += lds[w][lane][j];
+  write_row<Ot, ACCESS, ADD, VEC>(table + (i64)mine * stride_t, acc, scale, at, column, n);
 }
 
 }  // namespace nep

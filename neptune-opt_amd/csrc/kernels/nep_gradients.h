@@ -6,24 +6,27 @@
 // from the rounded norm, so that a norm computed before gives the same bits.  A norm that is an infinity or
 // NaN has no factor: the elements stay as they are.
 //
-// A launch takes up to kTensors tensors by value, in its arguments: nothing is copied to the device, and a
-// captured launch keeps its own list.  Their elements are dealt to the workgroups in turn, in pieces of
-// `piece` elements that do not cross tensors; a workgroup finds a piece's tensor by bisection (scalar loads
-// from the arguments).  Scaling walks the pieces from the last to the first: what the norm read last is still
-// in the memory-side cache.
+// Lists of up to kTensors tensors are given by value, in a launch's arguments: nothing is copied to the device, and
+// a captured launch keeps its own list.  Longer ones (up to kMostTensors a launch) are put together in device memory
+// by small launches that hold a part each (0.9 GB in 290 tensors: 131 us so, 148 by three launches of the sums).
+// The elements are dealt to the workgroups in turn, in pieces of `piece` elements that do not cross tensors; a
+// workgroup finds a piece's tensor among the first pieces' numbers, in LDS, by two ballots (the arguments lie far
+// away, so each is read once).  Scaling walks the pieces from the last to the first: what the norm read last is
+// still in the memory-side cache.
 #pragma once
 
 namespace nep {
 
 constexpr int kTensors = 112;                        // 3584 bytes; all arguments stay below 4096
+constexpr int kMostTensors = 4096;
 constexpr int kSumLanes = 1024;
 
-struct TensorEntry {
+struct alignas(16) TensorEntry {
   const void* in;
   void* out;
   u64 count;                                         // elements, at least one
   u32 first;                                         // number of its first piece
-  u32 kind;                                          // types of in and out, see visit
+  u32 kind;                                          // types of in and out
 };
 struct TensorList {
   TensorEntry entry[kTensors];
@@ -32,16 +35,39 @@ struct TensorList {
 // in and out
 constexpr u32 kF32 = 0, kBF16 = 1, kF16 = 2, kBF16ToF32 = 3, kF16ToF32 = 4;
 
-// The entry that piece p belongs to; entries [0, count) with ascending first pieces.
-__device__ __forceinline__ const TensorEntry& entry_of(const TensorList& list, int count, u32 p) {
-  int lo = 0, hi = count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (list.entry[mid].first <= p) lo = mid;
-    else hi = mid;
-  }
-  return list.entry[lo];
+__device__ __forceinline__ void copy_entry_words(u32x4* to, const TensorEntry* from, int count) {
+  for (int i = threadIdx.x; i < 2 * count; i += kSumLanes) to[i] = ((const u32x4*)from)[i];
 }
+// A part of a long list, to its place.
+__device__ __forceinline__ void gradient_list(const TensorList& list, int count, TensorEntry* __restrict__ to) {
+  copy_entry_words((u32x4*)to, list.entry, count);
+}
+
+// A list as a workgroup sees it: a short one is copied to LDS (FAR false), of a long one the numbers of the first
+// pieces.
+template <bool FAR>
+struct Tensors {
+  static constexpr int MOST = FAR ? kMostTensors : kTensors;
+  const TensorEntry* entries;
+  const u32* firsts;
+  int count, step;
+
+  // `lds`: room for a list by value; `numbers`: MOST words.  All lanes, once.
+  __device__ __forceinline__ Tensors(const TensorEntry* given, int n, u32x4* lds, u32* numbers)
+      : entries(FAR ? given : (const TensorEntry*)lds), firsts(numbers), count(n), step((n + 63) / 64) {
+    if constexpr (!FAR) copy_entry_words(lds, given, n);
+    for (int i = threadIdx.x; i < n; i += kSumLanes) numbers[i] = given[i].first;
+    __syncthreads();
+  }
+  // Number of the entry that piece p belongs to: the last with a first piece of p or less (the first one is 0).
+  __device__ __forceinline__ int of(u32 p) const {
+    const int lane = lane_id(), at = lane * step;
+    const u64 low = __builtin_amdgcn_ballot_w64(at < count && firsts[at < count ? at : 0] <= p);
+    const int begin = (__builtin_popcountll(low) - 1) * step, i = begin + lane;
+    const u64 in = __builtin_amdgcn_ballot_w64(lane < step && i < count && firsts[i < count ? i : 0] <= p);
+    return begin + __builtin_popcountll(in) - 1;
+  }
+};
 
 // Sum over the workgroup of kSumLanes lanes, the same in every lane.  (lds: a double per wavefront)
 __device__ __forceinline__ double workgroup_sum(double v, double* lds) {
@@ -90,12 +116,16 @@ __device__ __forceinline__ void add_squares(const typename St::T* p, i64 first, 
   }
 }
 
-__device__ __forceinline__ void gradient_sums(const TensorList& list, int count, u32 pieces, int piece,
+template <bool FAR>
+__device__ __forceinline__ void gradient_sums(const TensorEntry* list, int count, u32 pieces, int piece,
                                               double* __restrict__ sums) {
   __shared__ double lds[kSumLanes / 64];
+  __shared__ u32x4 words[FAR ? 1 : 2 * kTensors];
+  __shared__ u32 numbers[Tensors<FAR>::MOST];
+  const Tensors<FAR> tensors(list, count, words, numbers);
   double acc = 0.0;
   for (u32 p = blockIdx.x; p < pieces; p += gridDim.x) {
-    const TensorEntry& e = entry_of(list, count, p);
+    const TensorEntry e = tensors.entries[tensors.of(p)];
     const i64 first = (i64)(p - e.first) * piece;
     const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
     if (e.kind == kF32) add_squares<F32>((const float*)e.in, first, end, acc);
@@ -158,7 +188,8 @@ __device__ __forceinline__ void scale_elements(const typename St::T* p, typename
 }
 
 // `sums` null: the norm is given.  `copies`: whether an entry's out is not its in.
-__device__ __forceinline__ void gradient_scale(const TensorList& list, int count, u32 pieces, int piece,
+template <bool FAR>
+__device__ __forceinline__ void gradient_scale(const TensorEntry* list, int count, u32 pieces, int piece,
                                                const double* __restrict__ sums, int n_sums,
                                                const float* __restrict__ given, float* __restrict__ norm_out,
                                                float max_norm, int copies) {
@@ -166,9 +197,12 @@ __device__ __forceinline__ void gradient_scale(const TensorList& list, int count
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
   const float factor = is_finite(norm) && norm > max_norm ? div_rn(max_norm, norm) : 1.0f;
   if (factor == 1.0f && !copies) return;
+  __shared__ u32x4 words[FAR ? 1 : 2 * kTensors];
+  __shared__ u32 numbers[Tensors<FAR>::MOST];
+  const Tensors<FAR> tensors(list, count, words, numbers);
   for (u32 i = blockIdx.x; i < pieces; i += gridDim.x) {
     const u32 p = pieces - 1 - i;
-    const TensorEntry& e = entry_of(list, count, p);
+    const TensorEntry e = tensors.entries[tensors.of(p)];
     if (factor == 1.0f && e.in == e.out) continue;
     const i64 first = (i64)(p - e.first) * piece;
     const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;

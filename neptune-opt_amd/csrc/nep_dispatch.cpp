@@ -455,86 +455,80 @@ class CallTable {
   std::unordered_map<Key, std::shared_ptr<CallPlan>, KeyHash> plans_;
 };
 
-// The norm of many tensors and their scaling (csrc/kernels/nep_gradients.h), on one device.
+// The norm of many tensors and their scaling (csrc/kernels/nep_gradients.h).
 class GradientCalls {
  public:
-  // kernels' handles, tensors a launch takes, lanes of a workgroup, workgroups of a launch at most
-  GradientCalls(uint64_t sums, uint64_t norm, uint64_t scale, int tensors, int lanes, int workgroups)
-      : sums_(sums), norm_(norm), scale_(scale), tensors_(tensors), lanes_(lanes), workgroups_(workgroups) {
-    TORCH_CHECK(sums != 0 && norm != 0 && scale != 0 && tensors > 0 && lanes > 0 && workgroups > 0,
-                "GradientCalls: bad kernels");
+  // tensors of a list by value and of one in device memory, lanes of a workgroup, workgroups of a launch at most
+  GradientCalls(int by_value, int most, int lanes, int workgroups)
+      : by_value_(by_value), most_(most), lanes_(lanes), workgroups_(workgroups) {
+    TORCH_CHECK(by_value > 0 && most >= by_value && lanes > 0 && workgroups > 0, "GradientCalls: bad sizes");
   }
+
+  // A device's kernels: the norm; a part of a long list; sums and scaling of short lists, and of long ones.
+  void add(int device, const std::vector<uint64_t>& kernels) {
+    TORCH_CHECK(kernels.size() == 6 && device >= 0, "GradientCalls: expected six kernels");
+    for (uint64_t k : kernels) TORCH_CHECK(k != 0, "GradientCalls: bad kernel");
+    kernels_[device] = {kernels[0], kernels[1], {kernels[2], kernels[4]}, {kernels[3], kernels[5]}};
+  }
+  bool has(int device) const { return kernels_.count(device) != 0; }
 
   // The tensors' norm (fp32, no dimensions), or None for a list that this does not take.
   py::object norm(const py::handle& tensors) const {
-    std::vector<at::Tensor> in;
+    std::vector<const at::Tensor*> in;
     if (!collect(tensors, in)) return py::none();
-    const c10::Device device = in[0].device();
-    const c10::DeviceGuard guard(device);
-    hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
     std::vector<Entry> entries;
-    for (const at::Tensor& t : in) add(entries, t, t);
-    const Pieces pieces = deal(entries);
-    at::Tensor out = at::empty({}, at::TensorOptions().device(device).dtype(at::kFloat));
-    launch_norm(entries, pieces, device, stream, static_cast<float*>(out.data_ptr()));
+    entries.reserve(in.size());
+    for (const at::Tensor* t : in) push(entries, *t, *t);
+    Call call(*this, in[0]->device(), entries);
+    at::Tensor out = call.scalar();
+    call.norm(call.sums(), out);
     return py::cast(out);
   }
 
   // `out`: None (in place) or a list.  `given`: None or the norm.  The norm, or None for lists that this does
   // not take.
   py::object clip(const py::handle& tensors, const py::handle& out, const py::handle& given, float max_norm) const {
-    std::vector<at::Tensor> in, made;
+    std::vector<const at::Tensor*> in, made;
     if (!collect(tensors, in)) return py::none();
     const bool in_place = out.is_none();
     if (!in_place && (!collect(out, made) || made.size() != in.size())) return py::none();
-    const std::vector<at::Tensor>& to = in_place ? in : made;
-    const c10::Device device = in[0].device();
+    const std::vector<const at::Tensor*>& to = in_place ? in : made;
+    const c10::Device device = in[0]->device();
+    std::vector<Entry> entries;
+    entries.reserve(in.size());
+    int copies = 0;
     for (size_t i = 0; i < in.size(); ++i) {
-      const at::Tensor &a = in[i], &b = to[i];
-      if (b.requires_grad() || b.device() != device || !same_order(a, b) ||
-          (b.scalar_type() != a.scalar_type() && b.scalar_type() != at::kFloat))
+      const at::Tensor &a = *in[i], &b = *to[i];
+      if (b.requires_grad()) return py::none();
+      if (!in_place && (b.device() != device || !same_order(a, b) ||
+                        (b.scalar_type() != a.scalar_type() && b.scalar_type() != at::kFloat)))
         return py::none();
+      push(entries, a, b);
     }
-    if (!separate(in, to)) return py::none();
-    const float* known = nullptr;
+    for (const Entry& e : entries) copies |= e.in != e.out;
+    if (!separate(entries)) return py::none();
     at::Tensor norm;
-    if (!given.is_none()) {
+    const bool known = !given.is_none();
+    if (known) {
       if (!THPVariable_CheckExact(given.ptr())) return py::none();
       norm = THPVariable_Unpack(given.ptr());
       if (!plain(norm) || norm.device() != device || norm.scalar_type() != at::kFloat || norm.dim() != 0 ||
-          inside(norm, to))
+          inside(norm, entries))
         return py::none();
-      known = static_cast<const float*>(norm.data_ptr());
     }
-    const c10::DeviceGuard guard(device);
-    hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
-    std::vector<Entry> entries;
-    for (size_t i = 0; i < in.size(); ++i) add(entries, in[i], to[i]);
-    const Pieces pieces = deal(entries);
-    if (known == nullptr) norm = at::empty({}, at::TensorOptions().device(device).dtype(at::kFloat));
-    if (entries.empty()) {                           // nothing but its norm, 0
-      if (known == nullptr) launch_norm(entries, pieces, device, stream, static_cast<float*>(norm.data_ptr()));
-      return py::cast(norm);
-    }
+    Call call(*this, device, entries);
     at::Tensor sums;
-    if (known == nullptr) sums = launch_sums(entries, pieces, device, stream);
-    int copies = 0;
-    for (const Entry& e : entries) copies |= e.in != e.out;
-    // from the last list to the first, as the pieces of each
-    for (size_t i = pieces.launches.size(); i-- > 0;) {
-      const Part& part = pieces.launches[i];
-      Image image(entries, part, tensors_, pieces.piece);
-      image.put(known == nullptr ? sums.data_ptr() : nullptr);
-      image.put(static_cast<int32_t>(known == nullptr ? sums.numel() : 0));
-      image.align(8);
-      image.put(static_cast<const void*>(known));
-      image.put(known == nullptr && i + 1 == pieces.launches.size() ? norm.data_ptr() : nullptr);
-      image.put(max_norm);
-      image.put(static_cast<int32_t>(copies));
-      launch(scale_, grid(part), image, stream);
+    if (!known) {
+      norm = call.scalar();
+      sums = call.sums();
     }
-    for (const at::Tensor& t : to)
-      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    if (entries.empty()) {
+      if (!known) call.norm(sums, norm);             // of nothing: 0
+    } else {
+      call.scale(sums, norm, known, max_norm, copies);
+    }
+    for (const at::Tensor* t : to)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     return py::cast(norm);
   }
 
@@ -546,34 +540,142 @@ class GradientCalls {
     uint32_t first, kind;
   };
   static_assert(sizeof(Entry) == 32, "the kernels' layout");
-  struct Part {
-    size_t begin, end;                               // entries of one launch
-    uint32_t pieces;
-  };
-  struct Pieces {
-    int32_t piece;
-    std::vector<Part> launches;
+  struct Kernels {
+    uint64_t norm, list, sums[2], scale[2];          // of lists by value, and in device memory
   };
 
-  // A launch's arguments: its entries, their number, pieces and elements of a piece, then the rest.
+  // A launch's arguments.
   struct Image {
-    Image(const std::vector<Entry>& entries, const Part& part, int tensors, int32_t piece) {
-      bytes.resize(tensors * sizeof(Entry));
-      if (part.end > part.begin)
-        std::memcpy(bytes.data(), &entries[part.begin], (part.end - part.begin) * sizeof(Entry));
-      put(static_cast<int32_t>(part.end - part.begin));
-      put(part.pieces);
-      put(piece);
-      align(8);
-    }
     template <class T>
     void put(T value) {
+      bytes.resize((bytes.size() + sizeof(T) - 1) / sizeof(T) * sizeof(T));
       const size_t at = bytes.size();
       bytes.resize(at + sizeof(T));
       std::memcpy(bytes.data() + at, &value, sizeof(T));
     }
-    void align(size_t n) { bytes.resize((bytes.size() + n - 1) / n * n); }
     std::vector<uint8_t> bytes;
+  };
+
+  // One call's lists on its device and stream.
+  class Call {
+   public:
+    Call(const GradientCalls& of, c10::Device device, std::vector<Entry>& entries)
+        : of_(of), kernels_(of.kernels_.at(device.index())), guard_(device), entries_(entries),
+          options_(at::TensorOptions().device(device)),
+          stream_(c10::hip::getCurrentHIPStream(device.index()).stream()) {
+      uint64_t total = 0;
+      for (const Entry& e : entries_) total += e.count;
+      // at least one load of each lane, four where the pieces are many for the workgroups
+      while (piece_ < of.lanes_ * 32 && total / piece_ >= 16ull * of.workgroups_) piece_ *= 2;
+      piece_ = std::max(piece_, of.lanes_ * 8);
+      far_ = entries_.size() > static_cast<size_t>(of.by_value_);
+      const size_t most = far_ ? of.most_ : of.by_value_;
+      for (size_t begin = 0; begin < entries_.size(); begin += most) {
+        Part part{begin, std::min(entries_.size(), begin + most), 0};
+        uint64_t pieces = 0;
+        for (size_t i = part.begin; i < part.end; ++i) {
+          entries_[i].first = static_cast<uint32_t>(pieces);
+          pieces += (entries_[i].count + piece_ - 1) / piece_;
+          TORCH_CHECK_NOT_IMPLEMENTED(pieces < (1ull << 31), "gradients of more than 2^31 pieces of ", piece_,
+                                      " elements");
+        }
+        part.pieces = static_cast<uint32_t>(pieces);
+        parts_.push_back(part);
+      }
+      if (!far_) return;
+      // the lists, put together in device memory
+      list_ = at::empty({static_cast<int64_t>(entries_.size() * sizeof(Entry))}, options_.dtype(at::kByte));
+      for (size_t begin = 0; begin < entries_.size(); begin += of.by_value_) {
+        const size_t end = std::min(entries_.size(), begin + of.by_value_);
+        Image image;
+        by_value(image, begin, end);
+        image.put(static_cast<int32_t>(end - begin));
+        image.put(device_entries(begin));
+        launch(kernels_.list, 1, image);
+      }
+    }
+
+    at::Tensor scalar() const { return at::empty({}, options_.dtype(at::kFloat)); }
+
+    // One sum for each workgroup of all launches.
+    at::Tensor sums() const {
+      int64_t count = 0;
+      for (const Part& part : parts_) count += grid(part);
+      at::Tensor sums = at::empty({count}, options_.dtype(at::kDouble));
+      double* at = static_cast<double*>(sums.data_ptr());
+      for (const Part& part : parts_) {
+        Image image = head(part);
+        image.put(at);
+        launch(kernels_.sums[far_], grid(part), image);
+        at += grid(part);
+      }
+      return sums;
+    }
+
+    void norm(const at::Tensor& sums, at::Tensor& out) const {
+      Image image;
+      image.put(sums.data_ptr());
+      image.put(static_cast<int32_t>(sums.numel()));
+      image.put(out.data_ptr());
+      launch(kernels_.norm, 1, image);
+    }
+
+    // The parts from the last to the first, as the pieces of each; the first launch writes a norm that is not known.
+    void scale(const at::Tensor& sums, at::Tensor& norm, bool known, float max_norm, int copies) const {
+      for (size_t i = parts_.size(); i-- > 0;) {
+        const Part& part = parts_[i];
+        Image image = head(part);
+        image.put(known ? nullptr : sums.data_ptr());
+        image.put(static_cast<int32_t>(known ? 0 : sums.numel()));
+        image.put(known ? norm.data_ptr() : nullptr);
+        image.put(!known && i + 1 == parts_.size() ? norm.data_ptr() : nullptr);
+        image.put(max_norm);
+        image.put(static_cast<int32_t>(copies));
+        launch(kernels_.scale[far_], grid(part), image);
+      }
+    }
+
+   private:
+    struct Part {
+      size_t begin, end;                             // entries of one launch
+      uint32_t pieces;
+    };
+
+    uint32_t grid(const Part& part) const { return std::min<uint32_t>(part.pieces, of_.workgroups_); }
+    const void* device_entries(size_t begin) const {
+      return static_cast<const uint8_t*>(list_.data_ptr()) + begin * sizeof(Entry);
+    }
+    void by_value(Image& image, size_t begin, size_t end) const {
+      image.bytes.reserve(of_.by_value_ * sizeof(Entry) + 64);
+      image.bytes.resize(of_.by_value_ * sizeof(Entry));
+      if (end > begin) std::memcpy(image.bytes.data(), &entries_[begin], (end - begin) * sizeof(Entry));
+    }
+    // a part's list, its number of entries, its pieces and the elements of a piece
+    Image head(const Part& part) const {
+      Image image;
+      if (far_) image.put(device_entries(part.begin));
+      else by_value(image, part.begin, part.end);
+      image.put(static_cast<int32_t>(part.end - part.begin));
+      image.put(part.pieces);
+      image.put(static_cast<int32_t>(piece_));
+      return image;
+    }
+    void launch(uint64_t kernel, uint32_t workgroups, const Image& image) const {
+      const int rc = nep_launch_packed(kernel, workgroups, 1, 1, of_.lanes_, 0, stream_, image.bytes.data(),
+                                       image.bytes.size());
+      if (rc != NEP_OK) throw_hip_error(std::string("launch: ") + nep_last_error());
+    }
+
+    const GradientCalls& of_;
+    const Kernels& kernels_;
+    const c10::DeviceGuard guard_;
+    std::vector<Entry>& entries_;
+    const at::TensorOptions options_;
+    const hipStream_t stream_;
+    std::vector<Part> parts_;
+    at::Tensor list_;
+    int piece_ = 1024;
+    bool far_ = false;
   };
 
   static bool plain(const at::Tensor& t) {
@@ -582,7 +684,7 @@ class GradientCalls {
   }
 
   // The tensors of a list or tuple that is not empty: of the three types, on one device, without gaps.
-  static bool collect(const py::handle& list, std::vector<at::Tensor>& out) {
+  bool collect(const py::handle& list, std::vector<const at::Tensor*>& out) const {
     if (!PyList_CheckExact(list.ptr()) && !PyTuple_CheckExact(list.ptr())) return false;
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
     if (n == 0) return false;
@@ -591,13 +693,13 @@ class GradientCalls {
       PyObject* o = PySequence_Fast_GET_ITEM(list.ptr(), i);
       if (!THPVariable_CheckExact(o)) return false;
       const at::Tensor& t = THPVariable_Unpack(o);
-      if (!plain(t) || (!out.empty() && t.device() != out[0].device()) || !t.is_non_overlapping_and_dense())
+      if (!plain(t) || (i != 0 && t.device() != out[0]->device()) || !t.is_non_overlapping_and_dense())
         return false;
       if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf)
         return false;
-      out.push_back(t);
+      out.push_back(&t);
     }
-    return true;
+    return has(out[0]->get_device());
   }
 
   // Whether the elements of two tensors without gaps lie in one order.
@@ -608,29 +710,28 @@ class GradientCalls {
     return true;
   }
 
-  static void add(std::vector<Entry>& entries, const at::Tensor& in, const at::Tensor& out) {
+  static void push(std::vector<Entry>& entries, const at::Tensor& in, const at::Tensor& out) {
     if (in.numel() == 0) return;
     const bool wider = in.scalar_type() != at::kFloat && out.scalar_type() == at::kFloat;
     const uint32_t kind = in.scalar_type() == at::kFloat ? 0 : (in.scalar_type() == at::kBFloat16 ? 1 : 2) + 2 * wider;
     entries.push_back({in.data_ptr(), out.data_ptr(), static_cast<uint64_t>(in.numel()), 0, kind});
   }
+  static uintptr_t bytes_in(const Entry& e) { return e.count * (e.kind == 0 ? 4 : 2); }
+  static uintptr_t bytes_out(const Entry& e) { return e.count * (e.kind == 0 || e.kind > 2 ? 4 : 2); }
 
   // Whether what is written overlaps nothing else that is written or read, but for a tensor that is written
   // where it is read.
-  static bool separate(const std::vector<at::Tensor>& in, const std::vector<at::Tensor>& out) {
+  static bool separate(const std::vector<Entry>& entries) {
     struct Range {
       uintptr_t begin, end;
       bool written;
     };
     std::vector<Range> ranges;
-    auto range = [&](const at::Tensor& t, bool written) {
-      if (t.numel() == 0) return;
-      const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
-      ranges.push_back({begin, begin + t.numel() * t.element_size(), written});
-    };
-    for (size_t i = 0; i < in.size(); ++i) {
-      range(out[i], true);
-      if (out[i].data_ptr() != in[i].data_ptr() || out[i].scalar_type() != in[i].scalar_type()) range(in[i], false);
+    ranges.reserve(2 * entries.size());
+    for (const Entry& e : entries) {
+      const auto in = reinterpret_cast<uintptr_t>(e.in), out = reinterpret_cast<uintptr_t>(e.out);
+      ranges.push_back({out, out + bytes_out(e), true});
+      if (in != out || e.kind > 2) ranges.push_back({in, in + bytes_in(e), false});
     }
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
     uintptr_t any = 0, written = 0;                  // ends of the ranges so far
@@ -642,74 +743,17 @@ class GradientCalls {
     return true;
   }
 
-  static bool inside(const at::Tensor& t, const std::vector<at::Tensor>& all) {
+  static bool inside(const at::Tensor& t, const std::vector<Entry>& entries) {
     const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    for (const at::Tensor& a : all) {
-      const auto begin = reinterpret_cast<uintptr_t>(a.data_ptr());
-      if (at + 4 > begin && at < begin + a.numel() * a.element_size()) return true;
+    for (const Entry& e : entries) {
+      const auto begin = reinterpret_cast<uintptr_t>(e.out);
+      if (at + 4 > begin && at < begin + bytes_out(e)) return true;
     }
     return false;
   }
 
-  // Elements of a piece, and the lists' pieces.  At least one load of each lane, four where the pieces are
-  // many for the workgroups.
-  Pieces deal(std::vector<Entry>& entries) const {
-    Pieces p;
-    uint64_t total = 0;
-    for (const Entry& e : entries) total += e.count;
-    p.piece = lanes_ * 8;
-    while (p.piece < lanes_ * 32 && total / p.piece >= 16ull * workgroups_) p.piece *= 2;
-    for (size_t begin = 0; begin < entries.size(); begin += tensors_) {
-      Part part{begin, std::min(entries.size(), begin + tensors_), 0};
-      uint64_t pieces = 0;
-      for (size_t i = part.begin; i < part.end; ++i) {
-        entries[i].first = static_cast<uint32_t>(pieces);
-        pieces += (entries[i].count + p.piece - 1) / p.piece;
-      }
-      TORCH_CHECK_NOT_IMPLEMENTED(pieces < (1ull << 31), "gradients of more than 2^31 pieces of ", p.piece, " elements");
-      part.pieces = static_cast<uint32_t>(pieces);
-      p.launches.push_back(part);
-    }
-    return p;
-  }
-
-  uint32_t grid(const Part& part) const { return std::min<uint32_t>(part.pieces, workgroups_); }
-
-  void launch(uint64_t kernel, uint32_t workgroups, const Image& image, hipStream_t stream) const {
-    const int rc = nep_launch_packed(kernel, workgroups, 1, 1, lanes_, 0, stream, image.bytes.data(), image.bytes.size());
-    if (rc != NEP_OK) throw_hip_error(std::string("launch: ") + nep_last_error());
-  }
-
-  // One sum for each workgroup of all launches.
-  at::Tensor launch_sums(const std::vector<Entry>& entries, const Pieces& pieces, c10::Device device,
-                         hipStream_t stream) const {
-    int64_t count = 0;
-    for (const Part& part : pieces.launches) count += grid(part);
-    at::Tensor sums = at::empty({count}, at::TensorOptions().device(device).dtype(at::kDouble));
-    double* at = static_cast<double*>(sums.data_ptr());
-    for (const Part& part : pieces.launches) {
-      Image image(entries, part, tensors_, pieces.piece);
-      image.put(at);
-      launch(sums_, grid(part), image, stream);
-      at += grid(part);
-    }
-    return sums;
-  }
-
-  void launch_norm(const std::vector<Entry>& entries, const Pieces& pieces, c10::Device device, hipStream_t stream,
-                   float* out) const {
-    const at::Tensor sums = launch_sums(entries, pieces, device, stream);
-    Image image({}, Part{0, 0, 0}, 0, 0);
-    image.bytes.clear();
-    image.put(sums.data_ptr());
-    image.put(static_cast<int32_t>(sums.numel()));
-    image.align(8);
-    image.put(out);
-    launch(norm_, 1, image, stream);
-  }
-
-  const uint64_t sums_, norm_, scale_;
-  const int tensors_, lanes_, workgroups_;
+  const int by_value_, most_, lanes_, workgroups_;
+  std::unordered_map<int, Kernels> kernels_;
 };
 
 int64_t dtype_code(const at::Tensor& t) { return static_cast<int64_t>(t.scalar_type()); }
@@ -735,8 +779,10 @@ PYBIND11_MODULE(_neptune_dispatch, m) {
            py::arg("buffers"), py::arg("returns"), py::arg("bare"), py::arg("launches"))
       .def("run", &CallPlan::run, py::arg("tensors"));
   py::class_<GradientCalls>(m, "GradientCalls")
-      .def(py::init<uint64_t, uint64_t, uint64_t, int, int, int>(), py::arg("sums"), py::arg("norm"),
-           py::arg("scale"), py::arg("tensors"), py::arg("lanes"), py::arg("workgroups"))
+      .def(py::init<int, int, int, int>(), py::arg("by_value"), py::arg("most"), py::arg("lanes"),
+           py::arg("workgroups"))
+      .def("add", &GradientCalls::add, py::arg("device"), py::arg("kernels"))
+      .def("has", &GradientCalls::has, py::arg("device"))
       .def("norm", &GradientCalls::norm, py::arg("tensors"))
       .def("clip", &GradientCalls::clip, py::arg("tensors"), py::arg("out"), py::arg("given"), py::arg("max_norm"));
   py::class_<CallTable>(m, "CallTable")

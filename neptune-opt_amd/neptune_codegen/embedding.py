@@ -15,10 +15,12 @@ from __future__ import annotations
 import threading
 
 from neptune_codegen import calls, hip
-from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_order_name, embedding_sums_name,
+from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_few_name, embedding_order_name,
+                                      embedding_sums_name, emit_embedding_few_source,
                                       emit_embedding_order_source, emit_embedding_source,
                                       emit_embedding_sums_source)
 
+FEW = 256                # tokens that one launch takes
 MOST_KEYS = 1024         # rows that a workgroup counts the tokens of (nep_embedding.h kMostKeys)
 MOST_STRIDE = 1 << 20
 _PROGRAMS: dict = {}
@@ -29,6 +31,7 @@ _lock = threading.Lock()
 _LOOKUP_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.F32,)
 _ORDER_ARGS = (hip.PTR,) * 4 + (hip.I64,) * 3 + (hip.I32,)
 _SUMS_ARGS = (hip.PTR,) * 6 + (hip.I64, hip.I32) + (hip.I64,) * 3 + (hip.I32,) * 5 + (hip.F32,)
+_FEW_ARGS = (hip.PTR,) * 3 + (hip.I32,) * 2 + (hip.I64,) * 4 + (hip.I32,) * 4 + (hip.F32,)
 _JOIN_ARGS = (hip.PTR,) * 3 + (hip.I64, hip.I32) + (hip.I64,) * 2 + (hip.I32,) * 2 + (hip.F32,)
 
 
@@ -50,6 +53,11 @@ def _order_program(index: str, waves: int) -> hip.Program:
 
 def _sums_program(dtype, out, access: str, add: bool) -> hip.Program:
     return _program(embedding_sums_name("sums", dtype, out, access, add), emit_embedding_sums_source, dtype, out,
+                    access, add)
+
+
+def _few_program(dtype, out, index: str, access: str, add: bool) -> hip.Program:
+    return _program(embedding_few_name(dtype, out, index, access, add), emit_embedding_few_source, dtype, out, index,
                     access, add)
 
 
@@ -196,6 +204,31 @@ def _chunk(count: int, words: int) -> int:
     return chunk
 
 
+def _ordered(given, table, buffers, device, access, add, out, si, sg, st, scale, vocab, chunk, columns, clear,
+             log_lanes, log_tiles):
+    """Launches of a gradient with more than a few tokens; adds their scratch to the buffers."""
+    import torch
+
+    grad, tokens, _ = given
+    n, count, index = grad.shape[-1], tokens.numel(), _name(tokens)
+    log, waves, chunks = _shares(vocab), 16 if count > 1024 else 4, -(-count // chunk)
+    # keys, positions and the rows that are named; parts of runs over several chunks
+    keys, positions, named, parts = (calls.buffer(len(buffers) + i) for i in range(4))
+    buffers += [((count,), torch.int32)] * 2 + [((vocab,), torch.uint8)]
+    buffers.append(((chunks * 2 * 64 * columns * (16 // grad.element_size()),), torch.float32))
+    tag = (_name(grad), str(out), access, add)
+    prog = _sums_program(*tag)
+    launches = [(_order_program(index, waves).kernel(embedding_order_name(index, waves), _ORDER_ARGS, 64 * waves, device),
+                 (1 << log,), (calls.tensor(1), keys, positions, named, count, vocab, si, log)),
+                (prog.kernel(embedding_sums_name("sums", *tag), _SUMS_ARGS, 64, device), (chunks * columns + clear,),
+                 (calls.tensor(0), keys, positions, named, table, parts, count, n, vocab, sg, st, chunk, columns,
+                  chunks * columns, log_lanes, log_tiles, scale))]
+    if chunks > 1:
+        launches.append((prog.kernel(embedding_sums_name("join", *tag), _JOIN_ARGS, 256, device), (chunks, columns),
+                         (keys, parts, table, count, n, vocab, st, chunk, chunks, scale)))
+    return launches
+
+
 def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into=None):
     """Gradient [vocab, n] of the table for the output's gradient `grad` [..., n], in its dtype; or, with
     `into` [vocab, n] in that dtype or float32, the gradient added to `into` in place (one rounding for each
@@ -225,28 +258,22 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
     out = grad.dtype if into is None else into.dtype
     words = -(-n // (16 // grad.element_size()))
     access = _access(n, (g, sg), *([(into, st)] if add else []))
-    log, waves = _shares(vocab), 16 if count > 1024 else 4
-    chunk = _chunk(count, words)
-    chunks, columns = -(-count // chunk), -(-words // 64)
-    # result; keys, positions and the rows that are named; parts of runs over several chunks
-    buffers = [] if add else [((vocab, n), out)]
-    keys, positions, named, parts = (calls.buffer(len(buffers) + i) for i in range(4))
-    buffers += [((count,), torch.int32)] * 2 + [((vocab,), torch.uint8)]
-    buffers.append(((chunks * 2 * 64 * columns * (16 // grad.element_size()),), torch.float32))
-    table = calls.tensor(2) if add else calls.buffer(0)
-    tag = (_name(grad), str(out), access, add)
-    order, prog = embedding_order_name(_name(tokens), waves), _sums_program(*tag)
+    columns = -(-words // 64)
     # wavefronts that clear: four words a lane, of several short rows or a part of a long one
     log_lanes, log_tiles = min(7, (words - 1).bit_length()), (-(-words // 256) - 1).bit_length()
     clear = 0 if add else -(-vocab // (4 * (64 >> log_lanes))) if log_lanes < 7 else vocab << log_tiles
-    launches = [(_order_program(_name(tokens), waves).kernel(order, _ORDER_ARGS, 64 * waves, device), (1 << log,),
-                 (calls.tensor(1), keys, positions, named, count, vocab, si, log)),
-                (prog.kernel(embedding_sums_name("sums", *tag), _SUMS_ARGS, 64, device), (chunks * columns + clear,),
-                 (calls.tensor(0), keys, positions, named, table, parts, count, n, vocab, sg, st, chunk, columns,
-                  chunks * columns, log_lanes, log_tiles, scale))]
-    if chunks > 1:
-        launches.append((prog.kernel(embedding_sums_name("join", *tag), _JOIN_ARGS, 256, device),
-                         (chunks, columns), (keys, parts, table, count, n, vocab, st, chunk, chunks, scale)))
+    buffers = [] if add else [((vocab, n), out)]
+    table = calls.tensor(2) if add else calls.buffer(0)
+    if count <= FEW:
+        few = (_name(grad), str(out), _name(tokens), access, add)
+        launches = [(_few_program(*few).kernel(embedding_few_name(*few), _FEW_ARGS, 256, device),
+                     (count * columns + -(-clear // 4),),
+                     (calls.tensor(1), calls.tensor(0), table, count, n, vocab, si, sg, st, columns, count * columns,
+                      log_lanes, log_tiles, scale))]
+    else:
+        chunk = _chunk(count, words)
+        launches = _ordered(given, table, buffers, device, access, add, out, si, sg, st, scale, vocab, chunk, columns,
+                            clear, log_lanes, log_tiles)
     plan = calls.Plan(device, 3, buffers, () if add else (0,), launches)
     if calls.same(given, used):
         _BACKWARD.keep(given, (vocab, number), plan)

@@ -1006,17 +1006,43 @@ def emit_embedding_sums_source(dtype, out, access: str, add: bool) -> str:
             "chunk, chunks, scale);\n}\n")
 
 
+def embedding_few_name(dtype, out, index: str, access: str, add: bool) -> str:
+    return embedding_sums_name("few", dtype, out, f"{index[0]}{index[3:]}_{access}", add)
+
+
+def emit_embedding_few_source(dtype, out, index: str, access: str, add: bool) -> str:
+    """hiprtc unit of the gradient for up to 256 tokens, nep_embedding.h."""
+    st, ot, ix = dtype_tag(dtype)[1], dtype_tag(out)[1], _INDEX_TYPES[index]
+    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: few tokens' rows\n"
+            + kernel_header("nep_device.h", "nep_embedding.h")
+            + '\nextern "C" __global__ void __launch_bounds__(256) '
+            f"{embedding_few_name(dtype, out, index, access, add)}(const void* tokens, const void* grad, void* table, "
+            "int count, int n, long long vocab, long long stride_i, long long stride_g, long long stride_t, "
+            "int columns, unsigned sums, int log_lanes, int log_tiles, float scale) {\n"
+            f"  nep::embedding_few<{st}, {ot}, {ix}, {EMBEDDING_ACCESS[access]}, {str(add).lower()}>((const {ix}*)tokens, "
+            f"(const {st}::T*)grad, ({ot}::T*)table, count, n, (nep::u32)vocab, stride_i, stride_g, stride_t, columns, "
+            "sums, log_lanes, log_tiles, scale);\n}\n")
+
+
 # ---------------------------------------------------------------- gradients of a whole model
 def emit_gradients_source() -> str:
-    """hiprtc unit of the gradients' sums of squares, norm and scaling, nep_gradients.h."""
+    """hiprtc unit of the gradients' sums of squares, norm and scaling, for short lists by value and long ones
+    ("far") in device memory, nep_gradients.h."""
     bound = 'extern "C" __global__ void __launch_bounds__(1024)'
-    listed = "nep::TensorList list, int count, unsigned pieces, int piece"
-    return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// gradients' norm and scaling\n"
+    text = ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// gradients' norm and scaling\n"
             + kernel_header("nep_device.h", "nep_gradients.h")
-            + f"\n{bound} gradient_sums({listed}, double* sums) {{\n"
-            "  nep::gradient_sums(list, count, pieces, piece, sums);\n}\n"
-            f"{bound} gradient_norm(const double* sums, int count, float* norm) {{\n"
+            + f"\n{bound} gradient_norm(const double* sums, int count, float* norm) {{\n"
             "  nep::gradient_norm(sums, count, norm);\n}\n"
-            f"{bound} gradient_scale({listed}, const double* sums, int n_sums, const float* given, "
-            "float* norm, float max_norm, int copies) {\n"
-            "  nep::gradient_scale(list, count, pieces, piece, sums, n_sums, given, norm, max_norm, copies);\n}\n")
+            f"{bound} gradient_list(nep::TensorList list, int count, nep::TensorEntry* to) {{\n"
+            "  nep::gradient_list(list, count, to);\n}\n")
+    for far in (False, True):
+        tail, flag = ("_far", "true") if far else ("", "false")
+        listed = "const nep::TensorEntry* __restrict__ entries" if far else "nep::TensorList list"
+        entries = "entries" if far else "list.entry"
+        text += (f"{bound} gradient_sums{tail}({listed}, int count, unsigned pieces, int piece, double* sums) {{\n"
+                 f"  nep::gradient_sums<{flag}>({entries}, count, pieces, piece, sums);\n}}\n"
+                 f"{bound} gradient_scale{tail}({listed}, int count, unsigned pieces, int piece, const double* sums, "
+                 "int n_sums, const float* given, float* norm, float max_norm, int copies) {\n"
+                 f"  nep::gradient_scale<{flag}>({entries}, count, pieces, piece, sums, n_sums, given, norm, "
+                 "max_norm, copies);\n}\n")
+    return text

@@ -18,15 +18,19 @@ import threading
 from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.emitters import BASE_OPTIONS, emit_gradients_source
 
-TENSORS = 112            # kTensors and kSumLanes of nep_gradients.h
+TENSORS = 112            # kTensors, kMostTensors and kSumLanes of nep_gradients.h
+MOST_TENSORS = 4096
 LANES = 1024
 WORKGROUPS = 512         # two on a CU
-_LIST = (hip.I64,) * (4 * TENSORS) + (hip.I32,) * 3
-_SUMS_ARGS = _LIST + (hip.PTR,)
-_NORM_ARGS = (hip.PTR, hip.I32, hip.PTR)
-_SCALE_ARGS = _LIST + (hip.PTR, hip.I32, hip.PTR, hip.PTR, hip.F32, hip.I32)
+_HEAD = (hip.I32,) * 3
+_LIST, _FAR = (hip.I64,) * (4 * TENSORS), (hip.PTR,)
+_SCALE = (hip.PTR, hip.I32, hip.PTR, hip.PTR, hip.F32, hip.I32)
+# in the order in which the calls are given them (GradientCalls::add)
+_KERNELS = (("gradient_norm", (hip.PTR, hip.I32, hip.PTR)), ("gradient_list", _LIST + (hip.I32, hip.PTR)),
+            ("gradient_sums", _LIST + _HEAD + (hip.PTR,)), ("gradient_scale", _LIST + _HEAD + _SCALE),
+            ("gradient_sums_far", _FAR + _HEAD + (hip.PTR,)), ("gradient_scale_far", _FAR + _HEAD + _SCALE))
 _PROGRAM = None
-_CALLS: dict = {}
+_CALLS = None
 _OPS: dict = {}
 _lock = threading.Lock()
 
@@ -39,15 +43,15 @@ def _program() -> hip.Program:
         return _PROGRAM
 
 
-def _calls(device: int):
-    found = _CALLS.get(device)
-    if found is None:
+def _calls(device: int | None = None):
+    """The calls in C++, with the kernels of `device` among them."""
+    global _CALLS
+    if _CALLS is None:
+        _CALLS = dispatch.extension().GradientCalls(TENSORS, MOST_TENSORS, LANES, WORKGROUPS)
+    if device is not None and not _CALLS.has(device):
         prog = _program()
-        kernels = [prog.kernel(name, args, LANES, device) for name, args in
-                   (("gradient_sums", _SUMS_ARGS), ("gradient_norm", _NORM_ARGS), ("gradient_scale", _SCALE_ARGS))]
-        found = _CALLS[device] = dispatch.extension().GradientCalls(*(k.handle for k in kernels), TENSORS, LANES,
-                                                                    WORKGROUPS)
-    return found
+        _CALLS.add(device, [prog.kernel(name, args, LANES, device).handle for name, args in _KERNELS])
+    return _CALLS
 
 
 def _dense(t) -> bool:
@@ -104,37 +108,40 @@ def _refuse_written(tensors, out) -> None:
     raise ValueError("clipped gradients must not overlap one another, what is read, or the norm")
 
 
-def _ready(tensors):
-    """The device of a list's first tensor where kernels can be asked for, else None."""
-    import torch
-
+def _refuse_recording() -> None:
     if hip.recording_active():
         raise NotImplementedError("a call with a list of tensors has no launch plan and cannot be recorded")
-    first = tensors[0] if type(tensors) in (list, tuple) and tensors else None
-    return calls.device_index(first) if isinstance(first, torch.Tensor) and first.is_cuda \
-        and not calls.is_metadata(first) else None
 
 
-def _plain(tensors) -> list:
-    return [t.resolve_conj().resolve_neg() if _dense(t) else t.contiguous() for t in tensors]
+def _is_metadata(tensors) -> bool:
+    import torch
+
+    return isinstance(tensors, (list, tuple)) and bool(tensors) and isinstance(tensors[0], torch.Tensor) \
+        and calls.is_metadata(tensors[0])
+
+
+def _plain(tensors, copies: bool):
+    """The tensors without their subclasses; with `copies`, those with gaps (or a sign to come) copied."""
+    import torch
+
+    return None if tensors is None else [
+        ((t if _dense(t) else t.contiguous()).resolve_neg() if copies else t).as_subclass(torch.Tensor)
+        for t in tensors]
 
 
 def run_gradient_norm(tensors):
     """The 2-norm of all the tensors' elements together, fp32 without dimensions, on the current stream."""
     import torch
 
-    device = _ready(tensors)
-    if device is not None:
-        found = _calls(device).norm(tensors)
-        if found is not None:
-            return found
-    metadata = device is None and isinstance(tensors, (list, tuple)) and bool(tensors) and \
-        isinstance(tensors[0], torch.Tensor) and calls.is_metadata(tensors[0])
+    _refuse_recording()
+    found = _calls().norm(tensors)
+    if found is not None:
+        return found
+    metadata = _is_metadata(tensors)
     validate_gradient_inputs(tensors, metadata=metadata)
     if metadata:
         return torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    # (tensors with gaps are copied, subclasses taken as what they are)
-    return _calls(device).norm([t.as_subclass(torch.Tensor) for t in _plain(tensors)])
+    return _calls(calls.device_index(tensors[0])).norm(_plain(tensors, True))
 
 
 def _max_norm(max_norm) -> float:
@@ -149,18 +156,17 @@ def run_clip_gradients(tensors, max_norm: float, *, norm=None, out=None):
     the caller has it already (from run_gradient_norm, or of the shards of several devices)."""
     import torch
 
-    max_norm, device = _max_norm(max_norm), _ready(tensors)
-    if device is not None:
-        found = _calls(device).clip(tensors, out, norm, max_norm)
-        if found is not None:
-            return found
-    metadata = device is None and isinstance(tensors, (list, tuple)) and bool(tensors) and \
-        isinstance(tensors[0], torch.Tensor) and calls.is_metadata(tensors[0])
+    _refuse_recording()
+    max_norm = _max_norm(max_norm)
+    found = _calls().clip(tensors, out, norm, max_norm)
+    if found is not None:
+        return found
+    metadata = _is_metadata(tensors)
     validate_gradient_inputs(tensors, out, norm, metadata=metadata)
     if metadata:
         return torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    lists = [None if ts is None else [t.as_subclass(torch.Tensor) for t in ts] for ts in (tensors, out)]
-    found = _calls(device).clip(*lists, None if norm is None else norm.as_subclass(torch.Tensor), max_norm)
+    found = _calls(calls.device_index(tensors[0])).clip(_plain(tensors, False), _plain(out, False),
+                                                        None if norm is None else _plain([norm], False)[0], max_norm)
     if found is None:
         _refuse_written(tensors, out)
     return found

@@ -41,7 +41,7 @@ LISTS = {
     "empty": [((0,), F32), ((4, 0), BF16)], "some empty": [((0,), F32), ((9,), BF16), ((3, 0), F16), ((1,), F16)],
     "layer": [((96, 96), BF16), ((96,), F32), ((257, 33), BF16), ((31,), F16)],
     "many": [((1 + 37 * i % 101, 3), (F32, BF16, F16)[i % 3]) for i in range(300)],
-    "112": [((5,), BF16)] * 112, "113": [((5,), BF16)] * 113, "224": [((9,), F32)] * 224,
+    "112": [((5,), BF16)] * 112, "113": [((5,), BF16)] * 113, "224": [((9,), F32)] * 224, "4096": [((3,), F16)] * 4096, "4500": [((1 + i % 5,), F32) for i in range(4500)],
     "piece": [((8192,), F32), ((8193,), F32), ((8191,), F32), ((16384,), BF16), ((24577,), F16)],
     "large": [((4096, 2049), BF16), ((5000, 1111), F32), ((3000001,), F16)],
     "larger": [((20000, 4096), BF16), ((70000001,), BF16), ((4097, 4097), F32)],
@@ -106,6 +106,10 @@ def test_any_alignment_order_and_mixed_outputs():
     # with gaps, expanded or named twice: the norm reads what the tensors hold
     ts = [cube[:, :, 1:3], cube[:1, :1, :1, :1].expand(2, 3, 4, 5), cube[0], cube[0], cube[:1].transpose(1, 3)]
     check_norm(CG.run_gradient_norm(ts), ts)
+    ts = [torch._neg_view(base), torch.complex(base, base).conj().imag]     # negated when they are read
+    check_norm(CG.run_gradient_norm(ts), ts)
+    with pytest.raises(ValueError):
+        CG.run_clip_gradients(ts[:1], 1.0)
 
 
 def test_the_ends_of_the_range():

@@ -60,5 +60,6 @@ def test_tensors_without_gaps():
 
 def test_a_launch_fits_its_arguments():
     # 4096 bytes with the 256 that the compiler may add
-    for args in (GR._SUMS_ARGS, GR._SCALE_ARGS):
+    for _, args in GR._KERNELS:
         assert sum(4 if a in (GR.hip.I32, GR.hip.F32) else 8 for a in args) + 16 + 256 <= 4096
+    assert GR.TENSORS * 32 <= 3584 and GR.MOST_TENSORS <= 64 * 64        # two ballots find a tensor
