@@ -20,6 +20,7 @@ namespace nep {
 constexpr int kTensors = 112;                        // 3584 bytes; all arguments stay below 4096
 constexpr int kMostTensors = 4096;
 constexpr int kSumLanes = 1024;
+constexpr int kPieceLanes = 256;                     // lanes that share a piece: a workgroup has four at a time
 
 struct alignas(16) TensorEntry {
   const void* in;
@@ -59,13 +60,20 @@ struct Tensors {
     for (int i = threadIdx.x; i < n; i += kSumLanes) numbers[i] = given[i].first;
     __syncthreads();
   }
-  // Number of the entry that piece p belongs to: the last with a first piece of p or less (the first one is 0).
-  __device__ __forceinline__ int of(u32 p) const {
+  // The entry that piece p (of a wavefront) belongs to: the last with a first piece of p or less (the first has 0).
+  __device__ __forceinline__ TensorEntry entry(u32 p) const {
     const int lane = lane_id(), at = lane * step;
     const u64 low = __builtin_amdgcn_ballot_w64(at < count && firsts[at < count ? at : 0] <= p);
     const int begin = (__builtin_popcountll(low) - 1) * step, i = begin + lane;
     const u64 in = __builtin_amdgcn_ballot_w64(lane < step && i < count && firsts[i < count ? i : 0] <= p);
-    return begin + __builtin_popcountll(in) - 1;
+    const TensorEntry e = entries[begin + __builtin_popcountll(in) - 1];
+    // (the same in every lane, so that addresses are scalar)
+    auto same = [](u64 v) {
+      return (u64)(u32)__builtin_amdgcn_readfirstlane((int)(u32)v) |
+             (u64)(u32)__builtin_amdgcn_readfirstlane((int)(u32)(v >> 32)) << 32;
+    };
+    return {(const void*)same((u64)e.in), (void*)same((u64)e.out), same(e.count),
+            (u32)__builtin_amdgcn_readfirstlane((int)e.first), (u32)__builtin_amdgcn_readfirstlane((int)e.kind)};
   }
 };
 
@@ -88,17 +96,18 @@ __device__ __forceinline__ double workgroup_sum(double v, double* lds) {
   return total;
 }
 
-// Squares of elements [first, end) of p, added to acc.
+// Squares of elements [first, end) of p, added to acc, by kPieceLanes lanes.
 template <class St>
 __device__ __forceinline__ void add_squares(const typename St::T* p, i64 first, i64 end, double& acc) {
   constexpr int VEC = St::kVec, FLIGHT = 4;
+  const int lane = threadIdx.x % kPieceLanes;
   const i64 words = (end - first) / VEC;
   p += first;
-  for (i64 w0 = 0; w0 < words; w0 += kSumLanes * FLIGHT) {
+  for (i64 w0 = 0; w0 < words; w0 += kPieceLanes * FLIGHT) {
     u32x4 w[FLIGHT];
 #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
-      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      const i64 i = w0 + f * kPieceLanes + lane;
       w[f] = i < words ? load16_any_once(p + i * VEC) : u32x4{0u, 0u, 0u, 0u};
     }
 #pragma unroll
@@ -109,7 +118,7 @@ __device__ __forceinline__ void add_squares(const typename St::T* p, i64 first, 
       for (int j = 0; j < VEC; ++j) acc = __builtin_fma((double)v[j], (double)v[j], acc);
     }
   }
-  const i64 rest = words * VEC + threadIdx.x;
+  const i64 rest = words * VEC + lane;
   if (rest < end - first) {
     const double v = (double)St::load(p + rest);
     acc = __builtin_fma(v, v, acc);
@@ -124,8 +133,10 @@ __device__ __forceinline__ void gradient_sums(const TensorEntry* list, int count
   __shared__ u32 numbers[Tensors<FAR>::MOST];
   const Tensors<FAR> tensors(list, count, words, numbers);
   double acc = 0.0;
-  for (u32 p = blockIdx.x; p < pieces; p += gridDim.x) {
-    const TensorEntry e = tensors.entries[tensors.of(p)];
+  constexpr u32 AT_ONCE = kSumLanes / kPieceLanes;
+  const u32 group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieceLanes);
+  for (u32 p = blockIdx.x * AT_ONCE + group; p < pieces; p += gridDim.x * AT_ONCE) {
+    const TensorEntry e = tensors.entry(p);
     const i64 first = (i64)(p - e.first) * piece;
     const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
     if (e.kind == kF32) add_squares<F32>((const float*)e.in, first, end, acc);
@@ -156,14 +167,15 @@ __device__ __forceinline__ void scale_elements(const typename St::T* p, typename
                                                float factor) {
   typedef u32 u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
   constexpr int VEC = Ot::kVec, FLIGHT = St::kVec == VEC ? 4 : 8;
+  const int lane = threadIdx.x % kPieceLanes;
   const i64 words = (end - first) / VEC;
   p += first;
   q += first;
-  for (i64 w0 = 0; w0 < words; w0 += kSumLanes * FLIGHT) {
+  for (i64 w0 = 0; w0 < words; w0 += kPieceLanes * FLIGHT) {
     u32x4 w[FLIGHT];
 #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
-      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      const i64 i = w0 + f * kPieceLanes + lane;
       if (i >= words) continue;
       if constexpr (St::kVec == VEC) {
         w[f] = load16_any_once(p + i * VEC);
@@ -174,7 +186,7 @@ __device__ __forceinline__ void scale_elements(const typename St::T* p, typename
     }
 #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
-      const i64 i = w0 + f * kSumLanes + threadIdx.x;
+      const i64 i = w0 + f * kPieceLanes + lane;
       if (i >= words) continue;
       float v[St::kVec];
       St::unpack(w[f], v);
@@ -183,7 +195,7 @@ __device__ __forceinline__ void scale_elements(const typename St::T* p, typename
       store16_any(q + i * VEC, Ot::pack(v));
     }
   }
-  const i64 rest = words * VEC + threadIdx.x;
+  const i64 rest = words * VEC + lane;
   if (rest < end - first) Ot::store(q + rest, St::load(p + rest) * factor);
 }
 
@@ -200,9 +212,11 @@ __device__ __forceinline__ void gradient_scale(const TensorEntry* list, int coun
   __shared__ u32x4 words[FAR ? 1 : 2 * kTensors];
   __shared__ u32 numbers[Tensors<FAR>::MOST];
   const Tensors<FAR> tensors(list, count, words, numbers);
-  for (u32 i = blockIdx.x; i < pieces; i += gridDim.x) {
+  constexpr u32 AT_ONCE = kSumLanes / kPieceLanes;
+  const u32 group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieceLanes);
+  for (u32 i = blockIdx.x * AT_ONCE + group; i < pieces; i += gridDim.x * AT_ONCE) {
     const u32 p = pieces - 1 - i;
-    const TensorEntry e = tensors.entries[tensors.of(p)];
+    const TensorEntry e = tensors.entry(p);
     if (factor == 1.0f && e.in == e.out) continue;
     const i64 first = (i64)(p - e.first) * piece;
     const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;

@@ -540,6 +540,7 @@ class GradientCalls {
     uint32_t first, kind;
   };
   static_assert(sizeof(Entry) == 32, "the kernels' layout");
+  static constexpr int kPieceLanes = 256;            // as in nep_gradients.h
   struct Kernels {
     uint64_t norm, list, sums[2], scale[2];          // of lists by value, and in device memory
   };
@@ -565,9 +566,8 @@ class GradientCalls {
           stream_(c10::hip::getCurrentHIPStream(device.index()).stream()) {
       uint64_t total = 0;
       for (const Entry& e : entries_) total += e.count;
-      // at least one load of each lane, four where the pieces are many for the workgroups
-      while (piece_ < of.lanes_ * 32 && total / piece_ >= 16ull * of.workgroups_) piece_ *= 2;
-      piece_ = std::max(piece_, of.lanes_ * 8);
+      // two words of a lane (four of 32 bits), up to sixteen where the pieces are many for the workgroups
+      while (piece_ < 32 * kPieceLanes * 4 && total / piece_ >= 64ull * of.workgroups_) piece_ *= 2;
       far_ = entries_.size() > static_cast<size_t>(of.by_value_);
       const size_t most = far_ ? of.most_ : of.by_value_;
       for (size_t begin = 0; begin < entries_.size(); begin += most) {
@@ -641,7 +641,10 @@ class GradientCalls {
       uint32_t pieces;
     };
 
-    uint32_t grid(const Part& part) const { return std::min<uint32_t>(part.pieces, of_.workgroups_); }
+    uint32_t grid(const Part& part) const {
+      const uint32_t at_once = of_.lanes_ / kPieceLanes;
+      return std::min<uint32_t>((part.pieces + at_once - 1) / at_once, of_.workgroups_);
+    }
     const void* device_entries(size_t begin) const {
       return static_cast<const uint8_t*>(list_.data_ptr()) + begin * sizeof(Entry);
     }
@@ -674,7 +677,7 @@ class GradientCalls {
     const hipStream_t stream_;
     std::vector<Part> parts_;
     at::Tensor list_;
-    int piece_ = 1024;
+    int piece_ = 16 * kPieceLanes;
     bool far_ = false;
   };
 
