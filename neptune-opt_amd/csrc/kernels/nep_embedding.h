@@ -462,11 +462,12 @@ __device__ __forceinline__ void embedding_few(const Ix* __restrict__ tokens, con
   const i64 token = tid < count ? (i64)tokens[tid * stride_i] : -1;
   const u32 key = token >= 0 && token < (i64)vocab ? (u32)token : ~0u;
   if constexpr (!ADD) {
-    __shared__ unsigned char named[1024];
+    __shared__ u32 marks[256];                       // a byte for each of 1024 rows
+    unsigned char* named = (unsigned char*)marks;
     if (blockIdx.x >= sums) {
       const u32 block = blockIdx.x - sums, per = 64 >> (log_lanes < 6 ? log_lanes : 6);
       const u32 base = log_lanes < 7 ? block * (WAVES * 4 * per) : block * WAVES >> log_tiles;
-      ((u32*)named)[tid] = 0;
+      marks[tid] = 0;
       __syncthreads();
       if (key - base < 1024) named[key - base] = 1;  // (of at most 16 * 64 rows)
       __syncthreads();

@@ -141,8 +141,49 @@ def _rotary_programs():
                                      ("exchanged", False), ("exchanged", True))]
 
 
+def _quantized_norm_programs():
+    import torch
+
+    from neptune_codegen.residual_norm import _program, _variant
+
+    out = []
+    for rows, n, aligned in ((16384, 4096, True), (64, 4096, True), (8, 1024, True), (5331, 2999, False)):
+        x = torch.empty((rows, n), device="meta", dtype=torch.bfloat16)
+        for after, gate in ((True, "group"), (True, "none"), (False, "none")):
+            var = _variant(x, aligned, rows, n, after, gate, False)
+            out += [_program("quantized", dataclasses.replace(var, out="float8_e4m3fn", block=block, power_of_two=power))
+                    for block, power in ((0, False), (32, True), (128, False))]
+    return out
+
+
+def _embedding_programs():
+    import torch
+
+    from neptune_codegen.embedding import (_few_program, _lookup_program, _lookup_variant, _order_program,
+                                           _sums_program)
+
+    out = [_order_program(index, waves) for index in ("int32", "int64") for waves in (4, 16)]
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        name = str(dtype).replace("torch.", "")
+        for n, access in ((4096, "words"), (1024, "words"), (768, "words"), (1001, "any")):
+            table = torch.empty((1, n), device="meta", dtype=dtype)
+            out += [_lookup_program(_lookup_variant(table, torch.empty(0, device="meta", dtype=index), access, n))
+                    for index in (torch.int32, torch.int64)]
+        for access in ("words", "any"):
+            for into, add in ((name, False), (name, True), ("float32", True)):
+                out += [_sums_program(name, into, access, add), _few_program(name, into, "int64", access, add)]
+    return out
+
+
+def _gradient_programs():
+    from neptune_codegen.gradients import _program
+
+    return [_program()]
+
+
 def programs():
     # (a launch shape that two sizes share is listed once)
     return list(dict.fromkeys(_fold_programs() + _row_programs() + _segment_programs() + _attention_programs()
                               + _attention_backward_programs() + _distill_programs()
-                              + _residual_norm_programs() + _rotary_programs()))
+                              + _residual_norm_programs() + _rotary_programs() + _quantized_norm_programs()
+                              + _embedding_programs() + _gradient_programs()))
