@@ -121,20 +121,21 @@ __device__ __forceinline__ int exclusive_sum(int v, int* lds, int& all) {
 
 // The tokens by (token mod W, token / W), then by position, W = 2^log_shares workgroups: workgroup w has the
 // tokens that are w mod W, and its places are behind those of the workgroups before it.  Each of its wavefronts
-// walks a run of the positions, counts its tokens (and those of earlier workgroups) and lists them; when the
-// counters have become places, the list goes there.  Every workgroup reads all tokens (from L2, a few
-// instructions for 64 of them), and none waits for another.  Frequent tokens, often neighbours, spread over the
-// workgroups; a wavefront whose list is too short walks its run again.
+// walks a run of the positions (of less than 2^22), counts its tokens (and those of earlier workgroups) and lists
+// them; when the counters have become places, the list goes there.  Every workgroup reads all tokens (from L2, a
+// few instructions for 64 of them), and none waits for another.  Frequent tokens, often neighbours, spread over
+// the workgroups; a wavefront whose list is too short walks its run again, and empties it when it is full.
 // `named` gets a byte for each row of the table: whether a token names it.  Places behind the last token
 // have the key `vocab`.
 template <class Ix, int WAVES>
 __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u32* __restrict__ keys,
                                                 u32* __restrict__ positions, unsigned char* __restrict__ named,
                                                 i64 count, u32 vocab, i64 stride_i, int log_shares) {
-  constexpr int THREADS = WAVES * 64, BATCHES = 8, GROUP = 64 * BATCHES, LIST = 512;
+  constexpr int THREADS = WAVES * 64, BATCHES = 4, GROUP = 64 * BATCHES, LIST = 1024;
   __shared__ int counters[WAVES][kMostKeys];
-  __shared__ u32 list_keys[WAVES][LIST], list_positions[WAVES][LIST];
+  __shared__ u32 list[WAVES][LIST];                  // key / W, and the position in the run behind it
   __shared__ int sums[WAVES];
+  static_assert(kMostKeys <= 1 << 10, "32 bits hold an entry");
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const u32 share = blockIdx.x, mask = (1u << log_shares) - 1;
   const int mine = share < vocab ? (int)((vocab - 1 - share) >> log_shares) + 1 : 0;    // keys
@@ -176,7 +177,14 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
       each(i0 + GROUP, b);
     }
   };
-  int earlier = 0, listed = 0;
+  int listed = 0;
+  // a batch's own tokens, to the list
+  auto note = [&](bool own, u64 some, u32 key, i64 position) {
+    const int at = listed + __builtin_amdgcn_mbcnt_hi((u32)(some >> 32), __builtin_amdgcn_mbcnt_lo((u32)some, 0));
+    if (own && at < LIST) list[wave][at] = (key >> log_shares) << 22 | (u32)(position - first);
+    listed += __builtin_popcountll(some);
+  };
+  int earlier = 0;
   walk([&](i64 i0, const Ix* token) {
 #pragma unroll
     for (int b = 0; b < BATCHES; ++b) {
@@ -185,16 +193,10 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
       const bool own = of == share && key != ~0u;
       const u64 some = __builtin_amdgcn_ballot_w64(own);
       if (some == 0) continue;
-      const int at = listed + __builtin_amdgcn_mbcnt_hi((u32)(some >> 32), __builtin_amdgcn_mbcnt_lo((u32)some, 0));
-      if (own) {
+      if (own)
         __hip_atomic_fetch_add(&counters[wave][key >> log_shares], 1, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_WORKGROUP);
-        if (at < LIST) {
-          list_keys[wave][at] = key;
-          list_positions[wave][at] = (u32)(i0 + b * 64 + lane);
-        }
-      }
-      listed += __builtin_popcountll(some);
+      note(own, some, key, i0 + b * 64 + lane);
     }
   });
   int base;
@@ -221,41 +223,50 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
   __syncthreads();
   if (share == mask)
     for (i64 i = base + (int)threadIdx.x; i < count; i += THREADS) keys[i] = vocab;
-  // tokens in order of their positions, to their places
+  // the list's tokens, which are in order of their positions, to their places
   const int bits = mine > 1 ? 32 - __builtin_clz(mine - 1) : 0;
-  auto put = [&](bool own, u32 key, u32 position) {
-    const int k = own ? (int)(key >> log_shares) : 0;
-    u64 same = __builtin_amdgcn_ballot_w64(own);
-    for (int b = 0; b < bits; ++b) {
-      const bool bit = (k >> b) & 1;
-      const u64 set = __builtin_amdgcn_ballot_w64(bit);
-      same &= bit ? set : ~set;
-    }
-    const int before = __builtin_amdgcn_mbcnt_hi((u32)(same >> 32), __builtin_amdgcn_mbcnt_lo((u32)same, 0));
-    if (own) {
-      // (the wavefront's own counters: its reads and writes stay in order)
-      volatile int* counter = &counters[wave][k];
-      const int place = *counter + before;
-      if (before == 0) *counter = place + __builtin_popcountll(same);
-      keys[place] = key;
-      positions[place] = position;
+  auto empty = [&](int count) {
+    for (int l0 = 0; l0 < count; l0 += 64) {
+      const bool here = l0 + lane < count;
+      const u32 entry = here ? list[wave][l0 + lane] : 0;
+      const int k = (int)(entry >> 22);
+      u64 same = __builtin_amdgcn_ballot_w64(here);
+      for (int b = 0; b < bits; ++b) {
+        const bool bit = (k >> b) & 1;
+        const u64 set = __builtin_amdgcn_ballot_w64(bit);
+        same &= bit ? set : ~set;
+      }
+      const int before = __builtin_amdgcn_mbcnt_hi((u32)(same >> 32), __builtin_amdgcn_mbcnt_lo((u32)same, 0));
+      if (here) {
+        // (the wavefront's own counters: its reads and writes stay in order)
+        volatile int* counter = &counters[wave][k];
+        const int place = *counter + before;
+        if (before == 0) *counter = place + __builtin_popcountll(same);
+        keys[place] = (u32)k << log_shares | share;
+        positions[place] = (u32)first + (entry & 0x3fffffu);
+      }
     }
   };
   if (listed <= LIST) {
-    for (int l0 = 0; l0 < listed; l0 += 64) {
-      const bool here = l0 + lane < listed;
-      put(here, here ? list_keys[wave][l0 + lane] : 0, here ? list_positions[wave][l0 + lane] : 0);
-    }
-  } else {
-    walk([&](i64 i0, const Ix* token) {
-#pragma unroll
-      for (int b = 0; b < BATCHES; ++b) {
-        const u32 key = known(token[b]);
-        const bool own = (key & mask) == share && key != ~0u;
-        if (__builtin_amdgcn_ballot_w64(own) != 0) put(own, key, (u32)(i0 + b * 64 + lane));
-      }
-    });
+    empty(listed);
+    return;
   }
+  listed = 0;
+  walk([&](i64 i0, const Ix* token) {
+#pragma unroll
+    for (int b = 0; b < BATCHES; ++b) {
+      const u32 key = known(token[b]);
+      const bool own = (key & mask) == share && key != ~0u;
+      const u64 some = __builtin_amdgcn_ballot_w64(own);
+      if (some == 0) continue;
+      if (listed + 64 > LIST) {
+        empty(listed);
+        listed = 0;
+      }
+      note(own, some, key, i0 + b * 64 + lane);
+    }
+  });
+  empty(listed);
 }
 
 // ---------------------------------------------------------------- sums

@@ -31,6 +31,7 @@ def test_refusals(args, kw, error):
     ((G, I, True), {}, ValueError), ((G, I, 10.0), {}, ValueError), ((G, I.int().float(), 10), {}, TypeError),
     ((G.double(), I, 10), {}, TypeError), ((G, I, 10), {"scale": -math.inf}, ValueError),
     ((G, I, 1 << 31), {}, NotImplementedError),
+    ((meta(1 << 13, 1 << 13, 2), meta(1 << 13, 1 << 13, dtype=torch.int32), 10), {}, NotImplementedError),
     ((G, I, 10), {"into": meta(10, 15)}, ValueError), ((G, I, 10), {"into": meta(11, 16)}, ValueError),
     ((G, I, 10), {"into": meta(10, 16, dtype=torch.float16)}, TypeError),
     ((G.float(), I, 10), {"into": meta(10, 16)}, TypeError), ((G, I, 10), {"into": meta(16, 10).T}, ValueError),
