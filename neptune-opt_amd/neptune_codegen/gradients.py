@@ -131,12 +131,12 @@ def _plain(tensors, copies: bool):
 
 def run_gradient_norm(tensors):
     """The 2-norm of all the tensors' elements together, fp32 without dimensions, on the current stream."""
-    import torch
-
     _refuse_recording()
-    found = _calls().norm(tensors)
+    found = (_CALLS or _calls()).norm(tensors)
     if found is not None:
         return found
+    import torch
+
     metadata = _is_metadata(tensors)
     validate_gradient_inputs(tensors, metadata=metadata)
     if metadata:
@@ -154,13 +154,13 @@ def run_clip_gradients(tensors, max_norm: float, *, norm=None, out=None):
     """Scales the tensors to a common norm of at most `max_norm`, in place or into the tensors `out` (a copy,
     where the factor is 1), and returns their norm before, fp32 without dimensions.  `norm` is that norm where
     the caller has it already (from run_gradient_norm, or of the shards of several devices)."""
-    import torch
-
     _refuse_recording()
     max_norm = _max_norm(max_norm)
-    found = _calls().clip(tensors, out, norm, max_norm)
+    found = (_CALLS or _calls()).clip(tensors, out, norm, max_norm)
     if found is not None:
         return found
+    import torch
+
     metadata = _is_metadata(tensors)
     validate_gradient_inputs(tensors, out, norm, metadata=metadata)
     if metadata:

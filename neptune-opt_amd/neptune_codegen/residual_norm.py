@@ -194,10 +194,14 @@ BLOCKS = (32, 64, 128)
 _FORMATS = ("float8_e4m3fn", "float8_e5m2", "int8")
 
 
+_CODES: dict = {None: 0}     # of the types seen so far
+
+
 def _format(dtype) -> str:
     name = str(dtype).replace("torch.", "")
     if name not in _FORMATS:
         raise TypeError(f"residual norm's 8-bit outputs are {', '.join(_FORMATS)}, got {dtype}")
+    _CODES[dtype] = _FORMATS.index(name)
     return name
 
 
@@ -226,15 +230,16 @@ def run_residual_norm_quantized(x, y, gamma_after, gamma_before, *, gate=None, r
     type's largest value, or with `power_of_two` the least power of two that is no less, at least 2^-126 (0
     stays 0); values are rounded half to even.  Where a row or group holds an infinity or NaN, its scale is not
     finite.  The gradient is straight through: run_residual_norm_backward, with the rates."""
-    import torch
-
     given, return_stats, power_of_two = (x, y, gamma_after, gamma_before, gate), bool(return_stats), bool(power_of_two)
-    dtype = torch.float8_e4m3fn if dtype is None else dtype
-    out, block = _format(dtype), _block(group)
-    numbers = (residual_scale, eps, return_stats, _FORMATS.index(out), block, power_of_two)
+    numbers = (residual_scale, eps, return_stats, _CODES.get(dtype, ""), group, power_of_two)   # ("" has no key)
     found = _QUANTIZED.run(given, numbers)
     if found is not None:
         return found
+    import torch
+
+    dtype = torch.float8_e4m3fn if dtype is None else dtype
+    out, block = _format(dtype), _block(group)
+    numbers = (residual_scale, eps, return_stats, _CODES[dtype], group, power_of_two)
     metadata = isinstance(x, torch.Tensor) and calls.is_metadata(x)
     groups, group_rows = validate_residual_norm_inputs(*given, metadata=metadata)
     scale, eps = _scale(residual_scale), _eps(eps)

@@ -229,6 +229,20 @@ def test_captured_replays_and_the_registered_operator():
         assert all(same(a, b) for a, b in zip(out, ref)), i
 
 
+def test_a_seen_layout_does_not_lend_its_type():
+    dev = _dev()
+    x, g = torch.randn(4, 64, device=dev), torch.ones(64, device=dev)
+    values = [CG.run_residual_norm_quantized(x, x, None, g, **kw)[1] for kw in ({}, {"dtype": E4}, {"dtype": E5}, {"dtype": I8}) * 2]
+    assert [v.dtype for v in values] == [E4, E4, E5, I8] * 2
+    for kw in ({"dtype": torch.float16}, {"dtype": "float8_e4m3fn"}, {"dtype": 0}):
+        with pytest.raises(TypeError):
+            CG.run_residual_norm_quantized(x, x, None, g, **kw)
+    CG.run_residual_norm_quantized(x, x, None, g, group=32)
+    for group in (32.0, True, 33):
+        with pytest.raises(ValueError):
+            CG.run_residual_norm_quantized(x, x, None, g, group=group)
+
+
 def test_no_rows():
     dev = _dev()
     x, g = torch.empty(0, 64, dtype=torch.bfloat16, device=dev), torch.ones(64, dtype=torch.bfloat16, device=dev)
