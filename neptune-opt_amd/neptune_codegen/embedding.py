@@ -20,8 +20,9 @@ from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_
                                       emit_embedding_order_source, emit_embedding_source,
                                       emit_embedding_sums_source)
 
-FEW = 256                # tokens that one launch takes
+FEW = 512                # tokens that one launch takes (nep_embedding.h kFewTokens)
 MOST_TOKENS = 1 << 26    # of a gradient: sixteen wavefronts' runs of 2^22
+MOST_ROWS = 1 << 24      # (each thousand rows have a workgroup that reads all tokens)
 MOST_KEYS = 1024         # rows that a workgroup counts the tokens of (nep_embedding.h kMostKeys)
 MOST_STRIDE = 1 << 20
 _PROGRAMS: dict = {}
@@ -111,8 +112,8 @@ def validate_embedding_gradient_inputs(grad, tokens, vocab, into=None, *, metada
                          f"got {tuple(tokens.shape)}")
     n = grad.shape[-1]
     _check_sizes(tokens, vocab, n)
-    if tokens.numel() >= MOST_TOKENS:
-        raise NotImplementedError("embedding's gradient takes less than 2^26 tokens")
+    if tokens.numel() >= MOST_TOKENS or vocab > MOST_ROWS:
+        raise NotImplementedError("embedding's gradient takes less than 2^26 tokens, and up to 2^24 rows")
     if into is None:
         return
     calls.check_tensor(into, "embedding into", metadata=metadata)

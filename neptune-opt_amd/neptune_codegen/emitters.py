@@ -1011,7 +1011,7 @@ def embedding_few_name(dtype, out, index: str, access: str, add: bool) -> str:
 
 
 def emit_embedding_few_source(dtype, out, index: str, access: str, add: bool) -> str:
-    """hiprtc unit of the gradient for up to 256 tokens, nep_embedding.h."""
+    """hiprtc unit of the gradient for few tokens, nep_embedding.h."""
     st, ot, ix = dtype_tag(dtype)[1], dtype_tag(out)[1], _INDEX_TYPES[index]
     return ("// AUTO-GENERATED by neptune_codegen (HIP emitter) -- do not edit.\n// embedding: few tokens' rows\n"
             + kernel_header("nep_device.h", "nep_embedding.h")

@@ -144,15 +144,14 @@ def _rotary_programs():
 def _quantized_norm_programs():
     import torch
 
-    from neptune_codegen.residual_norm import _program, _variant
+    from neptune_codegen.residual_norm import _program, _quantized_variant
 
     out = []
     for rows, n, aligned in ((16384, 4096, True), (64, 4096, True), (8, 1024, True), (5331, 2999, False)):
         x = torch.empty((rows, n), device="meta", dtype=torch.bfloat16)
         for after, gate in ((True, "group"), (True, "none"), (False, "none")):
-            var = _variant(x, aligned, rows, n, after, gate, False)
-            out += [_program("quantized", dataclasses.replace(var, out="float8_e4m3fn", block=block, power_of_two=power))
-                    for block, power in ((0, False), (32, True), (128, False))]
+            out += [_program("quantized", _quantized_variant(x, aligned, rows, n, after, gate, "float8_e4m3fn", *kind))
+                    for kind in ((0, False), (32, True), (128, False))]
     return out
 
 

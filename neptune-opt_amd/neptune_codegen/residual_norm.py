@@ -211,6 +211,21 @@ def _block(group) -> int:
     return group or 0
 
 
+def _quantized_variant(x, aligned: bool, rows: int, n: int, after: bool, gate_kind: str, out: str, block: int,
+                       power_of_two: bool) -> ResidualNormVariant:
+    """The forward pass's lanes, but where the rows fill the chip, the two to five slots a lane that leave the
+    fewest lanes without columns (of equal ones the most slots).  With gamma_after and a gate per group, bf16 2464 x
+    8773 36.6 us by five slots, 50.2 by two; 1568 x 12544 34.1 by four, 42.7; 16384 x 4095 101 by four, 118; fp16
+    5331 x 2999 25.0 by three, 30.2; bf16 16384 x 4096 82.6 by four, 82.9 by two."""
+    var = _variant(x, aligned, rows, n, after, gate_kind, False)
+    slots = -(-n // (16 // x.element_size()))
+    if rows >= 4 * CUS and slots >= 128:
+        lanes = {nv: 1 << (-(-slots // nv) - 1).bit_length() for nv in (2, 3, 4, 5)}
+        nv = min((nv for nv in lanes if lanes[nv] <= 1024), key=lambda k: (lanes[k] * k, -k))
+        var = dataclasses.replace(var, tpr=lanes[nv], nv=nv, wg=max(256, lanes[nv]))
+    return dataclasses.replace(var, out=out, block=block, power_of_two=power_of_two)
+
+
 def _quantized_outputs(x, dtype, block: int, return_stats: bool):
     import torch
 
@@ -249,8 +264,8 @@ def run_residual_norm_quantized(x, y, gamma_after, gamma_before, *, gate=None, r
     n = x.shape[-1]
     rows = x.numel() // n
     used, strides, aligned = _operands((x, y), (gamma_after, gamma_before, gate), n)
-    var = _variant(x, aligned, rows, n, gamma_after is not None, _gate_kind(groups, group_rows), False)
-    var = dataclasses.replace(var, out=out, block=block, power_of_two=power_of_two)
+    var = _quantized_variant(x, aligned, rows, n, gamma_after is not None, _gate_kind(groups, group_rows), out, block,
+                             power_of_two)
     device = calls.device_index(x)
     kernel = _program("quantized", var).kernel(residual_norm_kernel_name("quantized", var), _QUANTIZED_ARGS, var.wg,
                                                device)

@@ -30,7 +30,7 @@ def test_refusals(args, kw, error):
     ((meta(2, 16), I, 10), {}, ValueError), ((meta(2, 3, 0), I, 10), {}, ValueError), ((G, I, 0), {}, ValueError),
     ((G, I, True), {}, ValueError), ((G, I, 10.0), {}, ValueError), ((G, I.int().float(), 10), {}, TypeError),
     ((G.double(), I, 10), {}, TypeError), ((G, I, 10), {"scale": -math.inf}, ValueError),
-    ((G, I, 1 << 31), {}, NotImplementedError),
+    ((G, I, 1 << 31), {}, NotImplementedError), ((G, I, (1 << 24) + 1), {}, NotImplementedError),
     ((meta(1 << 13, 1 << 13, 2), meta(1 << 13, 1 << 13, dtype=torch.int32), 10), {}, NotImplementedError),
     ((G, I, 10), {"into": meta(10, 15)}, ValueError), ((G, I, 10), {"into": meta(11, 16)}, ValueError),
     ((G, I, 10), {"into": meta(10, 16, dtype=torch.float16)}, TypeError),

@@ -107,7 +107,7 @@ def test_lookup(count, vocab, n, dtype):
     (1023, 511, 96, "past"), (1024, 512, 32, "one"), (1025, 513, 40, "one"), (1025, 2000, 33, "past"),
     (4096, 100000, 24, "zipf"), (4097, 300000, 17, "zipf"), (4097, 5, 130, "few"), (9000, 9000, 16, "distinct"),
     (12288, 70, 64, "past"), (12289, 31, 5, "one"), (777, 50, 2048, "few"), (64, 10, 16384, "few"), (50, 20, 20011, "zipf"),
-    (300, 10, 64, "none"), (40000, 50000, 8, "one"), (300000, 131072, 3, "few"), (300000, 2000, 2, "zipf"), (256, 300, 48, "zipf"), (255, 7, 1000, "past"), (256, 3000, 9, "one"), (257, 40, 520, "few"),
+    (300, 10, 64, "none"), (512, 90, 40, "zipf"), (511, 5000, 96, "past"), (513, 90, 40, "zipf"), (40000, 50000, 8, "one"), (300000, 131072, 3, "few"), (300000, 2000, 2, "zipf"), (256, 300, 48, "zipf"), (255, 7, 1000, "past"), (256, 3000, 9, "one"), (257, 40, 520, "few"),
     (200, 5000, 2048, "zipf"), (30, 70000, 24, "distinct"), (100, 2000, 513, "none"), (3, 1000, 5000, "past"), (20000, 32003, 101, "zipf"), (70000, 100, 8, "zipf")])
 def test_gradient(count, vocab, n, kind, dtype):
     dev = _dev()

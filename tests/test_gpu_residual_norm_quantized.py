@@ -3,8 +3,8 @@
 Tolerances.  The normed value h before its rounding is that of run_residual_norm: within 2^-16 of its terms' sizes
 (tests/test_gpu_residual_norm.py).  A scale is the largest of them over the format's largest value: within 2^-16 of
 the block's largest size, and an fp32 quotient (2^-23).  A value q is h / scale (a reciprocal, a product and a step from it, 2^-22),
-rounded: off by that, and by half a step of the format at h / scale.  With fp32 inputs h is what run_residual_norm
-returns, and scales and values are to the bit the quotient, reciprocal, product and step.
+rounded: off by that, and by half a step of the format at h / scale.  With fp32 inputs h is two products from the
+residual and the rate, and scales and values are to the bit the quotient, reciprocal, product and step.
 """
 import math
 
@@ -93,9 +93,8 @@ def check(t, dev, fmt, group, power, scale=0.5):
     assert ((values - ratio).abs() <= allowed).all()
     assert values.abs().max() <= MOST[fmt]
     if t["x"].dtype == torch.float32:
-        plain = CG.run_residual_norm(*args, **kw, return_stats=True)
-        assert torch.equal(r, plain[0]) and torch.equal(stats, plain[2])
-        hf = blocks(plain[1], group)
+        # (the residual is not rounded, and normed two products from it)
+        hf = blocks(r * stats[..., 1:] * d["before"], group)
         # quotients in 64 bits, then rounded, are those of fp32 (on the device torch divides by a number as it
         # multiplies by its reciprocal)
         if not power:
@@ -116,7 +115,8 @@ def check(t, dev, fmt, group, power, scale=0.5):
     ((4, 33), 1024, True, (4, 1)), ((700,), 96, True, ()), ((2, 3, 5), 333, True, (2, 3, 1)), ((5,), 8, False, None),
     ((1, 130), 4096, True, (1, 1)), ((1100,), 4096, False, None), ((40,), 2999, False, (40,)), ((1100,), 2999, True, None),
     ((5,), 8192, True, (5,)), ((2, 3), 16384, True, (2, 1)), ((3,), 10007, True, ()), ((600, 2), 128, True, (600, 1)),
-    ((1000,), 16, False, ()), ((17,), 40, True, None)])
+    ((1000,), 16, False, ()), ((17,), 40, True, None), ((1030,), 8773, True, (1030,)), ((1050,), 1110, True, ()),
+    ((1025,), 12544, False, None), ((1024,), 721, True, None)])
 def test_values_and_scales(lead, n, after, gate, dtype):
     dev = _dev()
     t = make(lead, n, dtype, after, gate, seed=n)

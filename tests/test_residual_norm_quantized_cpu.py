@@ -1,5 +1,4 @@
 """The residual norm's 8-bit output without a GPU: refusals, metadata calls, launch shapes."""
-import dataclasses
 import math
 
 import pytest
@@ -54,12 +53,17 @@ def test_metadata_calls():
 
 
 def test_blocks_lie_in_slots():
-    # (what the kernel asserts when it is compiled)
-    for n in (1, 7, 8, 31, 40, 200, 1000, 2048, 2999, 4096, 8192, 10007, 16384):
+    # (what the kernel asserts when it is compiled), and lanes hold every column
+    for n in (1, 7, 8, 31, 40, 200, 721, 1000, 1110, 2048, 2999, 4095, 4096, 7479, 8192, 8773, 10007, 12544, 16384):
         for dtype in (torch.float32, torch.bfloat16):
-            for rows in (1, 100000):
+            for rows in (1, 1023, 1024, 100000):
                 vec = 16 // meta(1, dtype=dtype).element_size()
-                var = RN._variant(meta(rows, n, dtype=dtype), n % 8 == 0, rows, n, True, "none", False)
-                for block in RN.BLOCKS:
-                    assert min(block // vec, var.tpr) <= 64 and (var.nv == 1 or var.tpr * vec % block == 0)
-                    assert dataclasses.replace(var, out="int8", block=block).tag() != var.tag()
+                tags = set()
+                for block in (0, *RN.BLOCKS):
+                    var = RN._quantized_variant(meta(rows, n, dtype=dtype), n % 8 == 0, rows, n, True, "none", "int8",
+                                                block, False)
+                    assert var.tpr * var.nv * vec >= n and var.tpr <= var.wg <= 1024 and var.wg % var.tpr == 0
+                    assert not block or (min(block // vec, var.tpr) <= 64
+                                         and (var.nv == 1 or var.tpr * vec % block == 0))
+                    tags.add(var.tag())
+                assert len(tags) == 4
