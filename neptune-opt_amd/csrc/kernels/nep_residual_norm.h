@@ -165,6 +165,8 @@ __device__ __forceinline__ void row_sums(float* v, float* lds) {
 //   scale = max|h| / M, M the format's largest value, or the least power of two that is no less (POWER),
 // and at least 2^-126, the least normal number; q = h / scale rounded to the format, half to even.  A block
 // with an infinity or NaN has that for a scale, so that scale q is not finite in any of its columns.
+// Seven bytes an element in 16 bits, as the forward pass's eight HBM-bound: bf16 16384 x 4096 gated 79.8 us (5.9
+// TB/s), fp16 5331 x 2999 in blocks of 32 20.2 (5.6).
 constexpr int kSameType = 0, kE4M3 = 1, kE5M2 = 2, kInt8 = 3;
 
 template <int FORMAT>

@@ -621,15 +621,14 @@ class GradientCalls {
       launch(kernels_.norm, 1, image);
     }
 
-    // The parts from the last to the first, as the pieces of each; the first launch writes a norm that is not known.
+    // The first launch writes a norm that is not known.
     void scale(const at::Tensor& sums, at::Tensor& norm, bool known, float max_norm, int copies) const {
-      for (size_t i = parts_.size(); i-- > 0;) {
-        const Part& part = parts_[i];
+      for (const Part& part : parts_) {
         Image image = head(part);
         image.put(known ? nullptr : sums.data_ptr());
         image.put(static_cast<int32_t>(known ? 0 : sums.numel()));
         image.put(known ? norm.data_ptr() : nullptr);
-        image.put(!known && i + 1 == parts_.size() ? norm.data_ptr() : nullptr);
+        image.put(!known && part.begin == 0 ? norm.data_ptr() : nullptr);
         image.put(max_norm);
         image.put(static_cast<int32_t>(copies));
         launch(kernels_.scale[far_], copies ? grid(part, kShort) : grid(part), image);

@@ -238,7 +238,8 @@ def run_residual_norm_quantized(x, y, gamma_after, gamma_before, *, gate=None, r
                                 eps: float = 1e-6, dtype=None, group: int | None = None,
                                 power_of_two: bool = False, return_stats: bool = False):
     """(residual, values, scales) on the current stream: run_residual_norm with the second result in 8 bits,
-    for an 8-bit matrix product, normed ~ values * scales, and with `return_stats` the rates as a fourth.
+    for an 8-bit matrix product, normed ~ values * scales, and with `return_stats` the rates as a fourth (its row
+    sums run in another order for some shapes).
 
     `dtype` is torch.float8_e4m3fn (the default), float8_e5m2 or int8; `scales` [..., 1] in fp32 has one number
     per row, or [..., ceil(n / group)] one per `group` (32, 64 or 128) columns: the largest magnitude over the
