@@ -22,7 +22,8 @@ namespace nep {
 constexpr int kTensors = 112;                        // 3584 bytes; all arguments stay below 4096
 constexpr int kMostTensors = 4096;
 constexpr int kSumLanes = 1024;
-constexpr int kPieceLanes = 256;                     // lanes that share a piece: a workgroup has four at a time
+constexpr int kPieceLanes = 256;                     // lanes that share a piece
+constexpr u32 kAtOnce = kSumLanes / kPieceLanes;     // pieces that a workgroup has at a time
 
 struct alignas(16) TensorEntry {
   const void* in;
@@ -127,6 +128,21 @@ __device__ __forceinline__ void add_squares(const typename St::T* p, i64 first, 
   }
 }
 
+// The squares of the pieces first, first + step, ...: a lane's share.
+template <class List>
+__device__ __forceinline__ double piece_squares(const List& tensors, u32 first, u32 step, u32 pieces, int piece) {
+  double acc = 0.0;
+  for (u32 p = first; p < pieces; p += step) {
+    const TensorEntry e = tensors.entry(p);
+    const i64 from = (i64)(p - e.first) * piece;
+    const i64 end = from + piece < (i64)e.count ? from + piece : (i64)e.count;
+    if (e.kind == kF32) add_squares<F32>((const float*)e.in, from, end, acc);
+    else if (e.kind == kBF16 || e.kind == kBF16ToF32) add_squares<BF16>((const u16*)e.in, from, end, acc);
+    else add_squares<F16>((const _Float16*)e.in, from, end, acc);
+  }
+  return acc;
+}
+
 template <bool FAR>
 __device__ __forceinline__ void gradient_sums(const TensorEntry* list, int count, u32 pieces, int piece,
                                               double* __restrict__ sums) {
@@ -134,17 +150,8 @@ __device__ __forceinline__ void gradient_sums(const TensorEntry* list, int count
   __shared__ u32x4 words[FAR ? 1 : 2 * kTensors];
   __shared__ u32 numbers[Tensors<FAR>::MOST];
   const Tensors<FAR> tensors(list, count, words, numbers);
-  double acc = 0.0;
-  constexpr u32 AT_ONCE = kSumLanes / kPieceLanes;
   const u32 group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieceLanes);
-  for (u32 p = blockIdx.x * AT_ONCE + group; p < pieces; p += gridDim.x * AT_ONCE) {
-    const TensorEntry e = tensors.entry(p);
-    const i64 first = (i64)(p - e.first) * piece;
-    const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
-    if (e.kind == kF32) add_squares<F32>((const float*)e.in, first, end, acc);
-    else if (e.kind == kBF16 || e.kind == kBF16ToF32) add_squares<BF16>((const u16*)e.in, first, end, acc);
-    else add_squares<F16>((const _Float16*)e.in, first, end, acc);
-  }
+  const double acc = piece_squares(tensors, blockIdx.x * kAtOnce + group, gridDim.x * kAtOnce, pieces, piece);
   const double total = workgroup_sum(acc, lds);
   if (threadIdx.x == 0) sums[blockIdx.x] = total;
 }
@@ -201,6 +208,27 @@ __device__ __forceinline__ void scale_elements(const typename St::T* p, typename
   if (rest < end - first) Ot::store(q + rest, St::load(p + rest) * factor);
 }
 
+__device__ __forceinline__ float factor_of(float norm, float max_norm) {
+  return is_finite(norm) && norm > max_norm ? div_rn(max_norm, norm) : 1.0f;
+}
+
+// The pieces first, first + step, ... times `factor`.
+template <class List>
+__device__ __forceinline__ void scale_pieces(const List& tensors, u32 first, u32 step, u32 pieces, int piece,
+                                             float factor) {
+  for (u32 p = first; p < pieces; p += step) {
+    const TensorEntry e = tensors.entry(p);
+    if (factor == 1.0f && e.in == e.out) continue;
+    const i64 from = (i64)(p - e.first) * piece;
+    const i64 end = from + piece < (i64)e.count ? from + piece : (i64)e.count;
+    if (e.kind == kF32) scale_elements<F32, F32>((const float*)e.in, (float*)e.out, from, end, factor);
+    else if (e.kind == kBF16) scale_elements<BF16, BF16>((const u16*)e.in, (u16*)e.out, from, end, factor);
+    else if (e.kind == kF16) scale_elements<F16, F16>((const _Float16*)e.in, (_Float16*)e.out, from, end, factor);
+    else if (e.kind == kBF16ToF32) scale_elements<BF16, F32>((const u16*)e.in, (float*)e.out, from, end, factor);
+    else scale_elements<F16, F32>((const _Float16*)e.in, (float*)e.out, from, end, factor);
+  }
+}
+
 // `sums` null: the norm is given.  `copies`: whether an entry's out is not its in.
 template <bool FAR>
 __device__ __forceinline__ void gradient_scale(const TensorEntry* list, int count, u32 pieces, int piece,
@@ -209,24 +237,29 @@ __device__ __forceinline__ void gradient_scale(const TensorEntry* list, int coun
                                                float max_norm, int copies) {
   const float norm = sums != nullptr ? norm_of(sums, n_sums) : *given;
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-  const float factor = is_finite(norm) && norm > max_norm ? div_rn(max_norm, norm) : 1.0f;
+  const float factor = factor_of(norm, max_norm);
   if (factor == 1.0f && !copies) return;
   __shared__ u32x4 words[FAR ? 1 : 2 * kTensors];
   __shared__ u32 numbers[Tensors<FAR>::MOST];
   const Tensors<FAR> tensors(list, count, words, numbers);
-  constexpr u32 AT_ONCE = kSumLanes / kPieceLanes;
   const u32 group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieceLanes);
-  for (u32 p = blockIdx.x * AT_ONCE + group; p < pieces; p += gridDim.x * AT_ONCE) {
-    const TensorEntry e = tensors.entry(p);
-    if (factor == 1.0f && e.in == e.out) continue;
-    const i64 first = (i64)(p - e.first) * piece;
-    const i64 end = first + piece < (i64)e.count ? first + piece : (i64)e.count;
-    if (e.kind == kF32) scale_elements<F32, F32>((const float*)e.in, (float*)e.out, first, end, factor);
-    else if (e.kind == kBF16) scale_elements<BF16, BF16>((const u16*)e.in, (u16*)e.out, first, end, factor);
-    else if (e.kind == kF16) scale_elements<F16, F16>((const _Float16*)e.in, (_Float16*)e.out, first, end, factor);
-    else if (e.kind == kBF16ToF32) scale_elements<BF16, F32>((const u16*)e.in, (float*)e.out, first, end, factor);
-    else scale_elements<F16, F32>((const _Float16*)e.in, (float*)e.out, first, end, factor);
-  }
+  scale_pieces(tensors, blockIdx.x * kAtOnce + group, gridDim.x * kAtOnce, pieces, piece, factor);
+}
+
+// A short list of few elements by one workgroup: the norm, and where `scale` is set the scaling behind it.
+__device__ __forceinline__ void gradient_one(const TensorEntry* list, int count, u32 pieces, int piece,
+                                             float* __restrict__ norm_out, float max_norm, int scale, int copies) {
+  __shared__ double lds[kSumLanes / 64];
+  __shared__ u32x4 words[2 * kTensors];
+  __shared__ u32 numbers[kTensors];
+  const Tensors<false> tensors(list, count, words, numbers);
+  const u32 group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPieceLanes);
+  // (the sum's barrier is behind all reads)
+  const float norm = (float)__builtin_sqrt(workgroup_sum(piece_squares(tensors, group, kAtOnce, pieces, piece), lds));
+  if (threadIdx.x == 0) *norm_out = norm;
+  const float factor = factor_of(norm, max_norm);
+  if (!scale || (factor == 1.0f && !copies)) return;
+  scale_pieces(tensors, group, kAtOnce, pieces, piece, factor);
 }
 
 }  // namespace nep

@@ -1034,7 +1034,10 @@ def emit_gradients_source() -> str:
             + f"\n{bound} gradient_norm(const double* sums, int count, float* norm) {{\n"
             "  nep::gradient_norm(sums, count, norm);\n}\n"
             f"{bound} gradient_list(nep::TensorList list, int count, nep::TensorEntry* to) {{\n"
-            "  nep::gradient_list(list, count, to);\n}\n")
+            "  nep::gradient_list(list, count, to);\n}\n"
+            f"{bound} gradient_one(nep::TensorList list, int count, unsigned pieces, int piece, float* norm, "
+            "float max_norm, int scale, int copies) {\n"
+            "  nep::gradient_one(list.entry, count, pieces, piece, norm, max_norm, scale, copies);\n}\n")
     for far in (False, True):
         tail, flag = ("_far", "true") if far else ("", "false")
         listed = "const nep::TensorEntry* __restrict__ entries" if far else "nep::TensorList list"

@@ -28,7 +28,8 @@ _SCALE = (hip.PTR, hip.I32, hip.PTR, hip.PTR, hip.F32, hip.I32)
 # in the order in which the calls are given them (GradientCalls::add)
 _KERNELS = (("gradient_norm", (hip.PTR, hip.I32, hip.PTR)), ("gradient_list", _LIST + (hip.I32, hip.PTR)),
             ("gradient_sums", _LIST + _HEAD + (hip.PTR,)), ("gradient_scale", _LIST + _HEAD + _SCALE),
-            ("gradient_sums_far", _FAR + _HEAD + (hip.PTR,)), ("gradient_scale_far", _FAR + _HEAD + _SCALE))
+            ("gradient_sums_far", _FAR + _HEAD + (hip.PTR,)), ("gradient_scale_far", _FAR + _HEAD + _SCALE),
+            ("gradient_one", _LIST + _HEAD + (hip.PTR, hip.F32, hip.I32, hip.I32)))
 _PROGRAM = None
 _CALLS = None
 _OPS: dict = {}

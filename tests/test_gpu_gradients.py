@@ -42,6 +42,7 @@ LISTS = {
     "layer": [((96, 96), BF16), ((96,), F32), ((257, 33), BF16), ((31,), F16)],
     "many": [((1 + 37 * i % 101, 3), (F32, BF16, F16)[i % 3]) for i in range(300)],
     "112": [((5,), BF16)] * 112, "113": [((5,), BF16)] * 113, "224": [((9,), F32)] * 224, "4096": [((3,), F16)] * 4096, "4500": [((1 + i % 5,), F32) for i in range(4500)],
+    "64 KB": [((16384,), F32)], "over 64 KB": [((16384,), F32), ((1,), F16)], "16 pieces": [((4096 * 3 + 5,), F16), ((4096,), BF16)],
     "piece": [((8192,), F32), ((8193,), F32), ((8191,), F32), ((16384,), BF16), ((24577,), F16)],
     "large": [((4096, 2049), BF16), ((5000, 1111), F32), ((3000001,), F16)],
     "larger": [((20000, 4096), BF16), ((70000001,), BF16), ((4097, 4097), F32)],
