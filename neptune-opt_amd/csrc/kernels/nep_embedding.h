@@ -99,6 +99,7 @@ __device__ __forceinline__ void embedding(const Ix* __restrict__ tokens, const t
 
 // ---------------------------------------------------------------- tokens in order
 constexpr int kMostKeys = 1024;                      // rows of the table that a workgroup counts
+constexpr int kMostTokenStride = 16;
 
 // Sums of the lanes before each lane, over the workgroup, and of all; `lds` holds an int per wavefront.
 template <int WAVES>
@@ -125,8 +126,8 @@ __device__ __forceinline__ int exclusive_sum(int v, int* lds, int& all) {
 
 // The tokens by (token mod W, token / W), then by position, W = 2^log_shares workgroups: workgroup w has the
 // tokens that are w mod W, and its places are behind those of the workgroups before it.  Each of its wavefronts
-// walks a run of the positions (of less than 2^22), counts its tokens (and those of earlier workgroups) and lists
-// them; when the counters have become places, the list goes there.  Every workgroup reads all tokens (from L2, a
+// walks a run of the positions (of less than 2^22), lists its tokens and counts them (and those of earlier
+// workgroups); when the counters have become places, the list goes there.  Every workgroup reads all tokens (from L2, a
 // few instructions for 64 of them), and none waits for another.  Frequent tokens, often neighbours, spread over
 // the workgroups; a wavefront whose list is too short walks its run again, and empties it when it is full.
 // `named` gets a byte for each row of the table: whether a token names it.  Places behind the last token
@@ -146,65 +147,78 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
   for (int k = lane; k < mine; k += 64) counters[wave][k] = 0;
   const i64 run = ((count + THREADS - 1) / THREADS) * 64;
   const i64 first = wave * run < count ? wave * run : count, end = first + run < count ? first + run : count;
-  const u32 lane_bytes = (u32)lane * (u32)stride_i * (u32)sizeof(Ix);    // (strides are below 2^20)
-  // a group of positions; absent tokens behind the end
-  auto load = [&](i64 i0, Ix* token) {
-    if (i0 + GROUP <= end) {
+  // A group of positions, through a buffer: no load is in a branch, so that the wait for one group leaves the next
+  // in flight (in branches 55087 tokens 18 us).  Past the run's end nothing is read and the tokens are absent.
+  // (strides are at most kMostTokenStride, so that a run's bytes stay below 2^30)
+  const u32 step = (u32)stride_i * (u32)sizeof(Ix);
+  const __amdgpu_buffer_rsrc_t run_words = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(tokens + first * stride_i), (short)0, end > first ? (int)((end - first - 1) * step + sizeof(Ix)) : 0,
+      (int)0x00020000);
+  const int size = (int)(end - first);
+  auto load = [&](int i0, Ix* token) {
 #pragma unroll
-      for (int b = 0; b < BATCHES; ++b)
-        token[b] = *(const Ix*)((const char*)(tokens + (i0 + b * 64) * stride_i) + lane_bytes);
-    } else {
-#pragma unroll
-      for (int b = 0; b < BATCHES; ++b) {
-        const i64 i = i0 + b * 64 + lane;
-        token[b] = i < end ? tokens[i * stride_i] : (Ix)-1;
+    for (int b = 0; b < BATCHES; ++b) {
+      const u32 at = (u32)(i0 + b * 64 + lane) * step;
+      if constexpr (sizeof(Ix) == 8) {
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(run_words, at, 0, 0);
+        token[b] = (Ix)((u64)w.x | (u64)w.y << 32);
+      } else {
+        token[b] = (Ix)__builtin_amdgcn_raw_buffer_load_b32(run_words, at, 0, 0);
       }
     }
   };
-  auto known = [&](Ix token) -> u32 {                // unknown tokens are of no workgroup
-    if constexpr (sizeof(Ix) == 8) {
-      const u64 t = (u64)token;
-      return (u32)(t >> 32) == 0 && (u32)t < vocab ? (u32)t : ~0u;
-    } else {
-      return (u32)token < vocab ? (u32)token : ~0u;
-    }
+  // The remainder of a token, which is the workgroup that it belongs to; an unknown token is of none.  (`left`:
+  // tokens of the run from the batch on)
+  auto owner = [&](Ix token, int left) -> u32 {
+    bool known = (u32)token < vocab;
+    if constexpr (sizeof(Ix) == 8) known = known && (u32)((u64)token >> 32) == 0;
+    u32 of = known ? (u32)token & mask : ~0u;
+    if (left < 64 * BATCHES) of = lane < left ? of : ~0u;                // (the run's last group)
+    return of;
   };
   // every group of the wavefront's run, the next one's tokens in flight
   auto walk = [&](auto each) {
     Ix a[BATCHES], b[BATCHES];
-    load(first, a);
-    for (i64 i0 = first; i0 < end; i0 += 2 * GROUP) {
+    load(0, a);
+    for (int i0 = 0; i0 < size; i0 += 2 * GROUP) {
       load(i0 + GROUP, b);
       each(i0, a);
-      if (i0 + GROUP >= end) break;
       load(i0 + 2 * GROUP, a);
       each(i0 + GROUP, b);
     }
   };
   int listed = 0;
-  // a batch's own tokens, to the list
-  auto note = [&](bool own, u64 some, u32 key, i64 position) {
+  // a batch's own tokens (there is room for a batch), to the list
+  auto note = [&](bool own, u64 some, u32 key, int position) {
     const int at = listed + __builtin_amdgcn_mbcnt_hi((u32)(some >> 32), __builtin_amdgcn_mbcnt_lo((u32)some, 0));
-    if (own && at < LIST) list[wave][at] = (key >> log_shares) << 22 | (u32)(position - first);
+    if (own) list[wave][at] = (key >> log_shares) << 22 | (u32)position;
     listed += __builtin_popcountll(some);
   };
-  int earlier = 0;
-  walk([&](i64 i0, const Ix* token) {
+  auto tally = [&]() {                               // counts the list's tokens
+    for (int l = lane; l < listed; l += 64)
+      __hip_atomic_fetch_add(&counters[wave][list[wave][l] >> 22], 1, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  int earlier = 0;                                   // of the wavefront
+  bool whole = true;                                 // the list holds all of them
+  walk([&](int i0, const Ix* token) {
 #pragma unroll
     for (int b = 0; b < BATCHES; ++b) {
-      const u32 key = known(token[b]), of = key & mask;
-      earlier += of < share ? 1 : 0;
-      const bool own = of == share && key != ~0u;
-      const u64 some = __builtin_amdgcn_ballot_w64(own);
+      const u32 of = owner(token[b], size - i0 - b * 64);
+      earlier += __builtin_popcountll(__builtin_amdgcn_uicmp(of, share, 36));    // less than
+      const u64 some = __builtin_amdgcn_uicmp(of, share, 32);                    // equal
       if (some == 0) continue;
-      if (own)
-        __hip_atomic_fetch_add(&counters[wave][key >> log_shares], 1, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_WORKGROUP);
-      note(own, some, key, i0 + b * 64 + lane);
+      if (listed + 64 > LIST) {
+        tally();
+        listed = 0;
+        whole = false;
+      }
+      note(of == share, some, (u32)token[b], i0 + b * 64 + lane);
     }
   });
+  tally();
   int base;
-  exclusive_sum<WAVES>(earlier, sums, base);         // (its barriers are behind all counts)
+  exclusive_sum<WAVES>(lane == 0 ? earlier : 0, sums, base);         // (its barriers are behind all counts)
   for (int k0 = 0; k0 < mine; k0 += THREADS) {
     const int k = k0 + threadIdx.x;
     int total = 0, all;
@@ -229,9 +243,9 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
     for (i64 i = base + (int)threadIdx.x; i < count; i += THREADS) keys[i] = vocab;
   // the list's tokens, which are in order of their positions, to their places
   const int bits = mine > 1 ? 32 - __builtin_clz(mine - 1) : 0;
-  auto empty = [&](int count) {
-    for (int l0 = 0; l0 < count; l0 += 64) {
-      const bool here = l0 + lane < count;
+  auto empty = [&]() {
+    for (int l0 = 0; l0 < listed; l0 += 64) {
+      const bool here = l0 + lane < listed;
       const u32 entry = here ? list[wave][l0 + lane] : 0;
       const int k = (int)(entry >> 22);
       u64 same = __builtin_amdgcn_ballot_w64(here);
@@ -251,26 +265,25 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
       }
     }
   };
-  if (listed <= LIST) {
-    empty(listed);
+  if (whole) {
+    empty();
     return;
   }
   listed = 0;
-  walk([&](i64 i0, const Ix* token) {
+  walk([&](int i0, const Ix* token) {
 #pragma unroll
     for (int b = 0; b < BATCHES; ++b) {
-      const u32 key = known(token[b]);
-      const bool own = (key & mask) == share && key != ~0u;
-      const u64 some = __builtin_amdgcn_ballot_w64(own);
+      const u32 of = owner(token[b], size - i0 - b * 64);
+      const u64 some = __builtin_amdgcn_uicmp(of, share, 32);
       if (some == 0) continue;
       if (listed + 64 > LIST) {
-        empty(listed);
+        empty();
         listed = 0;
       }
-      note(own, some, key, i0 + b * 64 + lane);
+      note(of == share, some, (u32)token[b], i0 + b * 64 + lane);
     }
   });
-  empty(listed);
+  empty();
 }
 
 // ---------------------------------------------------------------- sums

@@ -24,7 +24,7 @@ FEW = 512                # tokens that one launch takes (nep_embedding.h kFewTok
 MOST_TOKENS = 1 << 26    # of a gradient: sixteen wavefronts' runs of 2^22
 MOST_ROWS = 1 << 24      # (each thousand rows have a workgroup that reads all tokens)
 MOST_KEYS = 1024         # rows that a workgroup counts the tokens of (nep_embedding.h kMostKeys)
-MOST_STRIDE = 1 << 20
+MOST_STRIDE = 16         # of a gradient's tokens (nep_embedding.h kMostTokenStride)
 _PROGRAMS: dict = {}
 _OPS: dict = {}
 _FORWARD, _BACKWARD = calls.Table(), calls.Table()
@@ -147,10 +147,10 @@ def _name(t) -> str:
     return str(t.dtype).replace("torch.", "")
 
 
-def _flat(tokens):
-    """Tokens whose elements have one stride, and that stride."""
+def _flat(tokens, most: int | None = None):
+    """Tokens whose elements have one stride (of up to `most`), and that stride."""
     used, stride = calls.rows_of(tokens.unsqueeze(-1))
-    if stride >= MOST_STRIDE:                        # (a wavefront's are addressed with 32-bit offsets)
+    if most is not None and stride > most:
         used, stride = used.contiguous(), 1
     return (tokens if used.data_ptr() == tokens.data_ptr() else used), stride
 
@@ -256,7 +256,7 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
     n, count = grad.shape[-1], tokens.numel()
     if metadata or count == 0:
         return torch.zeros((vocab, n), dtype=grad.dtype, device=grad.device) if into is None else into
-    (g, sg), (flat, si) = calls.rows_of(grad), _flat(tokens)
+    (g, sg), (flat, si) = calls.rows_of(grad), _flat(tokens, MOST_STRIDE)
     used, device = (g, flat, into), calls.device_index(grad)
     st = n if into is None else into.stride(0) if vocab > 1 else n
     out = grad.dtype if into is None else into.dtype

@@ -79,3 +79,6 @@ def test_tokens_have_one_stride():
             assert flat.data_ptr() == t.data_ptr() and step == stride
         walked = flat.as_strided((t.numel(),), (step,), flat.storage_offset())
         assert torch.equal(walked, t.reshape(-1))
+    flat, step = EM._flat(x[:, 1], 5)                # further apart than a gradient reads them: copied
+    assert step == 1 and flat.data_ptr() != x[:, 1].data_ptr() and torch.equal(flat.reshape(-1), x[:, 1])
+    assert EM._flat(x[:, 1], 6)[1] == 6

@@ -142,6 +142,14 @@ def test_strides_and_alignments():
         ref = CG.run_embedding_backward(grad.to(dev), i, vocab, into=torch.ones(vocab, n, device=dev))
         assert torch.equal(part, ref)
         assert (into[:, :offset] == 1).all() and (into[:, offset + n:] == 1).all()
+    for apart in (16, 17):                           # read in place, and copied
+        i = tokens.to(dev).flatten().repeat_interleave(apart)[::apart]
+        for _ in range(2):
+            assert torch.equal(CG.run_embedding_backward(grad.to(dev).flatten(0, 1), i, vocab), want_grad)
+        many = make_tokens("past", 5000, vocab, 3).to(dev)
+        rows = torch.randn(5000, 16, device=dev)
+        assert torch.equal(CG.run_embedding_backward(rows, many.repeat_interleave(apart)[::apart], vocab),
+                           CG.run_embedding_backward(rows, many, vocab))
     # other orders: a table by columns, tokens by columns, a gradient of one row for all tokens
     assert same(CG.run_embedding(tokens.to(dev).T.contiguous().T, table.to(dev).T.contiguous().T), want)
     row = grad[:1, :1].to(dev).expand(b, s, n)
