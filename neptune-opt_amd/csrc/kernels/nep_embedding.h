@@ -14,8 +14,8 @@
 // or, of few tokens, by one launch in which each row's first token finds the others.
 //
 // HBM-bound: the lookup reads and writes a row per token (bf16 16384 x 4096 28 us, 7.1 TB/s), the gradient reads a
-// row per token and writes the table's (16384 tokens of 128256 x 4096 224 us: order 10, sums and clearing 202 at 5.8
-// TB/s, join 7; fp16 55087 tokens of 32003 x 1001 62 us: 18, 39, 5).
+// row per token and writes the table's (16384 tokens of 128256 x 4096 223 us: order 9, sums and clearing 202 at 5.8
+// TB/s, join 7; fp16 55087 tokens of 32003 x 1001 60 us: 16, 40, 5).
 #pragma once
 
 namespace nep {
@@ -148,7 +148,7 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
   const i64 run = ((count + THREADS - 1) / THREADS) * 64;
   const i64 first = wave * run < count ? wave * run : count, end = first + run < count ? first + run : count;
   // A group of positions, through a buffer: no load is in a branch, so that the wait for one group leaves the next
-  // in flight (in branches 55087 tokens 18 us).  Past the run's end nothing is read and the tokens are absent.
+  // in flight (in branches 55087 tokens 18 us, so 16).  Past the run's end nothing is read and the tokens are absent.
   // (strides are at most kMostTokenStride, so that a run's bytes stay below 2^30)
   const u32 step = (u32)stride_i * (u32)sizeof(Ix);
   const __amdgpu_buffer_rsrc_t run_words = __builtin_amdgcn_make_buffer_rsrc(

@@ -11,10 +11,10 @@
 // by small launches that hold a part each (0.9 GB in 290 tensors: 135 us so, 148 by three launches of the sums).
 // The elements are dealt to the workgroups in turn, in pieces of `piece` elements that do not cross tensors; a
 // workgroup finds a piece's tensor among the first pieces' numbers, in LDS, by two ballots (the arguments lie far
-// away, so each is read once).  (From the last piece to the first, scaling finds no more in the caches: 311 us, 314.)
+// away, so each is read once).
 //
 // HBM-bound: the norm reads its tensors once (0.89 GB bf16 135 us, 6.6 TB/s), a scaling reads them again and writes
-// (0.54 GB bf16 into fp32 83 + 297 us, 5.5 TB/s; 0.1 GB fp16 20 + 39).
+// (0.54 GB bf16 into fp32 83 + 295 us, 5.5 TB/s; 0.1 GB fp16 20 + 38).
 #pragma once
 
 namespace nep {

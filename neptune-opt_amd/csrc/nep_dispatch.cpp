@@ -659,7 +659,7 @@ class GradientCalls {
     };
 
     // Workgroups of a launch.  `more`: so many times more where the pieces suffice, since short
-    // workgroups keep what is written close together (0.54 GB into fp32 395 -> 384 us); not for a scaling in
+    // workgroups keep what is written close together (0.54 GB into fp32 395 us, so 384); not for a scaling in
     // place, whose workgroups often have nothing to do.
     uint32_t grid(const Part& part, uint32_t more = 1) const {
       const uint32_t at_once = of_.lanes_ / kPieceLanes, wanted = (part.pieces + at_once - 1) / at_once;
