@@ -92,6 +92,11 @@ def _check_sizes(tokens, vocab: int, n: int) -> None:
         raise NotImplementedError("embedding takes less than 2^31 tokens and rows, and rows of less than 2^28")
 
 
+def _check_gradient_sizes(tokens, vocab: int) -> None:
+    if tokens.numel() >= MOST_TOKENS or vocab > MOST_ROWS:
+        raise NotImplementedError("embedding's gradient takes less than 2^26 tokens, and up to 2^24 rows")
+
+
 def validate_embedding_inputs(tokens, table, *, metadata: bool = False) -> None:
     _check_rows(table, "table", metadata=metadata)
     if table.ndim != 2 or not table.numel():
@@ -112,8 +117,7 @@ def validate_embedding_gradient_inputs(grad, tokens, vocab, into=None, *, metada
                          f"got {tuple(tokens.shape)}")
     n = grad.shape[-1]
     _check_sizes(tokens, vocab, n)
-    if tokens.numel() >= MOST_TOKENS or vocab > MOST_ROWS:
-        raise NotImplementedError("embedding's gradient takes less than 2^26 tokens, and up to 2^24 rows")
+    _check_gradient_sizes(tokens, vocab)
     if into is None:
         return
     calls.check_tensor(into, "embedding into", metadata=metadata)
@@ -290,7 +294,7 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
 
 def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
     """Differentiable custom op `(Tensor tokens, Tensor table) -> Tensor` with the scale in its name; the
-    gradient is the table's."""
+    gradient is the table's, and a call that it would refuse is refused."""
     import torch
 
     from neptune_codegen.autotune import parameter_tag
@@ -303,10 +307,13 @@ def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
     name = f"embedding{parameter_tag({'scale': scale})}"
 
     def _forward(tokens, table):
-        return run_embedding(tokens, table, scale=scale)
+        out = run_embedding(tokens, table, scale=scale)
+        _check_gradient_sizes(tokens, table.shape[0])
+        return out
 
     def _forward_fake(tokens, table):
         validate_embedding_inputs(tokens, table, metadata=True)
+        _check_gradient_sizes(tokens, table.shape[0])
         return torch.empty((*tokens.shape, table.shape[1]), dtype=table.dtype, device=table.device)
 
     def _backward(grad, tokens, vocab):

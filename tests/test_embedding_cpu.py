@@ -56,6 +56,9 @@ def test_metadata_calls():
     assert grad.shape == (10, 16) and grad.dtype == torch.bfloat16
     into = meta(10, 16, dtype=torch.float32)
     assert CG.run_embedding_backward(G, I, 10, into=into) is into
+    assert CG.run_embedding(I, meta((1 << 24) + 1, 16)).shape == (2, 3, 16)
+    with pytest.raises(NotImplementedError):         # which its gradient would refuse
+        CG.as_embedding_op(2.0)(I, meta((1 << 24) + 1, 16))
     op = CG.as_embedding_op(2.0)
     assert op is CG.as_embedding_op(2) and op(I, T).shape == (2, 3, 16)
 
