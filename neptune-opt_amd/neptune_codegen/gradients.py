@@ -33,7 +33,7 @@ _KERNELS = (("gradient_norm", (hip.PTR, hip.I32, hip.PTR)), ("gradient_list", _L
 _PROGRAM = None
 _CALLS = None
 _OPS: dict = {}
-_lock = threading.Lock()
+_lock = threading.RLock()
 
 
 def _program() -> hip.Program:
@@ -45,14 +45,16 @@ def _program() -> hip.Program:
 
 
 def _calls(device: int | None = None):
-    """The calls in C++, with the kernels of `device` among them."""
+    """The calls in C++, with the kernels of `device` among them.  (One object for all threads: kernels that one
+    adds are in the object that every other one uses.)"""
     global _CALLS
-    if _CALLS is None:
-        _CALLS = dispatch.extension().GradientCalls(TENSORS, MOST_TENSORS, LANES, WORKGROUPS)
-    if device is not None and not _CALLS.has(device):
-        prog = _program()
-        _CALLS.add(device, [prog.kernel(name, args, LANES, device).handle for name, args in _KERNELS])
-    return _CALLS
+    with _lock:
+        if _CALLS is None:
+            _CALLS = dispatch.extension().GradientCalls(TENSORS, MOST_TENSORS, LANES, WORKGROUPS)
+        if device is not None and not _CALLS.has(device):
+            prog = _program()
+            _CALLS.add(device, [prog.kernel(name, args, LANES, device).handle for name, args in _KERNELS])
+        return _CALLS
 
 
 def _dense(t) -> bool:
