@@ -167,6 +167,8 @@ def check_tensor(t, name: str, *, metadata: bool) -> None:
         raise TypeError(f"{name} must be strided")
     if not metadata and t.device.type != "cuda":
         raise ValueError(f"{name} is on {t.device}; execution requires a ROCm (cuda) device")
+    if not metadata and t.numel() and t.data_ptr() == 0:         # a wrapper around others (DTensor, for one)
+        raise TypeError(f"{name} is a {type(t).__name__} without memory of its own; pass the tensor that it wraps")
 
 
 def overlap(a, b) -> bool:

@@ -108,7 +108,8 @@ def _refuse_written(tensors, out) -> None:
                                                  if n != 1 and t.numel()):
             raise ValueError("clipped gradients must fill their memory without gaps, outputs in their gradient's "
                              "order")
-    raise ValueError("clipped gradients must not overlap one another, what is read, or the norm")
+    raise ValueError("clipped gradients must be plain tensors (and no negated views) that do not overlap one another, "
+                     "what is read, or the norm")
 
 
 def _refuse_recording() -> None:
@@ -144,7 +145,10 @@ def run_gradient_norm(tensors):
     validate_gradient_inputs(tensors, metadata=metadata)
     if metadata:
         return torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    return _calls(calls.device_index(tensors[0])).norm(_plain(tensors, True))
+    found = _calls(calls.device_index(tensors[0])).norm(_plain(tensors, True))
+    if found is None:
+        raise TypeError("gradients must be plain tensors, or subclasses that are plain tensors without their class")
+    return found
 
 
 def _max_norm(max_norm) -> float:
