@@ -13,7 +13,9 @@ class Wrapper(torch.Tensor):
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
-        return args[0] if func is torch.ops.aten.alias.default else NotImplemented
+        if func is torch.ops.aten.alias.default:
+            return Wrapper(*args[0].shape, dtype=args[0].dtype)
+        return NotImplemented
 
 
 I64 = torch.int64
