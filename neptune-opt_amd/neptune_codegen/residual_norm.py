@@ -198,8 +198,10 @@ _CODES: dict = {None: 0}     # of the types seen so far
 
 
 def _format(dtype) -> str:
+    import torch
+
     name = str(dtype).replace("torch.", "")
-    if name not in _FORMATS:
+    if not isinstance(dtype, torch.dtype) or name not in _FORMATS:
         raise TypeError(f"residual norm's 8-bit outputs are {', '.join(_FORMATS)}, got {dtype}")
     _CODES[dtype] = _FORMATS.index(name)
     return name
