@@ -29,7 +29,7 @@ import functools
 import math
 import threading
 
-from neptune_codegen import hip
+from neptune_codegen import dispatch, hip
 from neptune_codegen.emitters import (ATTN_HEAD_DIMS, ATTN_SHORT_BLOCK_M, ATTN_SHORT_TILE,
                                       ATTN_SHORT_WAVES, BASE_OPTIONS, attention_block_m,
                                       attention_fold_threads, attention_kernel_name,
@@ -570,6 +570,7 @@ def exact_path_taken(exps) -> bool:
 attention_fold = run_attention
 
 
+@dispatch.one_at_a_time
 def as_attention_op(scale: float | None = None, causal: bool = True, lib: str = "neptune"):
     """Custom op `(Tensor q, Tensor k, Tensor v) -> Tensor` with scale and mask in its name."""
     import torch

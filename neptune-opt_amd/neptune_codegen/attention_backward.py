@@ -19,7 +19,7 @@ import functools
 import math
 import threading
 
-from neptune_codegen import calls, hip
+from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.attention import K_ROW_STRIDE_MAX, LOG2E, validate_attention_inputs
 from neptune_codegen.emitters import (ATTN_BWD_TILE, ATTN_BWD_WAVES, BASE_OPTIONS,
                                       attention_backward_blocks, attention_backward_kernel_name,
@@ -270,6 +270,7 @@ def _run(grad, q, k, v, out, lse, grad_lse, scale, causal, plan=None):
     return call.run(used)
 
 
+@dispatch.one_at_a_time
 def as_attention_grad_op(scale: float | None = None, causal: bool = True, lib: str = "neptune"):
     """Differentiable custom op `(Tensor q, Tensor k, Tensor v) -> (Tensor out, Tensor lse)` with
     scale and mask in its name: run_attention with its logsumexp, and run_attention_backward for

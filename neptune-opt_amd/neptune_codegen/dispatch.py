@@ -26,6 +26,7 @@ for example).
 """
 from __future__ import annotations
 
+import functools
 import importlib.util
 import struct
 import threading
@@ -33,6 +34,7 @@ import threading
 from neptune_codegen import hip
 
 _lock = threading.Lock()
+_defining = threading.RLock()
 _module = None
 MAX_PLANS = 1024      # per operator; later layouts keep using the Python body
 # qualname -> {"arguments": schema text after the name, "n_inputs": int,
@@ -59,6 +61,16 @@ def extension():
         spec.loader.exec_module(module)
         _module = module
         return module
+
+
+def one_at_a_time(make):
+    """`make`, which registers an operator, for one thread at a time: torch takes neither two definitions of a name
+    nor two at once, and a second caller finds what the first has kept."""
+    @functools.wraps(make)
+    def locked(*args, **kwargs):
+        with _defining:
+            return make(*args, **kwargs)
+    return locked
 
 
 def plan_of(recorder: hip.Recorder, inputs: tuple, outputs: tuple):

@@ -18,7 +18,7 @@ from __future__ import annotations
 import math
 import threading
 
-from neptune_codegen import calls, hip
+from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.emitters import (BASE_OPTIONS, DistillVariant, distill_kernel_name,
                                       emit_distill_source)
 from neptune_codegen.template import _validate_row_last
@@ -203,6 +203,7 @@ def run_distill_backward(grad, logits, top_logits, top_index, stats, *, temperat
     return plan.run(used)
 
 
+@dispatch.one_at_a_time
 def as_distill_op(temperature: float = 1.0, lib: str = "neptune"):
     """Differentiable custom op `(Tensor logits, Tensor top_logits, Tensor top_index) -> (Tensor loss,
     Tensor stats)` with the temperature in its name; the gradient is the logits'."""

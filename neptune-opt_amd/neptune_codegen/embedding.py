@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import threading
 
-from neptune_codegen import calls, hip
+from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.emitters import (BASE_OPTIONS, EmbeddingVariant, embedding_few_name, embedding_order_name,
                                       embedding_sums_name, emit_embedding_few_source,
                                       emit_embedding_order_source, emit_embedding_source,
@@ -292,6 +292,7 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
     return made[0]
 
 
+@dispatch.one_at_a_time
 def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
     """Differentiable custom op `(Tensor tokens, Tensor table) -> Tensor` with the scale in its name; the
     gradient is the table's, and a call that it would refuse is refused."""

@@ -179,6 +179,7 @@ def run_clip_gradients(tensors, max_norm: float, *, norm=None, out=None):
     return found
 
 
+@dispatch.one_at_a_time
 def as_gradient_norm_op(lib: str = "neptune"):
     """Custom op `(Tensor[] tensors) -> Tensor`: run_gradient_norm, without a gradient of its own."""
     import torch
@@ -198,6 +199,7 @@ def as_gradient_norm_op(lib: str = "neptune"):
         return _OPS.setdefault((lib, "norm"), op)
 
 
+@dispatch.one_at_a_time
 def as_clip_gradients_op(lib: str = "neptune"):
     """Custom op `(Tensor(a!)[] tensors, float max_norm) -> Tensor`: run_clip_gradients in place."""
     import torch

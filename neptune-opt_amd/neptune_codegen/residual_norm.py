@@ -23,7 +23,7 @@ import dataclasses
 import math
 import threading
 
-from neptune_codegen import calls, hip
+from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.emitters import (BASE_OPTIONS, ResidualNormVariant, emit_residual_norm_source,
                                       residual_norm_kernel_name)
 from neptune_codegen.template import _validate_row_last
@@ -283,6 +283,7 @@ def run_residual_norm_quantized(x, y, gamma_after, gamma_before, *, gate=None, r
     return plan.run(used)
 
 
+@dispatch.one_at_a_time
 def as_residual_norm_quantized_op(residual_scale: float = 1.0, eps: float = 1e-6, dtype=None,
                                   group: int | None = None, power_of_two: bool = False, lib: str = "neptune"):
     """Custom op `(Tensor x, Tensor y, Tensor? gamma_after, Tensor gamma_before, Tensor? gate) -> (Tensor
@@ -394,6 +395,7 @@ def run_residual_norm_backward(grad_residual, grad_normed, x, y, gamma_after, ga
     return plan.run(used)
 
 
+@dispatch.one_at_a_time
 def as_residual_norm_op(residual_scale: float = 1.0, eps: float = 1e-6, lib: str = "neptune"):
     """Differentiable custom op `(Tensor x, Tensor y, Tensor? gamma_after, Tensor gamma_before, Tensor? gate)
     -> (Tensor residual, Tensor normed, Tensor stats)` with the numbers in its name."""

@@ -16,7 +16,7 @@ from __future__ import annotations
 import math
 import threading
 
-from neptune_codegen import calls, hip
+from neptune_codegen import calls, dispatch, hip
 from neptune_codegen.emitters import BASE_OPTIONS, emit_rotary_source, rotary_kernel_name
 
 _PROGRAMS: dict = {}
@@ -178,6 +178,7 @@ def run_rotary_backward(grad_q, grad_k, positions, turns, *, magnitude: float = 
     return _run(grad_q, grad_k, positions, turns, magnitude, interleaved, -1.0)
 
 
+@dispatch.one_at_a_time
 def as_rotary_op(magnitude: float = 1.0, interleaved: bool = False, lib: str = "neptune"):
     """Differentiable custom op `(Tensor q, Tensor k, Tensor positions, Tensor turns) -> (Tensor, Tensor)`
     with the magnitude and the layout in its name (a k of no heads stands for none)."""

@@ -32,6 +32,7 @@ def _register(qualname: str, schema: str, impl, fake):
     return op
 
 
+@dispatch.one_at_a_time
 def as_triton_op(name: str, block: int | None = None, num_warps: int | None = None,
                  lib: str = "neptune", params: dict | None = None, keepdim: bool = False,
                  plan: str = "serial"):
@@ -107,6 +108,7 @@ def triton_op_name(name: str, lib: str = "neptune") -> str:
     return f"{lib}.{name}"
 
 
+@dispatch.one_at_a_time
 def as_readout_op(name: str, params: dict | None = None, nan_posinf_rows: bool = True,
                   lib: str = "neptune", block: int | None = None, num_warps: int | None = None):
     """Custom op `(Tensor x) -> Tensor`: the readout phi(x) - r of the exponential fold `name`
@@ -162,6 +164,7 @@ def readout_op_handle(name: str, params: dict | None = None, nan_posinf_rows: bo
 _STATE_OPS: dict[tuple, object] = {}
 
 
+@dispatch.one_at_a_time
 def as_state_op(name, params=None, plan="serial", lib="neptune"):
     """Structured op: rms_norm `(Tensor x, Tensor gamma) -> Tensor`, l2_normalize
     `(Tensor x) -> Tensor`; segment names go to as_segment_op."""
@@ -619,6 +622,7 @@ def run_segment_pool(data, segments, *, reduce="sum", offsets=False, initial=Non
     return _launch_segment(name, data, segments, params, plan)
 
 
+@dispatch.one_at_a_time
 def as_segment_op(name, params=None, plan="serial", lib="neptune"):
     """Custom op `(Tensor data, Tensor segments) -> Tensor`; constants live in its identity."""
     import torch
