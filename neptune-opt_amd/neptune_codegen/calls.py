@@ -173,14 +173,12 @@ def check_tensor(t, name: str, *, metadata: bool) -> None:
 
 def overlap(a, b) -> bool:
     """Whether the memory between two tensors' first and last elements overlaps."""
-    def ends(t):
-        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-        return t.data_ptr(), t.data_ptr() + span * t.element_size()
-
     if not a.numel() or not b.numel():
         return False
-    (a0, a1), (b0, b1) = ends(a), ends(b)
-    return a0 < b1 and b0 < a1
+    low, high = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
+    span = low.nbytes if low.is_contiguous() else \
+        (sum((n - 1) * s for n, s in zip(low.shape, low.stride())) + 1) * low.element_size()
+    return high.data_ptr() < low.data_ptr() + span
 
 
 def written(t) -> None:

@@ -131,11 +131,14 @@ def validate_embedding_gradient_inputs(grad, tokens, vocab, into=None, *, metada
         raise ValueError("embedding into must have unit column stride and rows that do not overlap")
 
 
-def _apart(grad, into) -> bool:
+def _apart(into, *read) -> bool:
+    """Whether `into` overlaps nothing that is read (what is no tensor or has no memory is refused elsewhere)."""
     import torch
 
-    return not isinstance(grad, torch.Tensor) or calls.is_metadata(grad) or calls.is_metadata(into) or \
-        not calls.overlap(grad, into)
+    def real(t):
+        return not t.is_meta if type(t) is torch.Tensor else isinstance(t, torch.Tensor) and not calls.is_metadata(t)
+
+    return not real(into) or not any(real(t) and calls.overlap(t, into) for t in read)
 
 
 def _access(n: int, *tensors) -> str:
@@ -245,7 +248,7 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
 
     given, add = (grad, tokens, into), into is not None
     # (what the layout of the tensors does not say; refused below)
-    apart = not add or (isinstance(into, torch.Tensor) and not into.requires_grad and _apart(grad, into))
+    apart = not add or (isinstance(into, torch.Tensor) and not into.requires_grad and _apart(into, grad, tokens))
     found = _BACKWARD.run(given, (vocab, scale)) if apart else None
     if found is not None:
         if not add:
@@ -255,7 +258,7 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
     metadata = isinstance(grad, torch.Tensor) and calls.is_metadata(grad)
     validate_embedding_gradient_inputs(grad, tokens, vocab, into, metadata=metadata)
     if not metadata and not apart:
-        raise ValueError("embedding into must not overlap the gradient that is added to it")
+        raise ValueError("embedding into must not overlap the gradient that is added to it, or the tokens")
     number, scale = scale, _scale(scale)
     n, count = grad.shape[-1], tokens.numel()
     if metadata or count == 0:
