@@ -158,13 +158,16 @@ def rows_of(t):
     return t, step or 0
 
 
-def check_tensor(t, name: str, *, metadata: bool) -> None:
+def check_tensor(t, name: str, *, metadata: bool, negated: bool = False) -> None:
+    """`negated`: whether the caller takes views whose memory holds their negated elements (a conjugate's imag)."""
     import torch
 
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.layout != torch.strided:
         raise TypeError(f"{name} must be strided")
+    if not metadata and not negated and t.is_neg():
+        raise ValueError(f"{name} is a view that negates what its memory holds; pass its resolve_neg()")
     if not metadata and t.device.type != "cuda":
         raise ValueError(f"{name} is on {t.device}; execution requires a ROCm (cuda) device")
     if not metadata and t.numel() and t.data_ptr() == 0:         # a wrapper around others (DTensor, for one)

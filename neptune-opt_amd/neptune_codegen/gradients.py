@@ -73,7 +73,7 @@ def _check_list(tensors, name: str, *, metadata: bool) -> None:
     if not isinstance(tensors, (list, tuple)) or not tensors:
         raise TypeError(f"{name} must be a list of at least one tensor")
     for t in tensors:
-        calls.check_tensor(t, name, metadata=metadata)
+        calls.check_tensor(t, name, metadata=metadata, negated=True)    # (the norm resolves, clipping refuses)
         if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
         if t.device != tensors[0].device:
