@@ -24,6 +24,7 @@ FEW = 512                # tokens that one launch takes (nep_embedding.h kFewTok
 MOST_TOKENS = 1 << 26    # of a gradient: sixteen wavefronts' runs of 2^22
 MOST_ROWS = 1 << 24      # (each thousand rows have a workgroup that reads all tokens)
 MOST_KEYS = 1024         # rows that a workgroup counts the tokens of (nep_embedding.h kMostKeys)
+MOST_ROW = 65535 << 10   # bytes, of more than FEW tokens' gradient (the join's grid: 65535 times 64 words)
 MOST_STRIDE = 16         # of a gradient's tokens (nep_embedding.h kMostTokenStride)
 _PROGRAMS: dict = {}
 _OPS: dict = {}
@@ -92,9 +93,11 @@ def _check_sizes(tokens, vocab: int, n: int) -> None:
         raise NotImplementedError("embedding takes less than 2^31 tokens and rows, and rows of less than 2^28")
 
 
-def _check_gradient_sizes(tokens, vocab: int) -> None:
+def _check_gradient_sizes(tokens, vocab: int, n: int, size: int) -> None:
     if tokens.numel() >= MOST_TOKENS or vocab > MOST_ROWS:
         raise NotImplementedError("embedding's gradient takes less than 2^26 tokens, and up to 2^24 rows")
+    if tokens.numel() > FEW and n * size > MOST_ROW:
+        raise NotImplementedError(f"embedding's gradient of more than {FEW} tokens takes rows of up to {MOST_ROW} bytes")
 
 
 def validate_embedding_inputs(tokens, table, *, metadata: bool = False) -> None:
@@ -117,7 +120,7 @@ def validate_embedding_gradient_inputs(grad, tokens, vocab, into=None, *, metada
                          f"got {tuple(tokens.shape)}")
     n = grad.shape[-1]
     _check_sizes(tokens, vocab, n)
-    _check_gradient_sizes(tokens, vocab)
+    _check_gradient_sizes(tokens, vocab, n, grad.element_size())
     if into is None:
         return
     calls.check_tensor(into, "embedding into", metadata=metadata)
@@ -298,7 +301,8 @@ def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into
 @dispatch.one_at_a_time
 def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
     """Differentiable custom op `(Tensor tokens, Tensor table) -> Tensor` with the scale in its name; the
-    gradient is the table's, and a call that it would refuse is refused."""
+    gradient is the table's, and a call that it would refuse is refused before anything runs, whether or not the table
+    requires grad (run_embedding takes larger tables and more tokens)."""
     import torch
 
     from neptune_codegen.autotune import parameter_tag
@@ -311,13 +315,13 @@ def as_embedding_op(scale: float = 1.0, lib: str = "neptune"):
     name = f"embedding{parameter_tag({'scale': scale})}"
 
     def _forward(tokens, table):
-        out = run_embedding(tokens, table, scale=scale)
-        _check_gradient_sizes(tokens, table.shape[0])
-        return out
+        if table.ndim == 2:
+            _check_gradient_sizes(tokens, *table.shape, table.element_size())
+        return run_embedding(tokens, table, scale=scale)
 
     def _forward_fake(tokens, table):
         validate_embedding_inputs(tokens, table, metadata=True)
-        _check_gradient_sizes(tokens, table.shape[0])
+        _check_gradient_sizes(tokens, *table.shape, table.element_size())
         return torch.empty((*tokens.shape, table.shape[1]), dtype=table.dtype, device=table.device)
 
     def _backward(grad, tokens, vocab):
