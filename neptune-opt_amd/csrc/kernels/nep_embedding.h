@@ -124,6 +124,13 @@ __device__ __forceinline__ int exclusive_sum(int v, int* lds, int& all) {
   return before + s - v;
 }
 
+// In a wavefront: what its lanes have stored in LDS is there for its other lanes' reads behind, and is read before their
+// stores behind.  (LDS takes a wavefront's accesses in order; this keeps the compiler to it.)
+__device__ __forceinline__ void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // The tokens by (token mod W, token / W), then by position, W = 2^log_shares workgroups: workgroup w has the
 // tokens that are w mod W, and its places are behind those of the workgroups before it.  Each of its wavefronts
 // walks a run of the positions (of less than 2^22), lists its tokens and counts them (and those of earlier
@@ -145,6 +152,7 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
   const u32 share = blockIdx.x, mask = (1u << log_shares) - 1;
   const int mine = share < vocab ? (int)((vocab - 1 - share) >> log_shares) + 1 : 0;    // keys
   for (int k = lane; k < mine; k += 64) counters[wave][k] = 0;
+  lanes_meet();
   const i64 run = ((count + THREADS - 1) / THREADS) * 64;
   const i64 first = wave * run < count ? wave * run : count, end = first + run < count ? first + run : count;
   // A group of positions, through a buffer: no load is in a branch, so that the wait for one group leaves the next
@@ -195,9 +203,11 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
     listed += __builtin_popcountll(some);
   };
   auto tally = [&]() {                               // counts the list's tokens
+    lanes_meet();
     for (int l = lane; l < listed; l += 64)
       __hip_atomic_fetch_add(&counters[wave][list[wave][l] >> 22], 1, __ATOMIC_RELAXED,
                              __HIP_MEMORY_SCOPE_WORKGROUP);
+    lanes_meet();
   };
   int earlier = 0;                                   // of the wavefront
   bool whole = true;                                 // the list holds all of them
@@ -244,6 +254,7 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
   // the list's tokens, which are in order of their positions, to their places
   const int bits = mine > 1 ? 32 - __builtin_clz(mine - 1) : 0;
   auto empty = [&]() {
+    lanes_meet();
     for (int l0 = 0; l0 < listed; l0 += 64) {
       const bool here = l0 + lane < listed;
       const u32 entry = here ? list[wave][l0 + lane] : 0;
@@ -263,6 +274,7 @@ __device__ __forceinline__ void embedding_order(const Ix* __restrict__ tokens, u
         keys[place] = (u32)k << log_shares | share;
         positions[place] = (u32)first + (entry & 0x3fffffu);
       }
+      lanes_meet();
     }
   };
   if (whole) {
