@@ -96,7 +96,7 @@ def _check_sizes(tokens, vocab: int, n: int) -> None:
 def _check_gradient_sizes(tokens, vocab: int, n: int, size: int) -> None:
     if tokens.numel() >= MOST_TOKENS or vocab > MOST_ROWS:
         raise NotImplementedError("embedding's gradient takes less than 2^26 tokens, and up to 2^24 rows")
-    if tokens.numel() > FEW and n * size > MOST_ROW:
+    if n * size > MOST_ROW and tokens.numel() > FEW:
         raise NotImplementedError(f"embedding's gradient of more than {FEW} tokens takes rows of up to {MOST_ROW} bytes")
 
 
