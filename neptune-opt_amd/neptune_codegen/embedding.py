@@ -246,7 +246,7 @@ def _ordered(given, table, buffers, device, access, add, out, si, sg, st, scale,
 def run_embedding_backward(grad, tokens, vocab: int, *, scale: float = 1.0, into=None):
     """Gradient [vocab, n] of the table for the output's gradient `grad` [..., n], in its dtype; or, with
     `into` [vocab, n] in that dtype or float32, the gradient added to `into` in place (one rounding for each
-    row that a token names, the others untouched), and `into`."""
+    row that a token names, the others untouched), and `into`, which overlaps nothing that the call reads."""
     import torch
 
     given, add = (grad, tokens, into), into is not None
