@@ -24,6 +24,7 @@
 // tensors and the numbers of a call.  GradientCalls runs the operators that take a list of tensors
 // (neptune_codegen/gradients.py), whose launches hold the tensors' addresses by value.
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
@@ -278,6 +279,16 @@ py::object key_of(const std::vector<at::Tensor>& tensors) {
   throw py::error_already_set();
 }
 
+// Whether a tensor's elements are in its storage: not those of a wrapper around other tensors, nor where the storage
+// was freed or made shorter behind them (storage.resize_).
+bool in_memory(const at::Tensor& t) {
+  if (!t.has_storage()) return false;
+  if (t.numel() == 0) return true;
+  const c10::Storage& storage = t.storage();
+  return storage.data() != nullptr && at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.itemsize(),
+                                                                       t.storage_offset()) <= storage.nbytes();
+}
+
 // One call layout of an entry point: the buffers it allocates (results first, then scratch) and its
 // launches, whose pointer arguments are each an input, or a buffer at a byte offset.
 class CallPlan {
@@ -418,7 +429,7 @@ class CallTable {
       if (!THPVariable_CheckExact(o)) return false;
       const at::Tensor& t = THPVariable_Unpack(o);
       if (!t.defined() || !t.device().is_cuda() || t.layout() != c10::kStrided || t.is_neg() || t.is_conj() ||
-          t.key_set().has(c10::DispatchKey::Python))
+          t.key_set().has(c10::DispatchKey::Python) || !in_memory(t))
         return false;
       key.push_back(static_cast<int64_t>(t.scalar_type()));
       key.push_back(t.get_device());
@@ -706,7 +717,7 @@ class GradientCalls {
 
   static bool plain(const at::Tensor& t) {
     return t.defined() && t.device().is_cuda() && t.layout() == c10::kStrided && !t.is_neg() && !t.is_conj() &&
-           !t.key_set().has(c10::DispatchKey::Python);
+           !t.key_set().has(c10::DispatchKey::Python) && in_memory(t);
   }
 
   // The tensors of a list or tuple that is not empty: of the three types, on one device, without gaps.
@@ -800,6 +811,7 @@ PYBIND11_MODULE(_neptune_dispatch, m) {
   m.def("installed", &installed, py::arg("qualname"));
   m.def("key_of", &key_of, py::arg("tensors"));
   m.def("dtype_code", &dtype_code, py::arg("tensor"));
+  m.def("in_memory", &in_memory, py::arg("tensor"));
   py::class_<CallPlan, std::shared_ptr<CallPlan>>(m, "CallPlan")
       .def(py::init<int, const py::tuple&, std::vector<int>, bool, const py::tuple&>(), py::arg("n_inputs"),
            py::arg("buffers"), py::arg("returns"), py::arg("bare"), py::arg("launches"))

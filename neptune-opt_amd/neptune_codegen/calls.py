@@ -170,8 +170,9 @@ def check_tensor(t, name: str, *, metadata: bool, negated: bool = False) -> None
         raise ValueError(f"{name} is a view that negates what its memory holds; pass its resolve_neg()")
     if not metadata and t.device.type != "cuda":
         raise ValueError(f"{name} is on {t.device}; execution requires a ROCm (cuda) device")
-    if not metadata and t.numel() and t.data_ptr() == 0:         # a wrapper around others (DTensor, for one)
-        raise TypeError(f"{name} is a {type(t).__name__} without memory of its own; pass the tensor that it wraps")
+    if not metadata and not dispatch.extension().in_memory(t):
+        raise TypeError(f"{name} is a {type(t).__name__} without memory of its own for its elements: a wrapper around "
+                        "other tensors (pass the one that it wraps), or one whose storage was freed")
 
 
 def overlap(a, b) -> bool:
